@@ -8,14 +8,13 @@
 #include <cstring>
 #include <mutex>
 
+#include "mq_check.h"
 #include "mq_internal.h"
 
 namespace mq {
 
 namespace {
 thread_local char g_err[512] = "";
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 }  // namespace
 
 void set_error(const char* fmt, ...) {
@@ -54,17 +53,7 @@ int launch_status(const char* what) {
 
 namespace {
 
-#define MQ_REQUIRE(cond, ...)        \
-    do {                             \
-        if (!(cond)) {               \
-            set_error(__VA_ARGS__);  \
-            return MQ_EINVAL;        \
-        }                            \
-    } while (0)
-
 constexpr int kEmpty = 1;   // check_gemm_common: valid shape with nothing to compute
-
-int dtype_bytes(int dt) { return dt == MQ_DT_F32 ? 4 : 2; }
 
 // Output and bias checks shared by the GEMM entry points: types, alignment and the row stride.
 int check_gemm_out(const char* what, const void* bias, int bias_dtype, const void* y, int y_dtype, int64_t ldy,

@@ -163,4 +163,111 @@ bool gemm_runs_few(const GemmArgs& a, WKind wk, Epi epi);
 // 256 x 256-tile kernel for large M (mq_gemm_wide.hip).
 int launch_gemm_wide(const GemmArgs& a, WKind wk, Epi epi, hipStream_t stream);
 
+// --- paged key-value cache (mq_kv.hip); strides in elements
+struct KvWriteArgs {
+    const void* k;            // [T, H, D], strides k_token / k_head
+    const void* v;
+    int64_t k_token, k_head, v_token, v_head;
+    int64_t T, H, D;
+    void* kc;                 // [pages, H, page size, D], K and V alike
+    void* vc;
+    int64_t c_page, c_head, c_token;
+    float* k_scale;           // [pages, H, page size] (int8 cache)
+    float* v_scale;
+    int64_t s_page, s_head, s_token;
+    int64_t pages;
+    int page_shift;
+    int row_shift;            // log2 of the lanes that hold a row
+    const int* table;         // [B, width]
+    int64_t ld_table, B, width;
+    const int* lens;
+    const int* cu_q;          // [B + 1], or null: one token per sequence
+};
+int launch_kv_write(const KvWriteArgs& a, int dtype, bool i8, hipStream_t stream);
+
+struct KvTables {
+    int* table;               // [rows, width]
+    int64_t ld_table, rows, width;
+    int* lens;                // [rows]
+    int* refs;                // [pages]
+    int64_t pages;
+    int page_shift;
+};
+struct KvCopyTensor {
+    void* base;
+    int64_t layer_bytes, page_pitch, page_bytes;
+};
+struct KvCopyArgs {
+    KvCopyTensor t[4];        // K, V and their scales
+    int tensors;
+    int64_t layers;
+    const int* moves;         // pairs (from, to); from < 0: none
+    int n;                    // moves, or the most there can be
+    const int* count;         // device count of the moves (null: n)
+    const int* place;         // compaction: new place of every page, applied to tb.table (null: none)
+    KvTables tb;
+};
+int launch_kv_fork(const KvTables& tb, const KvCopyArgs& copies, const int* src, const int* dst, int n, int* work,
+                   int* status, hipStream_t stream);
+int launch_kv_grow(const KvTables& tb, const int* rows, const int* counts, int n, int* work, int* status,
+                   hipStream_t stream);
+int launch_kv_free(const KvTables& tb, const int* rows, int n, hipStream_t stream);
+int launch_kv_compact(const KvTables& tb, const KvCopyArgs& copies, int* work, int* live, hipStream_t stream);
+
+// --- attention over the paged cache (mq_attn_*.hip)
+struct AttnArgs {
+    const void* q;            // [T, Hq, D]
+    int64_t q_token, q_head;
+    void* o;                  // [T, Hq, D]
+    int64_t o_token, o_head;
+    int64_t T;
+    int Hq, H, D;             // query heads, cache heads, head width
+    const void* kc;           // [pages, H, page size, D], K and V alike
+    const void* vc;
+    int64_t c_page, c_head, c_token;
+    const float* k_scale;     // int8 cache: [pages, H, page size]; else null
+    const float* v_scale;
+    int64_t s_page, s_head, s_token;
+    int64_t pages;
+    int page_shift;
+    const int* table;         // [B, width]
+    int64_t ld_table, B, width;
+    const int* lens;
+    const int* cu_q;          // [B + 1], or null: one token per sequence
+    float scale;              // of the scores
+    int64_t window;           // keys that a query sees, its own among them; 0: all
+    int64_t sinks;            // first keys that stay visible behind the window
+    int dtype;                // of q and o
+    void* work;
+    int64_t work_bytes;
+};
+int launch_attention(const AttnArgs& a, hipStream_t stream);
+int64_t attention_workspace_bytes(int64_t T, int Hq, int H, int D, int64_t B, bool ragged);
+
+// --- 4-bit weights, floating activations (mq_w4a16.hip)
+enum class W4Zero : int { Signed = 0, U4 = 1, Float = 2 };
+struct W4A16Args {
+    const void* x;            // [M, K] of type x_dtype
+    int x_dtype;
+    int64_t ldx;
+    int hblock;
+    const uint8_t* qw;        // [N, K / 2]
+    int64_t ldw;
+    const void* ws;           // [N, K / group] of type s_dtype
+    int s_dtype;
+    int64_t ldws;
+    const void* wz;           // packed uint4 [N, ceil(K / group / 2)] or [N, K / group] of type z_dtype
+    int z_dtype;
+    int64_t ldwz;
+    W4Zero zero;
+    int group;
+    const void* bias;
+    int bias_dtype;
+    void* y;
+    int y_dtype;
+    int64_t ldy;
+    int64_t M, N, K;
+};
+int launch_w4a16(const W4A16Args& a, hipStream_t stream);
+
 }  // namespace mq

@@ -11,6 +11,7 @@ keyword arguments, executed by hand-written HIP kernels in `libmq.so` through it
 """
 from . import weights
 from ._lib import LIB_PATH, MQError, load
+from .kv import PagedKVCache, kv_compact, kv_fork, kv_free, kv_grow, kv_write, paged_attention
 from .ops import (
     ExpandedW4,
     PreparedW4A8,
@@ -30,6 +31,7 @@ from .ops import (
     rotate_quantize,
     swiglu_quantize_int4_rowwise_convrot64,
     tile_int8_weight,
+    w4a16_linear,
     w4a8_int8_linear,
 )
 from .weights import (
@@ -48,4 +50,5 @@ __all__ = [
     "gemm_w4_group", "gemm_w4_group_partials", "gemm_rowscale", "gemm_rowscale_acc",
     "quantize_w4a8_asym_weight", "quantize_w4a4_group_weight", "quantize_convrot_w4a4_weight",
     "quantize_int8_convrot_weight",
+    "w4a16_linear", "paged_attention", "kv_write", "kv_fork", "kv_grow", "kv_free", "kv_compact", "PagedKVCache",
 ]

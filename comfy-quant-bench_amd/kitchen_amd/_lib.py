@@ -21,12 +21,14 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmq.so")
 
 _lib = None
-FAST_ENTRIES = ("mq_rotquant", "mq_swiglu_rotquant", "mq_linear_w4_group", "mq_linear_rowscale")
+FAST_ENTRIES = ("mq_rotquant", "mq_swiglu_rotquant", "mq_linear_w4_group", "mq_linear_rowscale", "mq_kv_write",
+                "mq_paged_attention", "mq_kv_grow", "mq_linear_w4a16")
 _entries: dict = {}   # entry point name -> callable
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_vp = ctypes.c_void_p
+c_float = ctypes.c_float
 
 _SIGNATURES = {
     "mq_abi_version": ([], c_int),
@@ -64,6 +66,23 @@ _SIGNATURES = {
                             c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp], c_int),
     "mq_linear_w4_group_noalloc": ([c_vp, c_int, c_i64, c_int, c_int, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                                     c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp], c_int),
+    "mq_kv_write": ([c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64,
+                     c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp],
+                    c_int),
+    "mq_paged_attention": ([c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64,
+                            c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_float,
+                            c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp], c_int),
+    "mq_paged_attention_workspace_bytes": ([c_i64, c_i64, c_i64, c_i64, c_i64, c_int], c_i64),
+    "mq_kv_workspace_bytes": ([c_i64, c_i64], c_i64),
+    "mq_kv_fork": ([c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+                    c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp], c_int),
+    "mq_kv_grow": ([c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp],
+                   c_int),
+    "mq_kv_free": ([c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp], c_int),
+    "mq_kv_compact": ([c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+                       c_vp, c_i64, c_vp, c_vp, c_i64, c_vp], c_int),
+    "mq_linear_w4a16": ([c_vp, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp,
+                         c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp], c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -75,7 +94,8 @@ W8_TILE16 = 0x100            # wbits flag: int8 weights in 16-row tiles (include
 ACT_I8, ACT_I4, ACT_X16ALT = 0, 1, 2
 W4_EXPANDED = 0x100          # act_mode / act_bits flag: 4-bit weights expanded to int8 tiles
 W4X_ROW = 3                  # mq_expand_weight_w4 layout for the row-scale GEMMs
-DT_BF16, DT_F16, DT_F32 = 0, 1, 2
+DT_BF16, DT_F16, DT_F32, DT_I8 = 0, 1, 2, 3
+W4Z_SIGNED, W4Z_U4, W4Z_FLOAT = 0, 1, 2   # zero-points of mq_linear_w4a16
 NOALLOC_SCRATCH_BYTES = 64 << 20   # MQ_NOALLOC_SCRATCH_BYTES
 DTYPE_CODE = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 

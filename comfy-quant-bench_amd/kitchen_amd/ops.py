@@ -772,3 +772,69 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     activations (after H_cg when convrot), full-K int32 accumulation."""
     return int8_rowscale_linear(x, weight, weight_scale, bias, out_dtype, convrot_groupsize if convrot else None,
                                 input_act)
+
+
+W4A16_GROUPS = (32, 64, 128)
+
+
+def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, wzeros=None, bias=None,
+                 group_size: int = INT4_GROUP_SIZE, convrot_groupsize: int | None = None, out_dtype=None) -> torch.Tensor:
+    """``x @ W.T + bias`` with 4-bit weights and activations in floating point, for few rows (one token each of a
+    batch's sequences: more rows than 16 read the weights again, and the W4A8 / W4A4 linears are the faster ones
+    for prompts). qweight: 8-bit [N, K/2] packed codes c (low nibble = even k); wscales: [N, K/group_size], the
+    scale s of a group of 32, 64 or 128. wzeros:
+
+    * None: signed int4 codes, w = s c (the configs' W4A4 weights)
+    * packed uint4 [N, ceil(K/group_size/2)] (8-bit type): w = s (c - z) (the configs' W4A8 weights' correction)
+    * floating [N, K/group_size]: w = s c + z (the lowbit_affine rule, custom_nodes/comfy-lowbit-loader/kernel.py:27-34)
+
+    convrot_groupsize: x is rotated by H per block first, as weights of a rotating converter ask for. Products
+    and sums are fp32; the output (out_dtype, x's type by default) is rounded once."""
+    k = x.shape[-1]
+    if qweight.dim() != 2 or qweight.element_size() != 1:
+        raise ValueError(f"qweight must be 8-bit [N, K/2], got {qweight.dtype} {list(qweight.shape)}")
+    n = qweight.shape[0]
+    if k != qweight.shape[1] * 2:
+        raise ValueError(f"Input K={k} does not match qweight K={qweight.shape[1] * 2}")
+    if group_size not in W4A16_GROUPS or k % group_size:
+        raise ValueError(f"group_size must be one of {W4A16_GROUPS} and divide K={k}, got {group_size}")
+    if convrot_groupsize and (convrot_groupsize not in CONVROT_GROUPSIZES or k % convrot_groupsize):
+        raise ValueError(f"convrot_groupsize must be one of {CONVROT_GROUPSIZES} and divide K={k}, got {convrot_groupsize}")
+    groups = k // group_size
+    x2 = _as_2d(x, k)
+    dev = x2.device
+    if x2.data_ptr() % 16:
+        x2 = x2.clone()
+    if wscales.shape != (n, groups) or wscales.dtype not in FLOAT_TYPES:
+        raise ValueError(f"wscales must be floating-point [{n}, {groups}], got {wscales.dtype} {list(wscales.shape)}")
+    ws = wscales if wscales.stride(1) == 1 else wscales.contiguous()
+    qw = qweight if qweight.stride(1) == 1 and qweight.stride(0) % 16 == 0 and qweight.data_ptr() % 16 == 0 \
+        else qweight.contiguous()
+    zero, zdt, zptr, ldz = _lib.W4Z_SIGNED, _lib.DT_BF16, None, 0
+    if wzeros is not None:
+        if wzeros.dtype in FLOAT_TYPES:
+            zero, zdt, want = _lib.W4Z_FLOAT, _lib.DTYPE_CODE[wzeros.dtype], (n, groups)
+        else:
+            zero, want = _lib.W4Z_U4, (n, (groups + 1) // 2)
+            if wzeros.element_size() != 1:
+                raise ValueError(f"zero-points must be packed uint4 or floating-point, got {wzeros.dtype}")
+        if wzeros.shape != want:
+            raise ValueError(f"zero-points must be {list(want)}, got {list(wzeros.shape)}")
+        if wzeros.device != dev:
+            raise ValueError(f"x is on {dev}, the weights are not")
+        wz = wzeros if wzeros.stride(1) == 1 else wzeros.contiguous()
+        zptr, ldz = wz.data_ptr(), max(wz.stride(0), want[1])
+    if qw.device != dev or ws.device != dev:
+        raise ValueError(f"x is on {dev}, the weights are not")
+    b = _bias(bias, n, dev)
+    dt = _out_dtype(out_dtype, x)
+    m = x2.shape[0]
+    y = torch.empty((m, n), dtype=dt, device=dev)
+    if m == 0 or n == 0:
+        return _finish(y, x, n)
+    _lib.call("mq_linear_w4a16", x2.data_ptr(), _lib.DTYPE_CODE[x2.dtype], k, int(convrot_groupsize or 0), qw.data_ptr(),
+              qw.stride(0) if n > 1 else k // 2, ws.data_ptr(), _lib.DTYPE_CODE[ws.dtype], max(ws.stride(0), groups), zptr,
+              zero, zdt, ldz, int(group_size), None if b is None else b.data_ptr(),
+              _lib.DT_BF16 if b is None else _lib.DTYPE_CODE[b.dtype], y.data_ptr(), _lib.DTYPE_CODE[dt], n, m, n, k,
+              _lib.stream_of_device(dev))
+    return _finish(y, x, n)

@@ -44,6 +44,7 @@ enum {
 #define MQ_DT_BF16 0
 #define MQ_DT_F16 1
 #define MQ_DT_F32 2
+#define MQ_DT_I8 3   /* paged caches only: int8 codes with an fp32 scale per token and head */
 
 /* Layouts of the activation codes written by mq_rotquant (its `packed` argument). */
 enum {
@@ -410,6 +411,108 @@ int mq_linear_w4_group_noalloc(const void* x, int x_dtype, int64_t ldx, int hblo
                                const uint8_t* qw, int64_t ldw, const uint16_t* ws, int64_t ldws, const uint8_t* wz,
                                int64_t ldwz, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy,
                                int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * Token generation: a paged key-value cache, attention over it, and linears with 4-bit weights and
+ * floating-point activations. No counterpart in the reference, whose attention and text generation run
+ * in the programs that call it.
+ *
+ * The cache of one layer is K and V [pages, H, page_size, D] of type cache_dtype: MQ_DT_BF16 or
+ * MQ_DT_F16 (the type of the tokens' rows), or MQ_DT_I8 with fp32 scales [pages, H, page_size] for
+ * each. K and V have the same strides c_page / c_head / c_token (elements, any order; D contiguous),
+ * their scales s_page / s_head / s_token. page_size is a power of two. Token j of sequence b lies in
+ * slot j % page_size of page page_table[b, j / page_size]; page_table is int32 [B, width], row stride
+ * ld_table. An entry that is no page of the cache (negative, or >= pages) holds nothing: its
+ * tokens are neither read nor written, and no query sees them. lens int32 [B]: tokens held, the new ones
+ * among them. cu_q int32 [B + 1] (ascending, cu_q[0] = 0): sequence b's new tokens are rows
+ * cu_q[b] .. cu_q[b + 1] - 1 of k, v, q and out; NULL: one new token per sequence (T = B). New token i
+ * of the n of sequence b stands at position lens[b] - n + i.
+ * Lengths, tables and cu_q are read on the device only. D % 8 == 0 (int8 cache: D % 16 == 0), D <= 256;
+ * rows of k, v, q, out and of the caches start at multiples of 16 bytes.
+ *
+ * mq_kv_write: k, v [T, H, D] of type dtype (bf16 or fp16) into their pages. int8 cache: per row of D
+ * values s = max(max |x| / 127, 1e-10), code = rne(x / s); a row with an infinity or NaN gets codes 0
+ * and scale NaN (it reads back as NaN). A token with a position below 0 or behind the table is dropped.
+ */
+int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                int dtype, int64_t T, int64_t H, int64_t D, void* k_cache, void* v_cache, int cache_dtype,
+                int64_t c_page, int64_t c_head, int64_t c_token, float* k_scale, float* v_scale, int64_t s_page,
+                int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
+                int64_t ld_table, int64_t B, int64_t width, const int32_t* lens, const int32_t* cu_q, void* stream);
+
+/*
+ * out[t, hq] = sum_j softmax_j(scale * q[t, hq] . k[j, h]) v[j, h] over the visible tokens j of t's sequence,
+ * h = hq / (Hq / H). The query at position p sees j <= p, of those (window > 0) the last `window`, its
+ * own among them, and the first `sinks`. A query that sees nothing (an idle sequence, a position below
+ * 0) gets zeros. Keys and values of tokens that a query does not see have no effect on its result, whatever
+ * they hold. Softmax statistics and sums are fp32; one rounding to dtype at the end.
+ *   q, out [T, Hq, D] of type dtype (bf16 or fp16; a 16-bit cache has the same), Hq % H == 0
+ *   workspace: mq_paged_attention_workspace_bytes(T, Hq, H, D, B, cu_q != NULL) bytes, 16-byte aligned
+ *   (nothing in it has to start at zero)
+ */
+int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int64_t Hq, int64_t H,
+                       int64_t D, const void* k_cache, const void* v_cache, int cache_dtype, int64_t c_page,
+                       int64_t c_head, int64_t c_token, const float* k_scale, const float* v_scale, int64_t s_page,
+                       int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
+                       int64_t ld_table, int64_t B, int64_t width, const int32_t* lens, const int32_t* cu_q, float scale,
+                       int64_t window, int64_t sinks, void* out, int64_t out_token, int64_t out_head, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged);
+
+/*
+ * Bookkeeping of the pages, on the device: page_table int32 [rows, width] (-1: none), lens int32 [rows],
+ * refs int32 [pages] (sequences that hold a page; 0: free). Pages are handed out lowest first. A
+ * call that cannot be done whole changes nothing. *status (int32 in device memory, or NULL): 0 done,
+ * > 0 that many pages missing, -1 an argument out of range (a row that does not exist, is given
+ * twice, is not empty where it has to be, or whose table is too short).
+ * The copies take the caches whole: `layers` layers layer_bytes apart, each of pages page_bytes long and
+ * page_pitch bytes apart (K and V alike; the scales of an int8 cache s_*, else NULL and 0).
+ *   workspace: mq_kv_workspace_bytes(pages, n) bytes, 16-byte aligned
+ *
+ * mq_kv_fork: sequence dst[i] (empty) becomes a copy of src[i], i < n: it shares the full pages and gets
+ * its own copy of a partly filled last one. mq_kv_grow: sequence rows[i] gets counts[i] tokens more
+ * (lens, and pages for them; their contents are written by mq_kv_write). mq_kv_free: sequences rows[i] are
+ * emptied and their pages given back (rows out of range are left out). mq_kv_compact: the pages held, n of
+ * them, move to 0 .. n - 1 in as few copies as there can be; *live = n.
+ */
+int64_t mq_kv_workspace_bytes(int64_t pages, int64_t n);
+int mq_kv_fork(void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t page_pitch, int64_t page_bytes,
+               float* k_scale, float* v_scale, int64_t s_layer_bytes, int64_t s_page_pitch, int64_t s_page_bytes,
+               int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, int32_t* lens, int32_t* refs,
+               int64_t pages, int page_size, const int32_t* src, const int32_t* dst, int64_t n, int32_t* status,
+               void* workspace, int64_t workspace_bytes, void* stream);
+int mq_kv_grow(int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, int32_t* lens, int32_t* refs,
+               int64_t pages, int page_size, const int32_t* seqs, const int32_t* counts, int64_t n, int32_t* status,
+               void* workspace, int64_t workspace_bytes, void* stream);
+int mq_kv_free(int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, int32_t* lens, int32_t* refs,
+               int64_t pages, const int32_t* seqs, int64_t n, void* stream);
+int mq_kv_compact(void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t page_pitch, int64_t page_bytes,
+                  float* k_scale, float* v_scale, int64_t s_layer_bytes, int64_t s_page_pitch, int64_t s_page_bytes,
+                  int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, int32_t* refs, int64_t pages,
+                  int32_t* live, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Zero-points of mq_linear_w4a16. */
+#define MQ_W4Z_SIGNED 0   /* signed int4 codes c:              w = s * c                            */
+#define MQ_W4Z_U4 1       /* uint4 codes, packed uint4 zeros:  w = s * (c - z)                      */
+#define MQ_W4Z_FLOAT 2    /* uint4 codes, floating zeros:      w = s * c + z (the lowbit_affine rule, */
+                          /* custom_nodes/comfy-lowbit-loader/kernel.py:27-34)                      */
+
+/*
+ * y[m, n] = T( sum_k x'[m, k] * w[n, k] + bias[n] ): 4-bit weights with a scale per group of K values
+ * and activations in floating point, x' = x or (hblock 16, 64, 256) x rotated by H_hblock in fp32
+ * as mq_rotquant rotates it. For few rows (one token of each of a batch's sequences): the weights are read
+ * once per 16 rows. Products and sums are fp32; nothing but the output is rounded.
+ *   x [M, K] of type x_dtype (bf16, fp16 or fp32), stride ldx (rows start at multiples of 16 bytes)
+ *   qw packed 4-bit [N, K/2], stride ldw bytes (ldw % 16 == 0, 16-byte aligned; low nibble = even k)
+ *   ws [N, K/group] of type s_dtype, stride ldws; wz by `zero` (MQ_W4Z_*): NULL, packed uint4
+ *   [N, ceil(K/group/2)] (stride ldwz bytes), or [N, K/group] of type z_dtype (stride ldwz elements)
+ *   group 32, 64 or 128; bias, y as mq_gemm_w4_group
+ * Requires K % group == 0, K % hblock == 0, K <= 32768.
+ */
+int mq_linear_w4a16(const void* x, int x_dtype, int64_t ldx, int hblock, const uint8_t* qw, int64_t ldw, const void* ws,
+                    int s_dtype, int64_t ldws, const void* wz, int zero, int z_dtype, int64_t ldwz, int group,
+                    const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                    void* stream);
 
 #ifdef __cplusplus
 }
