@@ -37,6 +37,7 @@ int check_cache(const char* what, int dtype, int64_t T, int64_t H, int64_t D, co
     MQ_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two (got %d)",
                what, page_size);
     MQ_REQUIRE(width * page_size < (int64_t(1) << 40), "%s: the tables hold too many tokens", what);
+    MQ_REQUIRE(pages * page_size < kMost, "%s: the cache holds too many tokens", what);
     MQ_REQUIRE(cu_q || T == B, "%s: without cu_q every sequence has one token (T=%lld, B=%lld)", what, (long long)T,
                (long long)B);
     if (T == 0 || B == 0) return MQ_OK;
@@ -85,7 +86,7 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
 }
 
 int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged) {
-    if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= kMost || D > 256) return 0;
+    if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256) return 0;
     return attention_workspace_bytes(T, static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D), B, ragged != 0);
 }
 
@@ -101,7 +102,7 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
                                k_scale, v_scale, s_page, s_head, s_token, pages, page_size, page_table, ld_table, B,
                                width, lens, cu_q);
     if (rc != MQ_OK) return rc;
-    MQ_REQUIRE(Hq > 0 && Hq % H == 0 && Hq < 65536, "paged_attention: %lld query heads for %lld cache heads (a multiple, < 65536)",
+    MQ_REQUIRE(Hq > 0 && Hq % H == 0 && Hq < 65536 && H > 0, "paged_attention: %lld query heads for %lld cache heads (a multiple, < 65536)",
                (long long)Hq, (long long)H);
     MQ_REQUIRE(window >= 0 && sinks >= 0, "paged_attention: window and sinks must be >= 0 (got %lld, %lld)",
                (long long)window, (long long)sinks);

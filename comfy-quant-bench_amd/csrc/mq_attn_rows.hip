@@ -85,9 +85,12 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
 
 }  // namespace
 
-int64_t attention_workspace_bytes(int64_t, int, int, int, int64_t, bool) { return 0; }
+int64_t attention_workspace_bytes(int64_t, int Hq, int H, int D, int64_t, bool ragged) {
+    return ragged ? 0 : attn_decode_workspace_bytes(Hq, H, D);
+}
 
 int launch_attention(const AttnArgs& a, hipStream_t stream) {
+    if (!a.cu_q) return launch_attn_decode(a, stream);
     const int64_t items = a.T * a.Hq;
     hipLaunchKernelGGL(attn_rows_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, a);
     return launch_status("paged_attention");
