@@ -24,7 +24,7 @@ FAST = os.path.join(HERE, "kitchen_amd", "_fast.so")
 SOURCES = ["mq_abi.hip", "mq_rotquant.hip", "mq_rotquant_f16.hip", "mq_rotquant_f32.hip", "mq_swiglu.hip",
            "mq_swiglu_f16.hip", "mq_swiglu_eager.hip", "mq_swiglu_eager_f16.hip",
            "mq_codebook.hip", "mq_wquant.hip", "mq_gemv.hip", "mq_gemm.hip", "mq_gemm_few.hip",
-           "mq_gemm_wide.hip", "mq_abi_serve.hip", "mq_kv.hip", "mq_attn_rows.hip", "mq_attn_decode.hip", "mq_w4a16.hip"]
+           "mq_gemm_wide.hip", "mq_abi_serve.hip", "mq_kv.hip", "mq_attn_decode.hip", "mq_attn_prompt.hip", "mq_w4a16.hip"]
 ARCH = "gfx950"
 
 

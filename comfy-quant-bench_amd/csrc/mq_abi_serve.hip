@@ -87,7 +87,7 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
 
 int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged) {
     if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256) return 0;
-    return attention_workspace_bytes(T, static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D), B, ragged != 0);
+    return ragged ? 0 : attn_decode_workspace_bytes(static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D));
 }
 
 int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int64_t Hq, int64_t H,
@@ -123,7 +123,7 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
     a.s_page = s_page; a.s_head = s_head; a.s_token = s_token; a.pages = pages; a.page_shift = log2_of(page_size);
     a.table = page_table; a.ld_table = ld_table; a.B = B; a.width = pages > 0 ? width : 0; a.lens = lens; a.cu_q = cu_q;
     a.scale = scale; a.window = window; a.sinks = sinks; a.dtype = dtype; a.work = workspace; a.work_bytes = workspace_bytes;
-    return launch_attention(a, static_cast<hipStream_t>(stream));
+    return cu_q ? launch_attn_prompt(a, static_cast<hipStream_t>(stream)) : launch_attn_decode(a, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,579 @@
+// Attention of ragged prompt chunks over a paged key-value cache (causal, sliding window, first tokens).
+//
+// MFMA-bound for long prompts: 4 D operations per query-key pair, against 32 score-sized VALU steps per lane
+// and 64 keys. A workgroup of four waves takes 128 rows of one cache head: row = (new token, query head of the
+// group), token-major, so the heads that share keys and values share their tiles too and a short prompt
+// fills a tile. Each wave keeps 32 rows; tiles of 64 keys go through LDS, double-buffered: the next tile's
+// loads are issued before this one's products and stored to the other half behind them, one barrier a tile.
+//
+//   S^T = K Q^T      32x32x16 products. A: 32 keys, from LDS rows of 16-byte chunks (chunk x of key k at
+//                    x ^ (k & 7): eight lanes read all banks). B: 32 query rows, kept in registers. Lane (q, h)
+//                    = (l & 31, l >> 5) gets row q, keys 8 (r / 4) + 4 h + r % 4, r < 16.
+//   softmax          in base 2, row by row in one lane and its partner l ^ 32. The reference maximum is only
+//                    moved (and the sums rescaled) when a row's maximum exceeds it by 2^8: any reference gives
+//                    the same quotient, and fp32 sums have the range.
+//   O^T = V^T P^T    B: a lane's 8 probabilities of keys 16 t + 4 h + {0 .. 3, 8 .. 11} as they are; A: V^T from
+//                    LDS, rows of one value over 64 keys, the keys in just that order, transposed by v_perm on
+//                    the way in.
+//
+// Rows of one tile may differ in what they see: hidden scores become -infinity, and their weight 0 leaves the sum
+// alone unless V holds an infinity or NaN there (0 times that is NaN). Tiles at an edge are looked through for
+// such values while they are stored; if there are any, the products run on V with them zeroed, and products of
+// ones count which rows see which kind, and add it.
+#include "mq_attn.h"
+
+namespace mq {
+namespace {
+
+constexpr int kRows = 128;     // rows per workgroup
+constexpr int kTile = 64;      // keys per step
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
+    if constexpr (DT == kDtF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float max2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Whether either 16-bit value of w is an infinity or NaN; w with such values zeroed.
+template <int DT>
+__device__ __forceinline__ bool has_wild(uint32_t w) {
+    constexpr uint32_t e = DT == kDtF16 ? 0x7c00u : 0x7f80u;
+    return (w & e) == e || (w >> 16 & e) == e;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t tame(uint32_t w) {
+    constexpr uint32_t e = DT == kDtF16 ? 0x7c00u : 0x7f80u;
+    return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
+}
+
+// 0: +infinity, 1: -infinity, 2: NaN, 3: a finite value.
+template <int DT>
+__device__ __forceinline__ int wild_kind(uint32_t w) {
+    constexpr uint32_t e = DT == kDtF16 ? 0x7c00u : 0x7f80u;
+    if ((w & 0x7fffu) < e) return 3;
+    return (w & 0x7fffu) > e ? 2 : static_cast<int>(w >> 15);
+}
+
+template <int DP>
+struct __attribute__((aligned(16))) Lds {
+    uint16_t k[2][kTile * DP];
+    uint16_t v[2][DP * kTile];
+    float ks[2][kTile], vs[2][kTile];
+    int code[3][kTile];        // a key's row: page << page_shift | slot, or -1
+    uint64_t held[3];          // bit x: key x is in a page of the cache
+    int wild;                  // an edge tile's values hold an infinity or NaN
+};
+
+// DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache.
+template <int DP, int DT, bool I8>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(AttnArgs a) {
+    constexpr int E = I8 ? 1 : 2;
+    constexpr bool kSplit = I8 && DT == kDtF16;         // fp16 rows against int8 keys: bf16 products of hi + lo
+    constexpr int MT = I8 ? kDtBf16 : DT;               // type of the products
+    constexpr float kSlack = 8.0f;                      // how far a row's maximum may pass its reference (log2)
+    constexpr float kLift = MT == kDtF16 ? 7.0f : 0.0f; // fp16 probabilities are held 2^7 times as large
+    constexpr int kSteps = DP / 16;                     // products over the width
+    constexpr int kBlocks = DP / 32;                    // value blocks of the output
+    constexpr int KC = DP / 32;                         // key chunks (8 values) a thread stages
+    constexpr int kPerKey = DP / 8;                     // chunks per key
+    constexpr int VE = DP / 16;                         // values of a row that a thread stages, of 4 keys
+    constexpr int VW = VE * E / 4;                      // dwords of them
+    extern __shared__ char lds_raw[];
+    Lds<DP>& sm = *reinterpret_cast<Lds<DP>*>(lds_raw);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = lane & 31, hf = lane >> 5;
+    const int group = a.Hq / a.H;
+    const int h = static_cast<int>(blockIdx.x % a.H);
+    // this workgroup's sequence and 128 rows of it; the last tiles, which see the most keys, come first
+    int64_t want = static_cast<int64_t>(gridDim.x) / a.H - 1 - blockIdx.x / a.H, b = -1, tile = 0;
+    for (int64_t b0 = 0; b0 < a.B; b0 += 64) {
+        int64_t n = 0;
+        if (b0 + lane < a.B) {
+            const int64_t tok = static_cast<int64_t>(a.cu_q[b0 + lane + 1]) - a.cu_q[b0 + lane];
+            n = tok > 0 ? (tok * group + kRows - 1) / kRows : 0;
+        }
+        int64_t x = n;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int64_t y = __shfl_up(x, s);
+            if (lane >= s) x += y;
+        }
+        const uint64_t past = __ballot(x > want);
+        if (past) {
+            const int first = __builtin_ctzll(past);
+            b = b0 + first;
+            tile = want - __shfl(x - n, first);
+            break;
+        }
+        want -= __shfl(x, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
+    tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile));
+    if (b < 0) return;
+    const int64_t tok0 = a.cu_q[b];
+    int64_t tok1 = a.cu_q[b + 1];
+    tok1 = tok1 < a.T ? tok1 : a.T;                     // nothing behind the rows of q, whatever cu_q says
+    if (tok0 < 0 || tok0 >= tok1) return;
+    const int64_t tokens = tok1 - tok0, rows = tokens * group;
+    const int64_t pos0 = static_cast<int64_t>(a.lens[b]) - (static_cast<int64_t>(a.cu_q[b + 1]) - tok0);
+    const int64_t row0 = tile * kRows;
+    if (row0 >= rows) return;
+    const int64_t cap = a.width << a.page_shift;
+    const int64_t most = rows - 1;
+
+    // positions: of this lane's row (rows past the end take the last one's), of the wave's and the workgroup's ends
+    const int64_t wrow = row0 + wave * 32;
+    const int64_t myrow = wrow + q < most ? wrow + q : most;
+    const int64_t tok = myrow / group;
+    const int64_t pos = pos0 + tok;
+    const int64_t wpos_lo = pos0 + (wrow < most ? wrow : most) / group;
+    const int64_t wpos_hi = pos0 + (wrow + 31 < most ? wrow + 31 : most) / group;
+    const int64_t pos_lo = pos0 + row0 / group;
+    const int64_t pos_hi = pos0 + (row0 + kRows - 1 < most ? row0 + kRows - 1 : most) / group;
+    auto first_of = [&](int64_t p) { return a.window > 0 && a.window <= p ? p - a.window + 1 : int64_t(0); };
+    const int64_t lo = first_of(pos), wlo_hi = first_of(wpos_hi), wlo_lo = first_of(wpos_lo);
+    const int64_t sinks = a.sinks;
+
+    // the tiles that some row sees: 0 .. ns - 1 (first tokens), then w0 ...
+    const int64_t last = pos_hi < cap ? pos_hi : cap - 1;
+    int ns = 0, nt = 0;
+    int64_t w0 = 0;
+    if (last >= 0) {
+        const int64_t start = first_of(pos_lo);
+        w0 = start / kTile;
+        const int64_t first = sinks < last + 1 ? sinks : last + 1;
+        int64_t s = start > 0 ? (first + kTile - 1) / kTile : 0;
+        int64_t nw = 0;
+        if (last >= start) {
+            nw = last / kTile - w0 + 1;
+            s = s < w0 ? s : w0;
+        }
+        ns = static_cast<int>(s);
+        nt = static_cast<int>(s + nw);
+    }
+    auto key_of = [&](int i) { return (i < ns ? static_cast<int64_t>(i) : w0 + (i - ns)) * kTile; };
+
+    // the query rows
+    Frag qf[kSteps], qf2[kSplit ? kSteps : 1];
+    const int64_t qrow = (tok0 + tok) * a.q_token + (h * group + myrow % group) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int d = 16 * s + 8 * hf;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (d < a.D) x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + qrow + d);
+        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+        qf[s] = Frag{{x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign}};
+        if constexpr (kSplit) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t hi, low;
+                split_f16(qf[s].w[j], &hi, &low);
+                qf[s].w[j] = hi;
+                qf2[s].w[j] = low;
+            }
+        }
+    }
+    f32x16 o[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+    float m = kNegInf, l = 0.0f;                        // reference maximum (of the scaled scores), sum of the lane's keys
+    bool any = false;
+    // the scores' scale, its sign moved into the query rows; a scale of 0 as one too small to tell, so that a
+    // hidden score's -infinity stays one
+    const float scale = __builtin_fmaxf(__builtin_fabsf(a.scale * kLog2e), 0x1p-100f);
+
+    const int* table = a.table + b * a.ld_table;
+    const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
+    const char* vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
+    const int mask = (1 << a.page_shift) - 1;
+    const int vg = tid >> 4, vc = tid & 15;             // V staging: keys 4 vg .. 4 vg + 3, values VE vc ..
+
+    // rows of tile i's keys (wave 0; lane x looks up key x)
+    auto look_up = [&](int i) -> int {
+        if (i >= nt) return -1;
+        const int64_t key = key_of(i) + lane, at = key >> a.page_shift;
+        if (key > last || at >= a.width) return -1;
+        const int p = table[at];
+        return p >= 0 && p < a.pages ? (p << a.page_shift) | (static_cast<int>(key) & mask) : -1;
+    };
+    auto put_codes = [&](int ring, int code) {
+        const uint64_t held = __ballot(code >= 0);
+        sm.code[ring][lane] = code;
+        if (lane == 0) sm.held[ring] = held;
+    };
+
+    uint4 kr[KC];
+    uint32_t vr[4][VW];
+    float sc = 0.0f;
+    // the tile whose codes are in sm.code[ring] into registers (a key that is not held: zeros)
+    auto load = [&](int ring) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KC; ++x) {
+            const int e = tid + 256 * x, key = e / kPerKey, d = 8 * (e % kPerKey);
+            const int code = sm.code[ring][key];
+            kr[x] = make_uint4(0, 0, 0, 0);
+            if (code >= 0 && d < a.D) {
+                const char* p = kbase + (static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + d) * E;
+                if constexpr (I8) {
+                    const uint2 y = *reinterpret_cast<const uint2*>(p);
+                    kr[x].x = y.x;
+                    kr[x].y = y.y;
+                } else {
+                    kr[x] = *reinterpret_cast<const uint4*>(p);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int code = sm.code[ring][4 * vg + r];
+            const char* p = vbase + (static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + VE * vc) * E;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[r][w] = 0;
+            if (code >= 0 && VE * vc < a.D) {
+                if constexpr (VW == 1) {
+                    vr[r][0] = *reinterpret_cast<const uint32_t*>(p);
+                } else if constexpr (VW == 2) {
+                    const uint2 y = *reinterpret_cast<const uint2*>(p);
+                    vr[r][0] = y.x;
+                    vr[r][1] = y.y;
+                } else {
+#pragma unroll
+                    for (int w = 0; w < VW / 4; ++w) {
+                        if (w > 0 && VE * vc + 16 / E * w >= a.D) break;
+                        const uint4 y = *reinterpret_cast<const uint4*>(p + 16 * w);
+                        vr[r][4 * w] = y.x;
+                        vr[r][4 * w + 1] = y.y;
+                        vr[r][4 * w + 2] = y.z;
+                        vr[r][4 * w + 3] = y.w;
+                    }
+                }
+            }
+        }
+        if constexpr (I8) {
+            if (tid < 128) {
+                const int code = sm.code[ring][tid & 63];
+                sc = code < 0 ? 0.0f
+                              : (tid < 64 ? a.k_scale : a.v_scale)[static_cast<int64_t>(code >> a.page_shift) * a.s_page +
+                                                                   h * a.s_head + (code & mask) * a.s_token];
+            }
+        }
+    };
+    // the registers into half `buf`; edge: infinities and NaN among the values become 0 and are noted
+    auto store = [&](int buf, bool edge) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KC; ++x) {
+            const int e = tid + 256 * x, key = e / kPerKey, chunk = e % kPerKey;
+            uint4 y = kr[x];
+            if constexpr (I8) {
+                float f0[4], f1[4];
+                i8x4(kr[x].x, f0);
+                i8x4(kr[x].y, f1);
+                y = make_uint4(bf16_exact2(f0[0], f0[1]), bf16_exact2(f0[2], f0[3]), bf16_exact2(f1[0], f1[1]),
+                               bf16_exact2(f1[2], f1[3]));
+            }
+            *reinterpret_cast<uint4*>(&sm.k[buf][key * DP + 8 * (chunk ^ (key & 7))]) = y;
+        }
+        if constexpr (!I8) {
+            if (edge) {
+                bool bad = false;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        bad = bad || has_wild<DT>(vr[r][w]);
+                        vr[r][w] = tame<DT>(vr[r][w]);
+                    }
+                if (bad) sm.wild = 1;
+            }
+        }
+        // value d of keys 4 vg .. 4 vg + 3: 8 bytes in chunk 2 (vg / 4) + vg % 2, half vg / 2 % 2
+        const int chunk = 2 * (vg >> 2) + (vg & 1), half = (vg >> 1) & 1;
+        auto put = [&](int d, uint32_t x, uint32_t y) {
+            *reinterpret_cast<uint2*>(&sm.v[buf][d * kTile + 8 * (chunk ^ ((d ^ (d >> 3)) & 7)) + 4 * half]) = make_uint2(x, y);
+        };
+        if constexpr (I8) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                float f[4][4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) i8x4(vr[r][w], f[r]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    put(VE * vc + 4 * w + e, bf16_exact2(f[0][e], f[1][e]), bf16_exact2(f[2][e], f[3][e]));
+            }
+            if (tid < 64) sm.ks[buf][tid] = sc;
+            else if (tid < 128) sm.vs[buf][tid - 64] = sc;
+        } else {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                put(VE * vc + 2 * w, pair16<0>(vr[0][w], vr[1][w]), pair16<0>(vr[2][w], vr[3][w]));
+                put(VE * vc + 2 * w + 1, pair16<1>(vr[0][w], vr[1][w]), pair16<1>(vr[2][w], vr[3][w]));
+            }
+        }
+    };
+    // whether some row of the workgroup sees a part of tile i only
+    auto edge_of = [&](int i) {
+        const int64_t j = key_of(i);
+        return !(j + kTile - 1 <= pos_lo && (j >= first_of(pos_hi) || j + kTile <= sinks));
+    };
+
+    // a lane's places in the LDS rows: chunk 2 s + h of key 32 u + q is at (2 s) ^ (h ^ (q & 7)), so four bases serve
+    // all steps; V^T's chunk 2 t + h of row 32 i + q at (2 t) ^ 4 (i % 2) ^ (h ^ (q ^ q / 8) % 8) likewise
+    const int kx = hf ^ (q & 7), vx = hf ^ ((q ^ (q >> 3)) & 7);
+    auto below = [](int64_t n) { return n >= 64 ? ~uint64_t(0) : n <= 0 ? uint64_t(0) : (uint64_t(1) << n) - 1; };
+
+    // the row's visible keys of the tile at j: bit 8 (r / 4) + r % 4 of each half
+    auto visible = [&](uint64_t held, int64_t j) {
+        return (held & below(pos - j + 1) & (~below(lo - j) | below(sinks - j))) >> (4 * hf);
+    };
+
+    auto work = [&](int buf, int i, int ring) __attribute__((always_inline)) {
+        const int64_t j = key_of(i);
+        if (wrow > most) return;                                                   // no rows in this wave
+        if (j > wpos_hi || (j + kTile <= wlo_lo && j >= sinks)) return;            // no row of the wave sees it
+        const char* kp[4];
+        const char* vp[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            kp[x] = reinterpret_cast<const char*>(sm.k[buf]) + q * DP * 2 + 16 * ((2 * x) ^ kx);
+            vp[x] = reinterpret_cast<const char*>(sm.v[buf]) + q * kTile * 2 + 16 * ((2 * x) ^ vx);
+        }
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                const uint4 x = *reinterpret_cast<const uint4*>(kp[st & 3] + (st >> 2) * 128 + u * 32 * DP * 2);
+                const Frag k{{x.x, x.y, x.z, x.w}};
+                s[u] = mfma32<MT>(k, qf[st], s[u]);
+                if constexpr (kSplit) s[u] = mfma32<MT>(k, qf2[st], s[u]);
+            }
+        }
+        if constexpr (I8) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const float4 x = *reinterpret_cast<const float4*>(&sm.ks[buf][32 * u + 8 * r4 + 4 * hf]);
+                    s[u][4 * r4] *= x.x;
+                    s[u][4 * r4 + 1] *= x.y;
+                    s[u][4 * r4 + 2] *= x.z;
+                    s[u][4 * r4 + 3] *= x.w;
+                }
+        }
+        const uint64_t held = sm.held[ring];
+        const bool whole = held == ~uint64_t(0) && j + kTile - 1 <= wpos_lo && (j >= wlo_hi || j + kTile <= sinks);
+        // bit 8 (r / 4) + r % 4 of see[u]: the row sees that key
+        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+        if (!whole) {
+            const uint64_t vis = visible(held, j);
+            see[0] = static_cast<uint32_t>(vis);
+            see[1] = static_cast<uint32_t>(vis >> 32);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = (see[u] >> (8 * (r >> 2) + (r & 3))) & 1 ? s[u][r] : kNegInf;
+        }
+        any = any || ((see[0] | see[1]) & 0x0f0f0f0fu) != 0;
+        float top = kNegInf;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[u][r]);
+        top = max2(top) * scale;
+        const bool move = top > m + kSlack;             // of this row: what other rows hold does not change it
+        if (__ballot(move)) {
+            const float f = move ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = move ? top : m;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= f;
+        }
+        const float base = kLift - (m == kNegInf ? 0.0f : m);
+        float sum[4] = {0, 0, 0, 0};
+        Frag p[4], p2[kSplit ? 4 : 1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                float e[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][4 * r4 + r], scale, base));
+                    sum[r] += e[r];
+                }
+                if constexpr (I8) {
+                    const float4 x = *reinterpret_cast<const float4*>(&sm.vs[buf][32 * u + 8 * r4 + 4 * hf]);
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)         // a hidden key has weight 0 whatever its scale holds
+                        e[r] = (see[u] >> (8 * r4 + r)) & 1 ? e[r] * xs[r] : 0.0f;
+                }
+                const int t = 2 * u + (r4 >> 1), w = 2 * (r4 & 1);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    p[t].w[w + x] = pack_16x2(e[2 * x], e[2 * x + 1], MT);
+                    if constexpr (kSplit)
+                        p2[t].w[w + x] = pack_16x2(e[2 * x] - bf16lo(p[t].w[w + x]), e[2 * x + 1] - bf16hi(p[t].w[w + x]), MT);
+                }
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        auto v_frag = [&](int i, int t) __attribute__((always_inline)) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vp[t ^ (2 * (i & 1))] + i * 32 * kTile * 2);
+            return Frag{{x.x, x.y, x.z, x.w}};
+        };
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const Frag v = v_frag(i, t);
+                o[i] = mfma32<MT>(v, p[t], o[i]);
+                if constexpr (kSplit) o[i] = mfma32<MT>(v, p2[t], o[i]);
+            }
+    };
+
+    // tile i is worked on from half i % 2 while tile i + 1 is loaded, and tile i + 2's rows are looked up; what says
+    // where a tile's keys are goes round three places, so one barrier a tile is enough
+    if (nt > 0) {
+        if (wave == 0) {
+            put_codes(0, look_up(0));
+            put_codes(1, look_up(1));
+        }
+        if (tid == 0) sm.wild = 0;
+        __syncthreads();
+        load(0);
+        store(0, edge_of(0));
+        __syncthreads();
+        int r0 = 0, r1 = 1, r2 = 2;
+        for (int i = 0; i < nt; ++i) {
+            const int cur = i & 1, nxt = cur ^ 1;
+            const bool more = i + 1 < nt;
+            int ahead = -1;
+            if (wave == 0) ahead = look_up(i + 2);
+            if (more) load(r1);
+            work(cur, i, r0);
+            if (wave == 0) put_codes(r2, ahead);
+            if (more) store(nxt, edge_of(i + 1));
+            __syncthreads();
+            const int r = r0;
+            r0 = r1;
+            r1 = r2;
+            r2 = r;
+        }
+        if constexpr (!I8) {
+            if (sm.wild) {
+                // values that are infinite or NaN at an edge: products of ones count, for every row and value, which
+                // kinds its keys hold, and they are added
+                for (int i = 0; i < nt; ++i) {
+                    if (!edge_of(i)) continue;
+                    __syncthreads();
+                    if (wave == 0) put_codes(0, look_up(i));
+                    __syncthreads();
+                    load(0);
+                    store(0, false);
+                    __syncthreads();
+                    const uint64_t vis = visible(sm.held[0], key_of(i));
+                    constexpr uint32_t kOne = MT == kDtF16 ? 0x3c00u : 0x3f80u;
+                    Frag one[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int bit = 16 * t + 8 * (x >> 1) + 2 * (x & 1);
+                            one[t].w[x] = ((vis >> bit) & 1 ? kOne : 0u) | ((vis >> (bit + 1)) & 1 ? kOne << 16 : 0u);
+                        }
+#pragma unroll
+                    for (int e = 0; e < kBlocks; ++e)
+#pragma unroll 1
+                        for (int kind = 0; kind < 3; ++kind) {
+                            f32x16 n;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) n[r] = 0.0f;
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(
+                                    reinterpret_cast<const char*>(sm.v[0]) + (32 * e + q) * kTile * 2 +
+                                    16 * ((2 * t) ^ (4 * (e & 1)) ^ vx));
+                                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                                Frag v;
+#pragma unroll
+                                for (int y = 0; y < 4; ++y)
+                                    v.w[y] = (wild_kind<MT>(w[y] & 0xffffu) == kind ? kOne : 0u) |
+                                             (wild_kind<MT>(w[y] >> 16) == kind ? kOne << 16 : 0u);
+                                n = mfma32<MT>(v, one[t], n);
+                            }
+                            const float w = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[e][r] += n[r] > 0.0f ? w : 0.0f;
+                        }
+                }
+            }
+        }
+    }
+    l = sum2(l);
+    any = (static_cast<int>(any) | __shfl_xor(static_cast<int>(any), 32)) != 0;
+    if (wrow + q <= most && wrow <= most) {
+        const float inv = any ? 1.0f / l : 0.0f;        // nothing seen: zeros
+        uint16_t* out = static_cast<uint16_t*>(a.o) + (tok0 + tok) * a.o_token + (h * group + myrow % group) * a.o_head;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int d = 32 * i + 8 * r4 + 4 * hf;
+                if (d < a.D)
+                    *reinterpret_cast<uint2*>(out + d) =
+                        make_uint2(pack_16x2(o[i][4 * r4] * inv, o[i][4 * r4 + 1] * inv, DT),
+                                   pack_16x2(o[i][4 * r4 + 2] * inv, o[i][4 * r4 + 3] * inv, DT));
+            }
+    }
+}
+
+template <int DP, int DT, bool I8>
+int launch_width(const AttnArgs& a, hipStream_t stream) {
+    const int64_t group = a.Hq / a.H;
+    const int64_t tiles = a.T * group / kRows + a.B;    // at least as many as the sequences' row tiles
+    const size_t lds = sizeof(Lds<DP>);
+    auto kern = attn_prompt_kernel<DP, DT, I8>;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(lds)) != hipSuccess) {
+        set_error("paged_attention: cannot reserve %zu bytes of LDS", lds);
+        return -3;
+    }
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles * a.H)), dim3(256), lds, stream, a);
+    return launch_status("paged_attention");
+}
+
+template <int DT, bool I8>
+int launch_type(const AttnArgs& a, hipStream_t stream) {
+    if (a.D <= 64) return launch_width<64, DT, I8>(a, stream);
+    if (a.D <= 128) return launch_width<128, DT, I8>(a, stream);
+    return launch_width<256, DT, I8>(a, stream);
+}
+
+}  // namespace
+
+int launch_attn_prompt(const AttnArgs& a, hipStream_t stream) {
+    const bool i8 = a.k_scale != nullptr;
+    if (a.dtype == kDtF16) return i8 ? launch_type<kDtF16, true>(a, stream) : launch_type<kDtF16, false>(a, stream);
+    return i8 ? launch_type<kDtBf16, true>(a, stream) : launch_type<kDtBf16, false>(a, stream);
+}
+
+}  // namespace mq

@@ -241,10 +241,9 @@ struct AttnArgs {
     void* work;
     int64_t work_bytes;
 };
-int launch_attention(const AttnArgs& a, hipStream_t stream);
+int launch_attn_prompt(const AttnArgs& a, hipStream_t stream);
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream);
 int64_t attn_decode_workspace_bytes(int Hq, int H, int D);
-int64_t attention_workspace_bytes(int64_t T, int Hq, int H, int D, int64_t B, bool ragged);
 
 // --- 4-bit weights, floating activations (mq_w4a16.hip)
 enum class W4Zero : int { Signed = 0, U4 = 1, Float = 2 };

@@ -424,7 +424,7 @@ int mq_linear_w4_group_noalloc(const void* x, int x_dtype, int64_t ldx, int hblo
  * slot j % page_size of page page_table[b, j / page_size]; page_table is int32 [B, width], row stride
  * ld_table. An entry that is no page of the cache (negative, or >= pages) holds nothing: its
  * tokens are neither read nor written, and no query sees them. lens int32 [B]: tokens held, the new ones
- * among them. cu_q int32 [B + 1] (ascending, cu_q[0] = 0): sequence b's new tokens are rows
+ * among them. cu_q int32 [B + 1] (ascending from 0 to T): sequence b's new tokens are rows
  * cu_q[b] .. cu_q[b + 1] - 1 of k, v, q and out; NULL: one new token per sequence (T = B). New token i
  * of the n of sequence b stands at position lens[b] - n + i.
  * Lengths, tables and cu_q are read on the device only. D % 8 == 0 (int8 cache: D % 16 == 0), D <= 256;
