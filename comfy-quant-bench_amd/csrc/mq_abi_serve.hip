@@ -290,6 +290,7 @@ int mq_linear_w4a16(const void* x, int x_dtype, int64_t ldx, int hblock, const u
                "linear_w4a16: x needs ldx >= K, ldx %% %lld == 0 and a 16-byte aligned base", (long long)per16);
     MQ_REQUIRE(ldw >= K / 2 && ldw % 16 == 0 && aligned(qw, 16),
                "linear_w4a16: qw needs ldw >= K/2 bytes, ldw %% 16 == 0 and a 16-byte aligned base");
+    MQ_REQUIRE(ldw < (1 << 25) && ldws < (1 << 25) && ldwz < (1 << 25), "linear_w4a16: row strides must be below 2^25");
     MQ_REQUIRE(ldws >= K / group && aligned(ws, dtype_bytes(s_dtype)), "linear_w4a16: ws needs ldws >= K/group and an aligned base");
     MQ_REQUIRE(zero != MQ_W4Z_U4 || ldwz >= (K / group + 1) / 2, "linear_w4a16: ldwz < ceil(K/group/2)");
     MQ_REQUIRE(zero != MQ_W4Z_FLOAT || (ldwz >= K / group && aligned(wz, dtype_bytes(z_dtype))),
