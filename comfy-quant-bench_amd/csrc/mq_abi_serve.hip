@@ -36,7 +36,7 @@ int check_cache(const char* what, int dtype, int64_t T, int64_t H, int64_t D, co
     MQ_REQUIRE(T < kMost && H < kMost && B < kMost && pages < kMost && width < kMost, "%s: shape too large", what);
     MQ_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two (got %d)",
                what, page_size);
-    MQ_REQUIRE(width * page_size < (int64_t(1) << 40), "%s: the tables hold too many tokens", what);
+    MQ_REQUIRE(width <= (kMost >> 1) / page_size, "%s: the tables hold too many tokens", what);
     MQ_REQUIRE(pages * page_size < kMost, "%s: the cache holds too many tokens", what);
     MQ_REQUIRE(cu_q || T == B, "%s: without cu_q every sequence has one token (T=%lld, B=%lld)", what, (long long)T,
                (long long)B);
@@ -49,6 +49,7 @@ int check_cache(const char* what, int dtype, int64_t T, int64_t H, int64_t D, co
     MQ_REQUIRE(kc && vc && aligned(kc, 16) && aligned(vc, 16) && c_page % per16 == 0 && c_head % per16 == 0 &&
                    c_token % per16 == 0,
                "%s: the caches need 16-byte aligned bases and strides that are multiples of 16 bytes", what);
+    MQ_REQUIRE(c_token < (1 << 25), "%s: token strides must be below 2^25 elements", what);
     MQ_REQUIRE(c_page >= 0 && c_head >= 0 && c_token >= 0 && s_page >= 0 && s_head >= 0 && s_token >= 0,
                "%s: negative stride", what);
     MQ_REQUIRE(!i8 || (ks && vs && aligned(ks, 4) && aligned(vs, 4)), "%s: an int8 cache needs its scales", what);
@@ -85,6 +86,11 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
     return launch_kv_write(a, dtype, cache_dtype == MQ_DT_I8, static_cast<hipStream_t>(stream));
 }
 
+int64_t mq_paged_attention_counters(int64_t T, int64_t Hq, int64_t H, int64_t B, int ragged) {
+    if (T <= 0 || Hq <= 0 || H <= 0 || B <= 0 || Hq >= 65536 || H > Hq || ragged) return 0;
+    return attn_decode_counters(static_cast<int>(Hq), static_cast<int>(H), B);
+}
+
 int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged) {
     if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256) return 0;
     return ragged ? 0 : attn_decode_workspace_bytes(static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D));
@@ -96,7 +102,7 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
                        int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
                        int64_t ld_table, int64_t B, int64_t width, const int32_t* lens, const int32_t* cu_q, float scale,
                        int64_t window, int64_t sinks, void* out, int64_t out_token, int64_t out_head, void* workspace,
-                       int64_t workspace_bytes, void* stream) {
+                       int64_t workspace_bytes, int32_t* counters, void* stream) {
     clear_error();
     const int rc = check_cache("paged_attention", dtype, T, H, D, k_cache, v_cache, cache_dtype, c_page, c_head, c_token,
                                k_scale, v_scale, s_page, s_head, s_token, pages, page_size, page_table, ld_table, B,
@@ -104,6 +110,9 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
     if (rc != MQ_OK) return rc;
     MQ_REQUIRE(Hq > 0 && Hq % H == 0 && Hq < 65536 && H > 0, "paged_attention: %lld query heads for %lld cache heads (a multiple, < 65536)",
                (long long)Hq, (long long)H);
+    // the kernels count tiles of at least 64 keys for every sequence, cache head and 16 query heads in 32 bits
+    MQ_REQUIRE((B + 1) * H * ((Hq / H + 15) / 16) < (int64_t(1) << 36) / (width * page_size + 256),
+               "paged_attention: the tables hold too many tokens");
     MQ_REQUIRE(window >= 0 && sinks >= 0, "paged_attention: window and sinks must be >= 0 (got %lld, %lld)",
                (long long)window, (long long)sinks);
     if (T == 0) return MQ_OK;
@@ -115,14 +124,17 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
     const int64_t need = mq_paged_attention_workspace_bytes(T, Hq, H, D, B, cu_q != nullptr);
     MQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need),
                "paged_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    MQ_REQUIRE(mq_paged_attention_counters(T, Hq, H, B, cu_q != nullptr) == 0 || (counters && aligned(counters, 4)),
+               "paged_attention: needs its counters (zeros)");
     AttnArgs a{};
+    a.counters = counters;
     a.q = q; a.q_token = q_token; a.q_head = q_head; a.o = out; a.o_token = out_token; a.o_head = out_head; a.T = T;
     a.Hq = static_cast<int>(Hq); a.H = static_cast<int>(H); a.D = static_cast<int>(D);
     a.kc = k_cache; a.vc = v_cache; a.c_page = c_page; a.c_head = c_head; a.c_token = c_token;
     if (cache_dtype == MQ_DT_I8) { a.k_scale = k_scale; a.v_scale = v_scale; }
     a.s_page = s_page; a.s_head = s_head; a.s_token = s_token; a.pages = pages; a.page_shift = log2_of(page_size);
     a.table = page_table; a.ld_table = ld_table; a.B = B; a.width = pages > 0 ? width : 0; a.lens = lens; a.cu_q = cu_q;
-    a.scale = scale; a.window = window; a.sinks = sinks; a.dtype = dtype; a.work = workspace; a.work_bytes = workspace_bytes;
+    a.scale = scale; a.window = window < kMost ? window : 0; a.sinks = sinks < kMost ? sinks : kMost - 1; a.dtype = dtype; a.work = workspace; a.work_bytes = workspace_bytes;
     return cu_q ? launch_attn_prompt(a, static_cast<hipStream_t>(stream)) : launch_attn_decode(a, static_cast<hipStream_t>(stream));
 }
 
@@ -138,7 +150,7 @@ int check_tables(const char* what, const int32_t* table, int64_t ld_table, int64
                (long long)pages, (long long)n);
     MQ_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two (got %d)",
                what, page_size);
-    MQ_REQUIRE(width * page_size < (int64_t(1) << 40), "%s: the tables hold too many tokens", what);
+    MQ_REQUIRE(width < kMost / page_size, "%s: the tables hold too many tokens", what);
     MQ_REQUIRE(rows == 0 || width == 0 || (table && aligned(table, 4) && ld_table >= width),
                "%s: page_table must be non-null and 4-byte aligned with ld_table >= width", what);
     MQ_REQUIRE((rows == 0 || (lens && aligned(lens, 4))) && (pages == 0 || (refs && aligned(refs, 4))),

@@ -14,105 +14,94 @@
 //                     values VE c .. VE c + VE - 1 (VE = width / 16, so 16 lanes read a whole row) and pairs the
 //                     keys' 16-bit values with v_perm. Product i gives values VE m + i of row m.
 //
-// A workgroup's four waves take 32 keys each of a 128-key tile. The tiles of all sequences and cache heads are
+// A workgroup's eight waves (four for heads of more than 128 values, whose operands take twice the registers) take
+// 32 keys each of a tile, one workgroup a compute unit. The tiles of all sequences and cache heads are
 // one line, cut into equal pieces for the resident workgroups (lengths are known on the device only, and a
-// ragged batch is balanced this way); a piece may end inside a sequence, which is then joined from its pieces'
-// maxima, sums and unnormalised outputs (fp32) by a second kernel in the order of the pieces, so the result is
-// the same every time.
+// ragged batch is balanced this way). A piece may end inside a sequence: its maxima, sums and unnormalised outputs
+// (fp32) then go to the workspace, and the workgroup that brings a sequence's last piece (a count per sequence
+// and cache head tells, which it sets back to zero) joins them in the order of the pieces, so the result is the
+// same every time.
 #include "mq_attn.h"
 
 namespace mq {
 namespace {
 
-constexpr int kTile = 128;     // keys per workgroup step
 constexpr int kKeys = 32;      // keys per wave and step
-constexpr int kWaves = 4;
+constexpr int waves_of(int dp) { return dp == 256 ? 4 : 8; }
 
-// What the query at position pos sees, as 128-key tiles: tiles 0 .. ns - 1 (first tokens), then w0 ...
+// What the query at position pos sees, as tiles of TILE keys: tiles 0 .. ns - 1 (first tokens), then w0 ... (Positions
+// and counts of tiles fit 32 bits: the host refuses tables that could hold more.)
 struct Visible {
-    int64_t pos, last, lo, sinks;   // last key that is held; first key of the window; first tokens that stay visible
-    int ns, nt;
-    int64_t w0;
+    int pos, last, lo, sinks;   // last key that is held; first key of the window; first tokens that stay visible
+    int ns, nt, w0;
 };
 
+template <int TILE>
 __device__ __forceinline__ Visible visible(const AttnArgs& a, int len) {
     Visible v;
-    const int64_t cap = a.width << a.page_shift;
-    v.pos = static_cast<int64_t>(len) - 1;
+    const int cap = static_cast<int>(a.width) << a.page_shift;
+    v.pos = len - 1;
     v.last = v.pos < cap ? v.pos : cap - 1;
-    v.lo = a.window > 0 && a.window <= v.pos ? v.pos - a.window + 1 : 0;
-    v.sinks = a.sinks < v.lo ? a.sinks : v.lo;
+    const int window = static_cast<int>(a.window), sinks = static_cast<int>(a.sinks);
+    v.lo = window > 0 && window <= v.pos ? v.pos - window + 1 : 0;
+    v.sinks = sinks < v.lo ? sinks : v.lo;
     v.ns = 0;
     v.nt = 0;
-    v.w0 = v.lo / kTile;
+    v.w0 = v.lo / TILE;
     if (v.last < 0) return v;
-    const int64_t first = v.sinks < v.last + 1 ? v.sinks : v.last + 1;
-    int64_t ns = (first + kTile - 1) / kTile, nw = 0;
+    const int first = v.sinks < v.last + 1 ? v.sinks : v.last + 1;
+    int nw = 0;
+    v.ns = (first + TILE - 1) / TILE;
     if (v.last >= v.lo) {
-        nw = v.last / kTile - v.w0 + 1;
-        ns = ns < v.w0 ? ns : v.w0;      // the window's first tile may hold first tokens too
+        nw = v.last / TILE - v.w0 + 1;
+        v.ns = v.ns < v.w0 ? v.ns : v.w0;       // the window's first tile may hold first tokens too
     }
-    v.ns = static_cast<int>(ns);
-    v.nt = static_cast<int>(ns + nw);
+    v.nt = v.ns + nw;
     return v;
 }
 
-// The line of tiles: sequence b has nt(b) tiles for each of `per` (cache head, row tile) pairs.
-struct Line {
-    int64_t total;     // tiles
-    int64_t piece;     // per workgroup
-};
+// A word that the kernel does not write, at an address that all lanes share: through the scalar unit.
+__device__ __forceinline__ int scalar_word(const int* p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
+}
 
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+// The line of tiles: sequence b has nt(b) tiles for each of `per` (cache head, row tile) pairs. total: tiles; and
+// the sequence that holds tile t of it, with the tiles before it. Every wave of a workgroup computes them for itself,
+// 64 sequences at a time.
+template <int TILE>
+__device__ __forceinline__ int line_total(const AttnArgs& a, int per) {
+    if (a.B == 1) return visible<TILE>(a, scalar_word(a.lens)).nt * per;
+    int n = 0;
+    for (int b = threadIdx.x & 63; b < a.B; b += 64) n += visible<TILE>(a, a.lens[b]).nt;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
-    return v;
+    for (int s = 1; s < 64; s <<= 1) n += __shfl_xor(n, s);
+    return __builtin_amdgcn_readfirstlane(n) * per;
 }
 
-// Sum of nt over sequences (every wave of the workgroup computes it for itself).
-__device__ __forceinline__ int64_t count_tiles(const AttnArgs& a, int64_t b0, int64_t b1) {
-    int64_t n = 0;
-    for (int64_t b = b0 + (threadIdx.x & 63); b < b1; b += 64) n += visible(a, a.lens[b]).nt;
-    return wave_sum(n);
-}
-
-// A value that all lanes hold, as the scalar unit sees it.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
-}
-
-__device__ __forceinline__ Line line_of(const AttnArgs& a, int64_t per, int64_t groups) {
-    Line l;
-    l.total = uniform(count_tiles(a, 0, a.B)) * per;
-    l.piece = (l.total + groups - 1) / groups;
-    return l;
-}
-
-// The sequence that holds tile t of the line, and the line's tiles before it (t < total).
-__device__ __forceinline__ void find_seq(const AttnArgs& a, int64_t per, int64_t t, int64_t* seq, int64_t* before) {
+template <int TILE>
+__device__ __forceinline__ void find_seq(const AttnArgs& a, int per, int t, int* seq, int* before) {
     const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    for (int64_t b0 = 0; b0 < a.B; b0 += 64) {
-        int64_t n = b0 + lane < a.B ? visible(a, a.lens[b0 + lane]).nt * per : 0;
-        int64_t x = n;
+    int base = 0;
+    *seq = 0;
+    *before = 0;
+    if (a.B == 1) return;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int n = b0 + lane < a.B ? visible<TILE>(a, a.lens[b0 + lane]).nt * per : 0;
+        int x = n;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
-            const int64_t y = __shfl_up(x, s);
+            const int y = __shfl_up(x, s);
             if (lane >= s) x += y;
         }
         const uint64_t past = __ballot(base + x > t);
         if (past) {
             const int first = __builtin_ctzll(past);
             *seq = b0 + first;
-            *before = base + __shfl(x - n, first);
+            *before = base + __builtin_amdgcn_readlane(x - n, first);
             return;
         }
-        base += __shfl(x, 63);
+        base += __builtin_amdgcn_readlane(x, 63);
     }
-    *seq = a.B;
-    *before = base;
 }
 
 // A split sequence's pieces: [slot][row][D] outputs, then [slot][row][2] maxima and sums. A workgroup's first
@@ -124,6 +113,22 @@ __device__ __forceinline__ float* part_stat(const AttnArgs& a, int rows, int64_t
     return static_cast<float*>(a.work) + slots * rows * a.D + slot * rows * 2;
 }
 
+// Pieces go from one workgroup to another, maybe on another die: stores and loads that are coherent on the
+// whole device (relaxed atomics of 8 bytes), so that no second level cache has to be written back for them.
+__device__ __forceinline__ void send(float* p, float x, float y) {
+    const uint64_t v = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 receive(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Keys and values are read once: past the caches' replacement (non-temporal), 10 % faster on a cache that does not
+// fit them.
 template <int BYTES>
 struct Raw;   // BYTES bytes of a row
 template <> struct Raw<4> { uint32_t w[1]; };
@@ -135,40 +140,124 @@ template <int BYTES>
 __device__ __forceinline__ Raw<BYTES> load_raw(const char* p) {
     Raw<BYTES> r;
     if constexpr (BYTES == 4) {
-        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
     } else if constexpr (BYTES == 8) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        r.w[0] = x.x; r.w[1] = x.y;
+        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+        r.w[0] = x[0]; r.w[1] = x[1];
     } else {
         static_assert(BYTES == 16);
-        const uint4 x = *reinterpret_cast<const uint4*>(p);
-        r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = x[i];
     }
     return r;
 }
 
-// BYTES of a value row from value d on, its head D wide: a piece of 16 bytes that begins behind the width reads
-// the row's first one instead (its products are never stored).
+// BYTES of a value row from value d on (at `off`), its head D wide: a piece of 16 bytes that begins behind the
+// width reads the one before it instead (its products are never stored).
 template <int BYTES, int E>
-__device__ __forceinline__ Raw<BYTES> load_row(const char* row, int d, int D) {
+__device__ __forceinline__ Raw<BYTES> load_row(const char* row, uint32_t off, int d, int D) {
     if constexpr (BYTES == 32) {
         Raw<32> r;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int at = d + i * 16 / E;
-            const uint4 x = *reinterpret_cast<const uint4*>(row + (at < D ? at : 0) * E);
-            r.w[4 * i] = x.x; r.w[4 * i + 1] = x.y; r.w[4 * i + 2] = x.z; r.w[4 * i + 3] = x.w;
+            const u32x4 x = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(row + (off + (d + i * 16 / E < D ? 16 * i : 0))));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.w[4 * i + e] = x[e];
         }
         return r;
     } else {
-        return load_raw<BYTES>(row + (d < D ? d : 0) * E);
+        return load_raw<BYTES>(row + off);
     }
+}
+
+// A split sequence's pieces p0 .. p1 together, for the query rows of one tile: groups of threads take every
+// parts-th piece with a running maximum, eight pieces' loads at a time, and are then added in LDS (buf).
+template <int DP, int DT>
+__device__ __forceinline__ void join_pieces(const AttnArgs& a, int rows, int rows_most, int slots, int s0, int piece, int p0,
+                                            int p1, int b, int hq0, float* buf) {
+    constexpr int kQuads = DP / 4;                      // float4 of a row
+    constexpr int kThreads = 64 * waves_of(DP);
+    const int items = rows * kQuads, parts = items >= kThreads ? 1 : kThreads / items;
+    constexpr int kAhead = 8;
+    for (int base = 0; base < items; base += kThreads) {
+        const int part = parts == 1 ? 0 : static_cast<int>(threadIdx.x) / items;
+        const int item = parts == 1 ? base + static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % items;
+        const int row = item / kQuads, d = 4 * (item % kQuads);
+        const bool mine = item < items && part < parts && d < a.D;
+        float m = kNegInf, l = 0.0f, x[4] = {0, 0, 0, 0};
+        bool some = false;
+        if (mine) {
+            for (int p = p0 + part; p <= p1; p += kAhead * parts) {
+                float pm[kAhead], pl[kAhead];
+                float4 px[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const int w = p + i * parts < p1 ? p + i * parts : p1;
+                    const int slot = 2 * w + (w * piece < s0);
+                    const float2 st = receive(part_stat(a, rows_most, slots, slot) + 2 * row);
+                    const float* x = part_out(a, rows_most, slot) + row * a.D + d;
+                    const float2 x0 = receive(x), x1 = receive(x + 2);
+                    pm[i] = st.x;
+                    pl[i] = p + i * parts <= p1 ? st.y : -1.0f;
+                    px[i] = make_float4(x0.x, x0.y, x1.x, x1.y);
+                }
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) top = pl[i] < 0.0f ? top : __builtin_fmaxf(top, pm[i]);
+                const float ref = top == kNegInf ? 0.0f : top;
+                const float f = __builtin_amdgcn_exp2f(m - ref);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= f;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (pl[i] < 0.0f) continue;         // nothing seen there
+                    some = true;
+                    const float fi = __builtin_amdgcn_exp2f(pm[i] - ref);
+                    l = __builtin_fmaf(fi, pl[i], l);
+                    x[0] = __builtin_fmaf(fi, px[i].x, x[0]);
+                    x[1] = __builtin_fmaf(fi, px[i].y, x[1]);
+                    x[2] = __builtin_fmaf(fi, px[i].z, x[2]);
+                    x[3] = __builtin_fmaf(fi, px[i].w, x[3]);
+                }
+            }
+        }
+        if (parts > 1) {
+            __syncthreads();
+            float* at = buf + 8 * threadIdx.x;
+            at[0] = m; at[1] = some ? l : -1.0f; at[2] = x[0]; at[3] = x[1]; at[4] = x[2]; at[5] = x[3];
+            __syncthreads();
+            if (part == 0 && mine) {
+                for (int o = 1; o < parts; ++o) {
+                    const float* y = buf + 8 * (o * items + item);
+                    if (y[1] < 0.0f) continue;
+                    some = true;
+                    const float top = __builtin_fmaxf(m, y[0]), ref = top == kNegInf ? 0.0f : top;
+                    const float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(y[0] - ref);
+                    m = top;
+                    l = l * f + y[1] * fo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = x[e] * f + y[2 + e] * fo;
+                }
+            }
+        }
+        if (mine && part == 0) {
+            const float inv = some ? 1.0f / l : 0.0f;
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + b * a.o_token + (hq0 + row) * a.o_head + d) =
+                make_uint2(pack_16x2(x[0] * inv, x[1] * inv, DT), pack_16x2(x[2] * inv, x[3] * inv, DT));
+        }
+    }
+    __syncthreads();
 }
 
 // DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache; SMALL: pages of less than
 // 16 tokens (a 16-key group may span pages, and every lane looks up its own keys).
 template <int DP, int DT, bool I8, bool SMALL>
-__global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_kernel(AttnArgs a, int row_tiles) {
+__global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_decode_kernel(AttnArgs a, int row_tiles, bool quads) {
+    constexpr int kWaves = waves_of(DP), kTile = kWaves * kKeys;
     constexpr int E = I8 ? 1 : 2;                       // bytes per cached value
     constexpr int VE = DP / 16;                         // values a lane holds of a value row
     constexpr int kSteps = DP / 32;                     // products over the width
@@ -181,38 +270,45 @@ __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_ke
     __shared__ float sm_out[kWaves][16][DP + 4];
     __shared__ float sm_m[kWaves][16], sm_l[kWaves][16];
     __shared__ int sm_any[kWaves];
+    __shared__ int sm_last;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int group = a.Hq / a.H;
     const int rows_most = group < 16 ? group : 16;
-    const int64_t per = static_cast<int64_t>(a.H) * row_tiles;
-    const Line line = line_of(a, per, gridDim.x);
-    const int64_t t0 = blockIdx.x * line.piece;
-    const int64_t t1 = t0 + line.piece < line.total ? t0 + line.piece : line.total;
+    const int per = a.H * row_tiles;
+    // sequences that see nothing have no tiles: zeros
+    for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
+        if (visible<kTile>(a, scalar_word(a.lens + e)).nt != 0) continue;
+        for (int x = threadIdx.x; x < a.Hq * (a.D / 8); x += 64 * kWaves) {
+            const int row = x / (a.D / 8), d = 8 * (x % (a.D / 8));
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + e * a.o_token + row * a.o_head + d) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    const int total = line_total<kTile>(a, per);
+    const int piece = (total + gridDim.x - 1) / gridDim.x;
+    const int t0 = blockIdx.x * piece;
+    const int t1 = t0 + piece < total ? t0 + piece : total;
     if (t0 >= t1) return;
-    int64_t b, before;
-    find_seq(a, per, t0, &b, &before);
-    b = uniform(b);
-    before = uniform(before);
+    int b, before;
+    find_seq<kTile>(a, per, t0, &b, &before);
     const int mask = (1 << a.page_shift) - 1;
     const int last_page = static_cast<int>(a.pages) - 1;
 
-    for (int64_t t = t0; t < t1;) {
-        Visible v = visible(a, a.lens[b]);
+    for (int t = t0; t < t1;) {
+        Visible v = visible<kTile>(a, scalar_word(a.lens + b));
         while (v.nt == 0 || t - before >= v.nt * per) {   // on to the next sequence that has tiles
             before += v.nt * per;
             ++b;
-            v = visible(a, a.lens[b]);
+            v = visible<kTile>(a, scalar_word(a.lens + b));
         }
-        const int pair = static_cast<int>((t - before) / v.nt);
-        const int i0 = static_cast<int>((t - before) - static_cast<int64_t>(pair) * v.nt);
-        const int64_t left = t1 - t;
-        const int i1 = i0 + (left < v.nt - i0 ? static_cast<int>(left) : v.nt - i0);   // this segment: tiles i0 .. i1 - 1
+        const int pair = (t - before) / v.nt;
+        const int i0 = t - before - pair * v.nt;
+        const int i1 = t1 - t < v.nt - i0 ? i0 + (t1 - t) : v.nt;   // this segment: tiles i0 .. i1 - 1
         const int h = pair / row_tiles, rt = pair % row_tiles;
         const int rows = group - 16 * rt < 16 ? group - 16 * rt : 16;
         const int hq0 = h * group + 16 * rt;
-        const int* table = a.table + b * a.ld_table;
+        const int* table = a.table + static_cast<int64_t>(b) * a.ld_table;
 
         // the query rows: B operand, lane (c, g) = row c, the values that the key loads' slots stand for
         Frag q[kSteps], q2[kSplit ? kSteps : 1];
@@ -242,78 +338,84 @@ __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_ke
         const float scale = a.scale * kLog2e;
         const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
         const char* vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
+        // the lane's places within 16 keys (bytes): key c, chunks 4 x + g; keys 4 g + r, values VE c ..
+        const uint32_t tok = static_cast<uint32_t>(a.c_token) * E;
+        uint32_t ko[KL], vo[4];
+#pragma unroll
+        for (int x = 0; x < KL; ++x) ko[x] = (SMALL ? 0 : c * tok) + (KB / E * (4 * x + g) < a.D ? KB * (4 * x + g) : 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vo[r] = (SMALL ? 0 : (4 * g + r) * tok) + (VE * c < a.D ? VE * E * c : 0);
+        const float* ksb = a.k_scale + (I8 ? h * a.s_head : 0);
+        const float* vsb = a.v_scale + (I8 ? h * a.s_head : 0);
 
         Raw<KB> kr[2][2][KL];       // [buffer][16-key group][load]
         Raw<VE * E> vr[2][8];       // [buffer][key]
         float ksc[2][2][4], vsc[2][2][4];   // int8: scales of the lane's 8 keys
         uint32_t held[2];           // bit 16 u + x: key x of group u is in a page of the cache
 
-        auto first_key = [&](int i) -> int64_t {
-            const int64_t tile = i < v.ns ? i : v.w0 + (i - v.ns);
-            return tile * kTile + wave * kKeys;
-        };
+        auto first_key = [&](int i) { return (i < v.ns ? i : v.w0 + (i - v.ns)) * kTile + wave * kKeys; };
         // the 32 keys from j on: every address is inside the cache (a key that is not held reads page 0)
-        auto load = [&](int buf, int64_t j) __attribute__((always_inline)) {
+        auto load = [&](int buf, int j) __attribute__((always_inline)) {
             held[buf] = 0;
-            const int64_t ne = a.width - 1;
+            const int ne = static_cast<int>(a.width) - 1;
             if constexpr (!SMALL) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int64_t at = (j + 16 * u) >> a.page_shift;
-                    const int p = table[at < ne ? at : ne];
+                    const int at = (j + 16 * u) >> a.page_shift;
+                    const int p = scalar_word(table + (at < ne ? at : ne));
                     const bool ok = p >= 0 && p <= last_page && at <= ne;
                     held[buf] |= ok ? 0xffffu << (16 * u) : 0u;
-                    const int pg = ok ? p : 0;
-                    const int slot = static_cast<int>(j + 16 * u) & mask;
+                    const int pg = ok ? p : 0, slot = (j + 16 * u) & mask;
                     const int64_t off = (pg * a.c_page + slot * a.c_token) * E;
-                    const int64_t tok = a.c_token * E;
+                    const char* kp = kbase + off;
+                    const char* vp = vbase + off;
 #pragma unroll
-                    for (int x = 0; x < KL; ++x) {
-                        const int d = KB / E * (4 * x + g);
-                        kr[buf][u][x] = load_raw<KB>(kbase + off + c * tok + (d < a.D ? d : 0) * E);
-                    }
+                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        vr[buf][4 * u + r] = load_row<VE * E, E>(vbase + off + (4 * g + r) * tok, VE * c, a.D);
-                        if constexpr (I8) {
-                            const int64_t so = pg * a.s_page + h * a.s_head + (slot + 4 * g + r) * a.s_token;
-                            ksc[buf][u][r] = a.k_scale[so];
-                            vsc[buf][u][r] = a.v_scale[so];
+                    for (int r = 0; r < 4; ++r) vr[buf][4 * u + r] = load_row<VE * E, E>(vp, vo[r], VE * c, a.D);
+                    if constexpr (I8) {
+                        const int64_t so = pg * a.s_page + slot * a.s_token;
+                        if (quads) {                    // four keys' scales are one aligned 16 bytes
+                            const float4 x = *reinterpret_cast<const float4*>(ksb + so + 4 * g);
+                            const float4 y = *reinterpret_cast<const float4*>(vsb + so + 4 * g);
+                            ksc[buf][u][0] = x.x; ksc[buf][u][1] = x.y; ksc[buf][u][2] = x.z; ksc[buf][u][3] = x.w;
+                            vsc[buf][u][0] = y.x; vsc[buf][u][1] = y.y; vsc[buf][u][2] = y.z; vsc[buf][u][3] = y.w;
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                ksc[buf][u][r] = ksb[so + (4 * g + r) * a.s_token];
+                                vsc[buf][u][r] = vsb[so + (4 * g + r) * a.s_token];
+                            }
                         }
                     }
                 }
             } else {
                 // lane x (and x + 32) looks up key x of the 32: its row as page << page_shift | slot, or -1
-                const int64_t mine = j + (lane & 31);
-                const int64_t at = mine >> a.page_shift;
+                const int mine = j + (lane & 31), at = mine >> a.page_shift;
                 const int p = table[at < ne ? at : ne];
                 const bool ok = p >= 0 && p <= last_page && at <= ne;
                 held[buf] = static_cast<uint32_t>(__ballot(ok));
-                const int code = ok ? (p << a.page_shift) | (static_cast<int>(mine) & mask) : 0;
+                const int code = ok ? (p << a.page_shift) | (mine & mask) : 0;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int ck = __shfl(code, 16 * u + c);
                     const char* kp = kbase + (static_cast<int64_t>(ck >> a.page_shift) * a.c_page + (ck & mask) * a.c_token) * E;
 #pragma unroll
-                    for (int x = 0; x < KL; ++x) {
-                        const int d = KB / E * (4 * x + g);
-                        kr[buf][u][x] = load_raw<KB>(kp + (d < a.D ? d : 0) * E);
-                    }
+                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int cv = __shfl(code, 16 * u + 4 * g + r);
                         const int64_t pg = cv >> a.page_shift, slot = cv & mask;
-                        vr[buf][4 * u + r] = load_row<VE * E, E>(vbase + (pg * a.c_page + slot * a.c_token) * E, VE * c, a.D);
+                        vr[buf][4 * u + r] = load_row<VE * E, E>(vbase + (pg * a.c_page + slot * a.c_token) * E, vo[r], VE * c, a.D);
                         if constexpr (I8) {
-                            const int64_t so = pg * a.s_page + h * a.s_head + slot * a.s_token;
-                            ksc[buf][u][r] = a.k_scale[so];
-                            vsc[buf][u][r] = a.v_scale[so];
+                            ksc[buf][u][r] = ksb[pg * a.s_page + slot * a.s_token];
+                            vsc[buf][u][r] = vsb[pg * a.s_page + slot * a.s_token];
                         }
                     }
                 }
             }
         };
-        auto work = [&](int buf, int64_t j) __attribute__((always_inline)) {
+        auto work = [&](int buf, int j) __attribute__((always_inline)) {
             // scores
             f32x4 s[2];
 #pragma unroll
@@ -356,7 +458,7 @@ __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_ke
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                     const int at = 16 * (x >> 2) + 4 * g + (x & 3);
-                    const int64_t key = j + at;
+                    const int key = j + at;
                     const bool ok = ((held[buf] >> at) & 1) && key <= v.last && (key >= v.lo || key < v.sinks);
                     see |= ok ? 1u << x : 0u;
                     p[x] = ok ? p[x] : kNegInf;
@@ -452,9 +554,10 @@ __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_ke
         }
         __syncthreads();
         const bool whole = i0 == 0 && i1 == v.nt;
-        const bool some = (sm_any[0] | sm_any[1] | sm_any[2] | sm_any[3]) != 0;
-        const int64_t slots = 2 * static_cast<int64_t>(gridDim.x);
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (t != t0);
+        int some = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) some |= sm_any[w];
+        const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t != t0);
         for (int e = threadIdx.x; e < rows * DP / 4; e += 64 * kWaves) {
             const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
             if (d >= a.D) continue;
@@ -480,75 +583,51 @@ __global__ void __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) attn_decode_ke
                 *reinterpret_cast<uint2*>(out) = make_uint2(pack_16x2(x[0] * inv, x[1] * inv, DT),
                                                             pack_16x2(x[2] * inv, x[3] * inv, DT));
             } else {
-                *reinterpret_cast<float4*>(part_out(a, rows_most, slot) + row * a.D + d) = make_float4(x[0], x[1], x[2], x[3]);
-                if (d == 0) {
-                    float* st = part_stat(a, rows_most, slots, slot) + 2 * row;
-                    st[0] = top;
-                    st[1] = some ? sum : -1.0f;                 // -1: nothing seen
-                }
+                float* to = part_out(a, rows_most, slot) + row * a.D + d;
+                send(to, x[0], x[1]);
+                send(to + 2, x[2], x[3]);
+                if (d == 0) send(part_stat(a, rows_most, slots, slot) + 2 * row, top, some ? sum : -1.0f);   // -1: nothing seen
+            }
+        }
+        if (!whole) {
+            // the sequence's pieces: workgroups p0 .. p1 of the line
+            const int s0 = before + pair * v.nt, p0 = s0 / piece, p1 = (s0 + v.nt - 1) / piece;
+            // every thread's stores have arrived (they are written through to where the device is coherent) before
+            // the workgroup is counted; the count's value says that the others' have too
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int* count = a.counters + static_cast<int64_t>(b) * per + pair;
+                const int old = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // the last one: zero again for the next call
+                if (old == p1 - p0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sm_last = old == p1 - p0;
+            }
+            __syncthreads();
+            if (sm_last) {
+                join_pieces<DP, DT>(a, rows, rows_most, slots, s0, piece, p0, p1, b, hq0, &sm_out[0][0][0]);
             }
         }
         t += i1 - i0;
     }
 }
 
-// One workgroup per (sequence, query head): joins a split sequence's pieces in their order; zeros for a
-// sequence that sees nothing. groups: the workgroups of the kernel before.
-__global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, int row_tiles, int groups) {
-    const int64_t b = blockIdx.x / a.Hq;
-    const int hq = static_cast<int>(blockIdx.x % a.Hq);
-    const int group = a.Hq / a.H, rows_most = group < 16 ? group : 16;
-    const int64_t per = static_cast<int64_t>(a.H) * row_tiles;
-    const Visible v = visible(a, a.lens[b]);
-    uint16_t* out = static_cast<uint16_t*>(a.o) + b * a.o_token + hq * a.o_head;
-    const int d = 4 * static_cast<int>(threadIdx.x);
-    if (v.nt == 0) {
-        if (d < a.D) *reinterpret_cast<uint2*>(out + d) = make_uint2(0, 0);
-        return;
-    }
-    const Line line = line_of(a, per, groups);
-    const int pair = hq / group * row_tiles + hq % group / 16, row = hq % group % 16;
-    const int64_t t0 = count_tiles(a, 0, b) * per + static_cast<int64_t>(pair) * v.nt, t1 = t0 + v.nt;
-    const int64_t w0 = t0 / line.piece, w1 = (t1 - 1) / line.piece;
-    if (w0 == w1 || d >= a.D) return;
-    const int64_t slots = 2 * static_cast<int64_t>(groups);
-    auto slot_of = [&](int64_t w) { return 2 * w + (w * line.piece < t0); };
-    float top = kNegInf;
-    for (int64_t w = w0; w <= w1; ++w) top = __builtin_fmaxf(top, part_stat(a, rows_most, slots, slot_of(w))[2 * row]);
-    const float base = top == kNegInf ? 0.0f : top;
-    float sum = 0.0f, x[4] = {0, 0, 0, 0};
-    bool some = false;
-#pragma unroll 4
-    for (int64_t w = w0; w <= w1; ++w) {
-        const int64_t slot = slot_of(w);
-        const float* st = part_stat(a, rows_most, slots, slot) + 2 * row;
-        if (st[1] < 0.0f) continue;
-        some = true;
-        const float f = __builtin_amdgcn_exp2f(st[0] - base);
-        sum = __builtin_fmaf(f, st[1], sum);
-        const float4 y = *reinterpret_cast<const float4*>(part_out(a, rows_most, slot) + row * a.D + d);
-        x[0] = __builtin_fmaf(f, y.x, x[0]);
-        x[1] = __builtin_fmaf(f, y.y, x[1]);
-        x[2] = __builtin_fmaf(f, y.z, x[2]);
-        x[3] = __builtin_fmaf(f, y.w, x[3]);
-    }
-    const float inv = some ? 1.0f / sum : 0.0f;
-    *reinterpret_cast<uint2*>(out + d) =
-        make_uint2(pack_16x2(x[0] * inv, x[1] * inv, a.dtype), pack_16x2(x[2] * inv, x[3] * inv, a.dtype));
-}
-
+// Workgroups: as many as are resident at once, one a compute unit.
 int decode_groups() {
     const int cus = device_cu_count();
-    return (cus > 0 ? cus : 256) * 2;
+    return cus > 0 ? cus : 256;
 }
 
 template <int DP, int DT, bool I8>
 int launch_width(const AttnArgs& a, int row_tiles, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(decode_groups()));
+    // int8 scales of 4 keys as 16 bytes: consecutive and aligned
+    const bool quads = I8 && a.s_token == 1 && a.s_page % 4 == 0 && a.s_head % 4 == 0 &&
+                       (reinterpret_cast<uintptr_t>(a.k_scale) | reinterpret_cast<uintptr_t>(a.v_scale)) % 16 == 0;
     if (a.page_shift >= 4)
-        hipLaunchKernelGGL((attn_decode_kernel<DP, DT, I8, false>), grid, dim3(64 * kWaves), 0, stream, a, row_tiles);
+        hipLaunchKernelGGL((attn_decode_kernel<DP, DT, I8, false>), grid, dim3(64 * waves_of(DP)), 0, stream, a, row_tiles, quads);
     else
-        hipLaunchKernelGGL((attn_decode_kernel<DP, DT, I8, true>), grid, dim3(64 * kWaves), 0, stream, a, row_tiles);
+        hipLaunchKernelGGL((attn_decode_kernel<DP, DT, I8, true>), grid, dim3(64 * waves_of(DP)), 0, stream, a, row_tiles, quads);
     return launch_status("paged_attention");
 }
 
@@ -569,15 +648,11 @@ int64_t attn_decode_workspace_bytes(int Hq, int H, int D) {
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream) {
     const int row_tiles = (a.Hq / a.H + 15) / 16;
     const bool i8 = a.k_scale != nullptr;
-    int rc;
     if (a.dtype == kDtF16)
-        rc = i8 ? launch_type<kDtF16, true>(a, row_tiles, stream) : launch_type<kDtF16, false>(a, row_tiles, stream);
-    else
-        rc = i8 ? launch_type<kDtBf16, true>(a, row_tiles, stream) : launch_type<kDtBf16, false>(a, row_tiles, stream);
-    if (rc) return rc;
-    hipLaunchKernelGGL(attn_join_kernel, dim3(static_cast<unsigned>(a.B * a.Hq)), dim3(64), 0, stream, a, row_tiles,
-                       decode_groups());
-    return launch_status("paged_attention");
+        return i8 ? launch_type<kDtF16, true>(a, row_tiles, stream) : launch_type<kDtF16, false>(a, row_tiles, stream);
+    return i8 ? launch_type<kDtBf16, true>(a, row_tiles, stream) : launch_type<kDtBf16, false>(a, row_tiles, stream);
 }
+
+int64_t attn_decode_counters(int Hq, int H, int64_t B) { return B * H * ((Hq / H + 15) / 16); }
 
 }  // namespace mq

@@ -91,11 +91,11 @@ ENTRY(mq_linear_rowscale, 21, B(0) | B(6) | B(9) | B(10) | B(12) | B(18) | B(20)
 ENTRY(mq_kv_write, 30, B(0) | B(3) | B(10) | B(11) | B(16) | B(17) | B(23) | B(27) | B(28) | B(29),
       fn_mq_kv_write(P(0), L(1), L(2), P(3), L(4), L(5), I(6), L(7), L(8), L(9), P(10), P(11), I(12), L(13), L(14), L(15),
                      P(16), P(17), L(18), L(19), L(20), L(21), I(22), P(23), L(24), L(25), L(26), P(27), P(28), P(29)))
-ENTRY_F(mq_paged_attention, 36,
-        B(0) | B(8) | B(9) | B(14) | B(15) | B(21) | B(25) | B(26) | B(30) | B(33) | B(35), B(27),
+ENTRY_F(mq_paged_attention, 37,
+        B(0) | B(8) | B(9) | B(14) | B(15) | B(21) | B(25) | B(26) | B(30) | B(33) | B(35) | B(36), B(27),
         fn_mq_paged_attention(P(0), L(1), L(2), I(3), L(4), L(5), L(6), L(7), P(8), P(9), I(10), L(11), L(12), L(13), P(14),
                               P(15), L(16), L(17), L(18), L(19), I(20), P(21), L(22), L(23), L(24), P(25), P(26), F(27),
-                              L(28), L(29), P(30), L(31), L(32), P(33), L(34), P(35)))
+                              L(28), L(29), P(30), L(31), L(32), P(33), L(34), P(35), P(36)))
 ENTRY(mq_kv_grow, 15, B(0) | B(4) | B(5) | B(8) | B(9) | B(11) | B(12) | B(14),
       fn_mq_kv_grow(P(0), L(1), L(2), L(3), P(4), P(5), L(6), I(7), P(8), P(9), L(10), P(11), P(12), L(13), P(14)))
 ENTRY(mq_linear_w4a16, 23, B(0) | B(4) | B(6) | B(9) | B(14) | B(16) | B(22),

@@ -240,10 +240,12 @@ struct AttnArgs {
     int dtype;                // of q and o
     void* work;
     int64_t work_bytes;
+    int* counters;            // zeros before and after a call
 };
 int launch_attn_prompt(const AttnArgs& a, hipStream_t stream);
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream);
 int64_t attn_decode_workspace_bytes(int Hq, int H, int D);
+int64_t attn_decode_counters(int Hq, int H, int64_t B);
 
 // --- 4-bit weights, floating activations (mq_w4a16.hip)
 enum class W4Zero : int { Signed = 0, U4 = 1, Float = 2 };

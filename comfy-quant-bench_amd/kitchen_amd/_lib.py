@@ -71,7 +71,8 @@ _SIGNATURES = {
                     c_int),
     "mq_paged_attention": ([c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64,
                             c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_float,
-                            c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp], c_int),
+                            c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp], c_int),
+    "mq_paged_attention_counters": ([c_i64, c_i64, c_i64, c_i64, c_int], c_i64),
     "mq_paged_attention_workspace_bytes": ([c_i64, c_i64, c_i64, c_i64, c_i64, c_int], c_i64),
     "mq_kv_workspace_bytes": ([c_i64, c_i64], c_i64),
     "mq_kv_fork": ([c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,

@@ -19,6 +19,8 @@ growth that cannot be done whole changes nothing and says so in `status`.
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _lib
@@ -27,6 +29,26 @@ from .ops import _scratch
 CACHE_TYPES = (torch.bfloat16, torch.float16, torch.int8)
 _CODE = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.int8: _lib.DT_I8}
 _ATTN_WS: dict = {}
+
+
+class _Counters(threading.local):
+    def __init__(self):
+        self.by_stream: dict = {}   # (device index, stream) -> zeros
+
+
+_COUNTERS = _Counters()
+
+
+def _counters(n: int, device, stream: int) -> torch.Tensor:
+    """Zeros that every call leaves as zeros: kept per thread, device and stream like the workspaces, whose calls
+    run in order; a captured call has its own, cleared by the graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=device)
+    kept, key = _COUNTERS.by_stream, (device.index, stream)
+    buf = kept.get(key)
+    if buf is None or buf.numel() < n:
+        buf = kept[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
+    return buf
 
 
 def _device_of(t: torch.Tensor, what: str):
@@ -144,17 +166,22 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with rows at multiples of 16 bytes")
     stream = _lib.stream_of_device(dev)
     key = (dev.index, t, heads, h, d, tables[2], cu_q is None)
-    nbytes = _ATTN_WS.get(key)
-    if nbytes is None:
+    sizes = _ATTN_WS.get(key)
+    if sizes is None:
+        lib, b, ragged = _lib.load(), tables[2], int(cu_q is not None)
         with torch.cuda.device(dev):
-            nbytes = int(_lib.load().mq_paged_attention_workspace_bytes(t, heads, h, d, tables[2], cu_q is not None))
+            sizes = (int(lib.mq_paged_attention_workspace_bytes(t, heads, h, d, b, ragged)),
+                     int(lib.mq_paged_attention_counters(t, heads, h, b, ragged)))
         if len(_ATTN_WS) > 4096:   # ragged batches come in any size: the sizes are only remembered, not needed
             _ATTN_WS.clear()
-        _ATTN_WS[key] = nbytes
+        _ATTN_WS[key] = sizes
+    nbytes, ncount = sizes
     work = _scratch(nbytes, dev, stream) if nbytes else None
+    count = _counters(ncount, dev, stream) if ncount else None
     _lib.call("mq_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), _CODE[q.dtype], t, heads, h, d, *cache,
               *tables, d ** -0.5 if scale is None else float(scale), window or 0, int(sinks), out.data_ptr(),
-              out.stride(0), out.stride(1), None if work is None else work.data_ptr(), nbytes, stream)
+              out.stride(0), out.stride(1), None if work is None else work.data_ptr(), nbytes,
+              None if count is None else count.data_ptr(), stream)
     return out
 
 

@@ -449,6 +449,8 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
  *   q, out [T, Hq, D] of type dtype (bf16 or fp16; a 16-bit cache has the same), Hq % H == 0
  *   workspace: mq_paged_attention_workspace_bytes(T, Hq, H, D, B, cu_q != NULL) bytes, 16-byte aligned
  *   (nothing in it has to start at zero)
+ *   counters: mq_paged_attention_counters(T, Hq, H, B, cu_q != NULL) int32 in device memory that are zero before the
+ *   call; they are zero again behind it, so calls in a row on one stream share them
  */
 int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int64_t Hq, int64_t H,
                        int64_t D, const void* k_cache, const void* v_cache, int cache_dtype, int64_t c_page,
@@ -456,8 +458,9 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
                        int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
                        int64_t ld_table, int64_t B, int64_t width, const int32_t* lens, const int32_t* cu_q, float scale,
                        int64_t window, int64_t sinks, void* out, int64_t out_token, int64_t out_head, void* workspace,
-                       int64_t workspace_bytes, void* stream);
+                       int64_t workspace_bytes, int32_t* counters, void* stream);
 int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged);
+int64_t mq_paged_attention_counters(int64_t T, int64_t Hq, int64_t H, int64_t B, int ragged);
 
 /*
  * Bookkeeping of the pages, on the device: page_table int32 [rows, width] (-1: none), lens int32 [rows],

@@ -18,7 +18,7 @@ WRITE = dict(k=A, k_token=512, k_head=128, v=A, v_token=512, v_head=128, dtype=0
 ATTN = dict(q=A, q_token=1024, q_head=128, dtype=0, T=3, Hq=8, H=4, D=128, kc=A, vc=A, cdt=0, c_page=8192, c_head=2048,
             c_token=128, ks=None, vs=None, s_page=0, s_head=0, s_token=0, pages=9, page=16, table=A, ld=4, B=3, width=4,
             lens=A, cu=None, scale=0.1, window=0, sinks=0, out=A, out_token=1024, out_head=128, work=None, work_bytes=0,
-            stream=None)
+            counters=None, stream=None)
 GROW = dict(table=A, ld=4, rows=3, width=4, lens=A, refs=A, pages=9, page=16, seqs=A, counts=A, n=2, status=None, work=A,
             work_bytes=1 << 20, stream=None)
 FORK = dict(k=A, v=A, layers=2, layer_bytes=1 << 16, pitch=4096, bytes=4096, ks=None, vs=None, sl=0, sp=0, sb=0, table=A, ld=4,
