@@ -65,28 +65,35 @@ __device__ __forceinline__ int scalar_word(const int* p) {
     return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// The line of tiles: sequence b has nt(b) tiles for each of `per` (cache head, row tile) pairs. total: tiles; and
-// the sequence that holds tile t of it, with the tiles before it. Every wave of a workgroup computes them for itself,
-// 64 sequences at a time.
+// The line of tiles: sequence b takes up `extra` places and its nt(b) tiles for each of `per` (cache head, row tile)
+// pairs; the places stand for what a workgroup pays to begin and end a sequence, so that those with many short ones
+// get fewer tiles. total: places; and the sequence that holds place t of it, with the places before it. Every wave
+// of a workgroup computes them for itself, 64 sequences at a time.
 template <int TILE>
-__device__ __forceinline__ int line_total(const AttnArgs& a, int per) {
-    if (a.B == 1) return visible<TILE>(a, scalar_word(a.lens)).nt * per;
+__device__ __forceinline__ int places(const AttnArgs& a, int len, int extra) {
+    const int nt = visible<TILE>(a, len).nt;
+    return nt ? nt + extra : 0;
+}
+
+template <int TILE>
+__device__ __forceinline__ int line_total(const AttnArgs& a, int per, int extra) {
+    if (a.B == 1) return places<TILE>(a, scalar_word(a.lens), extra) * per;
     int n = 0;
-    for (int b = threadIdx.x & 63; b < a.B; b += 64) n += visible<TILE>(a, a.lens[b]).nt;
+    for (int b = threadIdx.x & 63; b < a.B; b += 64) n += places<TILE>(a, a.lens[b], extra);
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) n += __shfl_xor(n, s);
     return __builtin_amdgcn_readfirstlane(n) * per;
 }
 
 template <int TILE>
-__device__ __forceinline__ void find_seq(const AttnArgs& a, int per, int t, int* seq, int* before) {
+__device__ __forceinline__ void find_seq(const AttnArgs& a, int per, int extra, int t, int* seq, int* before) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     *seq = 0;
     *before = 0;
     if (a.B == 1) return;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int n = b0 + lane < a.B ? visible<TILE>(a, a.lens[b0 + lane]).nt * per : 0;
+        const int n = b0 + lane < a.B ? places<TILE>(a, a.lens[b0 + lane], extra) * per : 0;
         int x = n;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
@@ -104,8 +111,8 @@ __device__ __forceinline__ void find_seq(const AttnArgs& a, int per, int t, int*
     }
 }
 
-// A split sequence's pieces: [slot][row][D] outputs, then [slot][row][2] maxima and sums. A workgroup's first
-// segment has slot 2 w, a last one that began inside its piece 2 w + 1.
+// A split sequence's pieces: [slot][row][D] outputs, then [slot][row][2] maxima and sums. The segment of a sequence
+// that began before workgroup w's piece has slot 2 w, one that goes on behind it 2 w + 1.
 __device__ __forceinline__ float* part_out(const AttnArgs& a, int rows, int64_t slot) {
     return static_cast<float*>(a.work) + slot * rows * a.D;
 }
@@ -173,14 +180,14 @@ __device__ __forceinline__ Raw<BYTES> load_row(const char* row, uint32_t off, in
 }
 
 // A split sequence's pieces p0 .. p1 together, for the query rows of one tile: groups of threads take every
-// parts-th piece with a running maximum, eight pieces' loads at a time, and are then added in LDS (buf).
+// parts-th piece with a running maximum, four pieces' loads at a time, and are then added in LDS (buf).
 template <int DP, int DT>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, int rows, int rows_most, int slots, int s0, int piece, int p0,
                                             int p1, int b, int hq0, float* buf) {
     constexpr int kQuads = DP / 4;                      // float4 of a row
     constexpr int kThreads = 64 * waves_of(DP);
     const int items = rows * kQuads, parts = items >= kThreads ? 1 : kThreads / items;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;
     for (int base = 0; base < items; base += kThreads) {
         const int part = parts == 1 ? 0 : static_cast<int>(threadIdx.x) / items;
         const int item = parts == 1 ? base + static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % items;
@@ -265,6 +272,11 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
     constexpr int KL = DP * E / 4 / KB;                 // key loads per row and lane
     constexpr bool kSplit = I8 && DT == kDtF16;         // fp16 rows against int8 keys: bf16 products of hi + lo
     constexpr int MT = I8 ? kDtBf16 : DT;               // type of the products
+    // beginning and ending a sequence takes about as long as 128 KB of keys and values: counted where there are more
+    // of them than workgroups (a ragged batch of 64: 85 -> 77 us); else every piece is a part of one anyway
+    constexpr int kExtra = (131072 + kTile * DP * E) / (2 * kTile * DP * E);
+    // the next segment's first tile is loaded ahead of this one's end where the registers for it are free
+    constexpr bool kAcross = DP != 256 && !kSplit;
     // fp16 probabilities are held 2^14 times as large: they stay normal down to 2^-28 of the largest
     constexpr float kLift = MT == kDtF16 ? 14.0f : 0.0f;
     __shared__ float sm_out[kWaves][16][DP + 4];
@@ -276,7 +288,7 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
     const int c = lane & 15, g = lane >> 4;
     const int group = a.Hq / a.H;
     const int rows_most = group < 16 ? group : 16;
-    const int per = a.H * row_tiles;
+    const int per = a.H * row_tiles, extra = a.B * per > gridDim.x ? kExtra : 0;
     // sequences that see nothing have no tiles: zeros
     for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
         if (visible<kTile>(a, scalar_word(a.lens + e)).nt != 0) continue;
@@ -285,41 +297,149 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + e * a.o_token + row * a.o_head + d) = make_uint4(0, 0, 0, 0);
         }
     }
-    const int total = line_total<kTile>(a, per);
+    const int total = line_total<kTile>(a, per, extra);
     const int piece = (total + gridDim.x - 1) / gridDim.x;
     const int t0 = blockIdx.x * piece;
     const int t1 = t0 + piece < total ? t0 + piece : total;
     if (t0 >= t1) return;
     int b, before;
-    find_seq<kTile>(a, per, t0, &b, &before);
+    find_seq<kTile>(a, per, extra, t0, &b, &before);
     const int mask = (1 << a.page_shift) - 1;
     const int last_page = static_cast<int>(a.pages) - 1;
 
-    for (int t = t0; t < t1;) {
-        Visible v = visible<kTile>(a, scalar_word(a.lens + b));
-        while (v.nt == 0 || t - before >= v.nt * per) {   // on to the next sequence that has tiles
-            before += v.nt * per;
-            ++b;
-            v = visible<kTile>(a, scalar_word(a.lens + b));
-        }
-        const int pair = (t - before) / v.nt;
-        const int i0 = t - before - pair * v.nt;
-        const int i1 = t1 - t < v.nt - i0 ? i0 + (t1 - t) : v.nt;   // this segment: tiles i0 .. i1 - 1
-        const int h = pair / row_tiles, rt = pair % row_tiles;
-        const int rows = group - 16 * rt < 16 ? group - 16 * rt : 16;
-        const int hq0 = h * group + 16 * rt;
-        const int* table = a.table + static_cast<int64_t>(b) * a.ld_table;
+    // the lane's places within 16 keys (bytes): key c, chunks 4 x + g; keys 4 g + r, values VE c ..
+    const uint32_t tok = static_cast<uint32_t>(a.c_token) * E;
+    uint32_t ko[KL], vo[4];
+#pragma unroll
+    for (int x = 0; x < KL; ++x) ko[x] = (SMALL ? 0 : c * tok) + (KB / E * (4 * x + g) < a.D ? KB * (4 * x + g) : 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vo[r] = (SMALL ? 0 : (4 * g + r) * tok) + (VE * c < a.D ? VE * E * c : 0);
 
-        // the query rows: B operand, lane (c, g) = row c, the values that the key loads' slots stand for
-        Frag q[kSteps], q2[kSplit ? kSteps : 1];
+    // the segment in hand: tiles i0 .. i1 - 1 of a sequence's cache head and row tile, whose tile 0 is place s0
+    Visible v;
+    int pair, s0, i0, i1;
+    const int* table;
+    const char *kbase, *vbase;
+    const float *ksb = nullptr, *vsb = nullptr;
+    // the next one at or behind place t; false: none in this workgroup's piece
+    auto open = [&](int t) __attribute__((always_inline)) {
+        while (t < t1) {
+            v = visible<kTile>(a, scalar_word(a.lens + b));
+            const int size = v.nt + extra;
+            if (v.nt == 0 || t - before >= size * per) {
+                before += v.nt ? size * per : 0;
+                ++b;
+                continue;
+            }
+            pair = (t - before) / size;
+            s0 = before + pair * size + extra;
+            i0 = t > s0 ? t - s0 : 0;
+            i1 = t1 - s0 < v.nt ? t1 - s0 : v.nt;
+            if (i0 < i1) break;
+            t = s0 + v.nt;                              // its extra places only
+        }
+        if (t >= t1) return false;
+        const int h = pair / row_tiles;
+        table = a.table + static_cast<int64_t>(b) * a.ld_table;
+        kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
+        vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
+        if constexpr (I8) {
+            ksb = a.k_scale + h * a.s_head;
+            vsb = a.v_scale + h * a.s_head;
+        }
+        return true;
+    };
+
+    // the query rows: B operand, lane (c, g) = row c, the values that the key loads' slots stand for
+    Frag q[kSteps], q2[kSplit ? kSteps : 1];
+    auto load_q = [&]() __attribute__((always_inline)) {
+        const int rt = pair % row_tiles, left = group - 16 * rt;
+        const uint16_t* row = static_cast<const uint16_t*>(a.q) + b * a.q_token +
+                              (pair / row_tiles * group + 16 * rt + (c < left ? c : 0)) * a.q_head;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int d = I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (c < rows && d < a.D)
-                x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + b * a.q_token +
-                                                    (hq0 + c) * a.q_head + d);
+            const uint4 x = *reinterpret_cast<const uint4*>(row + (d < a.D ? d : 0));
             q[s] = Frag{{x.x, x.y, x.z, x.w}};
+        }
+    };
+    Raw<KB> kr[2][2][KL];       // [buffer][16-key group][load]
+    Raw<VE * E> vr[2][8];       // [buffer][key]
+    float ksc[2][2][4], vsc[2][2][4];   // int8: scales of the lane's 8 keys
+    uint32_t held[2];           // bit 16 u + x: key x of group u is in a page of the cache
+
+    auto first_key = [&](int i) { return (i < v.ns ? i : v.w0 + (i - v.ns)) * kTile + wave * kKeys; };
+    // the 32 keys from j on: every address is inside the cache (a key that is not held reads page 0)
+    auto load = [&](int buf, int j) __attribute__((always_inline)) {
+        held[buf] = 0;
+        const int ne = static_cast<int>(a.width) - 1;
+        if constexpr (!SMALL) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int at = (j + 16 * u) >> a.page_shift;
+                const int p = scalar_word(table + (at < ne ? at : ne));
+                const bool ok = p >= 0 && p <= last_page && at <= ne;
+                held[buf] |= ok ? 0xffffu << (16 * u) : 0u;
+                const int pg = ok ? p : 0, slot = (j + 16 * u) & mask;
+                const int64_t off = (pg * a.c_page + slot * a.c_token) * E;
+                const char* kp = kbase + off;
+                const char* vp = vbase + off;
+#pragma unroll
+                for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vr[buf][4 * u + r] = load_row<VE * E, E>(vp, vo[r], VE * c, a.D);
+                if constexpr (I8) {
+                    const int64_t so = pg * a.s_page + slot * a.s_token;
+                    if (quads) {                    // four keys' scales are one aligned 16 bytes
+                        const float4 x = *reinterpret_cast<const float4*>(ksb + so + 4 * g);
+                        const float4 y = *reinterpret_cast<const float4*>(vsb + so + 4 * g);
+                        ksc[buf][u][0] = x.x; ksc[buf][u][1] = x.y; ksc[buf][u][2] = x.z; ksc[buf][u][3] = x.w;
+                        vsc[buf][u][0] = y.x; vsc[buf][u][1] = y.y; vsc[buf][u][2] = y.z; vsc[buf][u][3] = y.w;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            ksc[buf][u][r] = ksb[so + (4 * g + r) * a.s_token];
+                            vsc[buf][u][r] = vsb[so + (4 * g + r) * a.s_token];
+                        }
+                    }
+                }
+            }
+        } else {
+            // lane x (and x + 32) looks up key x of the 32: its row as page << page_shift | slot, or -1
+            const int mine = j + (lane & 31), at = mine >> a.page_shift;
+            const int p = table[at < ne ? at : ne];
+            const bool ok = p >= 0 && p <= last_page && at <= ne;
+            held[buf] = static_cast<uint32_t>(__ballot(ok));
+            const int code = ok ? (p << a.page_shift) | (mine & mask) : 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int ck = __shfl(code, 16 * u + c);
+                const char* kp = kbase + (static_cast<int64_t>(ck >> a.page_shift) * a.c_page + (ck & mask) * a.c_token) * E;
+#pragma unroll
+                for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int cv = __shfl(code, 16 * u + 4 * g + r);
+                    const int64_t pg = cv >> a.page_shift, slot = cv & mask;
+                    vr[buf][4 * u + r] = load_row<VE * E, E>(vbase + (pg * a.c_page + slot * a.c_token) * E, vo[r], VE * c, a.D);
+                    if constexpr (I8) {
+                        ksc[buf][u][r] = ksb[pg * a.s_page + slot * a.s_token];
+                        vsc[buf][u][r] = vsb[pg * a.s_page + slot * a.s_token];
+                    }
+                }
+            }
+        }
+    };
+    if (!open(t0)) return;
+    load_q();
+    load(0, first_key(i0));
+    for (bool more = true; more;) {
+        const int rt = pair % row_tiles, hq0 = pair / row_tiles * group + 16 * rt;
+        const int rows = group - 16 * rt < 16 ? group - 16 * rt : 16;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int d = I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+            if (c >= rows || d >= a.D) q[s] = Frag{{0, 0, 0, 0}};
             if constexpr (kSplit) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -336,85 +456,6 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
         float m = kNegInf, l = 0.0f;
         bool any = false;           // a key that the query sees (the same for all rows: it is one query's position)
         const float scale = a.scale * kLog2e;
-        const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
-        const char* vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
-        // the lane's places within 16 keys (bytes): key c, chunks 4 x + g; keys 4 g + r, values VE c ..
-        const uint32_t tok = static_cast<uint32_t>(a.c_token) * E;
-        uint32_t ko[KL], vo[4];
-#pragma unroll
-        for (int x = 0; x < KL; ++x) ko[x] = (SMALL ? 0 : c * tok) + (KB / E * (4 * x + g) < a.D ? KB * (4 * x + g) : 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vo[r] = (SMALL ? 0 : (4 * g + r) * tok) + (VE * c < a.D ? VE * E * c : 0);
-        const float* ksb = a.k_scale + (I8 ? h * a.s_head : 0);
-        const float* vsb = a.v_scale + (I8 ? h * a.s_head : 0);
-
-        Raw<KB> kr[2][2][KL];       // [buffer][16-key group][load]
-        Raw<VE * E> vr[2][8];       // [buffer][key]
-        float ksc[2][2][4], vsc[2][2][4];   // int8: scales of the lane's 8 keys
-        uint32_t held[2];           // bit 16 u + x: key x of group u is in a page of the cache
-
-        auto first_key = [&](int i) { return (i < v.ns ? i : v.w0 + (i - v.ns)) * kTile + wave * kKeys; };
-        // the 32 keys from j on: every address is inside the cache (a key that is not held reads page 0)
-        auto load = [&](int buf, int j) __attribute__((always_inline)) {
-            held[buf] = 0;
-            const int ne = static_cast<int>(a.width) - 1;
-            if constexpr (!SMALL) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int at = (j + 16 * u) >> a.page_shift;
-                    const int p = scalar_word(table + (at < ne ? at : ne));
-                    const bool ok = p >= 0 && p <= last_page && at <= ne;
-                    held[buf] |= ok ? 0xffffu << (16 * u) : 0u;
-                    const int pg = ok ? p : 0, slot = (j + 16 * u) & mask;
-                    const int64_t off = (pg * a.c_page + slot * a.c_token) * E;
-                    const char* kp = kbase + off;
-                    const char* vp = vbase + off;
-#pragma unroll
-                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) vr[buf][4 * u + r] = load_row<VE * E, E>(vp, vo[r], VE * c, a.D);
-                    if constexpr (I8) {
-                        const int64_t so = pg * a.s_page + slot * a.s_token;
-                        if (quads) {                    // four keys' scales are one aligned 16 bytes
-                            const float4 x = *reinterpret_cast<const float4*>(ksb + so + 4 * g);
-                            const float4 y = *reinterpret_cast<const float4*>(vsb + so + 4 * g);
-                            ksc[buf][u][0] = x.x; ksc[buf][u][1] = x.y; ksc[buf][u][2] = x.z; ksc[buf][u][3] = x.w;
-                            vsc[buf][u][0] = y.x; vsc[buf][u][1] = y.y; vsc[buf][u][2] = y.z; vsc[buf][u][3] = y.w;
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                ksc[buf][u][r] = ksb[so + (4 * g + r) * a.s_token];
-                                vsc[buf][u][r] = vsb[so + (4 * g + r) * a.s_token];
-                            }
-                        }
-                    }
-                }
-            } else {
-                // lane x (and x + 32) looks up key x of the 32: its row as page << page_shift | slot, or -1
-                const int mine = j + (lane & 31), at = mine >> a.page_shift;
-                const int p = table[at < ne ? at : ne];
-                const bool ok = p >= 0 && p <= last_page && at <= ne;
-                held[buf] = static_cast<uint32_t>(__ballot(ok));
-                const int code = ok ? (p << a.page_shift) | (mine & mask) : 0;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int ck = __shfl(code, 16 * u + c);
-                    const char* kp = kbase + (static_cast<int64_t>(ck >> a.page_shift) * a.c_page + (ck & mask) * a.c_token) * E;
-#pragma unroll
-                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int cv = __shfl(code, 16 * u + 4 * g + r);
-                        const int64_t pg = cv >> a.page_shift, slot = cv & mask;
-                        vr[buf][4 * u + r] = load_row<VE * E, E>(vbase + (pg * a.c_page + slot * a.c_token) * E, vo[r], VE * c, a.D);
-                        if constexpr (I8) {
-                            ksc[buf][u][r] = ksb[pg * a.s_page + slot * a.s_token];
-                            vsc[buf][u][r] = vsb[pg * a.s_page + slot * a.s_token];
-                        }
-                    }
-                }
-            }
-        };
         auto work = [&](int buf, int j) __attribute__((always_inline)) {
             // scores
             f32x4 s[2];
@@ -528,7 +569,6 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             }
         };
 
-        load(0, first_key(i0));
         int i = i0;
         for (; i + 1 < i1; i += 2) {
             load(1, first_key(i + 1));
@@ -538,8 +578,16 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
         }
         if (i < i1) work(0, first_key(i));
         l = sum4(l);
+        // the next segment's first tile and query rows are on their way while this one is written
+        const int cur_b = b, cur_pair = pair, cur_s0 = s0, nt = v.nt;
+        const bool whole = i0 == 0 && i1 == nt;
+        more = open(s0 + i1);
+        if (kAcross && more) {
+            load_q();
+            load(0, first_key(i0));
+        }
 
-        // the four waves' parts together: rows c, values VE (4 g + r) + i
+        // the waves' parts together: rows c, values VE (4 g + r) + i
         __syncthreads();
         if (lane == 0) sm_any[wave] = any;
         if (c < rows) {
@@ -553,11 +601,10 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
                 for (int e = 0; e < VE; ++e) sm_out[wave][c][VE * (4 * g + r) + e] = o[e][r];
         }
         __syncthreads();
-        const bool whole = i0 == 0 && i1 == v.nt;
         int some = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) some |= sm_any[w];
-        const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t != t0);
+        const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < cur_s0);
         for (int e = threadIdx.x; e < rows * DP / 4; e += 64 * kWaves) {
             const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
             if (d >= a.D) continue;
@@ -578,7 +625,7 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             }
             if (whole) {
                 const float inv = some ? 1.0f / sum : 0.0f;     // nothing seen: zeros
-                uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + b * a.o_token +
+                uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + cur_b * a.o_token +
                                                             (hq0 + row) * a.o_head + d);
                 *reinterpret_cast<uint2*>(out) = make_uint2(pack_16x2(x[0] * inv, x[1] * inv, DT),
                                                             pack_16x2(x[2] * inv, x[3] * inv, DT));
@@ -591,13 +638,13 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
         }
         if (!whole) {
             // the sequence's pieces: workgroups p0 .. p1 of the line
-            const int s0 = before + pair * v.nt, p0 = s0 / piece, p1 = (s0 + v.nt - 1) / piece;
+            const int p0 = cur_s0 / piece, p1 = (cur_s0 + nt - 1) / piece;
             // every thread's stores have arrived (they are written through to where the device is coherent) before
             // the workgroup is counted; the count's value says that the others' have too
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
             if (threadIdx.x == 0) {
-                int* count = a.counters + static_cast<int64_t>(b) * per + pair;
+                int* count = a.counters + static_cast<int64_t>(cur_b) * per + cur_pair;
                 const int old = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 // the last one: zero again for the next call
                 if (old == p1 - p0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -605,10 +652,13 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             }
             __syncthreads();
             if (sm_last) {
-                join_pieces<DP, DT>(a, rows, rows_most, slots, s0, piece, p0, p1, b, hq0, &sm_out[0][0][0]);
+                join_pieces<DP, DT>(a, rows, rows_most, slots, cur_s0, piece, p0, p1, cur_b, hq0, &sm_out[0][0][0]);
             }
         }
-        t += i1 - i0;
+        if (!kAcross && more) {
+            load_q();
+            load(0, first_key(i0));
+        }
     }
 }
 
