@@ -554,6 +554,7 @@ int launch_width(const AttnArgs& a, hipStream_t stream) {
     auto kern = attn_prompt_kernel<DP, DT, I8>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(lds)) != hipSuccess) {
+        (void)hipGetLastError();
         set_error("paged_attention: cannot reserve %zu bytes of LDS", lds);
         return -3;
     }

@@ -46,6 +46,8 @@ struct W4Plan {
     int parts;      // rows that a row of x becomes
     int rows_m;     // rows of x per workgroup (blockIdx.y)
     int chunk;      // K values staged at a time
+    int pitch;      // pairs of scale and zero-point a column in LDS
+    int pair_bufs;  // tiles' worth of them
 };
 
 // A stored value of type dt from its bits.
@@ -159,18 +161,34 @@ struct W4Piece {
     }
 };
 
-constexpr int kWaves = 4;
+// Scale and zero-point of a group as LDS holds them: two fp16 in a dword, or two floats.
+template <bool ANY>
+struct W4Pair;
+template <>
+struct W4Pair<false> {
+    uint32_t v;
+    __device__ __forceinline__ float scale() const { return f16_bits_to_f32(static_cast<uint16_t>(v & 0xffffu)); }
+    __device__ __forceinline__ float zero() const { return f16_bits_to_f32(static_cast<uint16_t>(v >> 16)); }
+};
+template <>
+struct W4Pair<true> {
+    float s, z;
+    __device__ __forceinline__ float scale() const { return s; }
+    __device__ __forceinline__ float zero() const { return z; }
+};
 
 // F16: fp16 rows and products, else bf16; Z: zero-points; G: groups of 64 or 128 with fp16 scales and zero-points,
-// or 0: any group and type; RT: 16-row tiles; CT: 16-column tiles; NE: registers of a product that
-// hold rows; KB: 128-value steps in flight.
-template <bool F16, W4Zero Z, int G, int RT, int CT, int NE, int KB>
-__global__ void __launch_bounds__(64 * kWaves, RT * CT >= 4 ? 2 : RT * CT >= 2 ? 3 : 4) w4a16_kernel(W4A16Args a, W4Plan pl) {
-    static_assert(RT == 1 || NE == 4, "more rows than a product has fill all its registers");
+// or 0: any group and type; CT: 16-column tiles; NE: registers of a product that hold rows (1: up to 4 rows, 4: up to
+// 16); KB: 128-value steps in flight; W: waves.
+template <bool F16, W4Zero Z, int G, int CT, int NE, int KB, int W>
+__global__ void __launch_bounds__(64 * W, W == 8 ? 2 : CT == 2 ? 3 : 4)
+w4a16_kernel(W4A16Args a, W4Plan pl) {
     constexpr bool ANY = G == 0;
     constexpr int kScales = ANY ? 4 : kBlk / G;         // scales that a step uses (any: the same ones again for larger groups)
-    constexpr int kHeld = ANY ? 4 : 1;                  // registers that hold them: two fp16 scales in one
     constexpr bool kSum = !F16 || Z == W4Zero::Float;   // the sum of x is needed
+    constexpr int kCols = 16 * CT;
+    constexpr bool kThrough = W == 8;                   // a workgroup goes through several tiles
+    using Pair = W4Pair<ANY>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -179,89 +197,119 @@ __global__ void __launch_bounds__(64 * kWaves, RT * CT >= 4 ? 2 : RT * CT >= 2 ?
     const int rows = static_cast<int>(a.M - m0 < pl.rows_m ? a.M - m0 : pl.rows_m);
     const int all = rows * pl.parts;                    // staged rows
     const int stride = pl.chunk + kPad;
+    const int gshift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7;
+    const int groups = K >> gshift, pitch = pl.pitch;
     uint16_t* xs = reinterpret_cast<uint16_t*>(lds);
-    uint16_t* zero = xs + pl.rows_m * pl.parts * stride;   // 16 bytes of zeros: the rows of a product that are not there
-    if (threadIdx.x < 8) zero[threadIdx.x] = 0;
+    Pair* pairs = reinterpret_cast<Pair*>(xs + pl.rows_m * pl.parts * stride);          // [pair_bufs][column][pitch]
+    float* red = reinterpret_cast<float*>(pairs + pl.pair_bufs * kCols * pitch);                // [wave][row][column]
 
     // loads complete in the order of their issue: the first piece of x ahead of the weights, so that x is
     // staged while the weights are on their way
     const int pieces = rows * (pl.chunk / (a.hblock ? 1024 : 8));
-    const int mine = a.hblock ? wave : static_cast<int>(threadIdx.x), step = a.hblock ? kWaves : 64 * kWaves;
-    W4Piece piece;
-    piece.load(a, pl, m0, mine, pieces, 0);
+    const int mine = a.hblock ? wave : static_cast<int>(threadIdx.x), step = a.hblock ? W : 64 * W;
+    constexpr int PB = kThrough ? 4 : 1;                // pieces a thread has in flight
+    W4Piece piece[PB];
+#pragma unroll
+    for (int i = 0; i < PB; ++i) piece[i].load(a, pl, m0, mine + i * step, pieces, 0);
     __builtin_amdgcn_sched_barrier(0);
 
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16 * CT;
-    // addresses as a scalar base and a 32-bit offset of the lane: its column's, within the workgroup's
-    const char* wbase = reinterpret_cast<const char*>(a.qw) + n0 * a.ldw;
-    const char* sbase = static_cast<const char*>(a.ws) + n0 * a.ldws * (ANY && a.s_dtype == kDtF32 ? 4 : 2);
-    const char* zbase = static_cast<const char*>(a.wz) +
-                        n0 * a.ldwz * (Z == W4Zero::U4 ? 1 : ANY && a.z_dtype == kDtF32 ? 4 : 2);
-    uint32_t wo[CT], so[CT], zo[CT];
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int left = static_cast<int>(a.N - 1 - n0 < 16 * CT ? a.N - 1 - n0 : 16 * CT);
-        const uint32_t col = 16 * t + c < left ? 16 * t + c : left;       // columns past N read the last one's weights
-        wo[t] = col * static_cast<uint32_t>(a.ldw);
-        so[t] = col * static_cast<uint32_t>(a.ldws);
-        zo[t] = col * static_cast<uint32_t>(a.ldwz);
-    }
-    const int gshift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7;
+    const int tiles = static_cast<int>((a.N + kCols - 1) / kCols);
     const uint32_t last = static_cast<uint32_t>(K / 2 - 16);
     uint4 w[KB][CT];
-    uint32_t sb[KB][CT][kHeld], zb[KB][CT][kHeld];      // scales and zero-points as they are stored
-    const int groups = K >> gshift;
-    // step `blk` (128 values) into ring place i; past the end of K the last values
-    auto fetch = [&](int i, int blk) __attribute__((always_inline)) {
+    // step `blk` (128 values) of tile `tile` into ring place i; past the end of K the last values
+    auto fetch = [&](int i, int tile, int blk) __attribute__((always_inline)) {
+        const int64_t n0 = static_cast<int64_t>(tile) * kCols;
+        // the address as a scalar base and a 32-bit offset of the lane: its column's, within the tile
+        const char* base = reinterpret_cast<const char*>(a.qw) + n0 * a.ldw;
         const uint32_t at = static_cast<uint32_t>(blk) * (kBlk / 2) + 16 * g;
         const uint32_t kk = at < last ? at : last;
+        const int left = static_cast<int>(a.N - 1 - n0 < kCols ? a.N - 1 - n0 : kCols);
 #pragma unroll
-        for (int t = 0; t < CT; ++t) w[i][t] = *reinterpret_cast<const uint4*>(wbase + (wo[t] + kk));
-        auto half = [](const char* base, int64_t at, uint32_t o) __attribute__((always_inline)) {
-            return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(base + 2 * at + 2 * o));
-        };
-        if constexpr (ANY) {
-            // one branch on a type around all its loads: inside a branch each, they would be waited for one by one
-            auto each = [&](auto&& f) __attribute__((always_inline)) {
-#pragma unroll
-                for (int s = 0; s < kScales; ++s) {
-                    const int ks = blk * kBlk + s * (kBlk / kScales);
-                    const int gi = (ks < K ? ks : K - 1) >> gshift;
-#pragma unroll
-                    for (int t = 0; t < CT; ++t) f(t, s, gi);
-                }
-            };
-            auto word = [](const char* base, int64_t at, uint32_t o) __attribute__((always_inline)) {
-                return *reinterpret_cast<const uint32_t*>(base + 4 * at + 4 * o);
-            };
-            if (a.s_dtype != kDtF32) each([&](int t, int s, int gi) { sb[i][t][s] = half(sbase, gi, so[t]); });
-            else each([&](int t, int s, int gi) { sb[i][t][s] = word(sbase, gi, so[t]); });
-            if constexpr (Z == W4Zero::U4) {
-                each([&](int t, int s, int gi) { zb[i][t][s] = *reinterpret_cast<const uint8_t*>(zbase + (gi >> 1) + zo[t]); });
-            } else if constexpr (Z == W4Zero::Float) {
-                if (a.z_dtype != kDtF32) each([&](int t, int s, int gi) { zb[i][t][s] = half(zbase, gi, zo[t]); });
-                else each([&](int t, int s, int gi) { zb[i][t][s] = word(zbase, gi, zo[t]); });
-            }
-        } else {
-            // both scales of a step in one dword (an odd last group's alone); its uint4 zero-points are one byte
-            const int gi = blk * kScales < groups ? blk * kScales : groups - 1;
-            auto pair = [&](const char* base, uint32_t o) __attribute__((always_inline)) {
-                if (kScales == 1 || gi + 1 >= groups) return half(base, gi, o);
-                uint32_t v;
-                __builtin_memcpy(&v, base + 2 * static_cast<int64_t>(gi) + 2 * o, 4);
-                return v;
-            };
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                sb[i][t][0] = pair(sbase, so[t]);
-                if constexpr (Z == W4Zero::U4) zb[i][t][0] = *reinterpret_cast<const uint8_t*>(zbase + (gi >> 1) + zo[t]);
-                else if constexpr (Z == W4Zero::Float) zb[i][t][0] = pair(zbase, zo[t]);
+        for (int t = 0; t < CT; ++t) {
+            const uint32_t col = 16 * t + c < left ? 16 * t + c : left;   // columns past N read the last one's weights
+            w[i][t] = *reinterpret_cast<const uint4*>(base + (col * static_cast<uint32_t>(a.ldw) + kk));
+        }
+    };
+    // each wave a run of consecutive steps of every chunk, so that it reads whole cache lines of a column; a tile's
+    // last step is followed by the next tile's first
+    const int blocks = (K + kBlk - 1) / kBlk, per = (pl.chunk / kBlk + W - 1) / W;
+    int f_tile = blockIdx.x, f_blk = wave * per, f_left = per;   // the next step to fetch, and the steps left in its run
+    auto fetch_next = [&](int i) __attribute__((always_inline)) {
+        if ((!kThrough || f_tile < tiles) && f_blk < blocks) fetch(i, f_tile, f_blk);
+        ++f_blk;
+        if (--f_left == 0) {
+            f_blk += pl.chunk / kBlk - per;
+            f_left = per;
+            if (kThrough && f_blk - wave * per >= blocks) {   // the runs of the last chunk are done
+                f_blk = wave * per;
+                f_tile += gridDim.x;
             }
         }
     };
-    const int blocks = (K + kBlk - 1) / kBlk;
 #pragma unroll
-    for (int i = 0; i < KB; ++i) fetch(i, wave + i * kWaves);
+    for (int i = 0; i < KB; ++i) fetch_next(i);
+
+    // A tile's scales and zero-points are read along the columns' rows, a pair of groups a load (one by one through the
+    // products' lanes they would cost as many cache lines as the weights do), and go to LDS: kAhead loads a thread
+    // ahead of the work before them, the rest (many groups) when they are stored.
+    constexpr int kAhead = CT == 2 ? 3 : 2;
+    const int halves = (groups + 1) / 2, items = kCols * halves;
+    uint32_t sb[kAhead], zb[kAhead];
+    auto load_item = [&](int tile, int e, uint32_t* s, uint32_t* z) __attribute__((always_inline)) {
+        const int64_t n0 = static_cast<int64_t>(tile) * kCols;
+        const int at = e < items ? e : 0, col = at / halves, gi = 2 * (at - col * halves);
+        const int64_t n = n0 + col < a.N ? n0 + col : a.N - 1;
+        const int g0 = gi + 1 < groups ? gi : groups - 2;   // an odd last group behind the one before it (there are two)
+        __builtin_memcpy(s, static_cast<const uint16_t*>(a.ws) + n * a.ldws + g0, 4);
+        if constexpr (Z == W4Zero::U4) *z = static_cast<const uint8_t*>(a.wz)[n * a.ldwz + (gi >> 1)];
+        if constexpr (Z == W4Zero::Float) __builtin_memcpy(z, static_cast<const uint16_t*>(a.wz) + n * a.ldwz + g0, 4);
+    };
+    auto store_item = [&](int e, uint32_t s, uint32_t z, Pair* to) __attribute__((always_inline)) {
+        if constexpr (!ANY) {
+            if (e >= items) return;
+            const int col = e / halves, gi = 2 * (e - col * halves);
+            uint32_t z0 = 0, z1 = 0;
+            const bool odd = gi + 1 >= groups;
+            if (odd) s >>= 16;
+            if constexpr (Z == W4Zero::U4) {
+                z0 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(z & 15));
+                z1 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(z >> 4));
+            } else if constexpr (Z == W4Zero::Float) {
+                if (odd) z >>= 16;
+                z0 = z & 0xffffu;
+                z1 = z >> 16;
+            }
+            *reinterpret_cast<uint2*>(to + col * pitch + gi) = make_uint2((s & 0xffffu) | z0 << 16, s >> 16 | z1 << 16);
+        }
+    };
+    auto load_pairs = [&](int tile) __attribute__((always_inline)) {
+        if constexpr (!ANY)
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) load_item(tile, threadIdx.x + i * 64 * W, sb + i, zb + i);
+    };
+    auto store_pairs = [&](int tile, Pair* to) __attribute__((always_inline)) {
+        if constexpr (!ANY) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) store_item(threadIdx.x + i * 64 * W, sb[i], zb[i], to);
+            for (int e = threadIdx.x + kAhead * 64 * W; e < items; e += 64 * W) {
+                uint32_t s, z = 0;
+                load_item(tile, e, &s, &z);
+                store_item(e, s, z, to);
+            }
+        } else {
+            const int64_t n0 = static_cast<int64_t>(tile) * kCols;
+            for (int e = threadIdx.x; e < kCols * groups; e += 64 * W) {
+                const int col = e / groups, gi = e - col * groups;
+                const int64_t n = n0 + col < a.N ? n0 + col : a.N - 1;
+                Pair p;
+                p.s = load_as_f32(a.ws, a.s_dtype, n * a.ldws + gi);
+                p.z = Z == W4Zero::U4 ? static_cast<float>((static_cast<const uint8_t*>(a.wz)[n * a.ldwz + (gi >> 1)] >> (4 * (gi & 1))) & 15)
+                      : Z == W4Zero::Float ? load_as_f32(a.wz, a.z_dtype, n * a.ldwz + gi) : 0.0f;
+                to[col * pitch + gi] = p;
+            }
+        }
+    };
+    load_pairs(blockIdx.x);
     __builtin_amdgcn_sched_barrier(0);
 
     // and-or takes one constant from a scalar register and one from a vector register, none from the instruction
@@ -271,22 +319,12 @@ __global__ void __launch_bounds__(64 * kWaves, RT * CT >= 4 ? 2 : RT * CT >= 2 ?
     constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
     const W4Frag ones{{kOne, kOne, kOne, kOne}};
 
-    w4_f32x4 y[RT][CT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int t = 0; t < CT; ++t) y[r][t] = w4_f32x4{0, 0, 0, 0};
+    w4_f32x4 y[CT];
     // row c of a product is row 4 (c % 4) + c / 4 of the tile
-    const uint16_t* xrow[RT];
-    bool there[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int row = 16 * r + 4 * (c & 3) + (c >> 2);
-        there[r] = row < all;
-        xrow[r] = there[r] ? xs + row * stride + 8 * g : zero;
-    }
+    const int row_c = 4 * (c & 3) + (c >> 2);
+    const uint16_t* xrow = xs + (row_c < all ? row_c : 0) * stride + 8 * g;   // a row that is not there: not stored either
 
-    auto compute = [&](int i, int blk, int k0) __attribute__((always_inline)) {
+    auto compute = [&](int i, int blk, int k0, const Pair* pr) __attribute__((always_inline)) {
         const int gb = blk * kBlk;
         uint32_t v[CT][4];
 #pragma unroll
@@ -302,35 +340,22 @@ __global__ void __launch_bounds__(64 * kWaves, RT * CT >= 4 ? 2 : RT * CT >= 2 ?
 #pragma unroll
         for (int s = 0; s < kScales; ++s) {
             float sc[CT], zp[CT];
-            const int gi = (gb + s * (kBlk / kScales)) >> gshift;
+            // a step that K ends in: its missing group's pair is not there, any will do (its x is zeros)
+            const int ks = gb + s * (kBlk / kScales), gi = (ks < K ? ks : K - 1) >> gshift;
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
-                if constexpr (ANY) {
-                    sc[t] = as_float(sb[i][t][s], a.s_dtype);
-                    if constexpr (Z == W4Zero::Float) zp[t] = as_float(zb[i][t][s], a.z_dtype);
-                } else {
-                    sc[t] = as_float(sb[i][t][0] >> (16 * s), kDtF16);
-                    if constexpr (Z == W4Zero::Float) zp[t] = as_float(zb[i][t][0] >> (16 * s), kDtF16);
-                }
-                if constexpr (Z == W4Zero::Signed) zp[t] = 8.0f;
-                else if constexpr (Z == W4Zero::U4) zp[t] = static_cast<float>((zb[i][t][ANY ? s : 0] >> (4 * (gi & 1))) & 15);
+                const Pair p = pr[(16 * t + c) * pitch + gi];
+                sc[t] = p.scale();
+                zp[t] = Z == W4Zero::Signed ? 8.0f : p.zero();
             }
-            w4_f32x4 acc[RT][CT], sum[RT];
+            w4_f32x4 acc[CT], sum = w4_f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                sum[r] = w4_f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < CT; ++t) acc[r][t] = w4_f32x4{0, 0, 0, 0};
-            }
+            for (int t = 0; t < CT; ++t) acc[t] = w4_f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int jj = 0; jj < 4 / kScales; ++jj) {
                 const int j = s * (4 / kScales) + jj;
-                W4Frag x[RT];
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(xrow[r] + (there[r] ? xo + 32 * j : 0));
-                    x[r] = W4Frag{{q.x, q.y, q.z, q.w}};
-                }
+                const uint4 q = *reinterpret_cast<const uint4*>(xrow + xo + 32 * j);
+                const W4Frag x{{q.x, q.y, q.z, q.w}};
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
                     W4Frag f;
@@ -344,104 +369,131 @@ __global__ void __launch_bounds__(64 * kWaves, RT * CT >= 4 ? 2 : RT * CT >= 2 ?
                         for (int e = 0; e < 4; ++e)
                             f.w[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(mq_f16x2, f.w[e]) + off2);
                     }
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[r][t] = w4_mfma<F16>(x[r], f, acc[r][t]);
+                    acc[t] = w4_mfma<F16>(x, f, acc[t]);
                 }
-                if constexpr (kSum)
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) sum[r] = w4_mfma<F16>(x[r], ones, sum[r]);
+                if constexpr (kSum) sum = w4_mfma<F16>(x, ones, sum);
             }
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
                 const float off = -128.0f - (Z == W4Zero::Float ? 0.0f : zp[t]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int e = 0; e < NE; ++e) {
-                        const float d = F16 ? acc[r][t][e] : __builtin_fmaf(off, sum[r][e], acc[r][t][e]);
-                        y[r][t][e] = __builtin_fmaf(sc[t], d, y[r][t][e]);
-                        if constexpr (Z == W4Zero::Float) y[r][t][e] = __builtin_fmaf(zp[t], sum[r][e], y[r][t][e]);
-                    }
+                for (int e = 0; e < NE; ++e) {
+                    const float d = F16 ? acc[t][e] : __builtin_fmaf(off, sum[e], acc[t][e]);
+                    y[t][e] = __builtin_fmaf(sc[t], d, y[t][e]);
+                    if constexpr (Z == W4Zero::Float) y[t][e] = __builtin_fmaf(zp[t], sum[e], y[t][e]);
+                }
             }
         }
     };
 
-    for (int k0 = 0; k0 < K; k0 += pl.chunk) {
-        if (k0 > 0) {
-            __syncthreads();                            // the last chunk has been read
-            piece.load(a, pl, m0, mine, pieces, k0);
-        }
-        for (int e = mine; e < pieces; e += step) {
-            if (e != mine) piece.load(a, pl, m0, e, pieces, k0);
-            piece.store(a, pl, xs, stride);
-        }
-        __syncthreads();
-        const int b0 = k0 / kBlk, b1 = b0 + pl.chunk / kBlk < blocks ? b0 + pl.chunk / kBlk : blocks;
-        for (int b = b0; b < b1; b += kWaves * KB) {
+    // A workgroup of eight waves takes every gridDim.x-th tile; x is staged once if it fits (one chunk), else for every tile anew.
+    store_pairs(blockIdx.x, pairs);
+    bool staged = false;
+    int buf = 0;
+    int tile = blockIdx.x;
+    do {
+        const Pair* pr = pairs + buf * kCols * pitch;
+        const bool more = kThrough && tile + static_cast<int>(gridDim.x) < tiles;
+        if (more) load_pairs(tile + gridDim.x);
 #pragma unroll
-            for (int i = 0; i < KB; ++i) {
-                const int blk = b + wave + i * kWaves;
-                if (blk < b1) compute(i, blk, k0);
-                if (blk + kWaves * KB < blocks) fetch(i, blk + kWaves * KB);
+        for (int t = 0; t < CT; ++t) y[t] = w4_f32x4{0, 0, 0, 0};
+        for (int k0 = 0; k0 < K; k0 += pl.chunk) {
+            if (!staged) {
+                if (k0 > 0 || (kThrough && tile != static_cast<int>(blockIdx.x))) {
+                    __syncthreads();                    // the last chunk has been read
+#pragma unroll
+                    for (int i = 0; i < PB; ++i) piece[i].load(a, pl, m0, mine + i * step, pieces, k0);
+                }
+                for (int e = mine; e < pieces; e += PB * step) {
+                    if (e != mine)
+#pragma unroll
+                        for (int i = 0; i < PB; ++i) piece[i].load(a, pl, m0, e + i * step, pieces, k0);
+#pragma unroll
+                    for (int i = 0; i < PB; ++i)
+                        if (e + i * step < pieces) piece[i].store(a, pl, xs, stride);
+                }
+                __syncthreads();
+                staged = pl.chunk >= K;
+            }
+            const int b0 = k0 / kBlk + wave * per, chunk_end = (k0 + pl.chunk) / kBlk;
+            const int b1 = b0 + per < chunk_end ? b0 + per : chunk_end, b2 = b1 < blocks ? b1 : blocks;
+            for (int b = b0; b < b0 + per; b += KB) {
+#pragma unroll
+                for (int i = 0; i < KB; ++i) {
+                    if (b + i < b2) compute(i, b + i, k0, pr);
+                    if (b + i < b0 + per) fetch_next(i);
+                }
             }
         }
-    }
-    // the waves' sums: [wave][row][column]
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(lds);
-    constexpr int kCols = 16 * CT;
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
+        if (more) store_pairs(tile + gridDim.x, pairs + (buf ^ 1) * kCols * pitch);
+        // the waves' sums, once the last tile's have been read
+        __syncthreads();
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                const int row = 16 * r + 4 * e + g;
-                if (row < all) red[(wave * all + row) * kCols + 16 * t + c] = y[r][t][e];
-            }
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows * kCols; e += 64 * kWaves) {
-        const int m = e / kCols, cc = e % kCols;
-        const int64_t n = n0 + cc;
-        if (n >= a.N) continue;
-        float s = 0.0f;
-        for (int p = 0; p < pl.parts; ++p)
+            for (int e = 0; e < NE; ++e)
+                if (4 * e + g < all) red[(wave * all + 4 * e + g) * kCols + 16 * t + c] = y[t][e];
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * kCols; e += 64 * W) {
+            const int m = e / kCols, cc = e % kCols;
+            const int64_t n = static_cast<int64_t>(tile) * kCols + cc;
+            if (n >= a.N) continue;
+            float s = 0.0f;
+            for (int p = 0; p < pl.parts; ++p)
 #pragma unroll
-            for (int wv = 0; wv < kWaves; ++wv) s += red[(wv * all + m * pl.parts + p) * kCols + cc];
-        if (a.bias) s += load_as_f32(a.bias, a.bias_dtype, n);
-        store_from_f32(a.y, a.y_dtype, (m0 + m) * a.ldy + n, s);
-    }
+                for (int wv = 0; wv < W; ++wv) s += red[(wv * all + m * pl.parts + p) * kCols + cc];
+            if (a.bias) s += load_as_f32(a.bias, a.bias_dtype, n);
+            store_from_f32(a.y, a.y_dtype, (m0 + m) * a.ldy + n, s);
+        }
+        tile += gridDim.x;
+        buf ^= 1;
+    } while (kThrough && tile < tiles);
 }
 
-template <bool F16, W4Zero Z, int G, int RT, int CT, int NE>
+template <bool F16, W4Zero Z, int G, int CT, int NE, int W>
 int launch_tiles(const W4A16Args& a, W4Plan pl, hipStream_t stream) {
-    constexpr int KB = RT == 1 && NE == 1 ? (G == 0 ? 3 : 4) : RT == 1 ? 2 : 1;
-    constexpr int round = kWaves * KB * kBlk;           // values of K that the waves' rings cover
+    constexpr int KB = CT == 2 ? 3 : 4;
+    constexpr int64_t kLds = 163840;                    // of a compute unit
     const int unit = a.hblock ? 1024 : kBlk;
-    const int rows = pl.rows_m * pl.parts;
-    // all of K if 40 KB hold it (four workgroups a compute unit), else whole rounds of the rings
+    const int64_t tiles = (a.N + 16 * CT - 1) / (16 * CT);
+    const int cus = device_cu_count();
+    pl.pitch = static_cast<int>((a.K / a.group + 1) / 4 * 4 + 2);   // even, and 16 columns on different banks
+    const bool through = W == 8 && tiles > cus && cus > 0 && 2 * 16 * CT * pl.pitch * sizeof(W4Pair<G == 0>) < kLds / 2;
+    const int64_t groups = through ? cus : tiles;
+    pl.pair_bufs = groups < tiles ? 2 : 1;
+    const int64_t pairs = static_cast<int64_t>(pl.pair_bufs) * 16 * CT * pl.pitch * sizeof(W4Pair<G == 0>);
+    int step = W * KB * kBlk;                           // x a chunk at a time: whole rounds of the rings and whole pieces
+    while (step % unit) step += W * KB * kBlk;
     const int64_t all = (a.K + unit - 1) / unit * unit;
-    int64_t chunk = all;
-    if (2 * rows * chunk > 40960) {
-        int step = round;                               // whole rounds and whole pieces of x
-        while (step % unit) step += round;
-        chunk = 40960 / (2 * rows) / step * step;
-        if (chunk < step) chunk = step;
-        if (chunk > all) chunk = all;
+    int64_t lds = 0;
+    for (;; pl.rows_m = (pl.rows_m + 1) / 2) {
+        const int64_t rows = pl.rows_m * pl.parts, red = W * rows * 16 * CT * 4;
+        // all of K if the workgroup's share of LDS holds it (W = 8: one workgroup a compute unit; else four)
+        int64_t room = W == 8 ? kLds : 40960;
+        if (room > kLds - pairs - red) room = kLds - pairs - red;
+        int64_t chunk = all;
+        if (rows * (chunk + kPad) * 2 > room) {
+            chunk = (room / (2 * rows) - kPad) / step * step;
+            if (chunk < step) chunk = step;
+            if (chunk > all) chunk = all;
+        }
+        pl.chunk = static_cast<int>(chunk);
+        lds = rows * (chunk + kPad) * 2 + pairs + red;
+        if (lds <= kLds) break;
+        if (pl.rows_m == 1) {
+            set_error("w4a16: %lld bytes of LDS for K=%lld", (long long)lds, (long long)a.K);
+            return -2;
+        }
     }
-    pl.chunk = static_cast<int>(chunk);
-    const size_t stage = static_cast<size_t>(rows) * (chunk + kPad) * 2 + 16;
-    const size_t red = static_cast<size_t>(kWaves) * rows * 16 * CT * 4;
-    const size_t lds = stage > red ? stage : red;
-    auto kern = w4a16_kernel<F16, Z, G, RT, CT, NE, KB>;
+    auto kern = w4a16_kernel<F16, Z, G, CT, NE, KB, W>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(lds)) != hipSuccess) {
-        set_error("w4a16: cannot reserve %zu bytes of LDS", lds);
+        (void)hipGetLastError();
+        set_error("w4a16: cannot reserve %lld bytes of LDS", (long long)lds);
         return -3;
     }
-    const dim3 grid(static_cast<unsigned>((a.N + 16 * CT - 1) / (16 * CT)),
-                    static_cast<unsigned>((a.M + pl.rows_m - 1) / pl.rows_m));
-    hipLaunchKernelGGL(kern, grid, dim3(64 * kWaves), lds, stream, a, pl);
+    const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>((a.M + pl.rows_m - 1) / pl.rows_m));
+    hipLaunchKernelGGL(kern, grid, dim3(64 * W), lds, stream, a, pl);
     return launch_status("w4a16");
 }
 
@@ -451,25 +503,23 @@ int launch_rows(const W4A16Args& a, hipStream_t stream) {
     // fp32 rows (and rotated rows for an fp32 output) need three bf16 parts; rotated 16-bit rows that are rounded
     // to 16 bits again two: 16 bits of every rotated value, an error of 2^-16 of it against the output's 2^-8
     pl.parts = a.x_dtype == kDtF32 || (a.hblock && a.y_dtype == kDtF32) ? 3 : a.hblock ? 2 : 1;
-    const int most = 64 / pl.parts;
+    const int most = 16 / pl.parts;                     // a product's rows; more go to another blockIdx.y
     pl.rows_m = static_cast<int>(a.M < most ? a.M : most);
-    const int rows = pl.rows_m * pl.parts, rt = (rows + 15) / 16;
     const int cus = device_cu_count();
-    // two column tiles a workgroup read the staged rows half as often; one where that would leave units idle
-    const bool two = G != 0 && (a.N + 31) / 32 >= 2 * (cus > 0 ? cus : 256);
-    if (rows <= 4) return launch_tiles<F16, Z, G, 1, 1, 1>(a, pl, stream);
-    if (rt <= 1) return launch_tiles<F16, Z, G, 1, 1, 4>(a, pl, stream);
-    if constexpr (G != 0) {
-        if (rt == 2 && two) return launch_tiles<F16, Z, G, 2, 2, 4>(a, pl, stream);
-        if (rt > 2 && two) return launch_tiles<F16, Z, G, 4, 2, 4>(a, pl, stream);
+    if (pl.rows_m * pl.parts <= 4) {
+        // two column tiles a workgroup stage x half as often; one where that would leave units idle
+        if constexpr (G != 0)
+            if ((a.N + 31) / 32 >= 2 * (cus > 0 ? cus : 256)) return launch_tiles<F16, Z, G, 2, 1, 4>(a, pl, stream);
+        return launch_tiles<F16, Z, G, 1, 1, 4>(a, pl, stream);
     }
-    return rt == 2 ? launch_tiles<F16, Z, G, 2, 1, 4>(a, pl, stream) : launch_tiles<F16, Z, G, 4, 1, 4>(a, pl, stream);
+    // more rows: one workgroup a compute unit keeps all of x in LDS and goes through the tiles
+    return launch_tiles<F16, Z, G, 1, 4, 8>(a, pl, stream);
 }
 
 template <bool F16>
 int launch_kind(const W4A16Args& a, hipStream_t stream) {
     const bool any = a.group == 32 || a.s_dtype != kDtF16 || (a.zero == W4Zero::Float && a.z_dtype != kDtF16);
-    const int g = any ? 0 : a.group;
+    const int g = any || a.K < 2 * a.group ? 0 : a.group;   // pairs of groups are read together
     auto go = [&](auto z) {
         constexpr W4Zero Z = decltype(z)::value;
         return g == 0 ? launch_rows<F16, Z, 0>(a, stream) : g == 64 ? launch_rows<F16, Z, 64>(a, stream)

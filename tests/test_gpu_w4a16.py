@@ -65,6 +65,20 @@ def test_long_rows(gpu_device, k, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,group,dtype", [(16, 4500, 16384, 64, torch.bfloat16), (16, 4500, 8192, 32, torch.float16),
+                                               (4, 10000, 32768, 32, torch.float32), (9, 8300, 4096, 128, torch.float16)])
+def test_many_columns(gpu_device, m, n, k, group, dtype):
+    """More columns than the compute units take at once, rows that do not fit LDS together with their scales."""
+    print(f"[w4a16] {m}x{n}x{k} group {group} {dtype}", flush=True)
+    qw, ws, wz = _weights(n, k, group, "float" if group == 128 else "u4", gpu_device)
+    x = torch.randn((m, k), device=gpu_device).to(dtype)
+    y = ck.w4a16_linear(x, qw, ws, wz, group_size=group)
+    at = torch.cat([torch.arange(40), torch.arange(n // 2, n // 2 + 40), torch.arange(n - 40, n)]).to(gpu_device)
+    _check(x, qw[at], ws[at], wz[at], None, y[:, at], group, 0)
+    assert torch.isfinite(y.float()).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("sdt", [torch.bfloat16, torch.float32])
 def test_types(gpu_device, out, sdt):
