@@ -70,10 +70,24 @@ struct __attribute__((aligned(16))) Lds {
     uint16_t k[2][kTile * DP];
     uint16_t v[2][DP * kTile];
     float ks[2][kTile], vs[2][kTile];
-    int code[3][kTile];        // a key's row: page << page_shift | slot, or -1
+    int64_t at[3][kTile];      // 16-bit caches: where a key's row begins (bytes; of a key that is not held: 0)
+    int code[3][kTile];        // int8 caches: page << page_shift | slot, or -1
     uint64_t held[3];          // bit x: key x is in a page of the cache
     int wild;                  // an edge tile's values hold an infinity or NaN
 };
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v* LdsShort4;
+
+// Sixteen bytes per active lane from `src` to LDS bytes dst + 16 lane (dst the same in all lanes). Written as asm: the
+// compiler would wait for the builtin's stores before any LDS read that it cannot tell apart.
+__device__ __forceinline__ void load_lds16(const char* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache.
 template <int DP, int DT, bool I8>
@@ -150,7 +164,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     const int64_t last = pos_hi < cap ? pos_hi : cap - 1;
     int ns = 0, nt = 0;
     int64_t w0 = 0;
-    if (last >= 0) {
+    if (last >= 0 && a.pages > 0) {
         const int64_t start = first_of(pos_lo);
         w0 = start / kTile;
         const int64_t first = sinks < last + 1 ? sinks : last + 1;
@@ -200,7 +214,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
     const char* vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
     const int mask = (1 << a.page_shift) - 1;
-    const int vg = tid >> 4, vc = tid & 15;             // V staging: keys 4 vg .. 4 vg + 3, values VE vc ..
+    const int vg = tid >> 4, vc = tid & 15;             // V staging (int8): keys 4 vg .. 4 vg + 3, values VE vc ..
 
     // rows of tile i's keys (wave 0; lane x looks up key x)
     auto look_up = [&](int i) -> int {
@@ -212,14 +226,50 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     };
     auto put_codes = [&](int ring, int code) {
         const uint64_t held = __ballot(code >= 0);
-        sm.code[ring][lane] = code;
+        if constexpr (I8)
+            sm.code[ring][lane] = code;
+        else
+            sm.at[ring][lane] = code < 0 ? 0 : 2 * (static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token);
         if (lane == 0) sm.held[ring] = held;
     };
 
-    uint4 kr[KC];
-    uint32_t vr[4][VW];
+    uint4 kr[I8 ? KC : 1];
+    uint32_t vr[I8 ? 4 : 1][VW];
     float sc = 0.0f;
-    // the tile whose codes are in sm.code[ring] into registers (a key that is not held: zeros)
+    // 16-bit caches: keys and values of the tile in sm.at[ring] straight into half `buf`, rows as they are, 16-byte
+    // chunk c of key k at c ^ kswap(k) and c ^ vswap(k). What is wider than the heads is not written (the keys' zeros stay).
+    const int slot = tid % kPerKey;
+    auto kswap = [](int key) { return key & 7; };
+    auto vswap = [](int key) { return DP == 64 ? 4 * (key >> 1 & 1) : 4 * (key & 3); };
+    const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_offset(sm.k[0]) + wave * 1024);
+    const uint32_t lds_v = __builtin_amdgcn_readfirstlane(lds_offset(sm.v[0]) + wave * 1024);
+    auto fetch = [&](int ring, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KC; ++x) {
+            const int key = (tid + 256 * x) / kPerKey, kc = slot ^ kswap(key), vc = slot ^ vswap(key);
+            const int64_t at = sm.at[ring][key];
+            const uint32_t to = buf * kTile * DP * 2 + 4096 * x;
+            if (8 * kc < a.D) load_lds16(kbase + at + 16 * kc, lds_k + to);
+            if (8 * vc < a.D) load_lds16(vbase + at + 16 * vc, lds_v + to);
+        }
+    };
+    // this thread's own values of half `buf`: infinities and NaN become 0 and are noted
+    auto tame_own = [&](int buf) {
+#pragma unroll
+        for (int x = 0; x < KC; ++x) {
+            uint4* p = reinterpret_cast<uint4*>(sm.v[buf]) + tid + 256 * x;
+            const uint4 y = *p;
+            bool bad = has_wild<DT>(y.x);
+            bad |= has_wild<DT>(y.y);
+            bad |= has_wild<DT>(y.z);
+            bad |= has_wild<DT>(y.w);
+            if (bad) {
+                sm.wild = 1;
+                *p = make_uint4(tame<DT>(y.x), tame<DT>(y.y), tame<DT>(y.z), tame<DT>(y.w));
+            }
+        }
+    };
+    // int8 caches: the tile whose codes are in sm.code[ring] into registers (a key that is not held: zeros)
     auto load = [&](int ring) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < KC; ++x) {
@@ -227,20 +277,16 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             const int code = sm.code[ring][key];
             kr[x] = make_uint4(0, 0, 0, 0);
             if (code >= 0 && d < a.D) {
-                const char* p = kbase + (static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + d) * E;
-                if constexpr (I8) {
-                    const uint2 y = *reinterpret_cast<const uint2*>(p);
-                    kr[x].x = y.x;
-                    kr[x].y = y.y;
-                } else {
-                    kr[x] = *reinterpret_cast<const uint4*>(p);
-                }
+                const uint2 y = *reinterpret_cast<const uint2*>(
+                    kbase + static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + d);
+                kr[x].x = y.x;
+                kr[x].y = y.y;
             }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int code = sm.code[ring][4 * vg + r];
-            const char* p = vbase + (static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + VE * vc) * E;
+            const char* p = vbase + static_cast<int64_t>(code >> a.page_shift) * a.c_page + (code & mask) * a.c_token + VE * vc;
 #pragma unroll
             for (int w = 0; w < VW; ++w) vr[r][w] = 0;
             if (code >= 0 && VE * vc < a.D) {
@@ -251,79 +297,49 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
                     vr[r][0] = y.x;
                     vr[r][1] = y.y;
                 } else {
-#pragma unroll
-                    for (int w = 0; w < VW / 4; ++w) {
-                        if (w > 0 && VE * vc + 16 / E * w >= a.D) break;
-                        const uint4 y = *reinterpret_cast<const uint4*>(p + 16 * w);
-                        vr[r][4 * w] = y.x;
-                        vr[r][4 * w + 1] = y.y;
-                        vr[r][4 * w + 2] = y.z;
-                        vr[r][4 * w + 3] = y.w;
-                    }
+                    const uint4 y = *reinterpret_cast<const uint4*>(p);
+                    vr[r][0] = y.x;
+                    vr[r][1] = y.y;
+                    vr[r][2] = y.z;
+                    vr[r][3] = y.w;
                 }
             }
         }
-        if constexpr (I8) {
-            if (tid < 128) {
-                const int code = sm.code[ring][tid & 63];
-                sc = code < 0 ? 0.0f
-                              : (tid < 64 ? a.k_scale : a.v_scale)[static_cast<int64_t>(code >> a.page_shift) * a.s_page +
-                                                                   h * a.s_head + (code & mask) * a.s_token];
-            }
+        if (tid < 128) {
+            const int code = sm.code[ring][tid & 63];
+            sc = code < 0 ? 0.0f
+                          : (tid < 64 ? a.k_scale : a.v_scale)[static_cast<int64_t>(code >> a.page_shift) * a.s_page +
+                                                               h * a.s_head + (code & mask) * a.s_token];
         }
     };
-    // the registers into half `buf`; edge: infinities and NaN among the values become 0 and are noted
-    auto store = [&](int buf, bool edge) __attribute__((always_inline)) {
+    // the registers into half `buf`, keys as above, values transposed: value d of keys 4 vg .. 4 vg + 3 is 8 bytes in
+    // chunk 2 (vg / 4) + vg % 2, half vg / 2 % 2
+    auto store = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < KC; ++x) {
             const int e = tid + 256 * x, key = e / kPerKey, chunk = e % kPerKey;
-            uint4 y = kr[x];
-            if constexpr (I8) {
-                float f0[4], f1[4];
-                i8x4(kr[x].x, f0);
-                i8x4(kr[x].y, f1);
-                y = make_uint4(bf16_exact2(f0[0], f0[1]), bf16_exact2(f0[2], f0[3]), bf16_exact2(f1[0], f1[1]),
-                               bf16_exact2(f1[2], f1[3]));
-            }
-            *reinterpret_cast<uint4*>(&sm.k[buf][key * DP + 8 * (chunk ^ (key & 7))]) = y;
+            float f0[4], f1[4];
+            i8x4(kr[x].x, f0);
+            i8x4(kr[x].y, f1);
+            *reinterpret_cast<uint4*>(&sm.k[buf][key * DP + 8 * (chunk ^ kswap(key))]) =
+                make_uint4(bf16_exact2(f0[0], f0[1]), bf16_exact2(f0[2], f0[3]), bf16_exact2(f1[0], f1[1]),
+                           bf16_exact2(f1[2], f1[3]));
         }
-        if constexpr (!I8) {
-            if (edge) {
-                bool bad = false;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        bad = bad || has_wild<DT>(vr[r][w]);
-                        vr[r][w] = tame<DT>(vr[r][w]);
-                    }
-                if (bad) sm.wild = 1;
-            }
-        }
-        // value d of keys 4 vg .. 4 vg + 3: 8 bytes in chunk 2 (vg / 4) + vg % 2, half vg / 2 % 2
         const int chunk = 2 * (vg >> 2) + (vg & 1), half = (vg >> 1) & 1;
-        auto put = [&](int d, uint32_t x, uint32_t y) {
-            *reinterpret_cast<uint2*>(&sm.v[buf][d * kTile + 8 * (chunk ^ ((d ^ (d >> 3)) & 7)) + 4 * half]) = make_uint2(x, y);
-        };
-        if constexpr (I8) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                float f[4][4];
+        for (int w = 0; w < VW; ++w) {
+            float f[4][4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) i8x4(vr[r][w], f[r]);
+            for (int r = 0; r < 4; ++r) i8x4(vr[r][w], f[r]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    put(VE * vc + 4 * w + e, bf16_exact2(f[0][e], f[1][e]), bf16_exact2(f[2][e], f[3][e]));
-            }
-            if (tid < 64) sm.ks[buf][tid] = sc;
-            else if (tid < 128) sm.vs[buf][tid - 64] = sc;
-        } else {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                put(VE * vc + 2 * w, pair16<0>(vr[0][w], vr[1][w]), pair16<0>(vr[2][w], vr[3][w]));
-                put(VE * vc + 2 * w + 1, pair16<1>(vr[0][w], vr[1][w]), pair16<1>(vr[2][w], vr[3][w]));
+            for (int e = 0; e < 4; ++e) {
+                const int d = VE * vc + 4 * w + e;
+                *reinterpret_cast<uint2*>(&sm.v[buf][d * kTile + 8 * (chunk ^ ((d ^ (d >> 3)) & 7)) + 4 * half]) =
+                    make_uint2(bf16_exact2(f[0][e], f[1][e]), bf16_exact2(f[2][e], f[3][e]));
             }
         }
+        if (tid < 64) sm.ks[buf][tid] = sc;
+        else if (tid < 128) sm.vs[buf][tid - 64] = sc;
     };
     // whether some row of the workgroup sees a part of tile i only
     auto edge_of = [&](int i) {
@@ -332,8 +348,26 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     };
 
     // a lane's places in the LDS rows: chunk 2 s + h of key 32 u + q is at (2 s) ^ (h ^ (q & 7)), so four bases serve
-    // all steps; V^T's chunk 2 t + h of row 32 i + q at (2 t) ^ 4 (i % 2) ^ (h ^ (q ^ q / 8) % 8) likewise
+    // all steps; int8: V^T's chunk 2 t + h of row 32 i + q at (2 t) ^ 4 (i % 2) ^ (h ^ (q ^ q / 8) % 8) likewise
     const int kx = hf ^ (q & 7), vx = hf ^ ((q ^ (q >> 3)) & 7);
+    // 16-bit: 16 lanes together read four keys of 16 values and get a value of four keys each; lane n reads key n / 4,
+    // values 4 (n % 4) .. of them
+    const int vn = lane & 15;
+    auto v_frag = [&](int buf, int i, int t) __attribute__((always_inline)) {
+        if constexpr (I8) {
+            const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(sm.v[buf]) + q * kTile * 2 +
+                                                            16 * ((2 * t) ^ (4 * (i & 1)) ^ vx) + i * 32 * kTile * 2);
+            return Frag{{x.x, x.y, x.z, x.w}};
+        } else {
+            const int row = 4 * hf + (vn >> 2);
+            const char* base = reinterpret_cast<const char*>(sm.v[buf]) + row * DP * 2 +
+                               16 * ((4 * (i & 3)) ^ vswap(row)) + 32 * (lane >> 4 & 1) + 8 * (vn & 3) + 256 * (i >> 2) + 16 * t * DP * 2;
+            const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(base));
+            const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(base + 8 * DP * 2));
+            const uint2 xw = __builtin_bit_cast(uint2, x), yw = __builtin_bit_cast(uint2, y);
+            return Frag{{xw.x, xw.y, yw.x, yw.y}};
+        }
+    };
     auto below = [](int64_t n) { return n >= 64 ? ~uint64_t(0) : n <= 0 ? uint64_t(0) : (uint64_t(1) << n) - 1; };
 
     // the row's visible keys of the tile at j: bit 8 (r / 4) + r % 4 of each half
@@ -346,12 +380,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
         if (wrow > most) return;                                                   // no rows in this wave
         if (j > wpos_hi || (j + kTile <= wlo_lo && j >= sinks)) return;            // no row of the wave sees it
         const char* kp[4];
-        const char* vp[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            kp[x] = reinterpret_cast<const char*>(sm.k[buf]) + q * DP * 2 + 16 * ((2 * x) ^ kx);
-            vp[x] = reinterpret_cast<const char*>(sm.v[buf]) + q * kTile * 2 + 16 * ((2 * x) ^ vx);
-        }
+        for (int x = 0; x < 4; ++x) kp[x] = reinterpret_cast<const char*>(sm.k[buf]) + q * DP * 2 + 16 * ((2 * x) ^ kx);
         f32x16 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -436,15 +466,11 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
                 }
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        auto v_frag = [&](int i, int t) __attribute__((always_inline)) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vp[t ^ (2 * (i & 1))] + i * 32 * kTile * 2);
-            return Frag{{x.x, x.y, x.z, x.w}};
-        };
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const Frag v = v_frag(i, t);
+                const Frag v = v_frag(buf, i, t);
                 o[i] = mfma32<MT>(v, p[t], o[i]);
                 if constexpr (kSplit) o[i] = mfma32<MT>(v, p2[t], o[i]);
             }
@@ -458,9 +484,24 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             put_codes(1, look_up(1));
         }
         if (tid == 0) sm.wild = 0;
+        if constexpr (!I8) {                            // what no load writes: keys beyond the heads' width
+            if (8 * kPerKey > a.D)
+                for (int e = tid; e < 2 * kTile * kPerKey; e += 256) reinterpret_cast<uint4*>(sm.k[0])[e] = make_uint4(0, 0, 0, 0);
+        }
         __syncthreads();
-        load(0);
-        store(0, edge_of(0));
+        // a tile that some row sees in part, or with keys that are not held
+        auto part = [&](int i, int ring) { return edge_of(i) || sm.held[ring] != ~uint64_t(0); };
+        auto arrive = [&](int i, int ring, int buf) __attribute__((always_inline)) {
+            if constexpr (I8) {
+                store(buf);
+            } else {
+                wait_loads();
+                if (part(i, ring)) tame_own(buf);
+            }
+        };
+        if constexpr (I8) load(0);
+        else fetch(0, 0);
+        arrive(0, 0, 0);
         __syncthreads();
         int r0 = 0, r1 = 1, r2 = 2;
         for (int i = 0; i < nt; ++i) {
@@ -468,10 +509,13 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             const bool more = i + 1 < nt;
             int ahead = -1;
             if (wave == 0) ahead = look_up(i + 2);
-            if (more) load(r1);
+            if (more) {
+                if constexpr (I8) load(r1);
+                else fetch(r1, nxt);
+            }
             work(cur, i, r0);
             if (wave == 0) put_codes(r2, ahead);
-            if (more) store(nxt, edge_of(i + 1));
+            if (more) arrive(i + 1, r1, nxt);
             __syncthreads();
             const int r = r0;
             r0 = r1;
@@ -483,12 +527,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
                 // values that are infinite or NaN at an edge: products of ones count, for every row and value, which
                 // kinds its keys hold, and they are added
                 for (int i = 0; i < nt; ++i) {
-                    if (!edge_of(i)) continue;
                     __syncthreads();
                     if (wave == 0) put_codes(0, look_up(i));
                     __syncthreads();
-                    load(0);
-                    store(0, false);
+                    if (!part(i, 0)) continue;
+                    fetch(0, 0);
+                    wait_loads();
                     __syncthreads();
                     const uint64_t vis = visible(sm.held[0], key_of(i));
                     constexpr uint32_t kOne = MT == kDtF16 ? 0x3c00u : 0x3f80u;
@@ -509,15 +553,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
                             for (int r = 0; r < 16; ++r) n[r] = 0.0f;
 #pragma unroll
                             for (int t = 0; t < 4; ++t) {
-                                const uint4 x = *reinterpret_cast<const uint4*>(
-                                    reinterpret_cast<const char*>(sm.v[0]) + (32 * e + q) * kTile * 2 +
-                                    16 * ((2 * t) ^ (4 * (e & 1)) ^ vx));
-                                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                                const Frag w = v_frag(0, e, t);
                                 Frag v;
 #pragma unroll
                                 for (int y = 0; y < 4; ++y)
-                                    v.w[y] = (wild_kind<MT>(w[y] & 0xffffu) == kind ? kOne : 0u) |
-                                             (wild_kind<MT>(w[y] >> 16) == kind ? kOne << 16 : 0u);
+                                    v.w[y] = (wild_kind<MT>(w.w[y] & 0xffffu) == kind ? kOne : 0u) |
+                                             (wild_kind<MT>(w.w[y] >> 16) == kind ? kOne << 16 : 0u);
                                 n = mfma32<MT>(v, one[t], n);
                             }
                             const float w = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
