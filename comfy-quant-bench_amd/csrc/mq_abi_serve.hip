@@ -87,13 +87,16 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
 }
 
 int64_t mq_paged_attention_counters(int64_t T, int64_t Hq, int64_t H, int64_t B, int ragged) {
-    if (T <= 0 || Hq <= 0 || H <= 0 || B <= 0 || Hq >= 65536 || H > Hq || ragged) return 0;
+    if (T <= 0 || Hq <= 0 || H <= 0 || B <= 0 || Hq >= 65536 || H > Hq || T * Hq >= kMost || B >= kMost) return 0;
+    if (ragged) return attn_prompt_counters(T, static_cast<int>(Hq), static_cast<int>(H), B);
     return attn_decode_counters(static_cast<int>(Hq), static_cast<int>(H), B);
 }
 
 int64_t mq_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t B, int ragged) {
-    if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256) return 0;
-    return ragged ? 0 : attn_decode_workspace_bytes(static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D));
+    if (T <= 0 || Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256 || T * Hq >= kMost || B >= kMost)
+        return 0;
+    if (ragged) return attn_prompt_workspace_bytes(T, static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D), B);
+    return attn_decode_workspace_bytes(static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D));
 }
 
 int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int64_t Hq, int64_t H,

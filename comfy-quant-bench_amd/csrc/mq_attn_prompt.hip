@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kRows = 128;     // rows per workgroup
 constexpr int kTile = 64;      // keys per step
+constexpr int kLeast = 8;      // tiles that a piece of a split sequence has at least
 
 template <int DT>
 __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
@@ -81,6 +82,14 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 }
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v* LdsShort4;
+
+// Between workgroups of one launch: past the caches that are not common to all of them.
+__device__ __forceinline__ void send1(float* p, float x) {
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float receive1(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 // Sixteen bytes per active lane from `src` to LDS bytes dst + 16 lane (dst the same in all lanes). Written as asm: the
 // compiler would wait for the builtin's stores before any LDS read that it cannot tell apart.
@@ -177,6 +186,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
         ns = static_cast<int>(s);
         nt = static_cast<int>(s + nw);
     }
+    // few rows over many tiles: this workgroup takes pieces' share `piece` of them, and the last to end joins them
+    const int piece = blockIdx.y, room = nt / kLeast;
+    const int pieces = room < 2 ? 1 : room < static_cast<int>(gridDim.y) ? room : static_cast<int>(gridDim.y);
+    if (piece >= pieces) return;
+    const int i0 = static_cast<int>(static_cast<int64_t>(nt) * piece / pieces);
+    const int i1 = static_cast<int>(static_cast<int64_t>(nt) * (piece + 1) / pieces);
     auto key_of = [&](int i) { return (i < ns ? static_cast<int64_t>(i) : w0 + (i - ns)) * kTile; };
 
     // the query rows
@@ -216,15 +231,15 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     const int mask = (1 << a.page_shift) - 1;
     const int vg = tid >> 4, vc = tid & 15;             // V staging (int8): keys 4 vg .. 4 vg + 3, values VE vc ..
 
-    // rows of tile i's keys (wave 0; lane x looks up key x)
+    // the table's entry for key x = lane of tile i (wave 0), as it is: a wait for it here would stop the wave
     auto look_up = [&](int i) -> int {
-        if (i >= nt) return -1;
-        const int64_t key = key_of(i) + lane, at = key >> a.page_shift;
-        if (key > last || at >= a.width) return -1;
-        const int p = table[at];
-        return p >= 0 && p < a.pages ? (p << a.page_shift) | (static_cast<int>(key) & mask) : -1;
+        const int64_t at = (key_of(i) + lane) >> a.page_shift;
+        return table[at < a.width ? at : a.width - 1];
     };
-    auto put_codes = [&](int ring, int code) {
+    auto put_codes = [&](int ring, int i, int p) {
+        const int64_t key = key_of(i) + lane;
+        const bool ok = i < i1 && key <= last && key >> a.page_shift < a.width && p >= 0 && p < a.pages;
+        const int code = ok ? (p << a.page_shift) | (static_cast<int>(key) & mask) : -1;
         const uint64_t held = __ballot(code >= 0);
         if constexpr (I8)
             sm.code[ring][lane] = code;
@@ -244,13 +259,20 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_offset(sm.k[0]) + wave * 1024);
     const uint32_t lds_v = __builtin_amdgcn_readfirstlane(lds_offset(sm.v[0]) + wave * 1024);
     auto fetch = [&](int ring, int buf) __attribute__((always_inline)) {
+        const int key = tid / kPerKey, kc = slot ^ kswap(key), vc = slot ^ vswap(key);   // the swaps are alike in all x
+        if (8 * kc < a.D) {
+            int64_t at[KC];
 #pragma unroll
-        for (int x = 0; x < KC; ++x) {
-            const int key = (tid + 256 * x) / kPerKey, kc = slot ^ kswap(key), vc = slot ^ vswap(key);
-            const int64_t at = sm.at[ring][key];
-            const uint32_t to = buf * kTile * DP * 2 + 4096 * x;
-            if (8 * kc < a.D) load_lds16(kbase + at + 16 * kc, lds_k + to);
-            if (8 * vc < a.D) load_lds16(vbase + at + 16 * vc, lds_v + to);
+            for (int x = 0; x < KC; ++x) at[x] = sm.at[ring][key + kTile / KC * x];
+#pragma unroll
+            for (int x = 0; x < KC; ++x) load_lds16(kbase + at[x] + 16 * kc, lds_k + buf * kTile * DP * 2 + 4096 * x);
+        }
+        if (8 * vc < a.D) {
+            int64_t at[KC];
+#pragma unroll
+            for (int x = 0; x < KC; ++x) at[x] = sm.at[ring][key + kTile / KC * x];
+#pragma unroll
+            for (int x = 0; x < KC; ++x) load_lds16(vbase + at[x] + 16 * vc, lds_v + buf * kTile * DP * 2 + 4096 * x);
         }
     };
     // this thread's own values of half `buf`: infinities and NaN become 0 and are noted
@@ -360,10 +382,11 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             return Frag{{x.x, x.y, x.z, x.w}};
         } else {
             const int row = 4 * hf + (vn >> 2);
-            const char* base = reinterpret_cast<const char*>(sm.v[buf]) + row * DP * 2 +
-                               16 * ((4 * (i & 3)) ^ vswap(row)) + 32 * (lane >> 4 & 1) + 8 * (vn & 3) + 256 * (i >> 2) + 16 * t * DP * 2;
-            const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(base));
-            const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(base + 8 * DP * 2));
+            const uint32_t base = lds_offset(sm.v[0]) + buf * kTile * DP * 2 + row * DP * 2 +
+                                  16 * ((4 * (i & 3)) ^ vswap(row)) + 32 * (lane >> 4 & 1) + 8 * (vn & 3);
+            const LdsShort4 p = (LdsShort4)(base) + (256 * (i >> 2) + 16 * t * DP * 2) / 8;
+            const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+            const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + DP * 2);
             const uint2 xw = __builtin_bit_cast(uint2, x), yw = __builtin_bit_cast(uint2, y);
             return Frag{{xw.x, xw.y, yw.x, yw.y}};
         }
@@ -478,10 +501,10 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
 
     // tile i is worked on from half i % 2 while tile i + 1 is loaded, and tile i + 2's rows are looked up; what says
     // where a tile's keys are goes round three places, so one barrier a tile is enough
-    if (nt > 0) {
+    if (i1 > i0) {
         if (wave == 0) {
-            put_codes(0, look_up(0));
-            put_codes(1, look_up(1));
+            put_codes(0, i0, look_up(i0));
+            put_codes(1, i0 + 1, look_up(i0 + 1));
         }
         if (tid == 0) sm.wild = 0;
         if constexpr (!I8) {                            // what no load writes: keys beyond the heads' width
@@ -501,20 +524,20 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
         };
         if constexpr (I8) load(0);
         else fetch(0, 0);
-        arrive(0, 0, 0);
+        arrive(i0, 0, 0);
         __syncthreads();
         int r0 = 0, r1 = 1, r2 = 2;
-        for (int i = 0; i < nt; ++i) {
-            const int cur = i & 1, nxt = cur ^ 1;
-            const bool more = i + 1 < nt;
-            int ahead = -1;
+        for (int i = i0; i < i1; ++i) {
+            const int cur = (i - i0) & 1, nxt = cur ^ 1;
+            const bool more = i + 1 < i1;
+            int ahead = 0;
             if (wave == 0) ahead = look_up(i + 2);
             if (more) {
                 if constexpr (I8) load(r1);
                 else fetch(r1, nxt);
             }
             work(cur, i, r0);
-            if (wave == 0) put_codes(r2, ahead);
+            if (wave == 0) put_codes(r2, i + 2, ahead);
             if (more) arrive(i + 1, r1, nxt);
             __syncthreads();
             const int r = r0;
@@ -526,9 +549,9 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             if (sm.wild) {
                 // values that are infinite or NaN at an edge: products of ones count, for every row and value, which
                 // kinds its keys hold, and they are added
-                for (int i = 0; i < nt; ++i) {
+                for (int i = i0; i < i1; ++i) {
                     __syncthreads();
-                    if (wave == 0) put_codes(0, look_up(i));
+                    if (wave == 0) put_codes(0, i, look_up(i));
                     __syncthreads();
                     if (!part(i, 0)) continue;
                     fetch(0, 0);
@@ -571,6 +594,50 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     }
     l = sum2(l);
     any = (static_cast<int>(any) | __shfl_xor(static_cast<int>(any), 32)) != 0;
+    if (pieces > 1 && wrow <= most) {
+        // a wave's pieces meet in memory; the last one adds all of them in their order, so the order of arrival
+        // changes nothing
+        constexpr int kPart = (16 * kBlocks + 2) * 64;
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+        float* parts = static_cast<float*>(a.work) + slot * gridDim.y * kPart + lane;
+        float* to = parts + static_cast<int64_t>(piece) * kPart;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) send1(to + 64 * (16 * i + r), o[i][r]);
+        send1(to + 64 * 16 * kBlocks, m);
+        send1(to + 64 * (16 * kBlocks + 1), any ? l : -1.0f);
+        __builtin_amdgcn_s_waitcnt(0);                  // all lanes' values are where other workgroups see them
+        int before = 0;
+        if (lane == 0) before = __hip_atomic_fetch_add(a.counters + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__builtin_amdgcn_readfirstlane(before) != pieces - 1) return;
+        if (lane == 0) __hip_atomic_store(a.counters + slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        m = kNegInf;
+        for (int x = 0; x < pieces; ++x)
+            m = __builtin_fmaxf(m, receive1(parts + static_cast<int64_t>(x) * kPart + 64 * 16 * kBlocks));
+        l = 0.0f;
+        any = false;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+#pragma unroll 1
+        for (int x = 0; x < pieces; ++x) {
+            const float* from = parts + static_cast<int64_t>(x) * kPart;
+            const float mx = receive1(from + 64 * 16 * kBlocks), lx = receive1(from + 64 * (16 * kBlocks + 1));
+            const float f = mx == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mx - m);
+            const bool some = !(lx == -1.0f);           // -1: the row sees nothing of this piece
+            any = any || some;
+            l += some ? lx * f : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float y = receive1(from + 64 * (16 * i + r));
+                    o[i][r] += some ? y * f : 0.0f;
+                }
+        }
+    }
     if (wrow + q <= most && wrow <= most) {
         const float inv = any ? 1.0f / l : 0.0f;        // nothing seen: zeros
         uint16_t* out = static_cast<uint16_t*>(a.o) + (tok0 + tok) * a.o_token + (h * group + myrow % group) * a.o_head;
@@ -587,10 +654,23 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     }
 }
 
+// Workgroups for whole sequences: at least as many as there are row tiles.
+int64_t row_tiles(int64_t T, int Hq, int H, int64_t B) { return (T * (Hq / H) / kRows + B) * H; }
+
+// Pieces that a sequence may be split in: as many as give every compute unit two workgroups (what fits beside each
+// other), 32 at most, and none for fewer than 2 x kLeast tiles.
+int64_t most_pieces(int64_t T, int Hq, int H, int64_t B) {
+    const int cus = device_cu_count();
+    const int64_t n = 2 * (cus > 0 ? cus : 256) / row_tiles(T, Hq, H, B);
+    return n < 2 ? 1 : n < 32 ? n : 32;
+}
+
 template <int DP, int DT, bool I8>
 int launch_width(const AttnArgs& a, hipStream_t stream) {
-    const int64_t group = a.Hq / a.H;
-    const int64_t tiles = a.T * group / kRows + a.B;    // at least as many as the sequences' row tiles
+    const int64_t tiles = row_tiles(a.T, a.Hq, a.H, a.B);
+    int64_t pieces = most_pieces(a.T, a.Hq, a.H, a.B);
+    const int64_t room = (a.width << a.page_shift) / (kTile * kLeast);
+    pieces = room < 2 ? 1 : pieces < room ? pieces : room;
     const size_t lds = sizeof(Lds<DP>);
     auto kern = attn_prompt_kernel<DP, DT, I8>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -599,7 +679,7 @@ int launch_width(const AttnArgs& a, hipStream_t stream) {
         set_error("paged_attention: cannot reserve %zu bytes of LDS", lds);
         return -3;
     }
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles * a.H)), dim3(256), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(pieces)), dim3(256), lds, stream, a);
     return launch_status("paged_attention");
 }
 
@@ -611,6 +691,15 @@ int launch_type(const AttnArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int64_t attn_prompt_workspace_bytes(int64_t T, int Hq, int H, int D, int64_t B) {
+    const int64_t pieces = most_pieces(T, Hq, H, B), wide = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    return pieces < 2 ? 0 : row_tiles(T, Hq, H, B) * pieces * 4 * (wide / 2 + 2) * 64 * 4;
+}
+
+int64_t attn_prompt_counters(int64_t T, int Hq, int H, int64_t B) {
+    return most_pieces(T, Hq, H, B) < 2 ? 0 : 4 * row_tiles(T, Hq, H, B);
+}
 
 int launch_attn_prompt(const AttnArgs& a, hipStream_t stream) {
     const bool i8 = a.k_scale != nullptr;

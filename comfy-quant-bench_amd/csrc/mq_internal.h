@@ -246,6 +246,8 @@ int launch_attn_prompt(const AttnArgs& a, hipStream_t stream);
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream);
 int64_t attn_decode_workspace_bytes(int Hq, int H, int D);
 int64_t attn_decode_counters(int Hq, int H, int64_t B);
+int64_t attn_prompt_workspace_bytes(int64_t T, int Hq, int H, int D, int64_t B);
+int64_t attn_prompt_counters(int64_t T, int Hq, int H, int64_t B);
 
 // --- 4-bit weights, floating activations (mq_w4a16.hip)
 enum class W4Zero : int { Signed = 0, U4 = 1, Float = 2 };

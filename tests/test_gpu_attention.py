@@ -292,3 +292,50 @@ def test_caches_past_4_gib_elements(gpu_device):
     small = ck.paged_attention(q, s.k, s.k, torch.where(s.table >= 0, s.table - (pages - n), s.table), s.kv_lens, cu_q=cu)
     assert torch.equal(y, small)
     del big
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,h,d", [(8, 2, 128), (3, 3, 64), (7, 1, 80), (2, 2, 256)])
+@pytest.mark.parametrize("dtype,int8", [(torch.bfloat16, False), (torch.float16, False), (torch.float16, True), (torch.bfloat16, True)])
+def test_few_rows_over_a_long_cache(gpu_device, hq, h, d, dtype, int8):
+    print(f"[attention] prompt pieces {hq}/{h} x {d} {dtype} int8 {int8}", flush=True)
+    s = Setup(gpu_device, [4099, 9, 1500, 0, 2048], hq, h, d, dtype=dtype, int8=int8, new=[3, 9, 40, 0, 1], page=64)
+    for kw in ({}, {"window": 1200, "sinks": 5}, {"window": 64}):
+        y = s.run(**kw)
+        s.check(y, **kw)
+        assert torch.equal(y, s.run(**kw))      # the counters are zeros again, the order of arrival changes nothing
+
+
+@pytest.mark.gpu
+def test_pieces_of_infinities_and_hidden_rows(gpu_device):
+    print("[attention] prompt pieces with infinities", flush=True)
+    s = Setup(gpu_device, [5000], 4, 2, 64, dtype=torch.bfloat16, new=[2], page=64)
+    y = s.run()
+    last = s.table[0, 4998 // 64]
+    s.v[last, 1, 4999 % 64, 3] = math.inf       # seen by the second token only, in the last piece
+    z = s.run()
+    assert torch.equal(z[0], y[0]) and torch.isinf(z[1, 2:, 3]).all()
+    z[1, 2:, 3] = y[1, 2:, 3]
+    assert torch.equal(z, y)
+    s.kv_lens[0] = 0                            # both tokens before the first one: nothing is seen
+    assert (s.run() == 0).all()
+
+
+@pytest.mark.gpu
+def test_pieces_in_a_graph(gpu_device):
+    print("[attention] prompt pieces in a graph", flush=True)
+    s = Setup(gpu_device, [6000, 3000], 8, 2, 128, new=[5, 7], page=64)
+    want = s.run()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        s.run()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            y = s.run()
+    for _ in range(4):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        assert torch.equal(s.run(), want)
