@@ -187,6 +187,9 @@ int copies_of(const char* what, void* k, void* v, int64_t layers, int64_t layer_
         MQ_REQUIRE(bytes > 0 && bytes % 4 == 0 && pitch >= bytes && pitch % 4 == 0 && layer_bytes >= 0 && layer_bytes % 4 == 0,
                    "%s: pages of %lld bytes, %lld apart: multiples of 4, not overlapping", what, (long long)bytes,
                    (long long)pitch);
+        // the copies count blocks of at least 4 KB of a page's layers in 32 bits
+        MQ_REQUIRE(bytes < kMost && 2 * layers * (bytes / 4096 + 1) < kMost && s_bytes <= bytes,
+                   "%s: a page of %lld bytes in %lld layers is too large", what, (long long)bytes, (long long)layers);
         c.t[c.tensors++] = {k, layer_bytes, pitch, bytes};
         c.t[c.tensors++] = {v, layer_bytes, pitch, bytes};
         MQ_REQUIRE((ks == nullptr) == (vs == nullptr), "%s: scales for both caches or none", what);

@@ -193,14 +193,14 @@ __global__ void __launch_bounds__(kPlan) fork_plan_kernel(KvTables a, const int*
     // a row that is forked to twice, or forked from while it is forked to
     check_distinct(dst, src, n, a.rows, sh);
     __syncthreads();
-    const int64_t cells = static_cast<int64_t>(n) * a.width;
     if (!sh.bad) {
         bool bad = false;
-        for (int64_t e = tid; e < cells; e += kPlan) {
-            const int64_t i = e / a.width, j = e - i * a.width;
-            if (j >= pages_of(a.lens[src[i]], a.page_shift)) continue;
-            const int p = a.table[src[i] * a.ld_table + j];
-            bad = bad || p < 0 || p >= a.pages;
+        for (int i = tid >> 6; i < n; i += kPlan / 64) {
+            const int s = src[i], held = pages_of(a.lens[s], a.page_shift);
+            for (int j = tid & 63; j < held; j += 64) {
+                const int p = a.table[s * a.ld_table + j];
+                bad = bad || p < 0 || p >= a.pages;
+            }
         }
         if (bad) sh.bad = 1;
     }
@@ -237,18 +237,16 @@ __global__ void __launch_bounds__(kPlan) fork_plan_kernel(KvTables a, const int*
         a.lens[d] = len;
     }
     __syncthreads();   // the moves are whole
-    for (int64_t e = tid; e < cells; e += kPlan) {
-        const int i = static_cast<int>(e / a.width);
-        const int64_t j = e - i * a.width;
-        const int s = src[i], full = a.lens[s] >> a.page_shift;
-        int p = -1;
-        if (j < full) {
-            p = a.table[s * a.ld_table + j];
-            atomicAdd(a.refs + p, 1);                       // integer: any order gives the same count
-        } else if (j == full) {
-            p = moves[2 * i + 1];
+    for (int i = tid >> 6; i < n; i += kPlan / 64) {       // a wave a child
+        const int s = src[i], d = dst[i], full = a.lens[s] >> a.page_shift, part = moves[2 * i + 1];
+        for (int64_t j = tid & 63; j < a.width; j += 64) {
+            int p = j == full ? part : -1;
+            if (j < full) {
+                p = a.table[s * a.ld_table + j];
+                atomicAdd(a.refs + p, 1);                   // integer: any order gives the same count
+            }
+            a.table[d * a.ld_table + j] = p;
         }
-        a.table[dst[i] * a.ld_table + j] = p;
     }
     if (tid == 0 && status) *status = 0;
 }
@@ -365,44 +363,48 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(int* refs, int64_t 
 
 // ---------------------------------------------------------------------------------------- page copies
 //
-// Pages moves[2 i] -> moves[2 i + 1] of every layer of up to four tensors (K, V and their scales). No
-// page is both read and written, so the copies need no order. HBM-bound: 16-byte loads and stores, a
-// unit of 16 KB per workgroup and step, with all its loads in flight before the first store.
+// Pages moves[2 i] -> moves[2 i + 1] of every layer of K and V, then of their scales. No page is both
+// read and written, so the copies need no order. HBM-bound: 16-byte loads and stores, a unit of 16 KB
+// per workgroup and step, with all its loads in flight before the first store; K and V in turns, so that
+// both fill the chip together.
 template <typename T>
 __global__ void __launch_bounds__(256) copy_pages_kernel(KvCopyArgs a) {
     const int count = a.count ? *a.count : a.n;
-    const int64_t step = static_cast<int64_t>(gridDim.x);
-    // compaction: the tables' entries to their pages' new places
-    if (a.place) {
-        const int64_t cells = a.tb.rows * a.tb.width;
-        for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < cells; e += step * 256) {
-            int* cell = a.tb.table + e / a.tb.width * a.tb.ld_table + e % a.tb.width;
-            const int p = *cell;
-            if (p >= 0 && p < a.tb.pages) *cell = a.place[p];
-        }
-    }
+    const uint32_t step = gridDim.x;
+    // compaction: the tables' entries to their pages' new places, a workgroup a row
+    if (a.place)
+        for (int64_t r = blockIdx.x; r < a.tb.rows; r += step)
+            for (int64_t j = threadIdx.x; j < a.tb.width; j += 256) {
+                int* cell = a.tb.table + r * a.tb.ld_table + j;
+                const int p = *cell;
+                if (p >= 0 && p < a.tb.pages) *cell = a.place[p];
+            }
     constexpr int kUnit = 256 * 4;                          // elements of T per unit
-    for (int w = 0; w < a.tensors; ++w) {
-        const KvCopyTensor t = a.t[w];
-        const int64_t per = t.page_bytes / static_cast<int64_t>(sizeof(T));
-        const int64_t units = (per + kUnit - 1) / kUnit;
-        const int64_t all = static_cast<int64_t>(count) * a.layers * units;
-        for (int64_t u = blockIdx.x; u < all; u += step) {
-            const int64_t unit = u % units, rest = u / units;
-            const int64_t layer = rest % a.layers, i = rest / a.layers;
+    for (int w = 0; w < a.tensors; w += 2) {                // K and V, then their scales: alike in pairs
+        const uint32_t per = static_cast<uint32_t>(a.t[w].page_bytes / static_cast<int64_t>(sizeof(T)));
+        const uint32_t units = (per + kUnit - 1) / kUnit, layers = static_cast<uint32_t>(a.layers);
+        const uint32_t blocks = 2 * layers * units;         // of a move: below 2^31, as the entry points see to
+        uint32_t u = blockIdx.x % blocks;
+        for (int64_t i = blockIdx.x / blocks; i < count;) {
             const int s = a.moves[2 * i], d = a.moves[2 * i + 1];
-            if (s < 0) continue;
-            char* base = static_cast<char*>(t.base) + layer * t.layer_bytes;
-            const T* from = reinterpret_cast<const T*>(base + s * t.page_pitch);
-            T* to = reinterpret_cast<T*>(base + d * t.page_pitch);
-            const int64_t e0 = unit * kUnit + threadIdx.x;
-            T x[4];
+            if (s >= 0) {
+                const uint32_t unit = u % units, rest = u / units, layer = rest >> 1;
+                const KvCopyTensor& t = a.t[w + (rest & 1)];
+                char* base = static_cast<char*>(t.base) + layer * t.layer_bytes;
+                const T* from = reinterpret_cast<const T*>(base + s * t.page_pitch);
+                T* to = reinterpret_cast<T*>(base + d * t.page_pitch);
+                const uint32_t e0 = unit * kUnit + threadIdx.x;
+                T x[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (e0 + j * 256 < per) x[j] = from[e0 + j * 256];
+                for (int j = 0; j < 4; ++j)
+                    if (e0 + j * 256 < per) x[j] = from[e0 + j * 256];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (e0 + j * 256 < per) to[e0 + j * 256] = x[j];
+                for (int j = 0; j < 4; ++j)
+                    if (e0 + j * 256 < per) to[e0 + j * 256] = x[j];
+            }
+            const uint64_t next = static_cast<uint64_t>(u) + step;
+            i += static_cast<int64_t>(next < blocks ? 0 : next < 2ull * blocks ? 1 : next / blocks);
+            u = static_cast<uint32_t>(next < blocks ? next : next < 2ull * blocks ? next - blocks : next % blocks);
         }
     }
 }
@@ -413,8 +415,11 @@ int launch_copies(const KvCopyArgs& a, hipStream_t stream) {
         wide = wide && a.t[w].page_bytes % 16 == 0 && a.t[w].page_pitch % 16 == 0 && a.t[w].layer_bytes % 16 == 0 &&
                reinterpret_cast<uintptr_t>(a.t[w].base) % 16 == 0;
     int64_t units = 0;
-    for (int w = 0; w < a.tensors; ++w)
-        units += static_cast<int64_t>(a.n) * a.layers * ((a.t[w].page_bytes / (wide ? 16 : 4) + 1023) / 1024);
+    for (int w = 0; w < a.tensors; w += 2) {
+        const int64_t blocks = 2 * a.layers * ((a.t[w].page_bytes / (wide ? 16 : 4) + 1023) / 1024);
+        const int64_t n = static_cast<int64_t>(a.n) * blocks;
+        units = units > n ? units : n;
+    }
     const int cus = device_cu_count();
     const int64_t most = static_cast<int64_t>(cus > 0 ? cus : 256) * 8;
     const int64_t grid = units < most ? (units > 0 ? units : 1) : most;
