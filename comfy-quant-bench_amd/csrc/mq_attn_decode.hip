@@ -21,6 +21,10 @@
 // (fp32) then go to the workspace, and the workgroup that brings a sequence's last piece (a count per sequence
 // and cache head tells, which it sets back to zero) joins them in the order of the pieces, so the result is the
 // same every time.
+//
+// Measured: 131071 tokens of 8 heads of 128, bf16: 87 us, 6.2 TB/s (a fill of memory reaches 6.7, a copy 5.1); 64 ragged
+// int8 sequences of up to 8000: 55 us, 3.4 TB/s, bound by unpacking and by the sequences' ends; one sequence of
+// 260 visible tokens: 10 us, a chain of dependent loads (length, table, rows) and the launch.
 #include "mq_attn.h"
 
 namespace mq {
@@ -273,7 +277,8 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
     constexpr bool kSplit = I8 && DT == kDtF16;         // fp16 rows against int8 keys: bf16 products of hi + lo
     constexpr int MT = I8 ? kDtBf16 : DT;               // type of the products
     // beginning and ending a sequence takes about as long as 128 KB of keys and values: counted where there are more
-    // of them than workgroups (a ragged batch of 64: 85 -> 77 us); else every piece is a part of one anyway
+    // of them than workgroups (64 ragged int8 sequences of 8 heads: 66 -> 58 us); else every piece is a part of one
+    // anyway (16 sequences of 2000: 30 us, 33 if counted)
     constexpr int kExtra = (131072 + kTile * DP * E) / (2 * kTile * DP * E);
     // the next segment's first tile is loaded ahead of this one's end where the registers for it are free
     constexpr bool kAcross = DP != 256 && !kSplit;

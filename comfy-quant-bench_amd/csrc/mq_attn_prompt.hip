@@ -1,10 +1,15 @@
 // Attention of ragged prompt chunks over a paged key-value cache (causal, sliding window, first tokens).
 //
-// MFMA-bound for long prompts: 4 D operations per query-key pair, against 32 score-sized VALU steps per lane
-// and 64 keys. A workgroup of four waves takes 128 rows of one cache head: row = (new token, query head of the
-// group), token-major, so the heads that share keys and values share their tiles too and a short prompt
-// fills a tile. Each wave keeps 32 rows; tiles of 64 keys go through LDS, double-buffered: the next tile's
-// loads are issued before this one's products and stored to the other half behind them, one barrier a tile.
+// Bound by MFMA and VALU together, which barely run side by side on this part: a wave's 64 keys of 32 rows are 32
+// products of 32 cycles (D = 128) and about 1000 cycles of softmax, of which the exponentials are half (two
+// waves' softmax beside each other's products, interleaved by hand, was slower). Long prompts: 880 TFLOP/s (8192
+// tokens, 32 heads of 128: 625 us; a large library matrix product reaches 1190).
+//
+// A workgroup of four waves takes 128 rows of one cache head: row = (new token, query head of the group),
+// token-major, so the heads that share keys and values share their tiles too and a short prompt fills a tile.
+// Each wave keeps 32 rows; tiles of 64 keys go through LDS, double-buffered, one barrier a tile: the next tile's
+// loads go there by themselves (16-bit caches; through registers: 795 us, half of that for stores and their
+// addresses) while this one is worked on. Two workgroups a compute unit.
 //
 //   S^T = K Q^T      32x32x16 products. A: 32 keys, from LDS rows of 16-byte chunks (chunk x of key k at
 //                    x ^ (k & 7): eight lanes read all banks). B: 32 query rows, kept in registers. Lane (q, h)
@@ -13,8 +18,13 @@
 //                    moved (and the sums rescaled) when a row's maximum exceeds it by 2^8: any reference gives
 //                    the same quotient, and fp32 sums have the range.
 //   O^T = V^T P^T    B: a lane's 8 probabilities of keys 16 t + 4 h + {0 .. 3, 8 .. 11} as they are; A: V^T from
-//                    LDS, rows of one value over 64 keys, the keys in just that order, transposed by v_perm on
-//                    the way in.
+//                    LDS in just that order: 16-bit caches lie there as in the pages and are transposed by the
+//                    LDS reads (16 lanes exchange 4 keys x 16 values); int8 ones are transposed by v_perm on the
+//                    way in, where they become bf16.
+//
+// Few rows over many keys would leave the chip idle: their tiles are split over several workgroups (the host gives
+// room for as many as fill it, the kernel takes as many as have tiles enough), whose sums meet in memory; of each
+// wave's pieces the last one to arrive adds all in their order. 5 tokens behind 32768: 845 -> 75 us.
 //
 // Rows of one tile may differ in what they see: hidden scores become -infinity, and their weight 0 leaves the sum
 // alone unless V holds an infinity or NaN there (0 times that is NaN). Tiles at an edge are looked through for
@@ -27,7 +37,9 @@ namespace {
 
 constexpr int kRows = 128;     // rows per workgroup
 constexpr int kTile = 64;      // keys per step
-constexpr int kLeast = 8;      // tiles that a piece of a split sequence has at least
+// Tiles that a piece of a split sequence has at least: a piece costs its first loads and its way through memory, some
+// three tiles' time (2000 tokens of 8 heads: 16 tiles 68 us, 8 43, 4 41; 64 tokens behind 1500: 54, 33, 29).
+constexpr int kLeast = 4;
 
 template <int DT>
 __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {

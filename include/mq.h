@@ -504,7 +504,8 @@ int mq_kv_compact(void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t
  * y[m, n] = T( sum_k x'[m, k] * w[n, k] + bias[n] ): 4-bit weights with a scale per group of K values
  * and activations in floating point, x' = x or (hblock 16, 64, 256) x rotated by H_hblock in fp32
  * as mq_rotquant rotates it. For few rows (one token of each of a batch's sequences): the weights are read
- * once per 16 rows. Products and sums are fp32; nothing but the output is rounded.
+ * once per 16 rows (rotated rows 8, fp32 rows 5). Products and sums are fp32 and the output is rounded once; rows rotated
+ * for a 16-bit output are held to 16 bits of each value.
  *   x [M, K] of type x_dtype (bf16, fp16 or fp32), stride ldx (rows start at multiples of 16 bytes)
  *   qw packed 4-bit [N, K/2], stride ldw bytes (ldw % 16 == 0, 16-byte aligned; low nibble = even k)
  *   ws [N, K/group] of type s_dtype, stride ldws; wz by `zero` (MQ_W4Z_*): NULL, packed uint4
