@@ -51,7 +51,17 @@ struct W4Plan {
     int chunk;      // K values staged at a time
     int pitch;      // pairs of scale and zero-point a column in LDS
     int pair_bufs;  // tiles' worth of them
+    // divisions as products: n / d = n m / 2^32 for n d < 2^32 with m = 2^32 / d rounded up
+    uint32_t by_pieces;   // pieces a staged row
+    uint32_t by_halves;   // pairs of groups a column
 };
+
+__host__ __device__ __forceinline__ uint32_t w4_inverse(int64_t d) {   // d = 1: 0, see w4_div
+    return static_cast<uint32_t>(((int64_t(1) << 32) + d - 1) / d);
+}
+__device__ __forceinline__ int w4_div(int n, uint32_t inverse) {
+    return inverse ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), inverse)) : n;
+}
 
 // A stored value of type dt from its bits.
 __device__ __forceinline__ float as_float(uint32_t b, int dt) {
@@ -82,7 +92,7 @@ struct W4Piece {
         const int lane = threadIdx.x & 63;
         const int width = a.hblock ? 1024 : 8, per = pl.chunk / width;
         const int at = e < all ? e : 0;
-        m = at / per;
+        m = w4_div(at, pl.by_pieces);
         kk = width * (at - m * per) + (a.hblock ? 16 * ((lane >> 2) + 16 * (lane & 3)) : 0);
         const int k = k0 + kk;
         ok = e < all && k < a.K;
@@ -151,9 +161,12 @@ struct W4Piece {
                 }
         }
     }
+    template <bool F16>
     __device__ __forceinline__ void store(const W4A16Args& a, const W4Plan& pl, uint16_t* xs, int stride) {
         uint16_t* to = xs + m * pl.parts * stride + kk;
-        if (a.hblock) {
+        if (F16) {
+            put<kDtF16, false>(a, pl, to, stride);
+        } else if (a.hblock) {
             if (a.x_dtype == kDtF32) put<kDtF32, true>(a, pl, to, stride);
             else if (a.x_dtype == kDtF16) put<kDtF16, true>(a, pl, to, stride);
             else put<kDtBf16, true>(a, pl, to, stride);
@@ -260,7 +273,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     uint32_t sb[kAhead], zb[kAhead];
     auto load_item = [&](int tile, int e, uint32_t* s, uint32_t* z) __attribute__((always_inline)) {
         const int64_t n0 = static_cast<int64_t>(tile) * kCols;
-        const int at = e < items ? e : 0, col = at / halves, gi = 2 * (at - col * halves);
+        const int at = e < items ? e : 0, col = w4_div(at, pl.by_halves), gi = 2 * (at - col * halves);
         const int64_t n = n0 + col < a.N ? n0 + col : a.N - 1;
         const int g0 = gi + 1 < groups ? gi : groups - 2;   // an odd last group behind the one before it (there are two)
         __builtin_memcpy(s, static_cast<const uint16_t*>(a.ws) + n * a.ldws + g0, 4);
@@ -270,7 +283,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     auto store_item = [&](int e, uint32_t s, uint32_t z, Pair* to) __attribute__((always_inline)) {
         if constexpr (!ANY) {
             if (e >= items) return;
-            const int col = e / halves, gi = 2 * (e - col * halves);
+            const int col = w4_div(e, pl.by_halves), gi = 2 * (e - col * halves);
             uint32_t z0 = 0, z1 = 0;
             const bool odd = gi + 1 >= groups;
             if (odd) s >>= 16;
@@ -413,7 +426,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
                         for (int i = 0; i < PB; ++i) piece[i].load(a, pl, m0, e + i * step, pieces, k0);
 #pragma unroll
                     for (int i = 0; i < PB; ++i)
-                        if (e + i * step < pieces) piece[i].store(a, pl, xs, stride);
+                        if (e + i * step < pieces) piece[i].template store<F16>(a, pl, xs, stride);
                 }
                 __syncthreads();
                 staged = pl.chunk >= K;
@@ -461,6 +474,7 @@ int launch_tiles(const W4A16Args& a, W4Plan pl, hipStream_t stream) {
     const int64_t tiles = (a.N + 16 * CT - 1) / (16 * CT);
     const int cus = device_cu_count();
     pl.pitch = static_cast<int>((a.K / a.group + 1) / 4 * 4 + 2);   // even, and 16 columns on different banks
+    pl.by_halves = w4_inverse((a.K / a.group + 1) / 2);             // at most 32 columns x 512 halves
     const bool through = W == 8 && tiles > cus && cus > 0 && 2 * 16 * CT * pl.pitch * sizeof(W4Pair<G == 0>) < kLds / 2;
     const int64_t groups = through ? cus : tiles;
     pl.pair_bufs = groups < tiles ? 2 : 1;
@@ -481,6 +495,7 @@ int launch_tiles(const W4A16Args& a, W4Plan pl, hipStream_t stream) {
             if (chunk > all) chunk = all;
         }
         pl.chunk = static_cast<int>(chunk);
+        pl.by_pieces = w4_inverse(chunk / (a.hblock ? 1024 : 8));   // at most 16 rows x 4096 pieces
         lds = rows * (chunk + kPad) * 2 + pairs + red;
         if (lds <= kLds) break;
         if (pl.rows_m == 1) {
