@@ -51,12 +51,13 @@ struct W4Plan {
     int chunk;      // K values staged at a time
     int pitch;      // pairs of scale and zero-point a column in LDS
     int pair_bufs;  // tiles' worth of them
-    // divisions as products: n / d = n m / 2^32 for n d < 2^32 with m = 2^32 / d rounded up
+    // divisions as products: n / d = n m / 2^32 for n d < 2^32 with m = 2^32 / d rounded up (a thread divides for
+    // every piece and pair, which took 2 us of 16 rows' 20)
     uint32_t by_pieces;   // pieces a staged row
     uint32_t by_halves;   // pairs of groups a column
 };
 
-__host__ __device__ __forceinline__ uint32_t w4_inverse(int64_t d) {   // d = 1: 0, see w4_div
+__host__ __device__ __forceinline__ uint32_t w4_inverse(int64_t d) {   // d = 1 wraps to 0
     return static_cast<uint32_t>(((int64_t(1) << 32) + d - 1) / d);
 }
 __device__ __forceinline__ int w4_div(int n, uint32_t inverse) {
@@ -223,7 +224,9 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     // staged while the weights are on their way
     const int pieces = rows * (pl.chunk / (a.hblock ? 1024 : 8));
     const int mine = a.hblock ? wave : static_cast<int>(threadIdx.x), step = a.hblock ? W : 64 * W;
-    constexpr int PB = kThrough ? 4 : 1;                // pieces a thread has in flight
+    // pieces a thread has in flight: as many as registers are free for (bf16 ones may be rotated or fp32 and take 16
+    // each: 16 rows of 4096 into 4096 12.6 us, with four 13.0; fp16 ones into 12288 17.4 us, with two 17.9)
+    constexpr int PB = !kThrough ? 1 : F16 ? 4 : 2;
     W4Piece piece[PB];
 #pragma unroll
     for (int i = 0; i < PB; ++i) piece[i].load(a, pl, m0, mine + i * step, pieces, 0);
@@ -532,7 +535,7 @@ int launch_rows(const W4A16Args& a, hipStream_t stream) {
         return launch_tiles<F16, Z, G, 1, 1, 4>(a, pl, stream);
     }
     // more rows: one workgroup a compute unit keeps all of x in LDS and goes through the tiles (16 rows of 4096 into
-    // 12288: 20 us, 36 a tile a workgroup; one row that way: 22 against 13 us)
+    // 12288: 17 us, over 30 a tile a workgroup; one row that way: 22 against 13 us)
     return launch_tiles<F16, Z, G, 1, 4, 8>(a, pl, stream);
 }
 
