@@ -532,6 +532,11 @@ int launch_rows(const W4A16Args& a, hipStream_t stream) {
         // one where that would leave units idle (4096 x 4096: 6.8 us, with two 9.2)
         if constexpr (G != 0)
             if ((a.N + 31) / 32 >= 2 * (cus > 0 ? cus : 256)) return launch_tiles<F16, Z, G, 2, 1, 4>(a, pl, stream);
+        // a workgroup a compute unit at most: eight waves, where four would need more than two rounds of their rings (a
+        // rotated row of 12288 into 3072: 15.7 us, with four 25.6; 4096 x 4096: 7.3, with four 6.6) or the pairs are
+        // loaded one by one (groups of 32 there: 9.5 us, with four 12.2)
+        if ((a.N + 15) / 16 <= (cus > 0 ? cus : 256) && (G == 0 || a.K > 2 * 4 * 4 * kBlk))
+            return launch_tiles<F16, Z, G, 1, 1, 8>(a, pl, stream);
         return launch_tiles<F16, Z, G, 1, 1, 4>(a, pl, stream);
     }
     // more rows: one workgroup a compute unit keeps all of x in LDS and goes through the tiles (16 rows of 4096 into

@@ -79,6 +79,17 @@ def test_many_columns(gpu_device, m, n, k, group, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,group,zeros,dtype", [(1, 100, 8192, 64, "none", torch.bfloat16), (3, 333, 5120, 128, "float", torch.float16),
+                                                     (4, 2000, 4160, 64, "u4", torch.float16), (2, 40, 9000 // 32 * 32, 32, "u4", torch.bfloat16),
+                                                     (1, 17, 32768, 128, "u4", torch.float32)])
+def test_few_columns_of_long_rows(gpu_device, m, n, k, group, zeros, dtype):
+    print(f"[w4a16] {m}x{n}x{k} group {group} {zeros} {dtype}", flush=True)
+    qw, ws, wz = _weights(n, k, group, zeros, gpu_device)
+    x = torch.randn((m, k), device=gpu_device).to(dtype)
+    _check(x, qw, ws, wz, None, ck.w4a16_linear(x, qw, ws, wz, group_size=group), group, 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("sdt", [torch.bfloat16, torch.float32])
 def test_types(gpu_device, out, sdt):
