@@ -24,6 +24,7 @@
 #include "mq_device.h"
 #include "mq_internal.h"
 #include "mq_rotate.h"
+#include "mq_w4a16_runs.h"
 
 namespace mq {
 namespace {
@@ -251,19 +252,12 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     };
     // each wave a run of consecutive steps of every chunk, so that it reads whole cache lines of a column; a tile's
     // last step is followed by the next tile's first
-    const int blocks = (K + kBlk - 1) / kBlk, per = (pl.chunk / kBlk + W - 1) / W;
-    int f_tile = blockIdx.x, f_blk = wave * per, f_left = per;   // the next step to fetch, and the steps left in its run
+    const int blocks = (K + kBlk - 1) / kBlk, chunk_steps = pl.chunk / kBlk;
+    const int per = w4_share<W>(chunk_steps), run = w4_run<KB>(per);
+    W4Fetch<kThrough> ahead(blockIdx.x, wave, per);
     auto fetch_next = [&](int i) __attribute__((always_inline)) {
-        if ((!kThrough || f_tile < tiles) && f_blk < blocks) fetch(i, f_tile, f_blk);
-        ++f_blk;
-        if (--f_left == 0) {
-            f_blk += pl.chunk / kBlk - per;
-            f_left = per;
-            if (kThrough && f_blk - wave * per >= blocks) {   // the runs of the last chunk are done
-                f_blk = wave * per;
-                f_tile += gridDim.x;
-            }
-        }
+        if (ahead.any(per, blocks, tiles)) fetch(i, ahead.tile, ahead.blk);
+        ahead.next(wave, per, run, chunk_steps, blocks, gridDim.x);
     };
 #pragma unroll
     for (int i = 0; i < KB; ++i) fetch_next(i);
@@ -436,11 +430,11 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
             }
             const int b0 = k0 / kBlk + wave * per, chunk_end = (k0 + pl.chunk) / kBlk;
             const int b1 = b0 + per < chunk_end ? b0 + per : chunk_end, b2 = b1 < blocks ? b1 : blocks;
-            for (int b = b0; b < b0 + per; b += KB) {
+            for (int b = b0; b < b0 + run; b += KB) {
 #pragma unroll
                 for (int i = 0; i < KB; ++i) {
                     if (b + i < b2) compute(i, b + i, k0, pr);
-                    if (b + i < b0 + per) fetch_next(i);
+                    fetch_next(i);
                 }
             }
         }
