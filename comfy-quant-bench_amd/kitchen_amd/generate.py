@@ -81,14 +81,16 @@ class Decoder:
                        for _ in range(c.layers)]
         self.cache = kv.PagedKVCache(c.layers, pages, c.kv_heads, c.head_dim, page_size, seqs, max_tokens, c.dtype, int8_cache, device)
 
-    def _forward(self, tokens: torch.Tensor, pos: torch.Tensor, cu_q) -> torch.Tensor:
-        """Hidden states of new tokens whose room the cache has; it holds their keys and values afterwards."""
+    def _forward(self, tokens: torch.Tensor, pos: torch.Tensor, cu_q, lens: torch.Tensor) -> torch.Tensor:
+        """Hidden states of new tokens whose room the cache has; it holds their keys and values afterwards. lens: the
+        cache's lengths of the sequences that take part, 0 of the others, whose tokens leave no trace."""
         c = self.config
         x = torch.nn.functional.embedding(tokens, self.embedding) * c.hidden ** 0.5
         for i, layer in enumerate(self.layers):
             q, k, v = layer["qkv"](_norm(x)).view(len(tokens), -1, c.head_dim).split([c.heads, c.kv_heads, c.kv_heads], 1)
-            self.cache.write(i, _turn(k, pos), v, cu_q)
-            y = self.cache.attend(i, _turn(q, pos), cu_q, window=c.window if i % 2 else None, sinks=c.sinks)
+            self.cache.write(i, _turn(k, pos), v, cu_q, lens=lens)
+            y = self.cache.attend(i, _turn(q, pos), cu_q, window=c.window if i % 2 else None, sinks=c.sinks,
+                                  lens=lens)
             x = x + layer["out"](y.view(len(tokens), -1))
             gate, up = layer["up"](_norm(x)).chunk(2, -1)
             x = x + layer["down"](torch.nn.functional.silu(gate) * up)
@@ -98,7 +100,8 @@ class Decoder:
         return torch.nn.functional.linear(x, self.embedding)
 
     def prompt(self, prompts: dict[int, list[int]]) -> torch.Tensor:
-        """New tokens (or a chunk of them) for some of the sequences; logits [len(prompts), vocab] behind the last of each."""
+        """New tokens (or a chunk of them) for some of the sequences; logits [len(prompts), vocab] behind the last of each.
+        Without room for all of them the cache stays as it is (cache.check() raises) and the logits say nothing."""
         cache, dev = self.cache, self.embedding.device
         rows = sorted(prompts)
         news = [len(prompts.get(b, ())) for b in range(cache.lens.shape[0])]
@@ -106,15 +109,19 @@ class Decoder:
         cu_q = torch.tensor([0] + news, device=dev).cumsum(0).to(torch.int32)
         tokens = torch.tensor([t for b in rows for t in prompts[b]], device=dev)
         seq = torch.tensor([b for b in rows for _ in prompts[b]], device=dev)
-        pos = cache.lens[seq] - cu_q[seq + 1] + torch.arange(len(tokens), device=dev)
-        x = self._forward(tokens, pos, cu_q)
+        lens = cache.lens * (cache.status == 0)          # nothing is written where nothing has grown
+        pos = lens[seq] - cu_q[seq + 1] + torch.arange(len(tokens), device=dev)
+        x = self._forward(tokens, pos, cu_q, lens)
         return self._logits(x[(cu_q[1:][rows] - 1).long()])
 
     def step(self, tokens: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
-        """A token more for the sequences `rows` (tokens [seqs], any value for the others); logits [seqs, vocab]."""
+        """A token more for the sequences `rows` (tokens [seqs], any token for the others, which keep what they hold);
+        logits [seqs, vocab]. Without room for all of them the cache stays as it is (cache.check() raises)."""
         cache = self.cache
         cache.grow(rows, torch.ones_like(rows))
-        return self._logits(self._forward(tokens, cache.lens - 1, None))
+        takes = (torch.arange(len(cache.lens), device=rows.device)[:, None] == rows).any(1) & (cache.status == 0)
+        lens = cache.lens * takes
+        return self._logits(self._forward(tokens, lens - 1, None, lens))
 
 
 def main(argv: list[str] | None = None) -> int:

@@ -357,11 +357,15 @@ class PagedKVCache:
         if code < 0:
             raise ValueError("a sequence is out of range, given twice, not empty, or too long for its page table")
 
-    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor | None = None) -> None:
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor | None = None,
+              lens: torch.Tensor | None = None) -> None:
+        """lens: other lengths than the cache's own, such as 0 for a sequence that gets no token in this call."""
         kc, vc, ks, vs = self._layer(layer)
-        kv_write(k, v, kc, vc, self.page_table, self.lens, cu_q, ks, vs)
+        kv_write(k, v, kc, vc, self.page_table, self.lens if lens is None else lens, cu_q, ks, vs)
 
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor | None = None, scale: float | None = None,
-               window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+               window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,
+               lens: torch.Tensor | None = None) -> torch.Tensor:
         kc, vc, ks, vs = self._layer(layer)
-        return paged_attention(q, kc, vc, self.page_table, self.lens, cu_q, scale, window, sinks, ks, vs, out)
+        return paged_attention(q, kc, vc, self.page_table, self.lens if lens is None else lens, cu_q, scale, window, sinks,
+                               ks, vs, out)
