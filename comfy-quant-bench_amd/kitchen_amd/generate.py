@@ -102,6 +102,8 @@ class Decoder:
     def prompt(self, prompts: dict[int, list[int]]) -> torch.Tensor:
         """New tokens (or a chunk of them) for some of the sequences; logits [len(prompts), vocab] behind the last of each.
         Without room for all of them the cache stays as it is (cache.check() raises) and the logits say nothing."""
+        if not prompts or not all(prompts.values()):
+            raise ValueError("a prompt needs tokens")
         cache, dev = self.cache, self.embedding.device
         rows = sorted(prompts)
         news = [len(prompts.get(b, ())) for b in range(cache.lens.shape[0])]

@@ -62,3 +62,12 @@ def test_a_step_without_room_changes_nothing(gpu_device):
     with pytest.raises(Exception, match="1 pages short"):
         model.cache.check()
     assert all(torch.equal(a, b) for a, b in zip(before, _state(model)))
+
+
+@pytest.mark.gpu
+def test_prompts_without_tokens_are_refused(gpu_device):
+    model = generate.Decoder(small(layers=1), seqs=2, pages=3, max_tokens=128)
+    for prompts in ({}, {0: [1, 2], 1: []}):
+        with pytest.raises(ValueError, match="tokens"):
+            model.prompt(prompts)
+    assert not model.cache.lens.any()
