@@ -100,6 +100,13 @@ def _cache_args(k, v, ks, vs, like: torch.Tensor, heads: int | None):
     return pages, h, page, (k.data_ptr(), v.data_ptr(), _CODE[dt], c0, c1, c2, *sp, pages, page)
 
 
+def _apart(page_table: torch.Tensor) -> torch.Tensor:
+    """A table that is only read, its rows behind each other (copied where they overlap, as an expanded one's do)."""
+    if page_table.dim() == 2 and page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+        return page_table.contiguous()
+    return page_table
+
+
 def _table_args(page_table, kv_lens, cu_q, tokens: int, dev):
     """The library's arguments of the tables: (page_table, ld, sequences, width, lens, cu_q)."""
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev:
@@ -135,6 +142,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     k, v = _rows(k, "k"), _rows(v, "v")
     t, h, d = k.shape
     pages, _, _, cache = _cache_args(k_cache, v_cache, k_scale, v_scale, k, h)
+    page_table = _apart(page_table)
     tables = _table_args(page_table, kv_lens, cu_q, t, dev)
     _lib.call("mq_kv_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
               _CODE[k.dtype], t, h, d, *cache, *tables, _lib.stream_of_device(dev))
@@ -156,6 +164,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     pages, h, _, cache = _cache_args(k_cache, v_cache, k_scale, v_scale, q, None)
     if h == 0 or heads % h:
         raise ValueError(f"{heads} query heads for {h} cache heads: expected a multiple")
+    page_table = _apart(page_table)
     tables = _table_args(page_table, kv_lens, cu_q, t, dev)
     if window is not None and window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 (None: no window) and sinks at least 0, got {window} and {sinks}")
@@ -201,6 +210,8 @@ def _tables(page_table, lens, refs):
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError("page_table must be int32 [sequences, width] with contiguous rows")
     rows, width = page_table.shape
+    if rows > 1 and page_table.stride(0) < width:
+        raise ValueError(f"the rows of page_table must not overlap (strides {page_table.stride()})")
     for t, n, what in ((lens, rows, "lens"), (refs, None, "refs")):
         if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.device != dev or not t.is_contiguous()
                               or (n is not None and t.shape[0] != n)):

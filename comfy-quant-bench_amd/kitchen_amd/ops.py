@@ -777,6 +777,11 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 W4A16_GROUPS = (32, 64, 128)
 
 
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """[n, k] with contiguous rows behind each other (copied where they overlap, as an expanded tensor's do)."""
+    return t if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
 def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, wzeros=None, bias=None,
                  group_size: int = INT4_GROUP_SIZE, convrot_groupsize: int | None = None, out_dtype=None) -> torch.Tensor:
     """``x @ W.T + bias`` with 4-bit weights and activations in floating point, for few rows (one token each of a
@@ -807,7 +812,7 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
         x2 = x2.clone()
     if wscales.shape != (n, groups) or wscales.dtype not in FLOAT_TYPES:
         raise ValueError(f"wscales must be floating-point [{n}, {groups}], got {wscales.dtype} {list(wscales.shape)}")
-    ws = wscales if wscales.stride(1) == 1 else wscales.contiguous()
+    ws = _rows_apart(wscales)
     qw = qweight if qweight.stride(1) == 1 and qweight.stride(0) % 16 == 0 and qweight.data_ptr() % 16 == 0 \
         else qweight.contiguous()
     zero, zdt, zptr, ldz = _lib.W4Z_SIGNED, _lib.DT_BF16, None, 0
@@ -822,7 +827,7 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
             raise ValueError(f"zero-points must be {list(want)}, got {list(wzeros.shape)}")
         if wzeros.device != dev:
             raise ValueError(f"x is on {dev}, the weights are not")
-        wz = wzeros if wzeros.stride(1) == 1 else wzeros.contiguous()
+        wz = _rows_apart(wzeros)
         zptr, ldz = wz.data_ptr(), max(wz.stride(0), want[1])
     if qw.device != dev or ws.device != dev:
         raise ValueError(f"x is on {dev}, the weights are not")
