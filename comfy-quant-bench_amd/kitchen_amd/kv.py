@@ -227,7 +227,7 @@ def _status_ptr(status, dev):
     return status.data_ptr()
 
 
-def _layers(k, v, ks, vs, pages: int):
+def _layers(k, v, ks, vs, pages: int, dev):
     """(page_size, the library's arguments of whole caches [layers, pages, kv_heads, page_size, head_dim], or one
     layer without the first dimension): every page one block of memory."""
     def block(t, dims, what):
@@ -246,6 +246,8 @@ def _layers(k, v, ks, vs, pages: int):
 
     if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
         raise ValueError("k and v must be alike")
+    if any(t is not None and t.device != dev for t in (k, ks, vs)):
+        raise ValueError(f"the caches and their scales must be on {dev}, like page_table")
     k5, args = block(k, 5, "the caches")
     sargs = (None, None, 0, 0, 0)
     if (ks is None) != (vs is None) or (k.dtype == torch.int8) != (ks is not None):
@@ -273,7 +275,7 @@ def kv_fork(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: to
     of range, given twice or not empty; nothing has changed unless it is 0."""
     dev, *tab = _tables(page_table, lens, refs)
     pages = refs.shape[0]
-    page, cache = _layers(k, v, k_scale, v_scale, pages)
+    page, cache = _layers(k, v, k_scale, v_scale, pages, dev)
     s, d = _index(src, dev, "src"), _index(dst, dev, "dst")
     n = s.shape[0]
     if d.shape[0] != n:
@@ -314,7 +316,7 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, refs:
     Returns n, int32 [1] on the device."""
     dev, *tab = _tables(page_table, None, refs)
     pages = refs.shape[0]
-    _, cache = _layers(k, v, k_scale, v_scale, pages)
+    _, cache = _layers(k, v, k_scale, v_scale, pages, dev)
     live = torch.empty(1, dtype=torch.int32, device=dev)
     stream = _lib.stream_of_device(dev)
     work, nbytes = _kv_scratch(pages, 0, dev, stream)
