@@ -95,7 +95,7 @@ constexpr int kPlan = 1024;
 constexpr int kSeenRows = 1 << 16;   // rows per window of the bitmap below
 
 struct PlanShared {
-    int wave[kPlan / 64];
+    int64_t wave[kPlan / 64];
     int bad;
     uint32_t seen[kSeenRows / 32];
 };
@@ -125,20 +125,21 @@ __device__ void check_distinct(const int* rows, const int* others, int n, int64_
     }
 }
 
-// Exclusive prefix sum over the workgroup; *total = the sum.
-__device__ __forceinline__ int block_scan(int v, PlanShared& sh, int* total) {
+// Exclusive prefix sum over the workgroup; *total = the sum (T: int, or int64_t where it may pass 32 bits).
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, PlanShared& sh, T* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+    T x = v;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-        const int y = __shfl_up(x, s);
+        const T y = __shfl_up(x, s);
         if (lane >= s) x += y;
     }
     if (lane == 63) sh.wave[wave] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    T before = 0, all = 0;
     for (int w = 0; w < kPlan / 64; ++w) {
-        const int y = sh.wave[w];
+        const T y = static_cast<T>(sh.wave[w]);
         if (w < wave) before += y;
         all += y;
     }
@@ -158,7 +159,7 @@ __device__ int find_free(const int* refs, int64_t pages, int need, int* list, Pl
         for (int j = 0; j < kPer; ++j)
             if (p + j < pages && refs[p + j] == 0) free |= 1u << j;
         int total;
-        int at = found + block_scan(__popc(free), sh, &total);
+        int at = found + block_scan<int>(__popc(free), sh, &total);
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
             if ((free >> j) & 1) {
@@ -274,11 +275,11 @@ __global__ void __launch_bounds__(kPlan) grow_plan_kernel(KvTables a, const int*
             }
             if (bad) { sh.bad = 1; more = 0; }
         }
-        int total;
-        const int at = static_cast<int>(need) + block_scan(more, sh, &total);
-        if (i < n) first[i] = at;
+        // 1024 sequences of 2^21 pages each pass 32 bits; places past `pages` are not used (nothing is changed then)
+        int64_t total;
+        const int64_t at = need + block_scan<int64_t>(more, sh, &total);
+        if (i < n) first[i] = at < a.pages ? static_cast<int>(at) : 0;
         need += total;
-        if (need > a.pages) break;                          // more than there can be (the same for all threads)
     }
     check_distinct(rows, nullptr, n, a.rows, sh);
     __syncthreads();
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(int* refs, int64_t 
                 place[p + j] = static_cast<int>(p + j);
             }
         int th, tm;
-        int ah = holes + block_scan(__popc(hole), sh, &th), am = movers + block_scan(__popc(mover), sh, &tm);
+        int ah = holes + block_scan<int>(__popc(hole), sh, &th), am = movers + block_scan<int>(__popc(mover), sh, &tm);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             if ((hole >> j) & 1) moves[2 * ah++ + 1] = static_cast<int>(p + j);
