@@ -104,9 +104,12 @@ __device__ __forceinline__ float receive1(const float* p) {
 }
 
 // Sixteen bytes per active lane from `src` to LDS bytes dst + 16 lane (dst the same in all lanes). Written as asm: the
-// compiler would wait for the builtin's stores before any LDS read that it cannot tell apart.
+// compiler would wait for the builtin's stores before any LDS read that it cannot tell apart. m0, which says where to,
+// is left as it was: the compiler may keep a value there and takes no word that it is overwritten (it is reserved).
 __device__ __forceinline__ void load_lds16(const char* src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory");
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
