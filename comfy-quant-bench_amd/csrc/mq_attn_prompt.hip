@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     uint32_t vr[I8 ? 4 : 1][VW];
     float sc = 0.0f;
     // 16-bit caches: keys and values of the tile in sm.at[ring] straight into half `buf`, rows as they are, 16-byte
-    // chunk c of key k at c ^ kswap(k) and c ^ vswap(k). What is wider than the heads is not written (the keys' zeros stay).
+    // chunk c of key k at c ^ kswap(k) and c ^ vswap(k). What is wider than the heads is not written (zeros stay there).
     const int slot = tid % kPerKey;
     auto kswap = [](int key) { return key & 7; };
     auto vswap = [](int key) { return DP == 64 ? 4 * (key >> 1 & 1) : 4 * (key & 3); };
@@ -522,9 +522,12 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
             put_codes(1, i0 + 1, look_up(i0 + 1));
         }
         if (tid == 0) sm.wild = 0;
-        if constexpr (!I8) {                            // what no load writes: keys beyond the heads' width
+        if constexpr (!I8) {                            // what no load writes: keys and values beyond the heads' width
             if (8 * kPerKey > a.D)
-                for (int e = tid; e < 2 * kTile * kPerKey; e += 256) reinterpret_cast<uint4*>(sm.k[0])[e] = make_uint4(0, 0, 0, 0);
+                for (int e = tid; e < 2 * kTile * kPerKey; e += 256) {
+                    reinterpret_cast<uint4*>(sm.k[0])[e] = make_uint4(0, 0, 0, 0);
+                    reinterpret_cast<uint4*>(sm.v[0])[e] = make_uint4(0, 0, 0, 0);
+                }
         }
         __syncthreads();
         // a tile that some row sees in part, or with keys that are not held
