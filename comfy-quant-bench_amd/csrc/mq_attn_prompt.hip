@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
     float m = kNegInf, l = 0.0f;                        // reference maximum (of the scaled scores), sum of the lane's keys
     bool any = false;
     // the scores' scale, its sign moved into the query rows; a scale of 0 as one too small to tell, so that a
-    // hidden score's -infinity stays one
-    const float scale = __builtin_fmaxf(__builtin_fabsf(a.scale * kLog2e), 0x1p-100f);
+    // hidden score's -infinity stays one (a NaN stays a NaN)
+    const float size = __builtin_fabsf(a.scale * kLog2e), scale = size < 0x1p-100f ? 0x1p-100f : size;
 
     const int* table = a.table + b * a.ld_table;
     const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
@@ -657,17 +657,18 @@ __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2) attn_prompt_kernel(Att
         }
     }
     if (wrow + q <= most && wrow <= most) {
-        const float inv = any ? 1.0f / l : 0.0f;        // nothing seen: zeros
+        const float inv = 1.0f / l;
         uint16_t* out = static_cast<uint16_t*>(a.o) + (tok0 + tok) * a.o_token + (h * group + myrow % group) * a.o_head;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int d = 32 * i + 8 * r4 + 4 * hf;
+                // nothing seen: zeros (hidden scores leave o as it was, but a scale that is NaN makes NaN of them too)
                 if (d < a.D)
                     *reinterpret_cast<uint2*>(out + d) =
-                        make_uint2(pack_16x2(o[i][4 * r4] * inv, o[i][4 * r4 + 1] * inv, DT),
-                                   pack_16x2(o[i][4 * r4 + 2] * inv, o[i][4 * r4 + 3] * inv, DT));
+                        make_uint2(any ? pack_16x2(o[i][4 * r4] * inv, o[i][4 * r4 + 1] * inv, DT) : 0u,
+                                   any ? pack_16x2(o[i][4 * r4 + 2] * inv, o[i][4 * r4 + 3] * inv, DT) : 0u);
             }
     }
 }
