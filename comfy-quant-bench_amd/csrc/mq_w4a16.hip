@@ -3,10 +3,12 @@
 // unpacking them: at 8 TB/s a SIMD has some 78 VALU operations for the 1 KB of a wave's step.
 //
 // The codes go through MFMA as 16-bit floats without being scaled first (a scaled weight would be rounded):
-// bits of a code are or-ed into the mantissa of a constant, which makes 128 + c in bf16 (1024 + c in fp16), seven
+// bits of a code are or-ed into the mantissa of a constant, which makes 16 + c in bf16 (1024 + c in fp16), eight
 // operations for the eight codes of a dword. What is too much is taken off exactly: in fp16 by a packed
-// subtraction (which takes the zero-point with it), in bf16 behind the product, where acc - (128 + z) sum(x)
-// needs the group's sum of x, a product with ones. Each group's fp32 sum is then scaled into the output's.
+// subtraction (which takes the zero-point with it), in bf16 behind the product, where acc - (16 + z) sum(x)
+// needs the group's sum of x, a product with ones. Both sums are rounded to fp32 at up to 31 |x| a value, so 16, the
+// least that has mantissa bits for a code, loses the least: 1.5e-7 of an fp32 output, 4096 normal values a row (128 + c,
+// one operation less, 13.4 us for 13.6 below: 7e-7). Each group's fp32 sum is then scaled into the output's.
 // Rows of x that have more bits than the 16-bit type are split into as many rows as hold them (fp32: three
 // bf16 rows, exactly), which the 16 rows of a product have room for, and the rows' outputs are added at the end.
 //
@@ -326,7 +328,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     __builtin_amdgcn_sched_barrier(0);
 
     // and-or takes one constant from a scalar register and one from a vector register, none from the instruction
-    uint32_t magic = F16 ? 0x64006400u : 0x43004300u, low = 0x000f000fu;
+    uint32_t magic = F16 ? 0x64006400u : 0x41804180u, low = F16 ? 0x000f000fu : 0x00780078u;
     asm volatile("" : "+v"(magic));
     asm volatile("" : "+s"(low));
     constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
@@ -373,7 +375,11 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
                 for (int t = 0; t < CT; ++t) {
                     W4Frag f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f.w[e] = ((v[t][j] >> (4 * e)) & low) | magic;
+                    for (int e = 0; e < 4; ++e) {
+                        // nibbles e and e + 4: to the lowest mantissa bits (fp16), or three above them
+                        const uint32_t n = F16 ? v[t][j] >> (4 * e) : e == 0 ? v[t][j] << 3 : v[t][j] >> (4 * e - 3);
+                        f.w[e] = (n & low) | magic;
+                    }
                     if constexpr (F16) {
                         // 1024 + c - (1024 + z): exact
                         const _Float16 off = static_cast<_Float16>(-1024.0f - (Z == W4Zero::Float ? 0.0f : zp[t]));
@@ -388,7 +394,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
             }
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
-                const float off = -128.0f - (Z == W4Zero::Float ? 0.0f : zp[t]);
+                const float off = -16.0f - (Z == W4Zero::Float ? 0.0f : zp[t]);
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
                     const float d = F16 ? acc[t][e] : __builtin_fmaf(off, sum[e], acc[t][e]);
