@@ -405,6 +405,42 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
         }
     };
 
+    // The wave's steps b0 .. b2 - 1 of a chunk as the formula stands, weight by weight in fp32, for the sums that are not
+    // finite: a shifted code's infinity less the shift's is NaN where the weight's alone is an infinity (or, for values
+    // near the end of the range, finite).
+    auto plain = [&](int tile, int b0, int b2, int k0, const Pair* pr, const w4_f32x4 (&before)[CT]) {
+#pragma unroll 1
+        for (int t = 0; t < CT; ++t) {
+            const int64_t n = static_cast<int64_t>(tile) * kCols + 16 * t + c;
+            const uint8_t* col = a.qw + (n < a.N ? n : a.N - 1) * a.ldw;
+            w4_f32x4 s = before[t];
+#pragma unroll 1
+            for (int k = b0 * kBlk; k < b2 * kBlk && k < K; k += 8) {
+                const uint32_t codes = *reinterpret_cast<const uint32_t*>(col + k / 2);
+                const Pair p = pr[(16 * t + c) * pitch + (k >> gshift)];
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    int code = codes >> (4 * i) & 15;
+                    if constexpr (Z == W4Zero::Signed) code = (code ^ 8) - 8;
+                    const float w = Z == W4Zero::Signed ? p.scale() * static_cast<float>(code)
+                                    : Z == W4Zero::U4   ? p.scale() * (static_cast<float>(code) - p.zero())
+                                                        : __builtin_fmaf(p.scale(), static_cast<float>(code), p.zero());
+                    const uint16_t* x = xs + (k - k0) + (i < 4 ? 2 * i : 2 * i - 7);    // in the order of the codes
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) {
+                        const uint32_t h = x[(4 * e + g < all ? 4 * e + g : 0) * stride];
+                        s[e] = __builtin_fmaf(as_float(h, F16 ? kDtF16 : kDtBf16), w, s[e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < CT; ++u)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+                    if (u == t && !__builtin_isfinite(y[u][e])) y[u][e] = s[e];
+        }
+    };
+
     // A workgroup of eight waves takes every gridDim.x-th tile; x is staged once if it fits (one chunk), else for every tile anew.
     store_pairs(blockIdx.x, pairs);
     bool staged = false;
@@ -436,6 +472,9 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
             }
             const int b0 = k0 / kBlk + wave * per, chunk_end = (k0 + pl.chunk) / kBlk;
             const int b1 = b0 + per < chunk_end ? b0 + per : chunk_end, b2 = b1 < blocks ? b1 : blocks;
+            w4_f32x4 before[CT];
+#pragma unroll
+            for (int t = 0; t < CT; ++t) before[t] = y[t];
             for (int b = b0; b < b0 + run; b += KB) {
 #pragma unroll
                 for (int i = 0; i < KB; ++i) {
@@ -443,6 +482,12 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
                     fetch_next(i);
                 }
             }
+            bool wild = false;
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int e = 0; e < NE; ++e) wild |= !__builtin_isfinite(y[t][e]);
+            if (__ballot(wild)) plain(tile, b0, b2, k0, pr, before);
         }
         if (more) store_pairs(tile + gridDim.x, pairs + (buf ^ 1) * kCols * pitch);
         // the waves' sums, once the last tile's have been read
