@@ -813,8 +813,9 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     if wscales.shape != (n, groups) or wscales.dtype not in FLOAT_TYPES:
         raise ValueError(f"wscales must be floating-point [{n}, {groups}], got {wscales.dtype} {list(wscales.shape)}")
     ws = _rows_apart(wscales)
-    qw = qweight if qweight.stride(1) == 1 and qweight.stride(0) % 16 == 0 and qweight.data_ptr() % 16 == 0 \
-        else qweight.contiguous()
+    qw = _rows_apart(qweight)
+    if qw.stride(0) % 16 or qw.data_ptr() % 16:
+        qw = qw.clone(memory_format=torch.contiguous_format)
     zero, zdt, zptr, ldz = _lib.W4Z_SIGNED, _lib.DT_BF16, None, 0
     if wzeros is not None:
         if wzeros.dtype in FLOAT_TYPES:

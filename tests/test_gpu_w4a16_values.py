@@ -107,3 +107,17 @@ def test_more_rows_than_a_grid_has(gpu_device):
     qw, ws, wz = weights(16, 64, 64, "u4", gpu_device)
     x = torch.randn((600000, 64), device=gpu_device).to(torch.bfloat16)
     check(ck.w4a16_linear(x, qw, ws, wz, None, 64, 64), x, qw, ws, wz, 64, 64)
+
+
+@pytest.mark.gpu
+def test_weights_at_any_place(gpu_device):
+    """Packed weights that begin between 16-byte boundaries, and one row of them for every column."""
+    qw, ws, wz = weights(50, 512, 64, "u4", gpu_device)
+    x = torch.randn((2, 512), device=gpu_device).to(torch.bfloat16)
+    want = ck.w4a16_linear(x, qw, ws, wz)
+    for shift in (1, 8):
+        flat = torch.zeros(50 * 256 + shift, dtype=torch.uint8, device=gpu_device)
+        flat[shift:] = qw.reshape(-1)
+        assert torch.equal(ck.w4a16_linear(x, flat[shift:].view(50, 256), ws, wz), want)
+    one = qw[:1].expand(50, 256)
+    assert torch.equal(ck.w4a16_linear(x, one, ws, wz), ck.w4a16_linear(x, one.contiguous(), ws, wz))
