@@ -176,6 +176,12 @@ KvTables tables_of(int32_t* table, int64_t ld_table, int64_t rows, int64_t width
     return t;
 }
 
+// A fork or growth of no sequence: done, which *status says in the order of the stream.
+int empty_plan(int32_t* status, void* stream) {
+    MQ_REQUIRE(aligned(status, 4), "status must be 4-byte aligned");
+    return status ? launch_kv_grow(KvTables{}, nullptr, nullptr, 0, nullptr, status, static_cast<hipStream_t>(stream)) : MQ_OK;
+}
+
 // The caches that a fork or a compaction copies pages of.
 int copies_of(const char* what, void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t pitch, int64_t bytes,
               float* ks, float* vs, int64_t s_layer, int64_t s_pitch, int64_t s_bytes, int64_t pages, KvCopyArgs* out) {
@@ -226,7 +232,8 @@ int mq_kv_fork(void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t pa
     KvCopyArgs c;
     rc = copies_of("kv_fork", k, v, layers, layer_bytes, page_pitch, page_bytes, k_scale, v_scale, s_layer_bytes,
                    s_page_pitch, s_page_bytes, pages, &c);
-    if (rc || n == 0) return rc;
+    if (rc) return rc;
+    if (n == 0) return empty_plan(status, stream);
     MQ_REQUIRE(src && dst && aligned(src, 4) && aligned(dst, 4) && aligned(status, 4), "kv_fork: src and dst must be non-null and 4-byte aligned");
     rc = check_work("kv_fork", workspace, workspace_bytes, pages, n);
     if (rc) return rc;
@@ -239,7 +246,8 @@ int mq_kv_grow(int32_t* page_table, int64_t ld_table, int64_t rows, int64_t widt
                void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
     int rc = check_tables("kv_grow", page_table, ld_table, rows, width, lens, refs, pages, page_size, n);
-    if (rc || n == 0) return rc;
+    if (rc) return rc;
+    if (n == 0) return empty_plan(status, stream);
     MQ_REQUIRE(seqs && counts && aligned(seqs, 4) && aligned(counts, 4) && aligned(status, 4),
                "kv_grow: the sequences and counts must be non-null and 4-byte aligned");
     rc = check_work("kv_grow", workspace, workspace_bytes, pages, n);

@@ -33,3 +33,15 @@ def test_grow_by_more_pages_than_32_bits_count(gpu_device):
         ck.kv_grow(table, lens, refs, range(1024), counts, 1, status)
         assert int(status) == 0x7fffffff
         assert lens[:-1].sum() == 0 and int(lens[-1]) == 1 - more and not refs.any() and (table[:, :8] == -1).all()
+
+
+@pytest.mark.gpu
+def test_a_call_for_no_sequence_is_done(gpu_device):
+    """The status of a growth or fork of nothing is 0, whatever the one before it was."""
+    c = ck.PagedKVCache(1, 2, 1, 8, 4, 3, 64, device=gpu_device)
+    for call in (lambda: c.grow([], []), lambda: c.fork([], [])):
+        c.grow([0], [60])
+        assert int(c.status) == 13
+        call()
+        assert int(c.status) == 0
+        c.check()
