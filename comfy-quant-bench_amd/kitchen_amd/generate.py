@@ -107,11 +107,12 @@ class Decoder:
         cache, dev = self.cache, self.embedding.device
         rows = sorted(prompts)
         news = [len(prompts.get(b, ())) for b in range(cache.lens.shape[0])]
+        before = cache.lens.clone()
         cache.grow(rows, [news[b] for b in rows])
         cu_q = torch.tensor([0] + news, device=dev).cumsum(0).to(torch.int32)
         tokens = torch.tensor([t for b in rows for t in prompts[b]], device=dev)
         seq = torch.tensor([b for b in rows for _ in prompts[b]], device=dev)
-        lens = cache.lens * (cache.status == 0)          # nothing is written where nothing has grown
+        lens = cache.lens * (cache.lens > before)        # nothing is written where nothing has grown
         pos = lens[seq] - cu_q[seq + 1] + torch.arange(len(tokens), device=dev)
         x = self._forward(tokens, pos, cu_q, lens)
         return self._logits(x[(cu_q[1:][rows] - 1).long()])
@@ -119,10 +120,9 @@ class Decoder:
     def step(self, tokens: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
         """A token more for the sequences `rows` (tokens [seqs], any token for the others, which keep what they hold);
         logits [seqs, vocab]. Without room for all of them the cache stays as it is (cache.check() raises)."""
-        cache = self.cache
+        cache, before = self.cache, self.cache.lens.clone()
         cache.grow(rows, torch.ones_like(rows))
-        takes = (torch.arange(len(cache.lens), device=rows.device)[:, None] == rows).any(1) & (cache.status == 0)
-        lens = cache.lens * takes
+        lens = cache.lens * (cache.lens > before)        # nothing is written where nothing has grown
         return self._logits(self._forward(tokens, lens - 1, None, lens))
 
 
