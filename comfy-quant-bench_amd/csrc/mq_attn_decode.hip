@@ -9,10 +9,14 @@
 //                     each 32; B: the query heads' rows. Lane (c, g) gets query row c, keys 4 g + r (r < 4).
 //   softmax           in base 2 over the running maximum of query row c: 8 scores a lane, joined over the four
 //                     lanes that hold the row.
-//   O^T = V^T P^T     a lane's 8 probabilities are the B operand as they are (the keys of a product may come in any
+//   O^T = V^T P^T     a lane's 8 probabilities, rounded to 16 bits, are the B operand (the keys of a product may come in any
 //                     order, so slot (g, j) is key 16 (j / 4) + 4 g + j % 4); for A a lane loads the same 8 keys'
 //                     values VE c .. VE c + VE - 1 (VE = width / 16, so 16 lanes read a whole row) and pairs the
-//                     keys' 16-bit values with v_perm. Product i gives values VE m + i of row m.
+//                     keys' 16-bit values with v_perm. Product i gives values VE m + i of row m. The rounding is
+//                     relative 2^-9 (bf16) or 2^-12 each, of random signs, in sums of thousands: 131071 bf16
+//                     tokens come out 2.2e-3 from the exact result, 1.7e-3 if only the output were rounded; the sum
+//                     that divides is of the unrounded ones. fp16 rows over an int8 cache, whose products are bf16,
+//                     take what is rounded off in a second product.
 //
 // A workgroup's eight waves (four for heads of more than 128 values, whose operands take twice the registers) take
 // 32 keys each of a tile, one workgroup a compute unit. The tiles of all sequences and cache heads are

@@ -2,8 +2,8 @@
 //
 // Bound by MFMA and VALU together, which barely run side by side on this part: a wave's 64 keys of 32 rows are 32
 // products of 32 cycles (D = 128) and about 1000 cycles of softmax, of which the exponentials are half (two
-// waves' softmax beside each other's products, interleaved by hand, was slower). Long prompts: 880 TFLOP/s (8192
-// tokens, 32 heads of 128: 625 us; a large library matrix product reaches 1190).
+// waves' softmax beside each other's products, interleaved by hand, was slower). Long prompts: 840 to 880
+// TFLOP/s from card to card (8192 tokens, 32 heads of 128: 624 to 654 us; a large library matrix product reaches 1190).
 //
 // A workgroup of four waves takes 128 rows of one cache head: row = (new token, query head of the group),
 // token-major, so the heads that share keys and values share their tiles too and a short prompt fills a tile.
@@ -14,10 +14,14 @@
 //   S^T = K Q^T      32x32x16 products. A: 32 keys, from LDS rows of 16-byte chunks (chunk x of key k at
 //                    x ^ (k & 7): eight lanes read all banks). B: 32 query rows, kept in registers. Lane (q, h)
 //                    = (l & 31, l >> 5) gets row q, keys 8 (r / 4) + 4 h + r % 4, r < 16.
-//   softmax          in base 2, row by row in one lane and its partner l ^ 32. The reference maximum is only
+//   softmax          in base 2 and fp32, row by row in one lane and its partner l ^ 32. The reference maximum is only
 //                    moved (and the sums rescaled) when a row's maximum exceeds it by 2^8: any reference gives
 //                    the same quotient, and fp32 sums have the range.
-//   O^T = V^T P^T    B: a lane's 8 probabilities of keys 16 t + 4 h + {0 .. 3, 8 .. 11} as they are; A: V^T from
+//   O^T = V^T P^T    B: a lane's 8 probabilities of keys 16 t + 4 h + {0 .. 3, 8 .. 11}, rounded to the products'
+//                    16 bits: relative 2^-9 (bf16) or 2^-12 each, of random signs, so less than the output's own
+//                    rounding (8192 tokens of bf16: 2.0e-3 from the exact result, 1.5e-3 if only the output were
+//                    rounded; a second product of what is rounded off would double the MFMA work of this half). The
+//                    sum that divides is of the unrounded ones. fp16 ones are held 2^7 times as large; A: V^T from
 //                    LDS in just that order: 16-bit caches lie there as in the pages and are transposed by the
 //                    LDS reads (16 lanes exchange 4 keys x 16 values); int8 ones are transposed by v_perm on the
 //                    way in, where they become bf16.

@@ -8,19 +8,21 @@
 // subtraction (which takes the zero-point with it), in bf16 behind the product, where acc - (16 + z) sum(x)
 // needs the group's sum of x, a product with ones. Both sums are rounded to fp32 at up to 31 |x| a value, so 16, the
 // least that has mantissa bits for a code, loses the least: 1.5e-7 of an fp32 output, 4096 normal values a row (128 + c,
-// one operation less, 13.4 us for 13.6 below: 7e-7). Each group's fp32 sum is then scaled into the output's.
+// one operation less, 0.2 us of the 13.9 below: 7e-7). Each group's fp32 sum is then scaled into the output's.
 // Rows of x that have more bits than the 16-bit type are split into as many rows as hold them (fp32: three
 // bf16 rows, exactly), which the 16 rows of a product have room for, and the rows' outputs are added at the end.
 //
 // A workgroup owns 16 CT output columns; its W waves share the K values, 128 at a time: lane (c, g) reads the
 // 16 bytes of column c that hold values 32 g .. 32 g + 31 (64 bytes of each of 16 rows a load), and two exchanges
 // of lane and register index bits leave in register j the dword of values 32 j + 8 g. A wave keeps KB steps'
-// loads in flight in a ring of registers. x is staged in LDS, as much of it as fits, in the order of the unpacked
+// loads in flight in a ring of registers (in which order: mq_w4a16_runs.h). x is staged in LDS, as much of it as fits, in the order of the unpacked
 // codes (0 4 1 5 2 6 3 7); the waves' sums are added there at the end. Row 4 e + g of x is row 4 g + e of
 // a product, so that up to 4 rows come out in one register of every lane, up to 16 in four.
 //
-// Measured: 4096 x 4096, one row: 6.8 us (the launch and one round of loads); 3072 -> 18432, one rotated row: 13.4 us,
-// 2.3 TB/s, bound by unpacking and the latency of the few rounds that each workgroup has.
+// Sums that are not finite are added again weight by weight (plain): the shifts would make NaN of an infinity.
+//
+// Measured: 4096 x 4096, one row: 6.0 us (the launch and one round of loads); 3072 -> 18432, one rotated row: 13.9 us,
+// 2.2 TB/s, bound by unpacking and the latency of the few rounds that each workgroup has.
 #include <type_traits>
 
 #include "mq_device.h"
@@ -228,7 +230,7 @@ w4a16_kernel(W4A16Args a, W4Plan pl) {
     const int pieces = rows * (pl.chunk / (a.hblock ? 1024 : 8));
     const int mine = a.hblock ? wave : static_cast<int>(threadIdx.x), step = a.hblock ? W : 64 * W;
     // pieces a thread has in flight: as many as registers are free for (bf16 ones may be rotated or fp32 and take 16
-    // each: 16 rows of 4096 into 4096 12.6 us, with four 13.0; fp16 ones into 12288 17.4 us, with two 17.9)
+    // each: 16 rows of 4096 into 4096 12.1 us, with four 12.7; fp16 ones into 12288 17.9 us, with two 18.2)
     constexpr int PB = !kThrough ? 1 : F16 ? 4 : 2;
     W4Piece piece[PB];
 #pragma unroll
@@ -573,19 +575,19 @@ int launch_rows(const W4A16Args& a, hipStream_t stream) {
     pl.rows_m = static_cast<int>(a.M < most ? a.M : most);
     const int cus = device_cu_count();
     if (pl.rows_m * pl.parts <= 4) {
-        // two column tiles a workgroup stage x half as often (a rotated row of 3072 into 18432: 13.4 us, with one 14.9);
-        // one where that would leave units idle (4096 x 4096: 6.8 us, with two 9.2)
+        // two column tiles a workgroup stage x half as often (a rotated row of 3072 into 18432: 13.9 us, with one 14.9);
+        // one where that would leave units idle (4096 x 4096: 6.0 us, with two 8.3)
         if constexpr (G != 0)
             if ((a.N + 31) / 32 >= 2 * (cus > 0 ? cus : 256)) return launch_tiles<F16, Z, G, 2, 1, 4>(a, pl, stream);
         // a workgroup a compute unit at most: eight waves, where four would need more than two rounds of their rings (a
-        // rotated row of 12288 into 3072: 15.7 us, with four 25.6; 4096 x 4096: 7.3, with four 6.6) or the pairs are
-        // loaded one by one (groups of 32 there: 9.5 us, with four 12.2)
+        // rotated row of 12288 into 3072: 15.4 us, with four 25.0; 4096 x 4096: 6.5, with four 6.0) or the pairs are
+        // loaded one by one (groups of 32 there: 7.7 to 8.8 us, with four 9.2)
         if ((a.N + 15) / 16 <= (cus > 0 ? cus : 256) && (G == 0 || a.K > 2 * 4 * 4 * kBlk))
             return launch_tiles<F16, Z, G, 1, 1, 8>(a, pl, stream);
         return launch_tiles<F16, Z, G, 1, 1, 4>(a, pl, stream);
     }
     // more rows: one workgroup a compute unit keeps all of x in LDS and goes through the tiles (16 rows of 4096 into
-    // 12288: 17 us, over 30 a tile a workgroup; one row that way: 22 against 13 us)
+    // 12288: 17.9 us, 30.9 a tile a workgroup; one rotated row of 3072 into 18432 that way: 20.4 against 13.9 us)
     return launch_tiles<F16, Z, G, 1, 4, 8>(a, pl, stream);
 }
 

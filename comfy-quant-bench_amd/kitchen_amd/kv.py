@@ -272,7 +272,8 @@ def kv_fork(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: to
     """Sequences dst (empty) become copies of src, pairwise: full pages are shared (refs), a partly filled last
     page is copied, in every layer, to the lowest free page. k, v: the whole cache [layers, pages, kv_heads,
     page_size, head_dim] (or one layer of it). status (int32 on the device): 0 done, > 0 pages missing, -1 a row out
-    of range, given twice or not empty; nothing has changed unless it is 0."""
+    of range, given twice or not empty, or a src without a page that its length asks for; nothing has changed unless it
+    is 0."""
     dev, *tab = _tables(page_table, lens, refs)
     pages = refs.shape[0]
     page, cache = _layers(k, v, k_scale, v_scale, pages, dev)
@@ -368,7 +369,8 @@ class PagedKVCache:
         if code > 0:
             raise _lib.MQError(f"the cache is {code} pages short")
         if code < 0:
-            raise ValueError("a sequence is out of range, given twice, not empty, or too long for its page table")
+            raise ValueError("a sequence is out of range, given twice, not empty, without a page that it should have, or too "
+                             "long for its page table")
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor | None = None,
               lens: torch.Tensor | None = None) -> None:

@@ -793,8 +793,9 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     * packed uint4 [N, ceil(K/group_size/2)] (8-bit type): w = s (c - z) (the configs' W4A8 weights' correction)
     * floating [N, K/group_size]: w = s c + z (the lowbit_affine rule, custom_nodes/comfy-lowbit-loader/kernel.py:27-34)
 
-    convrot_groupsize: x is rotated by H per block first, as weights of a rotating converter ask for. Products
-    and sums are fp32; the output (out_dtype, x's type by default) is rounded once."""
+    convrot_groupsize: x is rotated by H per block first, as weights of a rotating converter ask for. Products are
+    exact and sums fp32 (rows rotated for a 16-bit output are held to 16 bits of each value); the output (out_dtype, x's
+    type by default) is rounded once."""
     k = x.shape[-1]
     if qweight.dim() != 2 or qweight.element_size() != 1:
         raise ValueError(f"qweight must be 8-bit [N, K/2], got {qweight.dtype} {list(qweight.shape)}")

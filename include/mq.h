@@ -467,7 +467,7 @@ int64_t mq_paged_attention_counters(int64_t T, int64_t Hq, int64_t H, int64_t B,
  * refs int32 [pages] (sequences that hold a page; 0: free). Pages are handed out lowest first. A
  * call that cannot be done whole changes nothing. *status (int32 in device memory, or NULL): 0 done,
  * > 0 that many pages missing, -1 an argument out of range (a row that does not exist, is given
- * twice, is not empty where it has to be, or whose table is too short).
+ * twice, is not empty where it has to be, whose table is too short, or, forked from, lacks a page of its length).
  * The copies take the caches whole: `layers` layers layer_bytes apart, each of pages page_bytes long and
  * page_pitch bytes apart (K and V alike; the scales of an int8 cache s_*, else NULL and 0).
  *   workspace: mq_kv_workspace_bytes(pages, n) bytes, 16-byte aligned
@@ -504,8 +504,10 @@ int mq_kv_compact(void* k, void* v, int64_t layers, int64_t layer_bytes, int64_t
  * y[m, n] = T( sum_k x'[m, k] * w[n, k] + bias[n] ): 4-bit weights with a scale per group of K values
  * and activations in floating point, x' = x or (hblock 16, 64, 256) x rotated by H_hblock in fp32
  * as mq_rotquant rotates it. For few rows (one token of each of a batch's sequences): the weights are read
- * once per 16 rows (rotated rows 8, fp32 rows 5). Products and sums are fp32 and the output is rounded once; rows rotated
- * for a 16-bit output are held to 16 bits of each value.
+ * once per 16 rows (rotated rows 8, fp32 rows 5). Products are exact, sums fp32, and the output is rounded once; rows
+ * rotated for a 16-bit output are held to 16 bits of each value. bf16, fp32 and rotated rows are multiplied with 16 + code
+ * and (16 + zero-point) sum(x) is taken off each group's sum, which costs an fp32 output of 4096 normal values a row
+ * 1.5e-7. Infinities and NaN in x, ws or wz give what the formula gives.
  *   x [M, K] of type x_dtype (bf16, fp16 or fp32), stride ldx (rows start at multiples of 16 bytes)
  *   qw packed 4-bit [N, K/2], stride ldw bytes (ldw % 16 == 0, 16-byte aligned; low nibble = even k)
  *   ws [N, K/group] of type s_dtype, stride ldws; wz by `zero` (MQ_W4Z_*): NULL, packed uint4
