@@ -86,6 +86,41 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
     return launch_kv_write(a, dtype, cache_dtype == MQ_DT_I8, static_cast<hipStream_t>(stream));
 }
 
+int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t out_token, int64_t out_head, int64_t Hq,
+                 const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int dtype,
+                 int64_t T, int64_t H, int64_t D, void* k_cache, void* v_cache, int cache_dtype, int64_t c_page,
+                 int64_t c_head, int64_t c_token, float* k_scale, float* v_scale, int64_t s_page, int64_t s_head,
+                 int64_t s_token, int64_t pages, int page_size, const int32_t* page_table, int64_t ld_table, int64_t B,
+                 int64_t width, const int32_t* lens, const int32_t* cu_q, const uint64_t* freq, int64_t turn,
+                 int interleaved, float size, void* stream) {
+    clear_error();
+    const int rc = check_cache("kv_append", dtype, T, H, D, k_cache, v_cache, cache_dtype, c_page, c_head, c_token,
+                               k_scale, v_scale, s_page, s_head, s_token, pages, page_size, page_table, ld_table, B,
+                               width, lens, cu_q);
+    if (rc != MQ_OK) return rc;
+    MQ_REQUIRE(Hq >= 0 && Hq < 65536 && H < 65536, "kv_append: bad number of heads (%lld, %lld)", (long long)Hq, (long long)H);
+    MQ_REQUIRE(turn >= 0 && turn <= D && turn % 8 == 0, "kv_append: %lld of %lld values turned: expected a multiple of 8",
+               (long long)turn, (long long)D);
+    if (T == 0 || B == 0) return MQ_OK;
+    MQ_REQUIRE(turn == 0 || (freq && aligned(freq, 8)), "kv_append: the frequencies must be non-null and 8-byte aligned");
+    MQ_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16) && k_token % 8 == 0 && k_head % 8 == 0 && v_token % 8 == 0 &&
+                   v_head % 8 == 0,
+               "kv_append: k and v need 16-byte aligned bases and rows that start at multiples of 16 bytes");
+    MQ_REQUIRE(Hq == 0 || (q && out && aligned(q, 16) && aligned(out, 16) && q_token % 8 == 0 && q_head % 8 == 0 &&
+                           out_token % 8 == 0 && out_head % 8 == 0),
+               "kv_append: q and out need 16-byte aligned bases and rows that start at multiples of 16 bytes");
+    KvAppendArgs a{};
+    KvWriteArgs& w = a.w;
+    w.k = k; w.v = v; w.k_token = k_token; w.k_head = k_head; w.v_token = v_token; w.v_head = v_head;
+    w.T = T; w.H = H; w.D = D; w.kc = k_cache; w.vc = v_cache; w.c_page = c_page; w.c_head = c_head; w.c_token = c_token;
+    w.k_scale = k_scale; w.v_scale = v_scale; w.s_page = s_page; w.s_head = s_head; w.s_token = s_token;
+    w.pages = pages; w.page_shift = log2_of(page_size); w.table = page_table; w.ld_table = ld_table; w.B = B;
+    w.width = pages > 0 ? width : 0; w.lens = lens; w.cu_q = cu_q;
+    a.q = q; a.q_token = q_token; a.q_head = q_head; a.o = out; a.o_token = out_token; a.o_head = out_head; a.Hq = Hq;
+    a.freq = freq; a.turn = static_cast<int>(turn); a.interleaved = interleaved; a.size = size;
+    return launch_kv_append(a, dtype, cache_dtype == MQ_DT_I8, static_cast<hipStream_t>(stream));
+}
+
 int64_t mq_paged_attention_counters(int64_t T, int64_t Hq, int64_t H, int64_t B, int ragged) {
     if (T <= 0 || Hq <= 0 || H <= 0 || B <= 0 || Hq >= 65536 || H > Hq || T * Hq >= kMost || B >= kMost) return 0;
     if (ragged) return attn_prompt_counters(T, static_cast<int>(Hq), static_cast<int>(H), B);
@@ -139,6 +174,72 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
     a.table = page_table; a.ld_table = ld_table; a.B = B; a.width = pages > 0 ? width : 0; a.lens = lens; a.cu_q = cu_q;
     a.scale = scale; a.window = window < kMost ? window : 0; a.sinks = sinks < kMost ? sinks : kMost - 1; a.dtype = dtype; a.work = workspace; a.work_bytes = workspace_bytes;
     return cu_q ? launch_attn_prompt(a, static_cast<hipStream_t>(stream)) : launch_attn_decode(a, static_cast<hipStream_t>(stream));
+}
+
+int64_t mq_kv_shared_ints(int64_t rows) { return rows < 0 || rows >= (kMost >> 4) ? 0 : SharedPlan::ints(rows); }
+
+int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, const int32_t* lens,
+                 int page_size, int32_t* plan, void* stream) {
+    clear_error();
+    MQ_REQUIRE(rows >= 0 && width >= 0 && rows < (kMost >> 4) && width < kMost, "kv_shared: bad shape rows=%lld width=%lld",
+               (long long)rows, (long long)width);
+    MQ_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "kv_shared: page_size must be a power of two (got %d)",
+               page_size);
+    MQ_REQUIRE(width <= (kMost >> 1) / page_size, "kv_shared: the tables hold too many tokens");
+    MQ_REQUIRE(plan && aligned(plan, 4), "kv_shared: plan must be non-null and 4-byte aligned");
+    MQ_REQUIRE(rows == 0 || (lens && aligned(lens, 4)), "kv_shared: lens must be non-null and 4-byte aligned");
+    MQ_REQUIRE(rows == 0 || width == 0 || (page_table && aligned(page_table, 4) && ld_table >= width),
+               "kv_shared: page_table must be non-null and 4-byte aligned with ld_table >= width");
+    return launch_kv_shared(page_table, ld_table, rows, width, lens, log2_of(page_size), plan, static_cast<hipStream_t>(stream));
+}
+
+int64_t mq_paged_attention_shared_counters(int64_t Hq, int64_t H, int64_t B) {
+    if (Hq <= 0 || H <= 0 || B <= 0 || Hq >= 65536 || H > Hq || B * Hq >= kMost) return 0;
+    return attn_shared_counters(static_cast<int>(Hq), static_cast<int>(H), B);
+}
+
+int64_t mq_paged_attention_shared_workspace_bytes(int64_t Hq, int64_t H, int64_t D, int64_t B) {
+    if (Hq <= 0 || H <= 0 || D <= 0 || B <= 0 || Hq >= 65536 || H > Hq || D > 256 || B * Hq >= kMost) return 0;
+    return attn_shared_workspace_bytes(static_cast<int>(Hq), static_cast<int>(H), static_cast<int>(D), B);
+}
+
+int mq_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t B, int64_t Hq, int64_t H,
+                              int64_t D, const void* k_cache, const void* v_cache, int cache_dtype, int64_t c_page,
+                              int64_t c_head, int64_t c_token, const float* k_scale, const float* v_scale, int64_t s_page,
+                              int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
+                              int64_t ld_table, int64_t width, const int32_t* lens, const int32_t* plan, float scale,
+                              void* out, int64_t out_token, int64_t out_head, void* workspace, int64_t workspace_bytes,
+                              int32_t* counters, void* stream) {
+    clear_error();
+    const int rc = check_cache("paged_attention_shared", dtype, B, H, D, k_cache, v_cache, cache_dtype, c_page, c_head,
+                               c_token, k_scale, v_scale, s_page, s_head, s_token, pages, page_size, page_table, ld_table,
+                               B, width, lens, nullptr);
+    if (rc != MQ_OK) return rc;
+    MQ_REQUIRE(Hq > 0 && Hq % H == 0 && Hq < 65536, "paged_attention_shared: %lld query heads for %lld cache heads (a multiple, < 65536)",
+               (long long)Hq, (long long)H);
+    // the kernels count tiles of at least 64 keys for every sequence, cache head and 16 query heads in 32 bits
+    MQ_REQUIRE((B + 1) * H * ((Hq / H + 15) / 16) < (int64_t(1) << 36) / (width * page_size + 256),
+               "paged_attention_shared: the tables hold too many tokens");
+    if (B == 0) return MQ_OK;
+    MQ_REQUIRE(q && out && aligned(q, 16) && aligned(out, 16) && q_token % 8 == 0 && q_head % 8 == 0 &&
+                   out_token % 8 == 0 && out_head % 8 == 0,
+               "paged_attention_shared: q and out need 16-byte aligned bases and rows that start at multiples of 16 bytes");
+    MQ_REQUIRE(B * Hq < kMost && B < (kMost >> 4), "paged_attention_shared: too many rows");
+    MQ_REQUIRE(plan && aligned(plan, 4), "paged_attention_shared: plan must be non-null and 4-byte aligned");
+    const int64_t need = mq_paged_attention_shared_workspace_bytes(Hq, H, D, B);
+    MQ_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need,
+               "paged_attention_shared: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    MQ_REQUIRE(counters && aligned(counters, 4), "paged_attention_shared: needs its counters (zeros)");
+    AttnArgs a{};
+    a.counters = counters;
+    a.q = q; a.q_token = q_token; a.q_head = q_head; a.o = out; a.o_token = out_token; a.o_head = out_head; a.T = B;
+    a.Hq = static_cast<int>(Hq); a.H = static_cast<int>(H); a.D = static_cast<int>(D);
+    a.kc = k_cache; a.vc = v_cache; a.c_page = c_page; a.c_head = c_head; a.c_token = c_token;
+    if (cache_dtype == MQ_DT_I8) { a.k_scale = k_scale; a.v_scale = v_scale; }
+    a.s_page = s_page; a.s_head = s_head; a.s_token = s_token; a.pages = pages; a.page_shift = log2_of(page_size);
+    a.table = page_table; a.ld_table = ld_table; a.B = B; a.width = pages > 0 ? width : 0; a.lens = lens;
+    a.scale = scale; a.dtype = dtype; a.work = workspace; a.work_bytes = workspace_bytes; a.plan = plan;
+    return launch_attn_shared(a, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -185,6 +185,21 @@ struct KvWriteArgs {
 };
 int launch_kv_write(const KvWriteArgs& a, int dtype, bool i8, hipStream_t stream);
 
+// --- new tokens turned by their positions and written (mq_append.hip)
+struct KvAppendArgs {
+    KvWriteArgs w;
+    const void* q;            // [T, Hq, D], strides q_token / q_head
+    int64_t q_token, q_head;
+    void* o;                  // [T, Hq, D], the turned queries
+    int64_t o_token, o_head;
+    int64_t Hq;
+    const uint64_t* freq;     // [turn / 2], turns a position as 64-bit fractions
+    int turn;                 // values of a head that are turned
+    int interleaved;          // pairs are neighbours, else halves
+    float size;               // what cosines and sines are multiplied by
+};
+int launch_kv_append(const KvAppendArgs& a, int dtype, bool i8, hipStream_t stream);
+
 struct KvTables {
     int* table;               // [rows, width]
     int64_t ld_table, rows, width;
@@ -241,6 +256,11 @@ struct AttnArgs {
     void* work;
     int64_t work_bytes;
     int* counters;            // zeros before and after a call
+    // sequences that share beginnings (mq_attn_shared.hip), else null
+    const int* plan;          // groups (mq_kv_shared)
+    const int* start;         // [B], keys of a sequence that its group's part covers
+    float* shared_out;        // [B, Hq, D], the part over those keys, unnormalised
+    float* shared_stat;       // [B, Hq, 2], its maximum (base 2) and sum; sum -1: nothing seen
 };
 int launch_attn_prompt(const AttnArgs& a, hipStream_t stream);
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream);
@@ -248,6 +268,23 @@ int64_t attn_decode_workspace_bytes(int Hq, int H, int D);
 int64_t attn_decode_counters(int Hq, int H, int64_t B);
 int64_t attn_prompt_workspace_bytes(int64_t T, int Hq, int H, int D, int64_t B);
 int64_t attn_prompt_counters(int64_t T, int Hq, int H, int64_t B);
+int launch_attn_shared(const AttnArgs& a, hipStream_t stream);
+int64_t attn_shared_workspace_bytes(int Hq, int H, int D, int64_t B);
+int64_t attn_shared_counters(int Hq, int H, int64_t B);
+int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t width, const int* lens, int page_shift,
+                     int* plan, hipStream_t stream);
+
+// The groups of sequences that hold the same first pages, as int32: their number; three words unused; start[b], the
+// tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
+// shared, the sequence whose pages are read, its first member's place and their number; working space.
+struct SharedPlan {
+    static constexpr int kHead = 4, kGroup = 4;
+    static int64_t ints(int64_t B) { return kHead + 8 * B; }
+    __host__ __device__ static int64_t start() { return kHead; }
+    __host__ __device__ static int64_t members(int64_t B) { return kHead + B; }
+    __host__ __device__ static int64_t groups(int64_t B) { return kHead + 2 * B; }
+    __host__ __device__ static int64_t work(int64_t B) { return kHead + 4 * B; }
+};
 
 // --- 4-bit weights, floating activations (mq_w4a16.hip)
 enum class W4Zero : int { Signed = 0, U4 = 1, Float = 2 };
@@ -274,5 +311,41 @@ struct W4A16Args {
     int64_t M, N, K;
 };
 int launch_w4a16(const W4A16Args& a, hipStream_t stream);
+
+
+// --- norms (mq_norm.hip)
+struct NormArgs {
+    const void* x;            // [M, K] of type dtype
+    int64_t ldx;
+    const void* r;            // residual, or null
+    int64_t ldr;
+    const void* w;            // [K] of type w_dtype, or null
+    int w_dtype;
+    float eps;
+    void* h;                  // x + r (with a residual)
+    int64_t ldh;
+    void* y;                  // [M, K] of type dtype, or int8 codes
+    int64_t ldy;
+    float* s;                 // [M], the codes' scales
+    int dtype;
+    int hblock;               // -1: floating output; 0: codes; 16, 64, 256: codes of rotated rows
+    int64_t M, K;
+};
+int launch_norm(const NormArgs& a, hipStream_t stream);
+
+// --- the next token of rows of logits (mq_sample.hip)
+struct SampleArgs {
+    const void* x;            // [rows, V] of type dtype, row stride ld
+    int dtype;
+    int64_t ld, rows, V;
+    const float* u;           // [rows]
+    const float *temperature, *top_p, *min_p;   // [rows], or null: the values below
+    const int* top_k;
+    float temperature1, top_p1, min_p1;
+    int64_t top_k1;
+    int64_t* token;           // [rows]
+    void* work;
+};
+int launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace mq

@@ -11,7 +11,7 @@ keyword arguments, executed by hand-written HIP kernels in `libmq.so` through it
 """
 from . import weights
 from ._lib import LIB_PATH, MQError, load
-from .kv import PagedKVCache, kv_compact, kv_fork, kv_free, kv_grow, kv_write, paged_attention
+from .kv import PagedKVCache, Rotary, kv_append, kv_compact, kv_fork, kv_free, kv_grow, kv_shared, kv_write, paged_attention
 from .ops import (
     ExpandedW4,
     PreparedW4A8,
@@ -34,6 +34,7 @@ from .ops import (
     w4a16_linear,
     w4a8_int8_linear,
 )
+from .step import rms_norm, rms_norm_quantize, sample
 from .weights import (
     quantize_convrot_w4a4_weight,
     quantize_int8_convrot_weight,
@@ -51,4 +52,5 @@ __all__ = [
     "quantize_w4a8_asym_weight", "quantize_w4a4_group_weight", "quantize_convrot_w4a4_weight",
     "quantize_int8_convrot_weight",
     "w4a16_linear", "paged_attention", "kv_write", "kv_fork", "kv_grow", "kv_free", "kv_compact", "PagedKVCache",
+    "kv_append", "Rotary", "kv_shared", "rms_norm", "rms_norm_quantize", "sample",
 ]

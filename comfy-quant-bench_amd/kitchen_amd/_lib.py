@@ -22,7 +22,8 @@ LIB_PATH = os.path.join(_HERE, "libmq.so")
 
 _lib = None
 FAST_ENTRIES = ("mq_rotquant", "mq_swiglu_rotquant", "mq_linear_w4_group", "mq_linear_rowscale", "mq_kv_write",
-                "mq_paged_attention", "mq_kv_grow", "mq_linear_w4a16")
+                "mq_paged_attention", "mq_kv_grow", "mq_linear_w4a16", "mq_rms_norm", "mq_rms_norm_quant", "mq_kv_append",
+                "mq_kv_shared", "mq_paged_attention_shared", "mq_sample")
 _entries: dict = {}   # entry point name -> callable
 
 c_i64 = ctypes.c_int64
@@ -84,6 +85,22 @@ _SIGNATURES = {
                        c_vp, c_i64, c_vp, c_vp, c_i64, c_vp], c_int),
     "mq_linear_w4a16": ([c_vp, c_int, c_i64, c_int, c_vp, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp,
                          c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp], c_int),
+    "mq_rms_norm": ([c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_int, c_float, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64,
+                     c_vp], c_int),
+    "mq_rms_norm_quant": ([c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_int, c_float, c_int, c_vp, c_i64, c_vp, c_i64,
+                           c_vp, c_i64, c_i64, c_vp], c_int),
+    "mq_kv_append": ([c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int,
+                      c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                      c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_float, c_vp], c_int),
+    "mq_kv_shared_ints": ([c_i64], c_i64),
+    "mq_kv_shared": ([c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp], c_int),
+    "mq_paged_attention_shared_workspace_bytes": ([c_i64, c_i64, c_i64, c_i64], c_i64),
+    "mq_paged_attention_shared_counters": ([c_i64, c_i64, c_i64], c_i64),
+    "mq_paged_attention_shared": ([c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64,
+                                   c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_i64,
+                                   c_vp, c_vp, c_float, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp], c_int),
+    "mq_sample": ([c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_float, c_vp, c_i64, c_vp, c_float, c_vp, c_float,
+                   c_vp, c_vp], c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,13 +1,15 @@
 """A small text decoder on this package's linears and paged cache, and a program that answers with it.
 
-    python -m kitchen_amd.generate [--prompts 4] [--alternatives 2] [--tokens 32] [--int8-cache]
+    python -m kitchen_amd.generate [--prompts 4] [--alternatives 2] [--tokens 32] [--int8-cache] [--temperature 0.8 --top-p 0.9]
 
 Every layer's projections are held once, as the converters write them (uint4 codes rotated by Hadamard blocks, fp16
-scale and uint4 zero-point per group of 64), and used in two ways: prompts, with rows by the thousand, go through
-w4a8_int8_linear; steps of a token per sequence through w4a16_linear, whose activations stay in floating point. Keys
-and values live in a PagedKVCache: ragged prompts and single tokens are written to and attended in its pages, a
-prompt's alternatives are forks that share its pages, and when sequences end their pages are freed and the others'
-moved together. Weights are random: it shows the calls and their cost, not language."""
+scale and uint4 zero-point per group of 64), and used in two ways: prompts, with rows by the thousand, are multiplied as
+int8 codes, those of a norm's output made by the norm itself (rms_norm_quantize); steps of a token per sequence go through
+rms_norm and w4a16_linear, whose activations stay in floating point. Keys and values live in a PagedKVCache: ragged
+prompts and single tokens are turned by their positions, written to and attended in its pages, a prompt's alternatives
+are forks that share its pages, which a step reads once for all of them, and when sequences end their pages are freed
+and the others' moved together. Tokens are chosen by sample. Weights are random: it shows the calls and their cost, not
+language."""
 from __future__ import annotations
 
 import argparse
@@ -16,7 +18,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import kv, ops, weights
+from . import _lib, kv, ops, step, weights
 
 
 @dataclass
@@ -47,6 +49,19 @@ class Linear:
             return ops.w4a16_linear(x, self.q, self.s, self.z, None, self.GROUP, self.ROTATE)
         return ops.w4a8_int8_linear(x, self.q, self.s, None, None, self.z, None, self.GROUP, self.ROTATE, x.dtype)
 
+    def of_norm(self, delta: torch.Tensor | None, x: torch.Tensor):
+        """(projection of the norm of x + delta, x + delta); without a delta, of x."""
+        if x.shape[0] <= self.few:
+            y, x = (step.rms_norm(x), x) if delta is None else step.rms_norm(delta, None, x)
+            return self(y), x
+        q, s, *h = step.rms_norm_quantize(x, convrot_groupsize=self.ROTATE) if delta is None else \
+            step.rms_norm_quantize(delta, None, x, convrot_groupsize=self.ROTATE)
+        xw = ops._expansion(self.q, self.z, _lib.ACT_I8, *q.shape, self.s, _lib.stream_of(q))
+        y = ops.gemm_w4_group(q, s, self.q if xw is None else xw, self.s, self.z, None, self.q.shape[0], self.GROUP, _lib.ACT_I8, x.dtype)
+        return y, h[0] if h else x
+
+
+# Plain forms of the norm and of the turn by positions, to compare with.
 
 def _norm(x: torch.Tensor) -> torch.Tensor:
     f = x.float()
@@ -80,21 +95,24 @@ class Decoder:
                         "up": Linear(matrix(2 * c.inner, c.hidden), few), "down": Linear(matrix(c.hidden, c.inner), few)}
                        for _ in range(c.layers)]
         self.cache = kv.PagedKVCache(c.layers, pages, c.kv_heads, c.head_dim, page_size, seqs, max_tokens, c.dtype, int8_cache, device)
+        self.rotary = kv.Rotary(c.head_dim, device=device)
 
-    def _forward(self, tokens: torch.Tensor, pos: torch.Tensor, cu_q, lens: torch.Tensor) -> torch.Tensor:
+    def _forward(self, tokens: torch.Tensor, cu_q, lens: torch.Tensor, shared: torch.Tensor | None = None) -> torch.Tensor:
         """Hidden states of new tokens whose room the cache has; it holds their keys and values afterwards. lens: the
-        cache's lengths of the sequences that take part, 0 of the others, whose tokens leave no trace."""
+        cache's lengths of the sequences that take part, 0 of the others, whose tokens leave no trace. shared: the plan of
+        the pages that they share."""
         c = self.config
-        x = torch.nn.functional.embedding(tokens, self.embedding) * c.hidden ** 0.5
+        x, delta = torch.nn.functional.embedding(tokens, self.embedding) * c.hidden ** 0.5, None
         for i, layer in enumerate(self.layers):
-            q, k, v = layer["qkv"](_norm(x)).view(len(tokens), -1, c.head_dim).split([c.heads, c.kv_heads, c.kv_heads], 1)
-            self.cache.write(i, _turn(k, pos), v, cu_q, lens=lens)
-            y = self.cache.attend(i, _turn(q, pos), cu_q, window=c.window if i % 2 else None, sinks=c.sinks,
-                                  lens=lens)
-            x = x + layer["out"](y.view(len(tokens), -1))
-            gate, up = layer["up"](_norm(x)).chunk(2, -1)
-            x = x + layer["down"](torch.nn.functional.silu(gate) * up)
-        return _norm(x)
+            y, x = layer["qkv"].of_norm(delta, x)
+            q, k, v = y.view(len(tokens), -1, c.head_dim).split([c.heads, c.kv_heads, c.kv_heads], 1)
+            q = self.cache.append(i, q, k, v, self.rotary, cu_q, lens=lens)
+            window = c.window if i % 2 else None
+            y = self.cache.attend(i, q, cu_q, window=window, sinks=c.sinks, lens=lens, shared=None if window else shared)
+            y, x = layer["up"].of_norm(layer["out"](y.view(len(tokens), -1)), x)
+            gate, up = y.chunk(2, -1)
+            delta = layer["down"](torch.nn.functional.silu(gate) * up)
+        return step.rms_norm(x) if delta is None else step.rms_norm(delta, None, x)[0]
 
     def _logits(self, x: torch.Tensor) -> torch.Tensor:
         return torch.nn.functional.linear(x, self.embedding)
@@ -111,10 +129,8 @@ class Decoder:
         cache.grow(rows, [news[b] for b in rows])
         cu_q = torch.tensor([0] + news, device=dev).cumsum(0).to(torch.int32)
         tokens = torch.tensor([t for b in rows for t in prompts[b]], device=dev)
-        seq = torch.tensor([b for b in rows for _ in prompts[b]], device=dev)
         lens = cache.lens * (cache.lens > before)        # nothing is written where nothing has grown
-        pos = lens[seq] - cu_q[seq + 1] + torch.arange(len(tokens), device=dev)
-        x = self._forward(tokens, pos, cu_q, lens)
+        x = self._forward(tokens, cu_q, lens)
         return self._logits(x[(cu_q[1:][rows] - 1).long()])
 
     def step(self, tokens: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
@@ -123,7 +139,7 @@ class Decoder:
         cache, before = self.cache, self.cache.lens.clone()
         cache.grow(rows, torch.ones_like(rows))
         lens = cache.lens * (cache.lens > before)        # nothing is written where nothing has grown
-        return self._logits(self._forward(tokens, lens - 1, None, lens))
+        return self._logits(self._forward(tokens, None, lens, cache.shared(lens) if cache.forked else None))
 
 
 def main(argv: list[str] | None = None) -> int:
@@ -135,6 +151,10 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--window", type=int, default=None)
     ap.add_argument("--int8-cache", action="store_true")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest token always")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
     config = Config(layers=a.layers, window=a.window, sinks=4 if a.window else 0)
     most, seqs = a.length + a.tokens, a.prompts * a.alternatives
@@ -156,6 +176,7 @@ def main(argv: list[str] | None = None) -> int:
     tokens = logits.topk(a.alternatives).indices.t().reshape(-1)
     rows = torch.arange(seqs, dtype=torch.int32, device=tokens.device)
     answers = [tokens]
+    u = torch.rand((a.tokens, seqs), generator=torch.Generator(device=tokens.device).manual_seed(2), device=tokens.device)
     t2 = clock()
     for i in range(a.tokens):
         if i == a.tokens // 2 and a.alternatives > 1:      # the last alternatives have said enough
@@ -163,7 +184,7 @@ def main(argv: list[str] | None = None) -> int:
             live = cache.compact()
             rows = rows[:-a.prompts]
             print(f"{int(live)} pages are held after {a.prompts} sequences ended")
-        tokens = model.step(tokens, rows).argmax(-1)
+        tokens = step.sample(model.step(tokens, rows), u[i], a.temperature, a.top_k, a.top_p, a.min_p)
         answers.append(tokens)
     cache.check()
     t3 = clock()

@@ -13,12 +13,19 @@ tokens begin; None: one new token each) stay on the device: no call waits for it
     cache.write(layer, k, v)                    # k, v [16, 8, 128]
     y = cache.attend(layer, q)                  # q [16, 32, 128]
 
+or, with positions turned into queries and keys on the way and the pages that forks share read once:
+
+    rotary, shared = ck.Rotary(128), cache.shared()
+    q = cache.append(layer, q, k, v, rotary)
+    y = cache.attend(layer, q, shared=shared)
+
 Every call raises ValueError for tensors whose shapes, types, strides or devices do not fit. What only the
 device can see is bounded there: a table entry that is no page of the cache holds nothing, and a fork or
 growth that cannot be done whole changes nothing and says so in `status`.
 """
 from __future__ import annotations
 
+import math
 import threading
 
 import torch
@@ -148,15 +155,115 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
               _CODE[k.dtype], t, h, d, *cache, *tables, _lib.stream_of_device(dev))
 
 
+class Rotary:
+    """Rotary positions for kv_append: which values of a head are pairs and by how much a position turns them.
+
+    dim: how many of a head's values are turned, from the first on (a multiple of 8); interleaved: pairs are neighbours, else
+    values i and i + dim / 2. Pair i turns by base^(-2 i / dim) radians a position. scaling, for contexts `factor` times as
+    long as the `original` that a model was trained on:
+
+    * "linear": every frequency divided by factor
+    * "yarn": pairs that turn fewer than beta_slow times over the original context are divided by factor, those of more than
+      beta_fast turns stay, linearly between them by their number; queries and keys are multiplied by
+      0.1 ln(factor) + 1 (or by `size`)
+
+    The frequencies are held as 64-bit fractions of a turn on the device, so that positions of any size lose nothing."""
+
+    def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, scaling: str | None = None,
+                 factor: float = 1.0, original: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 size: float | None = None, device="cuda"):
+        if dim < 8 or dim % 8 or dim > 256:
+            raise ValueError(f"dim must be a multiple of 8 up to 256, got {dim}")
+        if not (base > 1 and factor > 0 and original > 0 and beta_fast > beta_slow > 0):
+            raise ValueError(f"base must be above 1, factor and original positive, beta_fast above beta_slow above 0; got {base}, "
+                             f"{factor}, {original}, {beta_fast}, {beta_slow}")
+        n = dim // 2
+        f = [base ** (-i / n) for i in range(n)]
+        own_size = 1.0
+        if scaling == "linear":
+            f = [x / factor for x in f]
+        elif scaling == "yarn":
+            # the pair that turns so many times over the original context
+            fast, slow = (n * math.log(original / (2 * math.pi * turns)) / math.log(base) for turns in (beta_fast, beta_slow))
+            lo, hi = max(math.floor(fast), 0), min(math.ceil(slow), dim - 1)
+            for i in range(n):
+                part = min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001)))
+                f[i] = f[i] / factor * part + f[i] * (1 - part)
+            own_size = 0.1 * math.log(factor) + 1.0
+        elif scaling is not None:
+            raise ValueError(f"scaling must be None, 'linear' or 'yarn', got {scaling!r}")
+        self.dim, self.interleaved = dim, bool(interleaved)
+        self.size = own_size if size is None else float(size)
+        turns = [round(x / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for x in f]
+        self.turns = torch.tensor([x - (1 << 64) if x >> 63 else x for x in turns], dtype=torch.int64).to(device)
+
+
+def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              page_table: torch.Tensor, kv_lens: torch.Tensor, rotary: Rotary, cu_q: torch.Tensor | None = None,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """kv_write of new tokens' keys and values, the keys turned by their positions, and the queries q [tokens, heads,
+    head_dim] turned likewise: returned, or in `out` (which may be q). Angles are exact at any position, the rest fp32, each
+    value rounded once (codes of an int8 cache are of the unrounded ones). A query without a position (of a sequence that
+    holds nothing) is passed as it is; rows behind the last sequence's are not written."""
+    dev = _device_of(q, "q")
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != dev or v.device != dev:
+        raise ValueError(f"k and v must be alike and on {dev}, got {list(k.shape)} {k.dtype} and {list(v.shape)} {v.dtype}")
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype:
+        raise ValueError(f"q must be [tokens, heads, head_dim] beside k, got {list(q.shape)} {q.dtype} and {list(k.shape)} {k.dtype}")
+    q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    t, h, d = k.shape
+    if rotary.dim > d:
+        raise ValueError(f"{rotary.dim} values to turn in heads of {d}")
+    if rotary.turns.device != dev:
+        raise ValueError(f"the rotary frequencies are on {rotary.turns.device}, the tokens on {dev}")
+    _, _, _, cache = _cache_args(k_cache, v_cache, k_scale, v_scale, k, h)
+    page_table = _apart(page_table)
+    tables = _table_args(page_table, kv_lens, cu_q, t, dev)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
+            or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+        raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with rows at multiples of 16 bytes")
+    _lib.call("mq_kv_append", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), q.shape[1],
+              k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _CODE[k.dtype], t, h, d, *cache,
+              *tables, rotary.turns.data_ptr(), rotary.dim, int(rotary.interleaved), rotary.size, _lib.stream_of_device(dev))
+    return out
+
+
+def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int) -> torch.Tensor:
+    """Which sequences hold the same first pages (forks of one another), as a plan for paged_attention(shared=): int32 on the
+    device, the same for all layers. It holds while sequences grow, and until one is freed or forked to, or a shared entry of
+    the table changes. page_size: the cache's."""
+    dev = _device_of(page_table, "page_table")
+    page_table = _apart(page_table)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError("page_table must be int32 [sequences, width] with contiguous rows")
+    b, width = page_table.shape
+    if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or kv_lens.shape[0] != b or kv_lens.device != dev \
+            or not kv_lens.is_contiguous():
+        raise ValueError(f"kv_lens must be contiguous int32 [{b}] on {dev}")
+    plan = torch.empty(_plan_ints(b), dtype=torch.int32, device=dev)
+    _lib.call("mq_kv_shared", page_table.data_ptr(), max(page_table.stride(0), width), b, width, kv_lens.data_ptr(),
+              int(page_size), plan.data_ptr(), _lib.stream_of_device(dev))
+    return plan
+
+
+def _plan_ints(b: int) -> int:
+    return 4 + 8 * b       # mq_kv_shared_ints
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     kv_lens: torch.Tensor, cu_q: torch.Tensor | None = None, scale: float | None = None,
                     window: int | None = None, sinks: int = 0, k_scale: torch.Tensor | None = None,
-                    v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    shared: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of new tokens q [tokens, heads, head_dim] over their sequences' pages, causal: the query at
     position p (new token i of n: kv_lens - n + i) sees tokens j <= p, with `window` only the last `window` of
     them (its own among them) and the first `sinks`. heads is a multiple of kv_heads (query head h reads cache
     head h // (heads // kv_heads)). scale: of the scores, head_dim ** -0.5 by default. A query that sees nothing
-    gets zeros. cu_q None: one new token per sequence (generation), else ragged prompt chunks.
+    gets zeros. cu_q None: one new token per sequence (generation), else ragged prompt chunks. shared: kv_shared's plan
+    of these tables, with which pages that sequences share are read once for all of them (one new token per sequence, no window).
     Returns out [tokens, heads, head_dim] in q's type."""
     dev = _device_of(q, "q")
     q = _rows(q, "q")
@@ -174,19 +281,34 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with rows at multiples of 16 bytes")
     stream = _lib.stream_of_device(dev)
-    key = (dev.index, t, heads, h, d, tables[2], cu_q is None)
+    if shared is not None:
+        if cu_q is not None or window is not None:
+            raise ValueError("shared pages are for one new token per sequence without a window")
+        if shared.dtype != torch.int32 or shared.shape != (_plan_ints(t),) or shared.device != dev or not shared.is_contiguous():
+            raise ValueError(f"shared must be kv_shared's plan of {t} sequences on {dev}")
+    key = (dev.index, t, heads, h, d, tables[2], cu_q is None, shared is None)
     sizes = _ATTN_WS.get(key)
     if sizes is None:
         lib, b, ragged = _lib.load(), tables[2], int(cu_q is not None)
         with torch.cuda.device(dev):
-            sizes = (int(lib.mq_paged_attention_workspace_bytes(t, heads, h, d, b, ragged)),
-                     int(lib.mq_paged_attention_counters(t, heads, h, b, ragged)))
+            if shared is not None:
+                sizes = (int(lib.mq_paged_attention_shared_workspace_bytes(heads, h, d, b)),
+                         int(lib.mq_paged_attention_shared_counters(heads, h, b)))
+            else:
+                sizes = (int(lib.mq_paged_attention_workspace_bytes(t, heads, h, d, b, ragged)),
+                         int(lib.mq_paged_attention_counters(t, heads, h, b, ragged)))
         if len(_ATTN_WS) > 4096:   # ragged batches come in any size: the sizes are only remembered, not needed
             _ATTN_WS.clear()
         _ATTN_WS[key] = sizes
     nbytes, ncount = sizes
     work = _scratch(nbytes, dev, stream) if nbytes else None
     count = _counters(ncount, dev, stream) if ncount else None
+    if shared is not None:
+        _lib.call("mq_paged_attention_shared", q.data_ptr(), q.stride(0), q.stride(1), _CODE[q.dtype], t, heads, h, d, *cache,
+                  *tables[:2], *tables[3:5], shared.data_ptr(), d ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                  out.stride(0), out.stride(1), None if work is None else work.data_ptr(), nbytes,
+                  None if count is None else count.data_ptr(), stream)
+        return out
     _lib.call("mq_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), _CODE[q.dtype], t, heads, h, d, *cache,
               *tables, d ** -0.5 if scale is None else float(scale), window or 0, int(sinks), out.data_ptr(),
               out.stride(0), out.stride(1), None if work is None else work.data_ptr(), nbytes,
@@ -346,6 +468,7 @@ class PagedKVCache:
         self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.forked = False                              # whether sequences may share pages
 
     def _layer(self, layer: int):
         return (self.k[layer], self.v[layer], None if self.k_scale is None else self.k_scale[layer],
@@ -356,6 +479,7 @@ class PagedKVCache:
 
     def fork(self, src, dst) -> None:
         kv_fork(self.k, self.v, self.page_table, self.lens, self.refs, src, dst, self.k_scale, self.v_scale, self.status)
+        self.forked = True
 
     def free(self, seqs) -> None:
         kv_free(self.page_table, self.lens, self.refs, seqs)
@@ -378,9 +502,20 @@ class PagedKVCache:
         kc, vc, ks, vs = self._layer(layer)
         kv_write(k, v, kc, vc, self.page_table, self.lens if lens is None else lens, cu_q, ks, vs)
 
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rotary: Rotary,
+               cu_q: torch.Tensor | None = None, lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """write with the positions turned into k, and into q, which is returned. lens: as for write."""
+        kc, vc, ks, vs = self._layer(layer)
+        return kv_append(q, k, v, kc, vc, self.page_table, self.lens if lens is None else lens, rotary, cu_q, ks, vs, out)
+
+    def shared(self, lens: torch.Tensor | None = None) -> torch.Tensor:
+        """The plan of the pages that sequences share, for attend: until a sequence is freed or forked to. lens: other lengths than
+        the cache's own (a sequence of length 0 takes no part)."""
+        return kv_shared(self.page_table, self.lens if lens is None else lens, self.page_size)
+
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor | None = None, scale: float | None = None,
                window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,
-               lens: torch.Tensor | None = None) -> torch.Tensor:
+               lens: torch.Tensor | None = None, shared: torch.Tensor | None = None) -> torch.Tensor:
         kc, vc, ks, vs = self._layer(layer)
         return paged_attention(q, kc, vc, self.page_table, self.lens if lens is None else lens, cu_q, scale, window, sinks,
-                               ks, vs, out)
+                               ks, vs, out, shared)

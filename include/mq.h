@@ -520,6 +520,75 @@ int mq_linear_w4a16(const void* x, int x_dtype, int64_t ldx, int hblock, const u
                     const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K,
                     void* stream);
 
+/*
+ * What a step of token generation does between its linears and behind them. No counterpart in the reference.
+ *
+ * mq_rms_norm: h = x + residual rounded to the rows' type (written to h; without a residual h is x and nothing is
+ * written), y = h * weight / sqrt(mean(h^2) + eps) in fp32, rounded once. mq_rms_norm_quant: the same y, unrounded, as
+ * int8 codes: rotated by H_hblock per block of hblock columns (0: not) as mq_rotquant rotates, scale = max(max |y| / 127,
+ * 1e-10) per row, code = rne(y / scale). A row with an infinity or NaN in y gets codes 0 and scale NaN. The sum of a
+ * row's squares has to fit fp32.
+ *   x, residual, h, y [M, K] of type dtype (bf16, fp16, fp32) at any address and row stride that the type allows; h may
+ *   be x or residual, y may be x; weight [K] of type w_dtype, or NULL for ones; q int8 [M, K]; scale [M]. K <= 32768.
+ */
+int mq_rms_norm(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int w_dtype,
+                float eps, void* h, int64_t ldh, void* y, int64_t ldy, int64_t M, int64_t K, void* stream);
+int mq_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                      int w_dtype, float eps, int hblock, void* h, int64_t ldh, int8_t* q, int64_t ldq, float* scale, int64_t M,
+                      int64_t K, void* stream);
+
+/*
+ * mq_kv_write of k and v with their positions turned into k, and into q [T, Hq, D], which goes to out (in place, or apart
+ * from it): pair i < turn / 2 of a head at position p becomes (a c - b s, a s + b c), c and s the cosine and sine of
+ * the turn's fraction p * freq[i] / 2^64 (modulo 1) times `size`. interleaved 0: a and b are values i and i + turn / 2 of
+ * the head, 1: values 2 i and 2 i + 1; values from `turn` on stay as they are. Computed in fp32 (angles in fp64), rounded
+ * once; an int8 cache takes codes of the unrounded values. Positions are mq_kv_write's; a query whose position is below 0
+ * is passed as it is, and rows of q behind the last sequence's are not written. turn % 8 == 0, turn <= D; Hq may be 0.
+ */
+int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t out_token, int64_t out_head, int64_t Hq,
+                 const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int dtype,
+                 int64_t T, int64_t H, int64_t D, void* k_cache, void* v_cache, int cache_dtype, int64_t c_page,
+                 int64_t c_head, int64_t c_token, float* k_scale, float* v_scale, int64_t s_page, int64_t s_head,
+                 int64_t s_token, int64_t pages, int page_size, const int32_t* page_table, int64_t ld_table, int64_t B,
+                 int64_t width, const int32_t* lens, const int32_t* cu_q, const uint64_t* freq, int64_t turn,
+                 int interleaved, float size, void* stream);
+
+/*
+ * mq_kv_shared: which sequences hold the same first pages, to plan: int32 [mq_kv_shared_ints(rows)], whose words only
+ * mq_paged_attention_shared reads. A group shares the tokens of the longest run of table entries that are equal in all its
+ * sequences. mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
+ * keys and values that a group shares are read once for all of it. The plan holds for any cache and layer with these tables,
+ * until a shared entry changes or a sequence that shares them is emptied and filled again; sequences may grow.
+ *   workspace, counters: as for mq_paged_attention, with the sizes of the functions below
+ */
+int64_t mq_kv_shared_ints(int64_t rows);
+int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, const int32_t* lens,
+                 int page_size, int32_t* plan, void* stream);
+int64_t mq_paged_attention_shared_workspace_bytes(int64_t Hq, int64_t H, int64_t D, int64_t B);
+int64_t mq_paged_attention_shared_counters(int64_t Hq, int64_t H, int64_t B);
+int mq_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t B, int64_t Hq, int64_t H,
+                              int64_t D, const void* k_cache, const void* v_cache, int cache_dtype, int64_t c_page,
+                              int64_t c_head, int64_t c_token, const float* k_scale, const float* v_scale, int64_t s_page,
+                              int64_t s_head, int64_t s_token, int64_t pages, int page_size, const int32_t* page_table,
+                              int64_t ld_table, int64_t width, const int32_t* lens, const int32_t* plan, float scale,
+                              void* out, int64_t out_token, int64_t out_head, void* workspace, int64_t workspace_bytes,
+                              int32_t* counters, void* stream);
+
+/*
+ * token[r] = the next token of logits row r for the random number u[r] in [0, 1): weights w_i = exp((l_i - max l) / T).
+ * In the order of l (descending, equal ones by index) the first top_k are kept (0: all), of those the shortest leading
+ * part whose weight reaches top_p of theirs (>= 1: all; at least one), of those w_i >= min_p; the token is the first i, in
+ * the order of i, whose kept weight up to i exceeds u times all kept weight. T <= 0 (or NaN): the first largest. Logits that
+ * are NaN count as -infinity; a row without any other gets -1; where +infinities are, only they have weight. u below
+ * 0 (or NaN) counts as 0, u >= 1 takes the last one kept. Weights are fp64, their sums exact in units of 2^-45 of the
+ * largest for V = 2^17 (2^(log2(V) - 62), at least 2^-51): the same inputs always give the same token.
+ *   logits [rows, V] of type dtype (bf16, fp16, fp32), row stride ld, V <= 2^24; temperature, top_p, min_p fp32 [rows]
+ *   and top_k int32 [rows], or NULL for the value *_all of every row
+ */
+int mq_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const float* u, const float* temperature,
+              float temperature_all, const int32_t* top_k, int64_t top_k_all, const float* top_p, float top_p_all,
+              const float* min_p, float min_p_all, int64_t* token, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

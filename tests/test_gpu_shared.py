@@ -1,0 +1,270 @@
+"""Attention of sequences that share pages (kv_shared's plan, paged_attention(shared=)) against plain loops in 64 bits over every
+sequence's own table.
+
+Tolerance as in tests/test_gpu_attention.py: the output is rounded once (u |o|); the probabilities are rounded to the
+products' 16 bits, relative u each (u W, W = sum_j p_j |v_j|); scores are fp32 sums of D exact products, off by
+(D + 4) 2^-24 R, which moves each p by twice that; sums over keys are fp32 (2^-11 W with the parts' joining). fp16
+probabilities are held 2^6 to 2^14 times as large as they are: what vanishes is below 2^-24 of a row's largest."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kitchen_amd as ck
+from oracle import serving, step
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+class Forks:
+    """Groups of sequences: groups[i] = (tokens that are shared, [every sequence's tokens beyond them, None: it has ended]); their
+    rows of the table in random order. Slots that hold no token are NaN."""
+
+    def __init__(self, dev, groups, hq, h, d, page=16, dtype=torch.bfloat16, int8=False, seed=0, order="phtd", spare=2, width=None):
+        g = torch.Generator().manual_seed(seed)
+        self.dtype, self.page = dtype, page
+        rows = [(i, own) for i, (_, owns) in enumerate(groups) for own in owns]
+        rows = [rows[i] for i in torch.randperm(len(rows), generator=g).tolist()]
+        self.lens = [0 if own is None else groups[i][0] + own for i, own in rows]
+        full = [n // page for n, _ in groups]
+        total = sum(full) + sum(max(0, -(-n // page) - full[i]) for n, (i, own) in zip(self.lens, rows) if own is not None) + spare
+        place = torch.randperm(total, generator=g).tolist()
+        common = [[place.pop() for _ in range(n)] for n in full]
+        width = width or max(1, max(-(-n // page) for n in self.lens))
+        table = torch.full((len(rows), width), -1, dtype=torch.int32)
+        used = torch.zeros(total, page, dtype=torch.bool)
+        for b, (i, own) in enumerate(rows):
+            if own is None:
+                continue
+            n = -(-self.lens[b] // page)
+            entries = (common[i] + [place.pop() for _ in range(max(0, n - full[i]))])[:n]
+            table[b, :n] = torch.tensor(entries, dtype=torch.int32)
+            for j in range(self.lens[b]):
+                used[entries[j // page], j % page] = True
+        shape = (total, h, page, d)
+        k, v = (torch.randn(shape, generator=g) for _ in range(2))
+        k[..., ::7] *= 3
+        self.q = torch.randn((len(rows), hq, d), generator=g).to(dtype).to(dev)
+        self.table, self.kv_lens = table.to(dev), torch.tensor(self.lens, dtype=torch.int32, device=dev)
+        hole = ~used[:, None, :, None].expand(shape)
+        self.ks = self.vs = None
+        if int8:
+            s = [(x.abs().amax(-1) / 127).clamp_min(1e-10) for x in (k, v)]
+            k, v = (torch.round(x / y[..., None]).to(torch.int8) for x, y in zip((k, v), s))
+            self.k64, self.v64 = (x.double() * y[..., None].double() for x, y in zip((k, v), s))
+            self.ks, self.vs = (self._order(y.masked_fill(~used[:, None, :].expand(shape[:3]), math.nan)[..., None], order, dev)[..., 0] for y in s)
+        else:
+            k, v = k.to(dtype), v.to(dtype)
+            self.k64, self.v64 = k.double(), v.double()
+            k, v = k.masked_fill(hole, math.nan), v.masked_fill(hole, math.nan)
+        self.k, self.v = (self._order(x, order, dev) for x in (k, v))
+
+    @staticmethod
+    def _order(x, order, dev):
+        perm = ["phtd".index(c) for c in order]
+        x = x.to(dev).permute(perm).contiguous()
+        return x.permute([perm.index(i) for i in range(4)])
+
+    def plan(self):
+        return ck.kv_shared(self.table, self.kv_lens, self.page)
+
+    def run(self, plan=None, **kw):
+        return ck.paged_attention(self.q, self.k, self.v, self.table, self.kv_lens, k_scale=self.ks, v_scale=self.vs,
+                                  shared=self.plan() if plan is None else plan, **kw)
+
+    def check(self, y, lens=None, **kw):
+        lens = self.lens if lens is None else lens
+        o, w, r = serving.attention(self.q.double().cpu().numpy(), self.k64.numpy(), self.v64.numpy(), self.table.cpu().numpy(), lens, None, **kw)
+        u, d = U[self.dtype], self.q.shape[2]
+        err = np.abs(y.double().cpu().numpy() - o)
+        tol = u * np.abs(o) + (u + 2 ** -11 + 2.2 * (d + 4) * 2.0 ** -24 * r[..., None]) * w \
+            + max(lens, default=0) * 2.0 ** -24 * float(self.v64.abs().max()) * (self.dtype == torch.float16) + 1e-30
+        tol[w == 0] = 0
+        assert np.isfinite(y.float().cpu().numpy()).all()
+        assert (err <= tol).all(), f"{(err > tol).mean():.3%} out, worst {(err / np.maximum(tol, 1e-300)).max():.2f} of the tolerance"
+
+
+def read(plan, b):
+    """(groups, start) of a plan, as the oracle gives them."""
+    p = plan.cpu().tolist()
+    n, start, members, groups = p[0], p[4:4 + b], p[4 + b:4 + 2 * b], p[4 + 2 * b:4 + 4 * b]
+    found = [groups[4 * i:4 * i + 4] for i in range(n)]
+    for tokens, lead, first, count in found:
+        assert lead == members[first]
+    return [(tokens, members[first:first + count]) for tokens, lead, first, count in found], start
+
+
+MIXED = [(33, [5, 1, 20, None]), (0, [7]), (64, [0, 3]), (200, [1] * 9), (16, [40, None]), (0, [None, 2, 3]), (150, [100, 0, 64])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 64, 256])
+@pytest.mark.parametrize("seed", [0, 1])
+def test_plan(gpu_device, page, seed):
+    s = Forks(gpu_device, MIXED, 2, 1, 8, page=page, seed=seed)
+    assert read(s.plan(), len(s.lens)) == step.shared(s.table.cpu().tolist(), s.lens, page)
+
+
+@pytest.mark.gpu
+def test_plans_of_other_tables(gpu_device):
+    """No sequence, one, entries that are no page, shared runs that end early, lengths beyond the table, thousands of rows."""
+    def plan(table, lens, page):
+        t = torch.tensor(table, dtype=torch.int32, device=gpu_device).view(len(lens), -1)
+        got = read(ck.kv_shared(t, torch.tensor(lens, dtype=torch.int32, device=gpu_device), page), len(lens))
+        assert got == step.shared(table, lens, page)
+        return got
+
+    assert ck.kv_shared(torch.zeros((0, 3), dtype=torch.int32, device=gpu_device), torch.zeros(0, dtype=torch.int32, device=gpu_device), 16).shape == (4,)
+    assert plan([[3, 4]], [20], 16) == ([], [0])
+    assert plan([[3, 4], [3, 5]], [20, 30], 16) == ([(16, [0, 1])], [16, 16])
+    assert plan([[3, 4], [3, 4]], [20, 19], 16) == ([(19, [0, 1])], [19, 19])
+    assert plan([[-1, 4], [-1, 4]], [20, 20], 16) == ([], [0, 0])
+    assert plan([[3, -1, 5], [3, -1, 5]], [40, 40], 16) == ([(16, [0, 1])], [16, 16])
+    assert plan([[7, 8], [7, 8]], [900, 1000], 16) == ([(32, [0, 1])], [32, 32])
+    assert plan([[7, 8], [7, 8], [7, 1]], [32, -4, 0], 16) == ([], [0, 0, 0])
+    g = torch.Generator().manual_seed(3)
+    table = torch.randint(0, 40, (2500, 1), generator=g).repeat(1, 70)
+    table[:, 65] += torch.randint(0, 3, (2500,), generator=g)
+    plan(table.tolist(), torch.randint(0, 71, (2500,), generator=g).tolist(), 1)
+
+
+HEADS = [(1, 1, 64), (4, 4, 128), (8, 2, 128), (32, 2, 64), (34, 2, 128), (6, 2, 80), (5, 1, 8), (14, 2, 96), (4, 1, 256), (16, 16, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,h,d", HEADS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_heads(gpu_device, hq, h, d, dtype):
+    print(f"[shared] {hq}/{h} x {d} {dtype}", flush=True)
+    s = Forks(gpu_device, MIXED, hq, h, d, dtype=dtype)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,h,d", [(8, 2, 128), (3, 3, 64), (17, 1, 16), (8, 8, 256), (6, 2, 80)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes(gpu_device, hq, h, d, dtype):
+    print(f"[shared] int8 {hq}/{h} x {d} {dtype}", flush=True)
+    s = Forks(gpu_device, MIXED, hq, h, d, dtype=dtype, int8=True)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 2, 8, 32, 128, 1024])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("order", ["phtd", "pthd", "htpd"])
+def test_pages(gpu_device, page, int8, order):
+    print(f"[shared] page {page} int8 {int8} {order}", flush=True)
+    s = Forks(gpu_device, [(300, [5, 200, 1]), (1030, [0, 9]), (70, [None, 3])], 8, 2, 64, page=page, int8=int8, order=order)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("members", [2, 5, 16, 17, 70])
+@pytest.mark.parametrize("tokens", [1, 16, 127, 129, 5000])
+def test_members(gpu_device, members, tokens):
+    """Rows that fill one tile, end inside one or take several, over one piece or many."""
+    print(f"[shared] {members} members of {tokens} tokens", flush=True)
+    s = Forks(gpu_device, [(tokens, [i % 3 for i in range(members)])], 8, 2, 128, page=1)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+def test_many_groups(gpu_device):
+    g = torch.Generator().manual_seed(5)
+    groups = [(int(torch.randint(1, 700, (1,), generator=g)), torch.randint(0, 90, (int(torch.randint(1, 7, (1,), generator=g)),), generator=g).tolist())
+              for _ in range(75)]
+    s = Forks(gpu_device, groups, 4, 2, 64, page=8)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+def test_nothing_shared(gpu_device):
+    """Without groups the results are the single-token kernel's, bit for bit."""
+    s = Forks(gpu_device, [(0, [n]) for n in (1, 333, 17, 1024)] + [(0, [None])], 8, 2, 128)
+    assert torch.equal(s.run(), ck.paged_attention(s.q, s.k, s.v, s.table, s.kv_lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_scale(gpu_device, scale):
+    s = Forks(gpu_device, MIXED, 8, 2, 64)
+    s.check(s.run(scale=scale), scale=scale)
+
+
+@pytest.mark.gpu
+def test_pages_that_are_none(gpu_device):
+    """Entries out of the cache's range, in what is shared and behind it."""
+    s = Forks(gpu_device, [(128, [20, 30, 40]), (64, [50, 0])], 8, 2, 64)
+    lead = s.table[:, 0].tolist()
+    first = [b for b in range(5) if lead[b] == lead[0]]
+    for b in first:
+        s.table[b, 3] = 10 ** 6
+    s.table[first[0], -1] = -1
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_plan_made_before(gpu_device, int8):
+    """Sequences that have grown since, one that has ended, one that is shorter than what was shared."""
+    s = Forks(gpu_device, [(100, [30, 40, 50, 60]), (40, [8, 9])], 8, 2, 64, int8=int8)
+    lens = s.lens
+    group = [b for b in range(6) if lens[b] > 100]
+    early = [n - 5 if n else 0 for n in lens]
+    s.kv_lens = torch.tensor(early, dtype=torch.int32, device=gpu_device)
+    plan = s.plan()
+    late = list(lens)
+    late[group[1]], late[group[2]] = 0, 70
+    s.kv_lens = torch.tensor(late, dtype=torch.int32, device=gpu_device)
+    s.check(s.run(plan), late)
+
+
+@pytest.mark.gpu
+def test_no_numbers_out_of_sight(gpu_device):
+    """Infinities and NaN behind a sequence's end in pages that others go on in do not reach its result (Forks fills them with NaN);
+    NaN in a shared key reaches the rows that see it alone."""
+    s = Forks(gpu_device, [(48, [5, 6]), (32, [9, 8])], 4, 2, 64)
+    base = s.run()
+    lead = s.table[:, 0].tolist()
+    s.v[lead[0], 0, 3, 5] = float("nan")
+    y = s.run()
+    hit = [b for b in range(4) if lead[b] == lead[0]]
+    bad = y.isnan()
+    assert bad[hit][:, :2, 5].all() and bad.sum() == 2 * len(hit)
+    other = [b for b in range(4) if b not in hit]
+    assert torch.equal(y[other], base[other])
+
+
+@pytest.mark.gpu
+def test_out_strides_streams_and_graphs(gpu_device):
+    s = Forks(gpu_device, MIXED, 8, 2, 64)
+    want = s.run()
+    wide = torch.full((len(s.lens), 8, 128), 7.0, dtype=torch.bfloat16, device=gpu_device)
+    s.run(out=wide[..., 32:96])
+    assert torch.equal(wide[..., 32:96], want) and (wide[..., :32] == 7).all() and (wide[..., 96:] == 7).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = s.run()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = s.plan()
+        y = [s.run(plan), s.run(plan, scale=0.5)]
+    for i in range(4):
+        s.q.copy_(torch.randn(s.q.shape, device=gpu_device))
+        graph.replay()
+        eager = [s.run(), s.run(scale=0.5)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(y, eager))
+
+
+@pytest.mark.gpu
+def test_the_same_every_time(gpu_device):
+    s = Forks(gpu_device, [(9000, [50] * 20), (300, [700] * 5)], 16, 2, 128)
+    want = s.run()
+    for _ in range(5):
+        assert torch.equal(s.run(), want)
