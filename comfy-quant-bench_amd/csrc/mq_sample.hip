@@ -4,10 +4,12 @@
 //   shortest leading part whose mass reaches p of theirs, and of those w_i >= min_p; the token is the first i, in
 //   the order of i, whose kept mass up to it exceeds u times all kept mass. T <= 0: the first largest.
 //
-// Weights are taken in fp64 (a polynomial of degree 12 on [-1/2, 1/2] octaves, 1e-16) and summed as integers, in
-// units of 2^-B of the largest with B = 62 - log2(V): sums are exact and the same in every order, so the result does
-// not depend on how a row is split or on which atomic comes first. (In fp32 the sum of a hundred thousand
-// weights would be off by more than the share of a single token.)
+// Weights are summed as integers, in units of 2^-B of the largest with B = 62 - log2(V): sums are exact and the same
+// in every order, so the result does not depend on how a row is split or on which atomic comes first. A weight
+// is a table's entry (fp64, 1e-16) for the nearest multiple of a power of two that cuts the row's reach into some 2048 bins, times
+// 1 + e for the rest of l, which is exact in fp32, is below 0.018 T and takes five fp32 products: 1e-9 at most, of random signs.
+// (With fp32 weights the sum of a hundred thousand of them would be off by more than the share of a single token; a fp64
+// exponential for every value takes four times as long as all of the rest.)
 //
 // A row is read three times, from memory and then from the caches: for its largest and smallest value; for a histogram,
 // numbers and masses, over 2048 bins of equal width in l, whose sums from the top say which bins the limits k and p cut;
@@ -29,6 +31,7 @@ constexpr int kPer = 8, kBlock = kThreads * kPer;   // consecutive values of a t
 constexpr int kBins = 2048;
 constexpr int kList = 4096;                         // values that are held in LDS
 constexpr int kMostBlocks = (1 << 24) / kBlock;
+constexpr double kLog2e64 = 1.4426950408889634074;
 constexpr float kNone = -__builtin_inff();          // of NaN too, which is never chosen
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -84,9 +87,10 @@ __device__ __forceinline__ uint64_t code_of(uint32_t key, int i) {
 }
 
 struct Lds {
+    double weight[kBins];           // of the bins' centres
     uint64_t mass[kBins];           // of the bins; of the blocks of a row
     uint32_t count[kBins];
-    uint64_t list[kList];           // key << 32 | index, in the order of the indexes
+    uint64_t list[kList];           // index << 32 | key
     uint64_t sort[kList];           // codes
     uint64_t wave[2 * kWavesOf];
     int found, n;
@@ -136,19 +140,20 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t s, Lds& sh) {
     return s;
 }
 
-// sh.sort[0 .. n) descending (n <= kList).
-__device__ void sort_codes(int n, Lds& sh) {
+// x[0 .. n) ascending or (DOWN) descending (n <= kList).
+template <bool DOWN>
+__device__ void sort_list(uint64_t* x, int n) {
     int size = 2;
     while (size < n) size *= 2;
     __syncthreads();
-    for (int i = n + threadIdx.x; i < size; i += kThreads) sh.sort[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) x[i] = DOWN ? 0 : ~uint64_t{0};
     for (int k = 2; k <= size; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
             __syncthreads();
             for (int t = threadIdx.x; t < size / 2; t += kThreads) {
                 const int a = 2 * t - (t & (j - 1)), b = a + j;
-                const uint64_t x = sh.sort[a], y = sh.sort[b];
-                if ((x < y) == ((a & k) == 0)) { sh.sort[a] = y; sh.sort[b] = x; }
+                const uint64_t u = x[a], v = x[b];
+                if ((u < v) == (((a & k) == 0) == DOWN)) { x[a] = v; x[b] = u; }
             }
         }
     __syncthreads();
@@ -165,33 +170,28 @@ struct Row {
     int first;              // its first index
     bool infinite;
     double scale, unit;     // log2(e) / T; 2^(52 - B)
-    float reach, per_bin;   // what is further below the best weighs nothing; bins per unit of l
+    float half, reach;      // half of the best; of how far below it a value may be and weigh anything (halves: no overflow)
+    float step, per_step;   // width of a bin, a power of two; its inverse
+    float top;              // the best's multiple of it
+    float inv, inv_rest;    // 1 / T in two parts
+    const double* weights;  // of the bins
 
     __device__ __forceinline__ float seen(float v) const { return infinite ? v == __builtin_inff() ? 0.0f : kNone : v; }
-    __device__ __forceinline__ bool heavy(float v) const { return best - v < reach; }
+    __device__ __forceinline__ bool heavy(float v) const { return __builtin_fmaf(v, -0.5f, half) < reach; }
     __device__ __forceinline__ int bin(float v) const {
-        const int b = static_cast<int>((best - v) * per_bin);
+        const int b = static_cast<int>(top - __builtin_rintf(v * per_step));
         return b < kBins - 1 ? b : kBins - 1;
     }
+    // The weight of a value that is heavy.
     __device__ __forceinline__ double weight(float v) const {
-        if (v == best) return 1.0;
-        const double y = (static_cast<double>(v) - static_cast<double>(best)) * scale;
-        if (!(y > -64.0)) return 0.0;
-        const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
-        double p = 1.0 / 479001600.0;
-        p = __builtin_fma(p, f, 1.0 / 39916800.0);
-        p = __builtin_fma(p, f, 1.0 / 3628800.0);
-        p = __builtin_fma(p, f, 1.0 / 362880.0);
-        p = __builtin_fma(p, f, 1.0 / 40320.0);
-        p = __builtin_fma(p, f, 1.0 / 5040.0);
-        p = __builtin_fma(p, f, 1.0 / 720.0);
-        p = __builtin_fma(p, f, 1.0 / 120.0);
-        p = __builtin_fma(p, f, 1.0 / 24.0);
-        p = __builtin_fma(p, f, 1.0 / 6.0);
-        p = __builtin_fma(p, f, 0.5);
-        p = __builtin_fma(p, f, 1.0);
-        p = __builtin_fma(p, f, 1.0);
-        return __builtin_ldexp(p, static_cast<int>(n));
+        const float n = __builtin_rintf(v * per_step), rest = __builtin_fmaf(-n, step, v);      // exact
+        const int b = static_cast<int>(top - n);
+        const float x = __builtin_fmaf(rest, inv, rest * inv_rest);
+        float e = __builtin_fmaf(x, 1.0f / 24.0f, 1.0f / 6.0f);
+        e = __builtin_fmaf(e, x, 0.5f);
+        e = __builtin_fmaf(e, x, 1.0f) * x;
+        const double w = weights[b < kBins - 1 ? b : kBins - 1];
+        return __builtin_fma(w, static_cast<double>(e), w);
     }
     // In units: the mantissa of unit + w.
     __device__ __forceinline__ uint64_t whole(double w) const {
@@ -274,11 +274,34 @@ __device__ __forceinline__ bool settle(Row& w, uint64_t best, float low, int64_t
     bits = bits < 51 ? bits : 51;
     w.unit = __builtin_ldexp(1.0, 52 - bits);
     // 2^-(bits + 1) is half a unit: 0 once rounded (a tie to even; the reach ends a little beyond it)
-    w.reach = static_cast<float>((bits + 1.01) / w.scale);
-    const float range = w.best - low, span = range < w.reach ? range : w.reach;
-    w.per_bin = span > 0.0f ? static_cast<float>(kBins) / span : 0.0f;
-    if (!(w.per_bin < 0x1p100f)) w.per_bin = 0x1p100f;
+    w.reach = static_cast<float>(0.5 * (bits + 1.01) / w.scale);
+    w.half = 0.5f * w.best;
+    const float range = w.half - 0.5f * low, span = range < w.reach ? range : w.reach;
+    // the smallest power of two that is at least span / 1023; none is needed below a 2^25th of the best (a value within
+    // reach that is no multiple of that is at least a quarter of the best away from it)
+    int at = 0, of_best = 0;
+    const float part = __builtin_frexpf(span * (2.0f / (kBins - 2)), &at);      // in [2^(at - 1), 2^at)
+    at -= part == 0.5f;
+    (void)__builtin_frexpf(w.best, &of_best);
+    at = span > 0.0f && at > of_best - 25 ? at : of_best - 25;
+    at = at > -120 ? at < 120 ? at : 120 : -120;
+    w.step = __builtin_ldexpf(1.0f, at);
+    w.per_step = __builtin_ldexpf(1.0f, -at);
+    w.top = __builtin_rintf(w.best * w.per_step);
+    const double inv = 1.0 / static_cast<double>(w.T);
+    w.inv = static_cast<float>(inv);
+    w.inv_rest = static_cast<float>(inv - static_cast<double>(w.inv));
     return false;
+}
+
+// The weights of the bins' centres.
+__device__ __forceinline__ void weigh_bins(Row& w, Lds& sh) {
+    for (int b = threadIdx.x; b < kBins; b += kThreads) {
+        const double d = (static_cast<double>(w.top) - b) * static_cast<double>(w.step) - static_cast<double>(w.best);
+        sh.weight[b] = exp2(d * w.scale);
+    }
+    w.weights = sh.weight;
+    __syncthreads();
 }
 
 // The second reading: numbers and (p) masses of the bins, added to count and mass.
@@ -327,7 +350,7 @@ __device__ __forceinline__ void each(const Row& w, int n, const Lds& sh, F f) {
     if (n >= 0) {
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t x = sh.list[i];
-            f(value_of(static_cast<uint32_t>(x >> 32)), static_cast<int>(static_cast<uint32_t>(x)));
+            f(value_of(static_cast<uint32_t>(x)), static_cast<int>(x >> 32));
         }
         return;
     }
@@ -425,7 +448,7 @@ __device__ Limit resolve(const Row& w, int n, int bin, Limit now, uint64_t need,
         }
         return limit;
     }
-    sort_codes(held, sh);
+    sort_list<true>(sh.sort, held);
     // four codes a thread, in order
     constexpr int kEach = kList / kThreads;
     uint64_t x[kEach], sum = 0;
@@ -466,6 +489,7 @@ __device__ __forceinline__ uint64_t place(float u, uint64_t all) {
 
 // The token of a value list in LDS.
 __device__ __forceinline__ int choose(const Row& w, int n, Limit limit, float u, Lds& sh) {
+    sort_list<false>(sh.list, n);
     constexpr int kEach = kList / kThreads;
     uint64_t x[kEach], sum = 0, all;
 #pragma unroll
@@ -474,8 +498,8 @@ __device__ __forceinline__ int choose(const Row& w, int n, Limit limit, float u,
         x[e] = 0;
         if (i < n) {
             const uint64_t y = sh.list[i];
-            const uint32_t k = static_cast<uint32_t>(y >> 32);
-            if (limit.keeps(k, static_cast<int>(static_cast<uint32_t>(y)))) x[e] = w.kept_units(value_of(k));
+            const uint32_t k = static_cast<uint32_t>(y);
+            if (limit.keeps(k, static_cast<int>(y >> 32))) x[e] = w.kept_units(value_of(k));
         }
         sum += x[e];
     }
@@ -483,7 +507,7 @@ __device__ __forceinline__ int choose(const Row& w, int n, Limit limit, float u,
     const uint64_t t = place(u, all);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-        if (to <= t && to + x[e] > t) sh.found = static_cast<int>(static_cast<uint32_t>(sh.list[kEach * threadIdx.x + e]));
+        if (to <= t && to + x[e] > t) sh.found = static_cast<int>(sh.list[kEach * threadIdx.x + e] >> 32);
         to += x[e];
     }
     __syncthreads();
@@ -589,42 +613,29 @@ __device__ Limit limit_of(const Row& w, int n, Cuts c, Lds& sh) {
     return limit;
 }
 
-// The third reading, of values b .. e - 1: those in bins 0 .. most, in order, to put(place, key << 32 | index) as far as there
-// is room; how many there are.
-template <int DT, typename F>
-__device__ __forceinline__ int collect(const Row& w, int b, int e, int most, F put, Lds& sh) {
-    int n = 0;
-    const int wave = threadIdx.x >> 6;
+// The third reading, of values b .. e - 1: those in bins 0 .. most to sh.list, in any order, as far as there is room; how many
+// there are.
+template <int DT>
+__device__ __forceinline__ int collect(const Row& w, int b, int e, int most, Lds& sh) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
     for (int i0 = b; i0 < e; i0 += kBlock) {
         const int i = i0 + kPer * threadIdx.x;
+        if (i >= e) break;
         float v[kPer];
-        uint32_t take = 0;
-        if (i < e) {
-            load8<DT>(w.x, i, e, v);
+        load8<DT>(w.x, i, e, v);
 #pragma unroll
-            for (int x = 0; x < kPer; ++x) {
-                v[x] = w.seen(v[x]);
-                take |= w.heavy(v[x]) && w.bin(v[x]) <= most ? 1u << x : 0u;
+        for (int x = 0; x < kPer; ++x) {
+            v[x] = w.seen(v[x]);
+            if (w.heavy(v[x]) && w.bin(v[x]) <= most) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kList) sh.list[at] = static_cast<uint64_t>(i + x) << 32 | key_of(v[x]);
             }
         }
-        const int mine = __popc(take), to = wave_incl(mine);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) sh.wave[wave] = to;
-        __syncthreads();
-        int at = n + to - mine;
-        for (int y = 0; y < kWavesOf; ++y) {
-            const int m = static_cast<int>(sh.wave[y]);
-            at += y < wave ? m : 0;
-            n += m;
-        }
-        if (take)
-#pragma unroll
-            for (int x = 0; x < kPer; ++x)
-                if (take >> x & 1) {
-                    if (at < kList) put(at, static_cast<uint64_t>(key_of(v[x])) << 32 | static_cast<uint32_t>(i + x));
-                    ++at;
-                }
     }
+    __syncthreads();
+    const int n = sh.n;
     __syncthreads();
     return n;
 }
@@ -632,7 +643,7 @@ __device__ __forceinline__ int collect(const Row& w, int b, int e, int most, F p
 // The last bin that w >= min_p can be in (min_p alone limits the row).
 __device__ __forceinline__ int least_bin(const Row& w) {
     const double d = -log(static_cast<double>(w.least < 1.0f ? w.least : 1.0f)) * static_cast<double>(w.T) * 1.000001;
-    const double b = d * w.per_bin + 1.0;
+    const double b = d * w.per_step + 2.0;
     return b < kBins - 1 ? static_cast<int>(b) : kBins - 1;
 }
 
@@ -661,8 +672,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     extremes<DT>(w, 0, w.V, &best, &low, sh);
     int64_t token;
     if (!settle(w, best, low, &token)) {
+        weigh_bins(w, sh);
         Cuts c{kBins, kBins, 0, 0, kBins - 1, 0};
-        const Limit all{0, w.V};
         if (w.limited()) {
             clear_bins(sh);
             histogram<DT>(w, 0, w.V, sh);
@@ -673,7 +684,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
         }
         int n = kList + 1;
         if ((w.limited() && c.held <= kList) || (!w.limited() && w.least > 0.0f) || w.V <= kList)
-            n = collect<DT>(w, 0, w.V, c.most, [&](int at, uint64_t x) { sh.list[at] = x; }, sh);
+            n = collect<DT>(w, 0, w.V, c.most, sh);
         token = finish<DT>(w, c, n, a.u[r], sh);
     }
     if (threadIdx.x == 0) a.token[r] = token;
