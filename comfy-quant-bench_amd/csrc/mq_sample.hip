@@ -5,21 +5,26 @@
 //   the order of i, whose kept mass up to it exceeds u times all kept mass. T <= 0: the first largest.
 //
 // Weights are summed as integers, in units of 2^-B of the largest with B = 62 - log2(V): sums are exact and the same
-// in every order, so the result does not depend on how a row is split or on which atomic comes first. A weight
-// is a table's entry (fp64, 1e-16) for the nearest multiple of a power of two that cuts the row's reach into some 2048 bins, times
-// 1 + e for the rest of l, which is exact in fp32, is below 0.018 T and takes five fp32 products: 1e-9 at most, of random signs.
-// (With fp32 weights the sum of a hundred thousand of them would be off by more than the share of a single token; a fp64
-// exponential for every value takes four times as long as all of the rest.)
+// in every order, so the result does not depend on how a row is split or on which atomic comes first. (With fp32 weights the
+// sum of a hundred thousand of them would be off by more than the share of a single token; a fp64 exponential for every
+// value takes four times as long as all of the rest.) A weight is a table's entry (fp64, 1e-15) for the nearest multiple of a
+// power of two, `step`, of which 4096 reach as far down as anything weighs (32 T), times 1 + e for the rest of l: that is
+// exact in fp32, below T / 128, and its series takes four fp32 products: 1e-9 at most, of random signs.
 //
-// A row is read three times, from memory and then from the caches: for its largest and smallest value; for a histogram,
-// numbers and masses, over 2048 bins of equal width in l, whose sums from the top say which bins the limits k and p cut;
-// and for the values of those bins and above, in the order of i, into LDS. There the cut bin is sorted and the
-// limits become one value and one index. Where more is kept than fits there (a flat row), only the cut bin is collected and
-// the row is read once more for the kept masses of its blocks of 8192, and the block that the token is in; where
-// even the cut bin does not fit (values alike by the thousand), its limit is found digit by digit of the values' bits.
+// First reading: the largest value, and numbers and masses of the 4096 bins around those multiples below it, in LDS. The
+// bins are places n modulo 4096, so that they stay where they are as the largest value seen rises; those that fall out of
+// reach are cleared. A bin is one 64-bit sum: a value adds 1 in the upper bits and 2^fine (e + 1/32) in the lower ones; the bin's
+// mass is its centre's weight times (number + sum of e). Sums over the bins from the top say which bin the limit cuts.
 //
-// A workgroup of 1024 takes a row, where there are enough of them or they are short; else every row is cut into parts, for
-// which the three readings are three launches, and the part that ends last has all to choose from.
+// Second reading: where k limits a row (few values), those of the cut bin and above, into LDS, where everything else is decided;
+// where p does, those of the cut bin alone and the masses of what is above it by blocks of 8192; without either, the masses of
+// the blocks. A limit inside a bin, a value and an index among equal ones, is found by sums over ranges of values (then of
+// indexes), narrowed by 4096 at a time; so is the token, in LDS or in the block that u is in, which is read once more.
+//
+// A workgroup of 1024 takes a row. Where there are fewer rows than compute units, long rows are cut into parts: a launch for the
+// first reading, one for the second, and the part that ends last has all to choose from. What fits neither (a limit k of
+// thousands, a cut bin of thousands, temperatures beyond 2^+-20 times what logits are like) is done by one workgroup that reads
+// the row again as often as it takes.
 #include "mq_device.h"
 #include "mq_internal.h"
 
@@ -28,53 +33,259 @@ namespace {
 
 constexpr int kThreads = 1024, kWavesOf = kThreads / 64;
 constexpr int kPer = 8, kBlock = kThreads * kPer;   // consecutive values of a thread; of the workgroup
-constexpr int kBins = 2048;
+constexpr int kBins = 4096, kMask = kBins - 1;
+constexpr int kEach = kBins / kThreads;             // bins, and values of the list, of a thread
 constexpr int kList = 4096;                         // values that are held in LDS
+constexpr int kFew = 256;
 constexpr int kMostBlocks = (1 << 24) / kBlock;
-constexpr double kLog2e64 = 1.4426950408889634074;
+constexpr int kMostParts = 16;
 constexpr float kNone = -__builtin_inff();          // of NaN too, which is never chosen
+constexpr float kBias = 1.0f / 32.0f;               // what makes e positive in a bin's sum
+static_assert(kMostBlocks <= kBins && kList == kBins);
 
+// Values as unsigned integers in their order, both zeros alike.
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-struct __attribute__((packed, aligned(2))) Eight16 {
+// --- reading a row
+
+struct __attribute__((packed, aligned(2))) Sixteen {
     uint32_t w[4];
 };
-struct __attribute__((packed, aligned(4))) Eight32 {
-    float f[4];
+// Eight values as they lie in memory.
+template <int DT>
+struct Raw8 {
+    Sixteen a[DT == kDtF32 ? 2 : 1];
+};
+// Values i .. i + 7 of a row; what is at `end` and behind it as -infinity.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8(const void* row, int i, int end) {
+    constexpr int kParts = DT == kDtF32 ? 2 : 1;
+    Raw8<DT> r;
+    if (i + kPer <= end) {
+        const char* p = static_cast<const char*>(row) + static_cast<int64_t>(i) * (DT == kDtF32 ? 4 : 2);
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) r.a[h] = *reinterpret_cast<const Sixteen*>(p + 16 * h);
+        return r;
+    }
+    constexpr uint32_t kLow = DT == kDtF16 ? 0xfc00u : 0xff80u;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        if constexpr (DT == kDtF32) {
+            r.a[e / 4].w[e % 4] = i + e < end ? static_cast<const uint32_t*>(row)[i + e] : 0xff800000u;
+        } else {
+            const uint32_t x = i + e < end ? static_cast<const uint16_t*>(row)[i + e] : kLow;
+            r.a[0].w[e / 2] = e & 1 ? r.a[0].w[e / 2] | x << 16 : x;
+        }
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void unpack8(const Raw8<DT>& r, float (&v)[kPer]) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        if constexpr (DT == kDtF32) {
+            v[e] = __uint_as_float(r.a[e / 4].w[e % 4]);
+        } else {
+            const uint32_t w = r.a[0].w[e / 2];
+            v[e] = DT == kDtF16 ? f16_bits_to_f32(static_cast<uint16_t>(e & 1 ? w >> 16 : w & 0xffffu)) : e & 1 ? bf16hi(w) : bf16lo(w);
+        }
+        v[e] = v[e] > kNone ? v[e] : kNone;         // NaN
+    }
+}
+
+// f(i, values i .. i + 7) for this thread's of values b .. e - 1, 32 or 64 bytes a thread in flight. All threads make all calls;
+// values behind the end are -infinity.
+template <int DT, typename F>
+__device__ __forceinline__ void scan(const void* row, int b, int e, F f) {
+    constexpr int kAhead = DT == kDtF32 ? 2 : 4;
+    const int mine = kPer * threadIdx.x;
+    Raw8<DT> raw[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x)
+        if (b + x * kBlock < e) raw[x] = load_raw8<DT>(row, b + x * kBlock + mine, e);
+    for (int i0 = b; i0 < e; i0 += kAhead * kBlock) {
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const int i = i0 + x * kBlock;
+            if (i >= e) break;
+            float v[kPer];
+            unpack8<DT>(raw[x], v);
+            if (i + kAhead * kBlock < e) raw[x] = load_raw8<DT>(row, i + kAhead * kBlock + mine, e);
+            f(i + mine, v);
+        }
+    }
+}
+
+struct Lds {
+    uint64_t weight[kBins];         // of the bins' centres in units, from the best's down
+    uint64_t bins[kBins + 64];      // first by place (n modulo 4096, and a place for each lane's values that are in none), then
+                                    // masses from the best's down; blocks' masses
+    uint64_t work[kBins];           // sums over ranges
+    uint64_t list[kList];           // index << 32 | key, in any order
+    uint64_t wave[2 * kWavesOf];
+    int found, n;
+    uint64_t left;
 };
 
-// Values i .. i + 7 of a row; NaN and what is behind the end as -infinity, both zeros alike.
-template <int DT>
-__device__ __forceinline__ void load8(const void* row, int i, int end, float (&v)[kPer]) {
-    if (i + kPer <= end) {
-        if constexpr (DT == kDtF32) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const Eight32 x = *reinterpret_cast<const Eight32*>(static_cast<const float*>(row) + i + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * h + e] = x.f[e];
-            }
-        } else {
-            const Eight16 x = *reinterpret_cast<const Eight16*>(static_cast<const uint16_t*>(row) + i);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const uint32_t w = x.w[e / 2];
-                v[e] = DT == kDtF16 ? f16_bits_to_f32(static_cast<uint16_t>(e & 1 ? w >> 16 : w & 0xffffu)) : e & 1 ? bf16hi(w) : bf16lo(w);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) v[e] = i + e < end ? load_as_f32(row, DT, i + e) : kNone;
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = v[e] == v[e] ? v[e] + 0.0f : kNone;
+// --- the workgroup together; every thread calls these
+
+// (Lane exchanges through LDS take ten times as long.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v), CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(v >> 32), CTRL, ROWS, 0xf, false);
+    return static_cast<uint64_t>(hi) << 32 | lo;
 }
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane));
+}
+// The sum over the lanes up to and including this one.
+__device__ __forceinline__ uint64_t wave_incl(uint64_t v) {
+    v += dpp64<0x111, 0xf>(v);      // from 1, 2, 4, 8 lanes before, within 16
+    v += dpp64<0x112, 0xf>(v);
+    v += dpp64<0x114, 0xf>(v);
+    v += dpp64<0x118, 0xf>(v);
+    v += dpp64<0x142, 0xa>(v);      // lane 15 to the next 16, lane 31 to the upper 32
+    v += dpp64<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane64(wave_incl(v), 63); }
+__device__ __forceinline__ uint32_t wave_max(uint32_t b) {
+    b = __builtin_elementwise_max(b, dpp_mov_u<kQuadXor1>(b));
+    b = __builtin_elementwise_max(b, dpp_mov_u<kQuadXor2>(b));
+    b = __builtin_elementwise_max(b, dpp_mov_u<kRowRor4>(b));
+    b = __builtin_elementwise_max(b, dpp_mov_u<kRowRor8>(b));
+    const uint32_t r0 = __builtin_amdgcn_readlane(b, 0), r1 = __builtin_amdgcn_readlane(b, 16);
+    const uint32_t r2 = __builtin_amdgcn_readlane(b, 32), r3 = __builtin_amdgcn_readlane(b, 48);
+    return __builtin_elementwise_max(__builtin_elementwise_max(r0, r1), __builtin_elementwise_max(r2, r3));
+}
+
+// The sum up to and including this thread's; *all = everybody's.
+__device__ __forceinline__ uint64_t block_incl(uint64_t v, uint64_t* all, Lds& sh) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_incl(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh.wave[wave] = v;
+    __syncthreads();
+    const uint64_t to = wave_incl(sh.wave[threadIdx.x & 15]);          // (each 16 lanes the same; the first 16's are read)
+    *all = lane64(to, 15);
+    return v + (wave ? lane64(to, wave - 1) : 0);
+}
+
+__device__ __forceinline__ uint64_t block_sum(uint64_t s, Lds& sh) {
+    s = wave_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return lane64(wave_incl(sh.wave[threadIdx.x & 15]), 15);
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t s, Lds& sh) {
+    s = wave_max(s);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return wave_max(static_cast<uint32_t>(sh.wave[threadIdx.x & 15]));
+}
+
+// Where the sum of x(0), x(1), ... x(4095) reaches `need` (> 0): the place (4096: nowhere) and what is missing in front of it.
+// Every wave sums 256 of them; the one where it is looks at its own again.
+template <typename F>
+__device__ __forceinline__ int cut(F x, uint64_t need, uint64_t* left, Lds& sh) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint64_t v[kEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        v[e] = x(256 * wave + 64 * e + lane);
+        sum += v[e];
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (lane == 0) sh.wave[wave] = sum;
+    __syncthreads();
+    const uint64_t to = wave_incl(sh.wave[lane & 15]);
+    const uint64_t upto = lane64(to, wave), before = upto - sum;
+    if (wave == 0 && lane64(to, 15) < need && lane == 0) sh.found = kBins;
+    if (before < need && upto >= need) {
+        uint64_t at = before;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const uint64_t y = at + wave_incl(v[e]);
+            if (y - v[e] < need && y >= need) {
+                sh.found = 256 * wave + 64 * e + lane;
+                sh.left = need - (y - v[e]);
+            }
+            at = lane64(y, 63);
+        }
+    }
+    __syncthreads();
+    const int found = __builtin_amdgcn_readfirstlane(sh.found);
+    *left = sh.left;
+    __syncthreads();
+    return found;
+}
+
+// The place, from 0 to `most`, where the sum of the values' x, in the order of their places `at`, reaches *need (> 0, reached):
+// over 4096 ranges of places, then over the parts of the one where it does. *need: what is missing in front of the place.
+// n: none of a thread's places from n on (of 1024 e + thread) has an x. Few: each against all.
+__device__ __forceinline__ uint32_t narrow(int n, const uint32_t (&at)[kEach], uint64_t (&x)[kEach], uint32_t most, uint64_t* need, Lds& sh) {
+    if (n <= kFew) {
+        uint32_t* places = reinterpret_cast<uint32_t*>(sh.work + kFew);
+        __syncthreads();
+        if (threadIdx.x < kFew) {
+            sh.work[threadIdx.x] = x[0];
+            places[threadIdx.x] = at[0];
+        }
+        __syncthreads();
+        const int i = threadIdx.x >> 2;
+        const uint32_t mine = places[i];
+        uint64_t before = 0, same = 0;
+        for (int j = threadIdx.x & 3; j < n; j += 4) {
+            const uint64_t y = sh.work[j];
+            const uint32_t p = places[j];
+            before += p < mine ? y : 0;
+            same += p == mine ? y : 0;
+        }
+        before += dpp64<kQuadXor1, 0xf>(before);
+        before += dpp64<kQuadXor2, 0xf>(before);
+        same += dpp64<kQuadXor1, 0xf>(same);
+        same += dpp64<kQuadXor2, 0xf>(same);
+        if (i < n && before < *need && before + same >= *need) {
+            sh.found = static_cast<int>(mine);
+            sh.left = *need - before;
+        }
+        __syncthreads();
+        *need = sh.left;
+        return static_cast<uint32_t>(sh.found);
+    }
+    int shift = 0;
+    uint32_t from = 0;
+    while (most >> shift >= kBins) ++shift;
+    for (;;) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sh.work[kThreads * e + threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (x[e]) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.work[(at[e] - from) >> shift]), static_cast<unsigned long long>(x[e]));
+        __syncthreads();
+        const int range = cut([&](int i) { return sh.work[i]; }, *need, need, sh);
+        from += static_cast<uint32_t>(range < kBins ? range : kBins - 1) << shift;
+        if (shift == 0) return from;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (at[e] < from || (at[e] - from) >> shift) x[e] = 0;
+        shift = shift > 12 ? shift - 12 : 0;
+    }
+}
+
+// --- a row
 
 // What is kept: keys above `key`, and those equal to it up to index `last`.
 struct Limit {
@@ -82,584 +293,589 @@ struct Limit {
     int last;
     __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
 };
-__device__ __forceinline__ uint64_t code_of(uint32_t key, int i) {
-    return static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~i);        // larger: earlier in the order
-}
-
-struct Lds {
-    double weight[kBins];           // of the bins' centres
-    uint64_t mass[kBins];           // of the bins; of the blocks of a row
-    uint32_t count[kBins];
-    uint64_t list[kList];           // index << 32 | key
-    uint64_t sort[kList];           // codes
-    uint64_t wave[2 * kWavesOf];
-    int found, n;
-    uint64_t left;
-};
-static_assert(kMostBlocks <= kBins);
-
-// --- sums over the workgroup; every thread calls them
-
-template <typename T>
-__device__ __forceinline__ T wave_incl(T v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const T y = __shfl_up(v, s);
-        if (lane >= s) v += y;
-    }
-    return v;
-}
-
-// The sum up to and including this thread's; *all = everybody's.
-__device__ __forceinline__ uint64_t block_incl(uint64_t v, uint64_t* all, Lds& sh) {
-    const int wave = threadIdx.x >> 6;
-    v = wave_incl(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) sh.wave[wave] = v;
-    __syncthreads();
-    uint64_t sum = 0;
-#pragma unroll
-    for (int y = 0; y < kWavesOf; ++y) {
-        if (y < wave) v += sh.wave[y];
-        sum += sh.wave[y];
-    }
-    *all = sum;
-    return v;
-}
-
-__device__ __forceinline__ uint64_t block_sum(uint64_t s, Lds& sh) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = 0;
-#pragma unroll
-    for (int y = 0; y < kWavesOf; ++y) s += sh.wave[y];
-    return s;
-}
-
-// x[0 .. n) ascending or (DOWN) descending (n <= kList).
-template <bool DOWN>
-__device__ void sort_list(uint64_t* x, int n) {
-    int size = 2;
-    while (size < n) size *= 2;
-    __syncthreads();
-    for (int i = n + threadIdx.x; i < size; i += kThreads) x[i] = DOWN ? 0 : ~uint64_t{0};
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int a = 2 * t - (t & (j - 1)), b = a + j;
-                const uint64_t u = x[a], v = x[b];
-                if ((u < v) == (((a & k) == 0) == DOWN)) { x[a] = v; x[b] = u; }
-            }
-        }
-    __syncthreads();
-}
-
-// --- a row
 
 struct Row {
     const void* x;
     int V;
-    float T, p, least;
+    float T, p, least, u;
     int64_t k;
-    float best;             // the largest value (rows with +infinities: 0, and these 0, all others -infinity)
+    float best;             // the largest value
     int first;              // its first index
-    bool infinite;
-    double scale, unit;     // log2(e) / T; 2^(52 - B)
-    float half, reach;      // half of the best; of how far below it a value may be and weigh anything (halves: no overflow)
-    float step, per_step;   // width of a bin, a power of two; its inverse
-    float top;              // the best's multiple of it
+    int bits, fine, number; // B; fractional bits of a bin's sum of e; where its number begins
+    float step, per_step;   // distance of the bins' centres, a power of two; its inverse
+    float top;              // the best's bin, as a multiple of the step
     float inv, inv_rest;    // 1 / T in two parts
-    const double* weights;  // of the bins
+    float floor;            // the smallest value that min_p keeps
 
-    __device__ __forceinline__ float seen(float v) const { return infinite ? v == __builtin_inff() ? 0.0f : kNone : v; }
-    __device__ __forceinline__ bool heavy(float v) const { return __builtin_fmaf(v, -0.5f, half) < reach; }
-    __device__ __forceinline__ int bin(float v) const {
-        const int b = static_cast<int>(top - __builtin_rintf(v * per_step));
-        return b < kBins - 1 ? b : kBins - 1;
-    }
-    // The weight of a value that is heavy.
-    __device__ __forceinline__ double weight(float v) const {
-        const float n = __builtin_rintf(v * per_step), rest = __builtin_fmaf(-n, step, v);      // exact
-        const int b = static_cast<int>(top - n);
+    // How many bins below the best's; 4096 or more (or NaN, for -infinity): out of reach.
+    __device__ __forceinline__ float depth(float v) const { return top - __builtin_rintf(v * per_step); }
+    // A value's weight over its bin's, less 1.
+    __device__ __forceinline__ float excess(float v) const {
+        const float rest = __builtin_fmaf(-__builtin_rintf(v * per_step), step, v);      // exact
         const float x = __builtin_fmaf(rest, inv, rest * inv_rest);
-        float e = __builtin_fmaf(x, 1.0f / 24.0f, 1.0f / 6.0f);
-        e = __builtin_fmaf(e, x, 0.5f);
-        e = __builtin_fmaf(e, x, 1.0f) * x;
-        const double w = weights[b < kBins - 1 ? b : kBins - 1];
-        return __builtin_fma(w, static_cast<double>(e), w);
+        const float e = __builtin_fmaf(x, 1.0f / 6.0f, 0.5f);
+        return __builtin_fmaf(e, x, 1.0f) * x;
     }
-    // In units: the mantissa of unit + w.
-    __device__ __forceinline__ uint64_t whole(double w) const {
-        return __builtin_bit_cast(uint64_t, unit + w) - __builtin_bit_cast(uint64_t, unit);
+    // A value's weight in units, from the table: the bin's and e times that, both to 31 fractional bits (0 out of reach).
+    __device__ __forceinline__ uint64_t units(float v, const Lds& sh) const {
+        const float d = depth(v), e = excess(v);
+        const bool in = d < static_cast<float>(kBins);
+        const uint64_t c = sh.weight[in ? static_cast<int>(d) : kMask];
+        const int64_t more = static_cast<int64_t>(static_cast<int32_t>(c >> (bits - 30))) * static_cast<int32_t>(e * 0x1p31f);
+        return in ? c + static_cast<uint64_t>(more >> (61 - bits)) : 0;
     }
-    __device__ __forceinline__ uint64_t units(float v) const { return whole(weight(v)); }
-    __device__ __forceinline__ uint64_t kept_units(float v) const {
-        const double w = weight(v);
-        return w < static_cast<double>(least) && v != best ? uint64_t{0} : whole(w);
+    // The same from its own exponential.
+    __device__ __forceinline__ uint64_t units(float v) const {
+        const double x = exp2((static_cast<double>(v) - static_cast<double>(best)) * (1.4426950408889634074 / static_cast<double>(T)));
+        return static_cast<uint64_t>(__builtin_rint(x * __builtin_ldexp(1.0, bits)));
     }
-    __device__ __forceinline__ bool limited() const { return (k > 0 && k < V) || p < 1.0f; }
+    __device__ __forceinline__ bool k_limits() const { return k > 0 && k < V; }
+    __device__ __forceinline__ bool p_limits() const { return p < 1.0f; }
+    __device__ __forceinline__ uint64_t place(uint64_t all) const {     // u's in all kept units
+        const double x = u, at = x > 0.0 ? x * static_cast<double>(all) : 0.0;
+        const uint64_t t = at < static_cast<double>(all) ? static_cast<uint64_t>(at) : all - 1;
+        return t < all ? t : all - 1;
+    }
+    // The least number or mass that reaches p of `all`.
+    __device__ __forceinline__ uint64_t part(uint64_t all) const {
+        const double need = __builtin_ceil(static_cast<double>(p) * static_cast<double>(all));
+        const uint64_t n = need > 1.0 ? static_cast<uint64_t>(need) : 1;
+        return n < all ? n : all;
+    }
 };
+
+// What is the same in all lanes, in scalar registers.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
+// Centres 2^at apart, for a temperature T.
+__device__ __forceinline__ void set_step(Row& w, int at) {
+    w.step = uniform(__builtin_ldexpf(1.0f, at));
+    w.per_step = uniform(__builtin_ldexpf(1.0f, -at));
+    const double inv = 1.0 / static_cast<double>(w.T);
+    w.inv = uniform(static_cast<float>(inv));
+    w.inv_rest = uniform(static_cast<float>(inv - static_cast<double>(w.inv)));
+}
+
+// The exponent of the smallest power of two of which 4094 reach as far as anything weighs: 2^-(B + 1) is half a unit.
+__device__ __forceinline__ int step_of(const Row& w) {
+    int at;
+    (void)__builtin_frexpf(static_cast<float>((w.bits + 1.01) * 0.69314718055994531 / (kBins - 2) * static_cast<double>(w.T)), &at);
+    return at;
+}
+__device__ __forceinline__ bool usual(float T) { return T >= 0x1p-20f && T <= 0x1p20f; }
 
 template <int DT>
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t r) {
     Row w;
     w.x = static_cast<const char*>(a.x) + r * a.ld * (DT == kDtF32 ? 4 : 2);
     w.V = static_cast<int>(a.V);
-    w.T = a.temperature ? a.temperature[r] : a.temperature1;
-    w.p = a.top_p ? a.top_p[r] : a.top_p1;
-    w.least = a.min_p ? a.min_p[r] : a.min_p1;
-    w.k = a.top_k ? a.top_k[r] : a.top_k1;
+    w.T = uniform(a.temperature ? a.temperature[r] : a.temperature1);
+    w.T = w.T < 0x1p120f ? w.T : w.T >= 0x1p120f ? 0x1p120f : 0.0f;     // (NaN: 0)
+    w.p = uniform(a.top_p ? a.top_p[r] : a.top_p1);
+    w.least = uniform(a.min_p ? a.min_p[r] : a.min_p1);
+    w.k = a.top_k ? __builtin_amdgcn_readfirstlane(a.top_k[r]) : a.top_k1;
+    w.u = uniform(a.u[r]);
+    int log2 = 0;
+    while ((1 << log2) < w.V) ++log2;
+    w.bits = 62 - log2 < 51 ? 62 - log2 : 51;
+    w.number = 63 - log2;                           // V values at most, each below 2^(fine - 4)
+    w.fine = 67 - 2 * log2 < 33 ? 67 - 2 * log2 : 33;
+    if (usual(w.T)) set_step(w, step_of(w));
     return w;
 }
 
-// The first reading, of values b .. e - 1: the code of the first largest, the smallest above -infinity.
+// The first largest of values b .. e - 1: w.best, w.first.
 template <int DT>
-__device__ __forceinline__ void extremes(const Row& w, int b, int e, uint64_t* best, float* low, Lds& sh) {
-    float top = kNone, least = __builtin_inff();
+__device__ __forceinline__ void largest(Row& w, int b, int e, Lds& sh) {
+    float top = kNone;
     int at = b;
-    for (int i0 = b; i0 < e; i0 += kBlock) {
-        const int i = i0 + kPer * threadIdx.x;
-        if (i >= e) break;
-        float v[kPer];
-        load8<DT>(w.x, i, e, v);
+    scan<DT>(w.x, b, e, [&](int i, const float (&v)[kPer]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
+        for (int x = 0; x < kPer; ++x)
             if (v[x] > top) { top = v[x]; at = i + x; }
-            least = v[x] > kNone ? __builtin_fminf(least, v[x]) : least;
-        }
-    }
-    uint64_t code = code_of(key_of(top), at);
+    });
+    const uint32_t best = block_max(key_of(top), sh);
+    w.best = uniform(value_of(best));
+    w.first = __builtin_amdgcn_readfirstlane(~block_max(key_of(top) == best ? ~static_cast<uint32_t>(at) : 0u, sh));
+}
+
+// The first reading of values b .. e - 1 with their bins (numbers, MASSES: and sums of e). known: w.top says where the best's bin
+// is; else it is found on the way, with w.best. *base: the place of the best's bin in sh.bins.
+template <int DT, bool MASSES>
+__device__ __forceinline__ void bins_of(Row& w, int b, int e, bool known, int* base, Lds& sh) {
+    constexpr int kDepth = DT == kDtF32 ? 2 : 4;    // blocks in hand; as many are on their way
+    const int mine = kPer * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < kBins + 64; i += kThreads) sh.bins[i] = 0;
+    const uint64_t one = uint64_t{1} << w.number;
+    const float scale = uniform(__builtin_ldexpf(1.0f, w.fine)), bias = uniform(kBias * scale);
+    int at = 0, parity = 0;
+    float top = known ? w.top : kNone;
+    uint32_t best = key_of(kNone);
+    Raw8<DT> raw[2][kDepth];
+    auto load = [&](int h, int i0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t y = __shfl_xor(code, d);
-        code = code > y ? code : y;
-        least = __builtin_fminf(least, __shfl_xor(least, d));
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        sh.wave[threadIdx.x >> 6] = code;
-        sh.wave[kWavesOf + (threadIdx.x >> 6)] = __float_as_uint(least);
-    }
-    __syncthreads();
-    for (int y = 0; y < kWavesOf; ++y) {
-        code = code > sh.wave[y] ? code : sh.wave[y];
-        least = __builtin_fminf(least, __uint_as_float(static_cast<uint32_t>(sh.wave[kWavesOf + y])));
-    }
-    *best = code;
-    *low = least;
-}
-
-// What follows from the extremes; true: the token is known (*token).
-__device__ __forceinline__ bool settle(Row& w, uint64_t best, float low, int64_t* token) {
-    w.best = value_of(static_cast<uint32_t>(best >> 32));
-    w.first = static_cast<int>(~static_cast<uint32_t>(best));
-    if (w.best == kNone) {
-        *token = -1;
-        return true;
-    }
-    if (!(w.T > 0.0f)) {
-        *token = w.first;
-        return true;
-    }
-    w.infinite = w.best == __builtin_inff();
-    if (w.infinite) { w.best = 0.0f; low = 0.0f; }
-    w.scale = 1.4426950408889634074 / static_cast<double>(w.T);
-    int bits = 62;
-    for (int64_t n = 1; n < w.V; n <<= 1) --bits;
-    bits = bits < 51 ? bits : 51;
-    w.unit = __builtin_ldexp(1.0, 52 - bits);
-    // 2^-(bits + 1) is half a unit: 0 once rounded (a tie to even; the reach ends a little beyond it)
-    w.reach = static_cast<float>(0.5 * (bits + 1.01) / w.scale);
-    w.half = 0.5f * w.best;
-    const float range = w.half - 0.5f * low, span = range < w.reach ? range : w.reach;
-    // the smallest power of two that is at least span / 1023; none is needed below a 2^25th of the best (a value within
-    // reach that is no multiple of that is at least a quarter of the best away from it)
-    int at = 0, of_best = 0;
-    const float part = __builtin_frexpf(span * (2.0f / (kBins - 2)), &at);      // in [2^(at - 1), 2^at)
-    at -= part == 0.5f;
-    (void)__builtin_frexpf(w.best, &of_best);
-    at = span > 0.0f && at > of_best - 25 ? at : of_best - 25;
-    at = at > -120 ? at < 120 ? at : 120 : -120;
-    w.step = __builtin_ldexpf(1.0f, at);
-    w.per_step = __builtin_ldexpf(1.0f, -at);
-    w.top = __builtin_rintf(w.best * w.per_step);
-    const double inv = 1.0 / static_cast<double>(w.T);
-    w.inv = static_cast<float>(inv);
-    w.inv_rest = static_cast<float>(inv - static_cast<double>(w.inv));
-    return false;
-}
-
-// The weights of the bins' centres.
-__device__ __forceinline__ void weigh_bins(Row& w, Lds& sh) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-        const double d = (static_cast<double>(w.top) - b) * static_cast<double>(w.step) - static_cast<double>(w.best);
-        sh.weight[b] = exp2(d * w.scale);
-    }
-    w.weights = sh.weight;
-    __syncthreads();
-}
-
-// The second reading: numbers and (p) masses of the bins, added to count and mass.
-template <int DT>
-__device__ __forceinline__ void histogram(const Row& w, int b, int e, Lds& sh) {
-    const bool masses = w.p < 1.0f;
-    for (int i0 = b; i0 < e; i0 += kBlock) {
-        const int i = i0 + kPer * threadIdx.x;
-        if (i >= e) break;
-        float v[kPer];
-        load8<DT>(w.x, i, e, v);
+        for (int x = 0; x < kDepth; ++x) raw[h][x] = load_raw8<DT>(w.x, i0 + x * kBlock + mine, e);
+    };
+    auto take = [&](int h) __attribute__((always_inline)) {
+        if (!known) {
+            // the best so far; places that have fallen out of reach are empty again
+            float most = kNone;
 #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-            const float y = w.seen(v[x]);
-            if (!w.heavy(y)) continue;
-            const int at = w.bin(y);
-            atomicAdd(&sh.count[at], 1u);
-            if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[at]), static_cast<unsigned long long>(w.units(y)));
+            for (int x = 0; x < kDepth; ++x) {
+                float v[kPer];
+                unpack8<DT>(raw[h][x], v);
+#pragma unroll
+                for (int y = 0; y < kPer; ++y) most = v[y] > most ? v[y] : most;
+            }
+            const uint32_t k = wave_max(key_of(most));
+            if (lane == 0) sh.wave[kWavesOf * parity + wave] = k;
+            __syncthreads();
+            uint32_t now = best;
+#pragma unroll
+            for (int y = 0; y < kWavesOf; ++y) {
+                const uint32_t z = static_cast<uint32_t>(sh.wave[kWavesOf * parity + y]);
+                now = now > z ? now : z;
+            }
+            parity ^= 1;
+            now = __builtin_amdgcn_readfirstlane(now);
+            if (now > best) {
+                best = now;
+                const float next = uniform(__builtin_rintf(value_of(best) * w.per_step));
+                if (next > top) {
+                    const float far = next - top;
+                    const int up = far < static_cast<float>(kBins) ? static_cast<int>(far) : kBins;
+                    at = (at - up) & kMask;
+                    for (int i = threadIdx.x; i < up; i += kThreads) sh.bins[(at + i) & kMask] = 0;
+                    top = next;
+                }
+                __syncthreads();
+            }
+        } else {
+            __syncthreads();
         }
+        w.top = top;
+#pragma unroll
+        for (int x = 0; x < kDepth; ++x) {
+            float v[kPer];
+            unpack8<DT>(raw[h][x], v);
+#pragma unroll
+            for (int y = 0; y < kPer; ++y) {
+                const float d = w.depth(v[y]);
+                const int to = d < static_cast<float>(kBins) ? (at + static_cast<int>(d)) & kMask : kBins + lane;
+                uint64_t add = one;
+                if constexpr (MASSES) add |= static_cast<uint32_t>(__builtin_fmaf(w.excess(v[y]), scale, bias));
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[to]), static_cast<unsigned long long>(add));
+            }
+        }
+    };
+    __syncthreads();
+    constexpr int kStep = kDepth * kBlock;
+    load(0, b);
+    for (int i0 = b; i0 < e; i0 += 2 * kStep) {
+        if (i0 + kStep < e) load(1, i0 + kStep);
+        take(0);
+        if (i0 + kStep >= e) break;
+        if (i0 + 2 * kStep < e) load(0, i0 + 2 * kStep);
+        take(1);
     }
+    if (!known) w.best = uniform(value_of(best));
+    *base = at;
+    __syncthreads();
 }
 
-// Where a sum over the bins from the top reaches `need` (> 0): the bin (kBins: nowhere) and what is missing in front of it.
-template <typename T>
-__device__ __forceinline__ int cut_bin(const T* bins, uint64_t need, uint64_t* left, Lds& sh) {
-    const uint64_t a = bins[2 * threadIdx.x], b = bins[2 * threadIdx.x + 1];
-    uint64_t all;
-    const uint64_t to = block_incl(a + b, &all, sh), from = to - a - b;
-    if (threadIdx.x == 0) sh.found = kBins;
-    __syncthreads();
-    if (from < need && to >= need) {
-        const bool second = from + a < need;
-        sh.found = 2 * threadIdx.x + second;
-        sh.left = need - from - (second ? a : 0);
+// The weights of the bins' centres: the best's times a power of the step's, from 64 and 64 of them.
+__device__ __forceinline__ void weigh_bins(const Row& w, Lds& sh) {
+    double* small = reinterpret_cast<double*>(sh.work);
+    const double scale = 1.4426950408889634074 / static_cast<double>(w.T) * static_cast<double>(w.step);
+    if (threadIdx.x < 128) {
+        const int i = threadIdx.x & 63;
+        small[threadIdx.x] = threadIdx.x < 64 ? exp2(-i * scale) : exp2(-64 * i * scale);
     }
+    if (threadIdx.x == 128)
+        small[128] = exp2((static_cast<double>(w.top) * static_cast<double>(w.step) - static_cast<double>(w.best)) * (1.4426950408889634074 / static_cast<double>(w.T)) + w.bits);
     __syncthreads();
-    const int found = sh.found;
-    *left = sh.left;
+    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.weight[b] = static_cast<uint64_t>(__builtin_rint(small[128] * small[64 + (b >> 6)] * small[b & 63]));
     __syncthreads();
-    return found;
 }
 
-// What there is to choose from: values in LDS (n >= 0), or the row.
-template <int DT, typename F>
-__device__ __forceinline__ void each(const Row& w, int n, const Lds& sh, F f) {
-    if (n >= 0) {
-        for (int i = threadIdx.x; i < n; i += kThreads) {
+// sh.bins from places and sums to masses, the best's first.
+__device__ __forceinline__ void masses_of(const Row& w, int base, Lds& sh) {
+    uint64_t x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int d = kThreads * e + threadIdx.x;
+        const uint64_t s = sh.bins[(base + d) & kMask], part = s & ((uint64_t{1} << w.number) - 1);
+        const double n = static_cast<double>(s >> w.number);
+        const double sum = static_cast<double>(part) * __builtin_ldexp(1.0, -w.fine) - n * static_cast<double>(kBias);
+        x[e] = static_cast<uint64_t>(__builtin_rint(static_cast<double>(sh.weight[d]) * (n + sum)));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sh.bins[kThreads * e + threadIdx.x] = x[e];
+    __syncthreads();
+}
+
+// The values of the list: f(value, index) in each of a thread's four places below n.
+template <typename F>
+__device__ __forceinline__ void listed(int n, const Lds& sh, F f) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = kThreads * e + threadIdx.x;
+        if (i < n) {
             const uint64_t x = sh.list[i];
-            f(value_of(static_cast<uint32_t>(x)), static_cast<int>(x >> 32));
+            f(e, value_of(static_cast<uint32_t>(x)), static_cast<int>(x >> 32));
         }
-        return;
     }
-    for (int i0 = 0; i0 < w.V; i0 += kBlock) {
-        const int i = i0 + kPer * threadIdx.x;
-        if (i >= w.V) break;
-        float v[kPer];
-        load8<DT>(w.x, i, w.V, v);
+}
+
+// Values b .. e - 1 whose bins are between `least` and `most` to sh.list, as far as there is room, behind the sh.n there are.
+template <int DT>
+__device__ __forceinline__ void collect(const Row& w, int b, int e, int least, int most, Lds& sh) {
+    scan<DT>(w.x, b, e, [&](int i, const float (&v)[kPer]) __attribute__((always_inline)) {
+        bool take[kPer], any = false;
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
-            const float y = w.seen(v[x]);
-            if (w.heavy(y)) f(y, i + x);
+            const float d = w.depth(v[x]);
+            take[x] = d <= static_cast<float>(most) && d >= static_cast<float>(least);
+            any |= take[x];
         }
-    }
-}
-
-// The last resort of `resolve`: the limit's value digit by digit, eight bits at a time, then the index among equal ones.
-template <int DT, bool MASS>
-__device__ Limit by_digits(const Row& w, int bin, Limit now, uint64_t need, Lds& sh) {
-    const int tid = threadIdx.x;
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (tid < 256) sh.sort[tid] = 0;
-        __syncthreads();
-        each<DT>(w, -1, sh, [&](float v, int i) {
-            const uint32_t k = key_of(v);
-            if (w.bin(v) != bin || !now.keeps(k, i) || (shift < 24 && k >> (shift + 8) != prefix >> (shift + 8))) return;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sort[k >> shift & 255]), MASS ? static_cast<unsigned long long>(w.units(v)) : 1ull);
-        });
-        __syncthreads();
-        if (tid == 0) {
-            int d = 255;
-            for (; d > 0 && sh.sort[d] < need; --d) need -= sh.sort[d];
-            sh.found = d;
-            sh.left = need;
-        }
-        __syncthreads();
-        prefix |= static_cast<uint32_t>(sh.found) << shift;
-        need = sh.left;
-    }
-    if (MASS) {
-        const uint64_t one = w.units(value_of(prefix));
-        need = one ? (need + one - 1) / one : 1;
-    }
-    // the need-th of the values that are equal to it
-    uint64_t before = 0;
-    __syncthreads();
-    if (tid == 0) sh.found = w.V;
-    for (int i0 = 0; i0 < w.V; i0 += kBlock) {
-        const int i = i0 + kPer * tid;
-        float v[kPer];
-        int n = 0;
-        if (i < w.V) {
-            load8<DT>(w.x, i, w.V, v);
+        if (!any) return;
 #pragma unroll
-            for (int x = 0; x < kPer; ++x) n += key_of(w.seen(v[x])) == prefix;
-        }
-        uint64_t all;
-        uint64_t to = before + block_incl(n, &all, sh) - n;
-        if (n)
-#pragma unroll
-            for (int x = 0; x < kPer; ++x)
-                if (key_of(w.seen(v[x])) == prefix && ++to == need) sh.found = i + x;
-        before += all;
-        if (before >= need) break;
-    }
+        for (int x = 0; x < kPer; ++x)
+            if (take[x]) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kList) sh.list[at] = static_cast<uint64_t>(i + x) << 32 | key_of(v[x]);
+            }
+    });
     __syncthreads();
-    const int last = sh.found;
-    return Limit{prefix, last < now.last || prefix != now.key ? last : now.last};
 }
-
-// The limit inside a bin: the shortest leading part, of what `now` keeps of it, with `need` (> 0) elements, or (MASS) units.
-// *mass: the units of that part (numbers only, and only where the bin fits LDS or `masses` asks for them).
-template <int DT, bool MASS>
-__device__ Limit resolve(const Row& w, int n, int bin, Limit now, uint64_t need, bool masses, uint64_t* mass, Lds& sh) {
+__device__ __forceinline__ void empty_list(Lds& sh) {
     __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    each<DT>(w, n, sh, [&](float v, int i) {
-        const uint32_t k = key_of(v);
-        if (w.bin(v) != bin || !now.keeps(k, i)) return;
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kList) sh.sort[at] = code_of(k, i);
+}
+
+// Kept masses of the blocks of values b .. e - 1 to sh.bins[block]: of values in bins above `cut` (and, cut < 4096, those in it
+// to sh.list), or within a limit.
+template <int DT, bool LIMIT>
+__device__ __forceinline__ void block_masses(const Row& w, int b, int e, int cut, Limit limit, Lds& sh) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
+    __syncthreads();
+    scan<DT>(w.x, b, e, [&](int i, const float (&v)[kPer]) __attribute__((always_inline)) {
+        uint64_t s = 0;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+            const float d = w.depth(v[x]);
+            const bool ok = (LIMIT ? d < static_cast<float>(kBins) && limit.keeps(key_of(v[x]), i + x) : d < static_cast<float>(cut)) && v[x] >= w.floor;
+            const uint64_t units = w.units(v[x], sh);
+            s += ok ? units : 0;
+            if (!LIMIT && cut < kBins && d == static_cast<float>(cut)) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kList) sh.list[at] = static_cast<uint64_t>(i + x) << 32 | key_of(v[x]);
+            }
+        }
+        s = wave_sum(s);
+        if ((threadIdx.x & 63) == 0 && s)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[i / kBlock]), static_cast<unsigned long long>(s));
     });
     __syncthreads();
-    const int held = sh.n;
-    Limit limit;
-    if (held > kList) {
-        limit = by_digits<DT, MASS>(w, bin, now, need, sh);
-        if (!MASS && masses) {
-            uint64_t s = 0;
-            each<DT>(w, n, sh, [&](float v, int i) { s += w.bin(v) == bin && limit.keeps(key_of(v), i) ? w.units(v) : 0; });
-            *mass = block_sum(s, sh);
-        }
-        return limit;
-    }
-    sort_list<true>(sh.sort, held);
-    // four codes a thread, in order
-    constexpr int kEach = kList / kThreads;
-    uint64_t x[kEach], sum = 0;
-    const bool weigh = MASS || masses;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int i = kEach * threadIdx.x + e;
-        x[e] = i >= held || (!MASS && static_cast<uint64_t>(i) >= need) ? 0 : weigh ? w.units(value_of(static_cast<uint32_t>(sh.sort[i] >> 32))) : 0;
-        sum += x[e];
-    }
-    uint64_t all = 0;
-    if (weigh) {
-        uint64_t to = block_incl(sum, &all, sh) - sum;
-        if (MASS) {
-            if (threadIdx.x == 0) sh.found = held - 1;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                if (to < need && to + x[e] >= need) sh.found = kEach * threadIdx.x + e;
-                to += x[e];
-            }
-            __syncthreads();
-        }
-    }
-    *mass = all;
-    const int last = MASS ? sh.found : static_cast<int>(need) - 1;
-    const uint64_t c = sh.sort[last < held ? last : held - 1];
-    __syncthreads();
-    return Limit{static_cast<uint32_t>(c >> 32), static_cast<int>(~static_cast<uint32_t>(c))};
 }
 
-// u's place in all kept units.
-__device__ __forceinline__ uint64_t place(float u, uint64_t all) {
-    const double x = u, at = x > 0.0 ? x * static_cast<double>(all) : 0.0;
-    const uint64_t t = at < static_cast<double>(all) ? static_cast<uint64_t>(at) : all - 1;
-    return t < all ? t : all - 1;
-}
-
-// The token of a value list in LDS.
-__device__ __forceinline__ int choose(const Row& w, int n, Limit limit, float u, Lds& sh) {
-    sort_list<false>(sh.list, n);
-    constexpr int kEach = kList / kThreads;
-    uint64_t x[kEach], sum = 0, all;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int i = kEach * threadIdx.x + e;
-        x[e] = 0;
-        if (i < n) {
-            const uint64_t y = sh.list[i];
-            const uint32_t k = static_cast<uint32_t>(y);
-            if (limit.keeps(k, static_cast<int>(y >> 32))) x[e] = w.kept_units(value_of(k));
-        }
-        sum += x[e];
-    }
-    uint64_t to = block_incl(sum, &all, sh) - sum;
-    const uint64_t t = place(u, all);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        if (to <= t && to + x[e] > t) sh.found = static_cast<int>(sh.list[kEach * threadIdx.x + e] >> 32);
-        to += x[e];
-    }
-    __syncthreads();
-    return sh.found;
-}
-
-// Kept units of values i0 .. i0 + 8191 of a row, this thread's eight.
+// The token of a row whose blocks' masses are in sh.bins: in bins above `cut` or within the limit.
 template <int DT>
-__device__ __forceinline__ uint64_t block_units(const Row& w, int i0, int e, Limit limit, uint64_t (&x)[kPer]) {
-    const int i = i0 + kPer * threadIdx.x;
-    uint64_t sum = 0;
+__device__ __forceinline__ int choose_block(const Row& w, Limit limit, Lds& sh) {
+    uint64_t s = 0, left, all;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
+    all = block_sum(s, sh);
+    const int i0 = cut([&](int i) { return sh.bins[i]; }, w.place(all) + 1, &left, sh) * kBlock, i = i0 + kPer * threadIdx.x;
     float v[kPer];
-    if (i < e) load8<DT>(w.x, i, e, v);
+    uint64_t x[kPer], sum = 0;
+    unpack8<DT>(load_raw8<DT>(w.x, i, w.V), v);
 #pragma unroll
     for (int y = 0; y < kPer; ++y) {
-        x[y] = 0;
-        if (i < e) {
-            const float z = w.seen(v[y]);
-            if (w.heavy(z) && limit.keeps(key_of(z), i + y)) x[y] = w.kept_units(z);
-        }
+        x[y] = v[y] >= w.floor && limit.keeps(key_of(v[y]), i + y) ? w.units(v[y], sh) : 0;
         sum += x[y];
     }
-    return sum;
-}
-
-// The masses of blocks b / 8192 ... of a row, to mass[block].
-template <int DT>
-__device__ __forceinline__ void block_masses(const Row& w, int b, int e, Limit limit, uint64_t* mass, Lds& sh) {
-    for (int i0 = b; i0 < e; i0 += kBlock) {
-        uint64_t x[kPer];
-        const uint64_t s = block_sum(block_units<DT>(w, i0, e, limit, x), sh);
-        if (threadIdx.x == 0) mass[i0 / kBlock] = s;
-    }
-}
-
-// The token of a row whose blocks' masses are in sh.mass.
-template <int DT>
-__device__ __forceinline__ int choose_block(const Row& w, Limit limit, float u, Lds& sh) {
-    __syncthreads();
-    const int blocks = (w.V + kBlock - 1) / kBlock;
-    for (int i = blocks + threadIdx.x; i < kBins; i += kThreads) sh.mass[i] = 0;
-    __syncthreads();
-    uint64_t s = 0;
-    for (int i = threadIdx.x; i < blocks; i += kThreads) s += sh.mass[i];
-    const uint64_t all = block_sum(s, sh);
-    uint64_t left;
-    const int at = cut_bin(sh.mass, place(u, all) + 1, &left, sh);
-    uint64_t x[kPer], sum;
-    const int i0 = at * kBlock;
-    const uint64_t mine = block_units<DT>(w, i0, w.V, limit, x);
-    uint64_t to = block_incl(mine, &sum, sh) - mine;
+    uint64_t to = block_incl(sum, &all, sh) - sum;
 #pragma unroll
     for (int y = 0; y < kPer; ++y) {
-        if (to < left && to + x[y] >= left) sh.found = i0 + kPer * threadIdx.x + y;
+        if (to < left && to + x[y] >= left) sh.found = i + y;
         to += x[y];
     }
     __syncthreads();
     return sh.found;
 }
 
-// What the histogram says: how far down values are to be collected.
-struct Cuts {
-    int k_bin, p_bin;           // the bins that the limits cut (kBins: none)
-    uint64_t k_left, p_left;    // what of them is kept
-    int most;                   // collect bins 0 .. most
-    uint64_t held;              // how many values those are (no limits: not known)
-};
-
-__device__ __forceinline__ Cuts cuts_of(const Row& w, Lds& sh) {
-    Cuts c{kBins, kBins, 0, 0, kBins - 1, 0};
-    if (w.k > 0 && w.k < w.V) c.k_bin = cut_bin(sh.count, static_cast<uint64_t>(w.k), &c.k_left, sh);
-    if (w.p < 1.0f && c.k_bin == kBins) {
-        const uint64_t all = block_sum(sh.mass[2 * threadIdx.x] + sh.mass[2 * threadIdx.x + 1], sh);
-        const double need = __builtin_ceil(static_cast<double>(w.p) * static_cast<double>(all));
-        c.p_bin = cut_bin(sh.mass, need > 1.0 ? static_cast<uint64_t>(need) : 1, &c.p_left, sh);
+// The limit among n values of the list: the shortest leading part, of those of one bin that `now` keeps, with `need` (> 0) of them,
+// or (MASS) units.
+template <bool MASS, typename W>
+__device__ __forceinline__ Limit limit_in(const Row& w, int n, int bin, Limit now, uint64_t need, W units, Lds& sh) {
+    uint32_t at[kEach], high = 0, low = 0xffffffffu, key[kEach];
+    int index[kEach];
+    uint64_t x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = 0;
+    listed(n, sh, [&](int e, float v, int i) {
+        key[e] = key_of(v);
+        index[e] = i;
+        if (w.depth(v) != static_cast<float>(bin) || !now.keeps(key[e], i)) return;
+        x[e] = MASS ? units(v) : 1;
+        if (MASS && x[e] == 0) x[e] = 1;            // (less than half a unit; there is nothing below to choose from)
+        high = high > key[e] ? high : key[e];
+        low = low < key[e] ? low : key[e];
+    });
+    high = block_max(high, sh);
+    low = ~block_max(~low, sh);
+    uint64_t y[kEach], all = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        at[e] = x[e] ? high - key[e] : 0;
+        y[e] = x[e];
+        all += x[e];
     }
-    c.most = c.k_bin < kBins ? c.k_bin : c.p_bin < kBins ? c.p_bin : kBins - 1;
-    const int b = 2 * threadIdx.x;
-    c.held = block_sum((b <= c.most ? sh.count[b] : 0) + (b + 1 <= c.most ? sh.count[b + 1] : 0), sh);
-    return c;
-}
-
-// The one limit of both, from n values in LDS (or the row).
-template <int DT>
-__device__ Limit limit_of(const Row& w, int n, Cuts c, Lds& sh) {
-    Limit limit{0, w.V};
-    uint64_t mass = 0;
-    if (c.k_bin < kBins) {
-        limit = resolve<DT, false>(w, n, c.k_bin, limit, c.k_left, w.p < 1.0f, &mass, sh);
-        if (w.p < 1.0f) {
-            // the mass of what k keeps, and where p of it ends: in a bin above the cut one or in that
-            const int b = 2 * threadIdx.x;
-            const uint64_t above = block_sum((b < c.k_bin ? sh.mass[b] : 0) + (b + 1 < c.k_bin ? sh.mass[b + 1] : 0), sh);
-            double need = __builtin_ceil(static_cast<double>(w.p) * static_cast<double>(above + mass));
-            need = need > 1.0 ? need : 1.0;
-            const uint64_t units = static_cast<uint64_t>(need) < above + mass ? static_cast<uint64_t>(need) : above + mass;
-            c.p_bin = c.k_bin;
-            c.p_left = units - above;
-            if (units <= above) c.p_bin = cut_bin(sh.mass, units, &c.p_left, sh);
-        }
+    all = block_sum(all, sh);
+    need = need < all ? need : all;
+    Limit limit{high - narrow(n, at, y, high - low, &need, sh), w.V};
+    // among equal ones
+    uint64_t same = 0, of = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        y[e] = x[e] != 0 && key[e] == limit.key;
+        at[e] = y[e] ? index[e] : 0;
+        same += y[e];
+        of = y[e] ? x[e] : of;
     }
-    if (c.p_bin < kBins) limit = resolve<DT, true>(w, n, c.p_bin, limit, c.p_left, false, &mass, sh);
+    same = block_sum(same, sh);
+    if (MASS) {
+        // (all of them weigh the same)
+        const uint32_t high_of = block_max(static_cast<uint32_t>(of >> 32), sh), low_of = block_max(static_cast<uint32_t>(of), sh);
+        of = static_cast<uint64_t>(high_of) << 32 | low_of;
+        need = (need + of - 1) / of;
+    }
+    if (need < same) limit.last = static_cast<int>(narrow(n, at, y, static_cast<uint32_t>(w.V - 1), &need, sh));
+    else if (limit.key == now.key) limit.last = now.last;
     return limit;
 }
 
-// The third reading, of values b .. e - 1: those in bins 0 .. most to sh.list, in any order, as far as there is room; how many
-// there are.
-template <int DT>
-__device__ __forceinline__ int collect(const Row& w, int b, int e, int most, Lds& sh) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
-    for (int i0 = b; i0 < e; i0 += kBlock) {
-        const int i = i0 + kPer * threadIdx.x;
-        if (i >= e) break;
-        float v[kPer];
-        load8<DT>(w.x, i, e, v);
+// The same from the row, where the bin's values do not fit the list: digit by digit of the values' bits.
+template <int DT, bool MASS>
+__device__ __forceinline__ Limit limit_by_digits(const Row& w, int bin, Limit now, uint64_t need, Lds& sh) {
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.work[i] = 0;
+        __syncthreads();
+        scan<DT>(w.x, 0, w.V, [&](int i, const float (&v)[kPer]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-            v[x] = w.seen(v[x]);
-            if (w.heavy(v[x]) && w.bin(v[x]) <= most) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kList) sh.list[at] = static_cast<uint64_t>(i + x) << 32 | key_of(v[x]);
+            for (int x = 0; x < kPer; ++x) {
+                const uint32_t k = key_of(v[x]);
+                if (w.depth(v[x]) != static_cast<float>(bin) || !now.keeps(k, i + x) || (shift < 24 && k >> (shift + 8) != prefix >> (shift + 8)))
+                    continue;
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.work[255 - (k >> shift & 255)]),
+                          MASS ? static_cast<unsigned long long>(w.units(v[x], sh)) : 1ull);
             }
-        }
+        });
+        __syncthreads();
+        const int d = cut([&](int i) { return sh.work[i]; }, need, &need, sh);
+        prefix |= static_cast<uint32_t>(255 - (d < 256 ? d : 255)) << shift;
+        if (d >= 256) need = 1;
+    }
+    if (MASS) {
+        const uint64_t of = w.units(value_of(prefix), sh);
+        need = of ? (need + of - 1) / of : 1;
+    }
+    // the need-th of the values that are equal to it
+    uint64_t before = 0, all;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = w.V;
+    for (int i0 = 0; i0 < w.V && before < need; i0 += kBlock) {
+        const int i = i0 + kPer * threadIdx.x;
+        float v[kPer];
+        unpack8<DT>(load_raw8<DT>(w.x, i, w.V), v);
+        uint64_t n = 0;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) n += i + x < w.V && key_of(v[x]) == prefix;
+        uint64_t to = before + block_incl(n, &all, sh) - n;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x)
+            if (i + x < w.V && key_of(v[x]) == prefix && ++to == need) sh.found = i + x;
+        before += all;
     }
     __syncthreads();
+    const int last = sh.found;
+    __syncthreads();
+    return Limit{prefix, prefix == now.key && now.last < last ? now.last : last};
+}
+
+// The limit in a bin of the row.
+template <int DT, bool MASS>
+__device__ __forceinline__ Limit limit_in_row(const Row& w, int bin, Limit now, uint64_t need, Lds& sh) {
+    empty_list(sh);
+    collect<DT>(w, 0, w.V, bin, bin, sh);
     const int n = sh.n;
-    __syncthreads();
-    return n;
+    if (n > kList) return limit_by_digits<DT, MASS>(w, bin, now, need, sh);
+    return limit_in<MASS>(w, n, bin, now, need, [&](float v) { return w.units(v, sh); }, sh);
 }
 
-// The last bin that w >= min_p can be in (min_p alone limits the row).
-__device__ __forceinline__ int least_bin(const Row& w) {
-    const double d = -log(static_cast<double>(w.least < 1.0f ? w.least : 1.0f)) * static_cast<double>(w.T) * 1.000001;
-    const double b = d * w.per_step + 2.0;
-    return b < kBins - 1 ? static_cast<int>(b) : kBins - 1;
+// The token of n values in LDS, all that k (the bin that it cuts and what it keeps of that; 4096: none) may keep.
+__device__ __forceinline__ int choose_listed(const Row& w, int n, int k_bin, uint64_t k_left, Lds& sh) {
+    Limit limit{0, w.V};
+    auto units = [&](float v) { return w.units(v); };
+    if (k_bin < kBins) limit = limit_in<false>(w, n, k_bin, limit, k_left, units, sh);
+    uint64_t x[kEach], y[kEach];
+    uint32_t at[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        x[e] = y[e] = 0;
+        at[e] = 0;
+    }
+    if (w.p_limits()) {
+        uint64_t s = 0, left;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.work[i] = 0;
+        __syncthreads();
+        listed(n, sh, [&](int e, float v, int i) {
+            if (!limit.keeps(key_of(v), i)) return;
+            const uint64_t z = units(v);
+            s += z;
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.work[static_cast<int>(w.depth(v))]), static_cast<unsigned long long>(z));
+        });
+        s = block_sum(s, sh);
+        const int bin = cut([&](int i) { return sh.work[i]; }, w.part(s), &left, sh);
+        limit = limit_in<true>(w, n, bin, limit, left, units, sh);
+    }
+    uint64_t s = 0;
+    listed(n, sh, [&](int e, float v, int i) {
+        at[e] = i;
+        x[e] = v >= w.floor && limit.keeps(key_of(v), i) ? w.units(v) : 0;
+        s += x[e];
+    });
+    uint64_t need = w.place(block_sum(s, sh)) + 1;
+    return static_cast<int>(narrow(n, at, x, static_cast<uint32_t>(w.V - 1), &need, sh));
 }
 
-// The token once what the histogram says is in LDS: from n values in sh.list, or (n > kList) from the row.
+// The token of a row that p alone limits, from the cut bin's n values in LDS and the masses of the blocks above it in sh.bins.
 template <int DT>
-__device__ int finish(const Row& w, const Cuts& c, int n, float u, Lds& sh) {
-    const bool in_lds = n <= kList;
-    const Limit limit = limit_of<DT>(w, in_lds ? n : -1, c, sh);
-    if (in_lds) return choose(w, n, limit, u, sh);
-    block_masses<DT>(w, 0, w.V, limit, sh.mass, sh);
-    return choose_block<DT>(w, limit, u, sh);
+__device__ __forceinline__ int choose_cut(const Row& w, int n, int bin, uint64_t left, Lds& sh) {
+    auto units = [&](float v) { return w.units(v, sh); };
+    Limit limit{0, w.V};
+    if (n <= kList) {
+        limit = limit_in<true>(w, n, bin, limit, left, units, sh);
+        listed(n, sh, [&](int e, float v, int i) {
+            if (v >= w.floor && limit.keeps(key_of(v), i))
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[i / kBlock]), static_cast<unsigned long long>(units(v)));
+        });
+        __syncthreads();
+    } else {
+        limit = limit_by_digits<DT, true>(w, bin, limit, left, sh);
+        block_masses<DT, true>(w, 0, w.V, kBins, limit, sh);
+    }
+    return choose_block<DT>(w, limit, sh);
 }
 
-__device__ __forceinline__ void clear_bins(Lds& sh) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) { sh.mass[i] = 0; sh.count[i] = 0; }
+// The token of a row with +infinities: all of them weigh the same, and nothing else does.
+template <int DT>
+__device__ __forceinline__ int among_infinities(const Row& w, Lds& sh) {
+    uint64_t n = 0, before = 0;
+    scan<DT>(w.x, 0, w.V, [&](int, const float (&v)[kPer]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) n += v[x] == __builtin_inff();
+    });
+    n = block_sum(n, sh);
+    if (w.k > 0 && static_cast<uint64_t>(w.k) < n) n = static_cast<uint64_t>(w.k);
+    if (w.p_limits()) n = w.part(n);
+    const uint64_t t = w.place(n);
+    for (int i0 = 0; before <= t; i0 += kBlock) {
+        float v[kPer];
+        unpack8<DT>(load_raw8<DT>(w.x, i0 + kPer * threadIdx.x, w.V), v);
+        uint64_t mine = 0, all;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) mine += v[x] == __builtin_inff();
+        uint64_t to = before + block_incl(mine, &all, sh) - mine;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x)
+            if (v[x] == __builtin_inff() && to++ == t) sh.found = i0 + kPer * threadIdx.x + x;
+        before += all;
+    }
     __syncthreads();
+    return sh.found;
+}
+
+// w.floor from the best: w >= min_p is l >= best + T log(min_p), rounded up to fp32 (the best is kept in any case).
+__device__ __forceinline__ void set_floor(Row& w) {
+    w.floor = kNone;
+    if (!(w.least > 0.0f)) return;
+    const double x = static_cast<double>(w.best) + static_cast<double>(w.T) * log(static_cast<double>(w.least));
+    float f = static_cast<float>(x);
+    if (static_cast<double>(f) < x) f = value_of(key_of(f) + 1);
+    w.floor = uniform(f < w.best ? f : w.best);
+}
+
+// Whether the best's bin is far from what fp32 loses places in; else the step is chosen anew, from the best: none is needed below a
+// 2^25th of it (a value within reach that is no multiple of that is at least a quarter of the best away).
+__device__ __forceinline__ bool well_placed(const Row& w) { return usual(w.T) && __builtin_fabsf(w.best * w.per_step) < 0x1p60f; }
+__device__ __forceinline__ void place_again(Row& w) {
+    int of_best = -120, at = step_of(w);
+    if (w.best != 0.0f) (void)__builtin_frexpf(w.best, &of_best);
+    at = at > of_best - 25 ? at : of_best - 25;
+    set_step(w, at > -120 ? at < 120 ? at : 120 : -120);
+    w.top = uniform(__builtin_rintf(w.best * w.per_step));
+}
+
+// Where numbers of the bins (by place) cut k: the bin (4096: nowhere), what it keeps, and how many values that bin and those above
+// it have.
+__device__ __forceinline__ int cut_number(const Row& w, int base, uint64_t* left, uint64_t* held, Lds& sh) {
+    auto number = [&](int d) { return sh.bins[(base + d) & kMask] >> w.number; };
+    const int bin = cut(number, static_cast<uint64_t>(w.k), left, sh);
+    uint64_t s = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int d = kThreads * e + threadIdx.x;
+        s += d <= bin ? number(d) : 0;
+    }
+    *held = block_sum(s, sh);
+    return bin;
+}
+
+// The token of a whole row with known best, one workgroup, as many readings as it takes (k of thousands, odd temperatures).
+template <int DT>
+__device__ __attribute__((noinline)) int by_readings(Row w, Lds& sh) {
+    if (!well_placed(w)) place_again(w);
+    else w.top = uniform(__builtin_rintf(w.best * w.per_step));
+    weigh_bins(w, sh);
+    Limit limit{0, w.V};
+    uint64_t left, held, mass = 0;
+    int base, bin = kBins;
+    if (w.k_limits()) {
+        bins_of<DT, false>(w, 0, w.V, true, &base, sh);
+        bin = cut_number(w, base, &left, &held, sh);
+        if (bin < kBins) limit = limit_in_row<DT, false>(w, bin, limit, left, sh);
+    }
+    if (w.p_limits()) {
+        if (bin < kBins) {
+            // what k keeps of its bin
+            uint64_t s = 0;
+            scan<DT>(w.x, 0, w.V, [&](int i, const float (&v)[kPer]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 0; x < kPer; ++x)
+                    if (w.depth(v[x]) == static_cast<float>(bin) && limit.keeps(key_of(v[x]), i + x)) s += w.units(v[x], sh);
+            });
+            mass = block_sum(s, sh);
+        }
+        bins_of<DT, true>(w, 0, w.V, true, &base, sh);
+        masses_of(w, base, sh);
+        uint64_t s = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) s += kThreads * e + threadIdx.x < bin ? sh.bins[kThreads * e + threadIdx.x] : 0;
+        const uint64_t above = block_sum(s, sh), need = w.part(above + mass);
+        left = need - above;
+        if (need <= above) bin = cut([&](int i) { return sh.bins[i]; }, need, &left, sh);
+        if (bin < kBins) limit = limit_in_row<DT, true>(w, bin, limit, left, sh);
+    }
+    block_masses<DT, true>(w, 0, w.V, kBins, limit, sh);
+    return choose_block<DT>(w, limit, sh);
 }
 
 template <int DT>
@@ -667,32 +883,51 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     __shared__ Lds sh;
     const int64_t r = blockIdx.x;
     Row w = row_of<DT>(a, r);
-    uint64_t best;
-    float low;
-    extremes<DT>(w, 0, w.V, &best, &low, sh);
-    int64_t token;
-    if (!settle(w, best, low, &token)) {
+    const bool limited = w.k_limits() || w.p_limits(), greedy = w.T < 0x1p-100f;
+    int base = 0;
+    if (greedy || !limited || !usual(w.T)) largest<DT>(w, 0, w.V, sh);
+    else if (w.k_limits()) bins_of<DT, false>(w, 0, w.V, false, &base, sh);
+    else bins_of<DT, true>(w, 0, w.V, false, &base, sh);
+    set_floor(w);
+    int token;
+    if (w.best == kNone) {
+        token = -1;
+    } else if (greedy) {
+        token = w.first;
+    } else if (w.best == __builtin_inff()) {
+        token = among_infinities<DT>(w, sh);
+    } else if (!well_placed(w)) {
+        token = by_readings<DT>(w, sh);
+    } else if (!limited) {
+        w.top = uniform(__builtin_rintf(w.best * w.per_step));
         weigh_bins(w, sh);
-        Cuts c{kBins, kBins, 0, 0, kBins - 1, 0};
-        if (w.limited()) {
-            clear_bins(sh);
-            histogram<DT>(w, 0, w.V, sh);
-            __syncthreads();
-            c = cuts_of(w, sh);
-        } else if (w.least > 0.0f) {
-            c.most = least_bin(w);
+        block_masses<DT, false>(w, 0, w.V, kBins, Limit{0, w.V}, sh);
+        token = choose_block<DT>(w, Limit{0, w.V}, sh);
+    } else if (w.k_limits()) {
+        uint64_t left, held;
+        const int bin = cut_number(w, base, &left, &held, sh);
+        if (held <= kList) {
+            empty_list(sh);
+            collect<DT>(w, 0, w.V, 0, bin < kBins ? bin : kBins - 1, sh);
+            token = choose_listed(w, sh.n, bin, left, sh);
+        } else {
+            token = by_readings<DT>(w, sh);
         }
-        int n = kList + 1;
-        if ((w.limited() && c.held <= kList) || (!w.limited() && w.least > 0.0f) || w.V <= kList)
-            n = collect<DT>(w, 0, w.V, c.most, sh);
-        token = finish<DT>(w, c, n, a.u[r], sh);
+    } else {
+        weigh_bins(w, sh);
+        masses_of(w, base, sh);
+        uint64_t s = 0, left;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
+        const int bin = cut([&](int i) { return sh.bins[i]; }, w.part(block_sum(s, sh)), &left, sh);
+        empty_list(sh);
+        block_masses<DT, false>(w, 0, w.V, bin, Limit{0, w.V}, sh);
+        token = choose_cut<DT>(w, sh.n, bin, left, sh);
     }
     if (threadIdx.x == 0) a.token[r] = token;
 }
 
 }  // namespace
-
-int64_t sample_workspace_bytes(int64_t, int64_t) { return 0; }
 
 int launch_sample(const SampleArgs& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(a.rows)), block(kThreads);

@@ -114,8 +114,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     Weights are exp((l - max l) / temperature). In the order of l (descending, ties by index) the first top_k are kept (0: all), of
     those the shortest leading part whose weight reaches top_p of theirs (>= 1: all), of those the ones of weight >= min_p; the
     token is the first, in the order of its number, whose kept weight up to it exceeds u times all kept weight. temperature 0: the first
-    largest logit. Each setting is a number or a tensor [rows]. Logits that are NaN count as -infinity; a row that holds nothing
-    else gives -1. The same inputs always give the same tokens."""
+    largest logit. Each setting is a number or a tensor [rows]. Logits that are NaN count as -infinity; where +infinities
+    are, only they have weight; a row of -infinities gives -1. The same inputs always give the same tokens."""
     _device_check(logits, "logits")
     if logits.dim() != 2 or logits.dtype not in FLOAT_TYPES:
         raise ValueError(f"logits must be bfloat16, float16 or float32 [rows, V], got {logits.dtype} {list(logits.shape)}")
