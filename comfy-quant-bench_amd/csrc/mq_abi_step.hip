@@ -76,9 +76,13 @@ int mq_rms_norm_quant(const void* x, int dtype, int64_t ldx, const void* residua
     return launch_norm(a, static_cast<hipStream_t>(stream));
 }
 
+int64_t mq_sample_workspace_bytes(int64_t rows, int64_t V) {
+    return rows <= 0 || V <= 0 || rows >= kMost || V > (int64_t(1) << 24) ? 0 : sample_workspace_bytes(rows, V);
+}
+
 int mq_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const float* u, const float* temperature,
               float temperature_all, const int32_t* top_k, int64_t top_k_all, const float* top_p, float top_p_all,
-              const float* min_p, float min_p_all, int64_t* token, void* stream) {
+              const float* min_p, float min_p_all, int64_t* token, void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
     MQ_REQUIRE(float_type(dtype), "sample: unknown type %d", dtype);
     MQ_REQUIRE(rows >= 0 && rows < kMost && V > 0, "sample: bad shape rows=%lld V=%lld", (long long)rows, (long long)V);
@@ -92,7 +96,11 @@ int mq_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V
     MQ_REQUIRE(aligned(logits, dtype_bytes(dtype)) && aligned(u, 4) && aligned(temperature, 4) && aligned(top_k, 4) &&
                    aligned(top_p, 4) && aligned(min_p, 4) && aligned(token, 8),
                "sample: operands must be aligned to their element size");
+    const int64_t need = mq_sample_workspace_bytes(rows, V);
+    MQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need),
+               "sample: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
     SampleArgs a{};
+    a.work = workspace;
     a.x = logits; a.dtype = dtype; a.ld = ld; a.rows = rows; a.V = V; a.u = u; a.temperature = temperature; a.top_p = top_p;
     a.min_p = min_p; a.top_k = top_k; a.temperature1 = temperature_all; a.top_p1 = top_p_all; a.min_p1 = min_p_all;
     a.top_k1 = top_k_all; a.token = token;

@@ -127,11 +127,11 @@ ENTRY_F(mq_paged_attention_shared, 34,
                                      P(9), I(10), L(11), L(12), L(13), P(14), P(15), L(16), L(17), L(18), L(19), I(20),
                                      P(21), L(22), L(23), P(24), P(25), F(26), P(27), L(28), L(29), P(30), L(31), P(32),
                                      P(33)))
-ENTRY_F(mq_sample, 16,
-        B(0) | B(5) | B(6) | B(8) | B(10) | B(12) | B(14) | B(15),
+ENTRY_F(mq_sample, 18,
+        B(0) | B(5) | B(6) | B(8) | B(10) | B(12) | B(14) | B(15) | B(17),
         B(7) | B(11) | B(13),
         fn_mq_sample(P(0), I(1), L(2), L(3), L(4), P(5), P(6), F(7), P(8), L(9), P(10), F(11), P(12), F(13),
-                     P(14), P(15)))
+                     P(14), P(15), L(16), P(17)))
 
 /* bind(rotquant, swiglu_rotquant, linear_w4_group, linear_rowscale, kv_write, paged_attention, kv_grow,
  * linear_w4a16, rms_norm, rms_norm_quant, kv_append, kv_shared, paged_attention_shared, sample): the functions' addresses */

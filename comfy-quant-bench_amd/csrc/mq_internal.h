@@ -347,5 +347,6 @@ struct SampleArgs {
     void* work;
 };
 int launch_sample(const SampleArgs& a, hipStream_t stream);
+int64_t sample_workspace_bytes(int64_t rows, int64_t V);
 
 }  // namespace mq

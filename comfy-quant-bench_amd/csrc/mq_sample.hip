@@ -38,8 +38,9 @@ constexpr int kEach = kBins / kThreads;             // bins, and values of the l
 constexpr int kList = 4096;                         // values that are held in LDS
 constexpr int kFew = 256;
 constexpr int kMostBlocks = (1 << 24) / kBlock;
-constexpr int kMostParts = 16;
+constexpr int kMostParts = 8;
 constexpr float kNone = -__builtin_inff();          // of NaN too, which is never chosen
+constexpr float kLeastT = 0x1p-100f;                // below it the first largest is taken
 constexpr float kBias = 1.0f / 32.0f;               // what makes e positive in a bin's sum
 static_assert(kMostBlocks <= kBins && kList == kBins);
 
@@ -878,63 +879,238 @@ __device__ __attribute__((noinline)) int by_readings(Row w, Lds& sh) {
     return choose_block<DT>(w, limit, sh);
 }
 
+// What the first reading of values b .. e - 1 leaves in w.best and w.first, or (limited, usual temperatures) w.best and the bins.
+template <int DT>
+__device__ __forceinline__ void first_reading(Row& w, int b, int e, int* base, Lds& sh) {
+    if (w.T < kLeastT || !usual(w.T) || !(w.k_limits() || w.p_limits())) largest<DT>(w, b, e, sh);
+    else if (w.k_limits()) bins_of<DT, false>(w, b, e, false, base, sh);
+    else bins_of<DT, true>(w, b, e, false, base, sh);
+}
+
+// Rows whose token needs no second reading of parts: true, and the token.
+template <int DT>
+__device__ __forceinline__ bool known(Row& w, int* token) {
+    if (w.best != kNone && w.T >= kLeastT) return false;
+    *token = w.best == kNone ? -1 : w.first;
+    return true;
+}
+
+// The bin that p cuts, from the masses in sh.bins.
+__device__ __forceinline__ int cut_mass(const Row& w, uint64_t* left, Lds& sh) {
+    uint64_t s = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
+    return cut([&](int i) { return sh.bins[i]; }, w.part(block_sum(s, sh)), left, sh);
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     __shared__ Lds sh;
     const int64_t r = blockIdx.x;
     Row w = row_of<DT>(a, r);
-    const bool limited = w.k_limits() || w.p_limits(), greedy = w.T < 0x1p-100f;
-    int base = 0;
-    if (greedy || !limited || !usual(w.T)) largest<DT>(w, 0, w.V, sh);
-    else if (w.k_limits()) bins_of<DT, false>(w, 0, w.V, false, &base, sh);
-    else bins_of<DT, true>(w, 0, w.V, false, &base, sh);
-    set_floor(w);
-    int token;
-    if (w.best == kNone) {
-        token = -1;
-    } else if (greedy) {
-        token = w.first;
-    } else if (w.best == __builtin_inff()) {
-        token = among_infinities<DT>(w, sh);
-    } else if (!well_placed(w)) {
-        token = by_readings<DT>(w, sh);
-    } else if (!limited) {
-        w.top = uniform(__builtin_rintf(w.best * w.per_step));
-        weigh_bins(w, sh);
-        block_masses<DT, false>(w, 0, w.V, kBins, Limit{0, w.V}, sh);
-        token = choose_block<DT>(w, Limit{0, w.V}, sh);
-    } else if (w.k_limits()) {
+    int base = 0, token;
+    first_reading<DT>(w, 0, w.V, &base, sh);
+    if (!known<DT>(w, &token)) {
+        set_floor(w);
         uint64_t left, held;
-        const int bin = cut_number(w, base, &left, &held, sh);
-        if (held <= kList) {
-            empty_list(sh);
-            collect<DT>(w, 0, w.V, 0, bin < kBins ? bin : kBins - 1, sh);
-            token = choose_listed(w, sh.n, bin, left, sh);
-        } else {
+        if (w.best == __builtin_inff()) {
+            token = among_infinities<DT>(w, sh);
+        } else if (!well_placed(w)) {
             token = by_readings<DT>(w, sh);
+        } else if (w.k_limits()) {
+            const int bin = cut_number(w, base, &left, &held, sh);
+            if (held <= kList) {
+                empty_list(sh);
+                collect<DT>(w, 0, w.V, 0, bin < kBins ? bin : kBins - 1, sh);
+                token = choose_listed(w, sh.n, bin, left, sh);
+            } else {
+                token = by_readings<DT>(w, sh);
+            }
+        } else {
+            w.top = uniform(__builtin_rintf(w.best * w.per_step));
+            weigh_bins(w, sh);
+            int bin = kBins;
+            if (w.p_limits()) {
+                masses_of(w, base, sh);
+                bin = cut_mass(w, &left, sh);
+            }
+            empty_list(sh);
+            block_masses<DT, false>(w, 0, w.V, bin, Limit{0, w.V}, sh);
+            token = bin < kBins ? choose_cut<DT>(w, sh.n, bin, left, sh) : choose_block<DT>(w, Limit{0, w.V}, sh);
         }
-    } else {
-        weigh_bins(w, sh);
-        masses_of(w, base, sh);
-        uint64_t s = 0, left;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
-        const int bin = cut([&](int i) { return sh.bins[i]; }, w.part(block_sum(s, sh)), &left, sh);
-        empty_list(sh);
-        block_masses<DT, false>(w, 0, w.V, bin, Limit{0, w.V}, sh);
-        token = choose_cut<DT>(w, sh.n, bin, left, sh);
     }
     if (threadIdx.x == 0) a.token[r] = token;
 }
 
+// --- rows in parts: a row's share of the workspace
+
+struct Share {
+    uint32_t *best, *first;     // [kMostParts], of the parts
+    int *n, *done;              // values in the list; parts that have ended
+    uint64_t *bins, *list, *blocks;
+};
+constexpr int64_t kShareHead = 8 * kMostParts + 64;
+__host__ __device__ constexpr int64_t share_bytes(int64_t V, int parts) {
+    return kShareHead + 8 * (static_cast<int64_t>(parts) * kBins + kList + (V + kBlock - 1) / kBlock);
+}
+__device__ __forceinline__ Share share_of(const SampleArgs& a, int64_t r, int parts) {
+    char* p = static_cast<char*>(a.work) + r * share_bytes(a.V, parts);
+    Share s;
+    s.best = reinterpret_cast<uint32_t*>(p);
+    s.first = s.best + kMostParts;
+    s.n = reinterpret_cast<int*>(s.first + kMostParts);
+    s.done = s.n + 1;
+    s.bins = reinterpret_cast<uint64_t*>(p + kShareHead);
+    s.list = s.bins + static_cast<int64_t>(parts) * kBins;
+    s.blocks = s.list + kList;
+    return s;
+}
+// Between workgroups of one launch: past the caches that are not common to all of them.
+__device__ __forceinline__ void send(uint64_t* p, uint64_t x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t receive(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+struct Part {
+    int b, e;
+};
+__device__ __forceinline__ Part part_of(int V, int part, int parts) {
+    const int blocks = (V + kBlock - 1) / kBlock, b = blocks * part / parts * kBlock, e = blocks * (part + 1) / parts * kBlock;
+    return Part{b, e < V ? e : V};
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_first_kernel(SampleArgs a) {
+    __shared__ Lds sh;
+    const int parts = gridDim.x, part = blockIdx.x;
+    const Share s = share_of(a, blockIdx.y, parts);
+    Row w = row_of<DT>(a, blockIdx.y);
+    const Part p = part_of(w.V, part, parts);
+    int base = 0;
+    w.first = p.b;
+    first_reading<DT>(w, p.b, p.e, &base, sh);
+    if (threadIdx.x == 0) {
+        s.best[part] = key_of(w.best);
+        s.first[part] = static_cast<uint32_t>(w.first);
+        if (part == 0) { *s.n = 0; *s.done = 0; }
+    }
+    if (w.T >= kLeastT && usual(w.T) && (w.k_limits() || w.p_limits()))
+        for (int d = threadIdx.x; d < kBins; d += kThreads) s.bins[part * kBins + d] = sh.bins[(base + d) & kMask];
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_second_kernel(SampleArgs a) {
+    __shared__ Lds sh;
+    const int parts = gridDim.x, part = blockIdx.x;
+    const Share s = share_of(a, blockIdx.y, parts);
+    Row w = row_of<DT>(a, blockIdx.y);
+    uint32_t best = 0;
+    int of = 0, token;
+    for (int y = 0; y < parts; ++y)
+        if (s.best[y] > best) { best = s.best[y]; of = y; }
+    w.best = uniform(value_of(__builtin_amdgcn_readfirstlane(best)));
+    w.first = static_cast<int>(s.first[of]);
+    // what one workgroup does alone
+    bool alone = known<DT>(w, &token);
+    set_floor(w);
+    if (!alone && (w.best == __builtin_inff() || !well_placed(w))) {
+        if (part != 0) return;
+        alone = true;
+        token = w.best == __builtin_inff() ? among_infinities<DT>(w, sh) : by_readings<DT>(w, sh);
+    }
+    if (alone) {
+        if (part == 0 && threadIdx.x == 0) a.token[blockIdx.y] = token;
+        return;
+    }
+    w.top = uniform(__builtin_rintf(w.best * w.per_step));
+    const Part p = part_of(w.V, part, parts);
+    uint64_t left = 0, held;
+    int bin = kBins;
+    if (w.k_limits() || w.p_limits()) {
+        // the parts' bins together, those of a lower best further down
+        uint64_t x[kEach] = {0, 0, 0, 0};
+        for (int y = 0; y < parts; ++y) {
+            const float far = w.top - __builtin_rintf(value_of(s.best[y]) * w.per_step);
+            if (!(far < static_cast<float>(kBins))) continue;
+            const int up = static_cast<int>(far);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int d = kThreads * e + static_cast<int>(threadIdx.x) - up;
+                if (d >= 0) x[e] += s.bins[y * kBins + d];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sh.bins[kThreads * e + threadIdx.x] = x[e];
+        __syncthreads();
+    }
+    empty_list(sh);
+    if (w.k_limits()) {
+        bin = cut_number(w, 0, &left, &held, sh);
+        if (held > kList) {
+            if (part != 0) return;
+            token = by_readings<DT>(w, sh);
+            if (threadIdx.x == 0) a.token[blockIdx.y] = token;
+            return;
+        }
+        collect<DT>(w, p.b, p.e, 0, bin < kBins ? bin : kBins - 1, sh);
+    } else {
+        weigh_bins(w, sh);
+        if (w.p_limits()) {
+            masses_of(w, 0, sh);
+            bin = cut_mass(w, &left, sh);
+        }
+        block_masses<DT, false>(w, p.b, p.e, bin, Limit{0, w.V}, sh);
+        for (int i = p.b / kBlock + threadIdx.x; i * kBlock < p.e; i += kThreads) send(s.blocks + i, sh.bins[i]);
+    }
+    // the part's values to the row's list; the last part takes them all
+    if (threadIdx.x == 0) sh.found = sh.n ? __hip_atomic_fetch_add(s.n, sh.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    __syncthreads();
+    const int mine = sh.n < kList ? sh.n : kList, to = sh.found;
+    for (int i = threadIdx.x; i < mine && to + i < kList; i += kThreads) send(s.list + to + i, sh.list[i]);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = __hip_atomic_fetch_add(s.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (sh.found != parts - 1) return;
+    const int n = __hip_atomic_load(s.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = threadIdx.x; i < n && i < kList; i += kThreads) sh.list[i] = receive(s.list + i);
+    if (!w.k_limits())
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = static_cast<int64_t>(i) * kBlock < w.V ? receive(s.blocks + i) : 0;
+    __syncthreads();
+    if (w.k_limits()) token = choose_listed(w, n, bin, left, sh);
+    else token = bin < kBins ? choose_cut<DT>(w, n, bin, left, sh) : choose_block<DT>(w, Limit{0, w.V}, sh);
+    if (threadIdx.x == 0) a.token[blockIdx.y] = token;
+}
+
+// Parts of a row: as many as fill the device, of at least a block each.
+int parts_of(int64_t rows, int64_t V) {
+    const int cus = device_cu_count();
+    const int64_t blocks = (V + kBlock - 1) / kBlock, room = (cus > 0 ? cus : 256) / (rows > 0 ? rows : 1);
+    const int64_t n = blocks < room ? blocks : room;
+    return static_cast<int>(n < 1 ? 1 : n < kMostParts ? n : kMostParts);
+}
+
+template <int DT>
+int launch_type(const SampleArgs& a, hipStream_t stream) {
+    const int parts = parts_of(a.rows, a.V);
+    if (parts == 1) {
+        hipLaunchKernelGGL((sample_kernel<DT>), dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, stream, a);
+    } else {
+        const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(a.rows));
+        hipLaunchKernelGGL((sample_first_kernel<DT>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((sample_second_kernel<DT>), grid, dim3(kThreads), 0, stream, a);
+    }
+    return launch_status("sample");
+}
+
 }  // namespace
 
+int64_t sample_workspace_bytes(int64_t rows, int64_t V) {
+    const int parts = parts_of(rows, V);
+    return parts == 1 ? 0 : rows * share_bytes(V, parts);
+}
+
 int launch_sample(const SampleArgs& a, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(a.rows)), block(kThreads);
-    if (a.dtype == kDtF32) hipLaunchKernelGGL((sample_kernel<kDtF32>), grid, block, 0, stream, a);
-    else if (a.dtype == kDtF16) hipLaunchKernelGGL((sample_kernel<kDtF16>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((sample_kernel<kDtBf16>), grid, block, 0, stream, a);
-    return launch_status("sample");
+    if (a.dtype == kDtF32) return launch_type<kDtF32>(a, stream);
+    return a.dtype == kDtF16 ? launch_type<kDtF16>(a, stream) : launch_type<kDtBf16>(a, stream);
 }
 
 }  // namespace mq

@@ -99,8 +99,9 @@ _SIGNATURES = {
     "mq_paged_attention_shared": ([c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64,
                                    c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_i64,
                                    c_vp, c_vp, c_float, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp], c_int),
-    "mq_sample": ([c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_float, c_vp, c_i64, c_vp, c_float, c_vp, c_float,
-                   c_vp, c_vp], c_int),
+    "mq_sample": ([c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_float, c_vp, c_i64, c_vp, c_float, c_vp, c_float, c_vp, c_vp,
+                   c_i64, c_vp], c_int),
+    "mq_sample_workspace_bytes": ([c_i64, c_i64], c_i64),
 }
 
 EXPORTED = tuple(_SIGNATURES)

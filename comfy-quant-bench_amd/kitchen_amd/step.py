@@ -15,9 +15,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import CONVROT_GROUPSIZES, FLOAT_TYPES
+from .ops import CONVROT_GROUPSIZES, FLOAT_TYPES, _scratch
 
 MOST_COLUMNS = 32768
+_SAMPLE_WS: dict = {}
 
 
 def _device_check(x: torch.Tensor, what: str) -> None:
@@ -132,6 +133,16 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     least = _setting(min_p, "min_p", rows, torch.float32, dev)
     token = torch.empty(rows, dtype=torch.int64, device=dev)
     if rows:
+        stream, key = _lib.stream_of_device(dev), (dev.index, rows, vocab)
+        nbytes = _SAMPLE_WS.get(key)
+        if nbytes is None:
+            with torch.cuda.device(dev):
+                nbytes = int(_lib.load().mq_sample_workspace_bytes(rows, vocab))
+            if len(_SAMPLE_WS) > 4096:
+                _SAMPLE_WS.clear()
+            _SAMPLE_WS[key] = nbytes
+        work = _scratch(nbytes, dev, stream) if nbytes else None
         _lib.call("mq_sample", x.data_ptr(), _lib.DTYPE_CODE[x.dtype], x.stride(0), rows, vocab, u.data_ptr(), t[0], float(t[1]),
-                  k[0], int(k[1]), p[0], float(p[1]), least[0], float(least[1]), token.data_ptr(), _lib.stream_of_device(dev))
+                  k[0], int(k[1]), p[0], float(p[1]), least[0], float(least[1]), token.data_ptr(),
+                  None if work is None else work.data_ptr(), nbytes, stream)
     return token

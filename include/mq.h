@@ -584,10 +584,12 @@ int mq_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, in
  * units of 2^-45 of the largest for V = 2^17 (2^(log2(V) - 62), at least 2^-51): the same inputs always give the same token.
  *   logits [rows, V] of type dtype (bf16, fp16, fp32), row stride ld, V <= 2^24; temperature, top_p, min_p fp32 [rows]
  *   and top_k int32 [rows], or NULL for the value *_all of every row
+ *   workspace: mq_sample_workspace_bytes(rows, V) bytes, 16-byte aligned (nothing in it has to start at zero)
  */
 int mq_sample(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const float* u, const float* temperature,
               float temperature_all, const int32_t* top_k, int64_t top_k_all, const float* top_p, float top_p_all,
-              const float* min_p, float min_p_all, int64_t* token, void* stream);
+              const float* min_p, float min_p_all, int64_t* token, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t mq_sample_workspace_bytes(int64_t rows, int64_t V);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,7 @@ SHARED = dict(q=A, q_token=1024, q_head=128, dtype=0, B=3, Hq=8, H=4, D=128, kc=
               c_token=128, ks=None, vs=None, s_page=0, s_head=0, s_token=0, pages=9, page=16, table=A, ld=4, width=4,
               lens=A, plan=A, scale=0.1, out=A, out_token=1024, out_head=128, work=A, work_bytes=1 << 30, counters=A, stream=None)
 SAMPLE = dict(x=A, dtype=0, ld=100, rows=3, V=100, u=A, t=None, t1=1.0, k=None, k1=0, p=None, p1=1.0, m=None, m1=0.0, token=A,
-              stream=None)
+              work=None, work_bytes=0, stream=None)
 
 REFUSED = [
     ("mq_rms_norm", NORM, dict(dtype=3), "input type"), ("mq_rms_norm", NORM, dict(w_dtype=-1), "weight type"),
@@ -59,6 +59,7 @@ REFUSED = [
     ("mq_sample", SAMPLE, dict(rows=-1), "bad shape"), ("mq_sample", SAMPLE, dict(ld=99), "row stride"),
     ("mq_sample", SAMPLE, dict(u=None), "null"), ("mq_sample", SAMPLE, dict(token=None), "null"),
     ("mq_sample", SAMPLE, dict(t=A + 2), "aligned"), ("mq_sample", SAMPLE, dict(token=A + 4), "aligned"),
+    ("mq_sample", SAMPLE, dict(V=1 << 20, ld=1 << 20), "workspace"), ("mq_sample", SAMPLE, dict(V=1 << 20, ld=1 << 20, work=A + 4, work_bytes=1 << 40), "workspace"),
 ]
 
 
@@ -127,6 +128,7 @@ def host(monkeypatch):
     monkeypatch.setattr(kv, "_scratch", lambda n, dev, stream: torch.zeros(4))
     monkeypatch.setattr(kv, "_counters", lambda n, dev, stream: torch.zeros(4, dtype=torch.int32))
     monkeypatch.setattr(module, "_device_check", lambda t, what: None)
+    monkeypatch.setattr(module, "_SAMPLE_WS", {(None, 3, 50): 0})
     return seen
 
 
