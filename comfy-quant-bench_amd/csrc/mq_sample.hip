@@ -127,7 +127,7 @@ struct Lds {
     uint64_t weight[kBins];         // of the bins' centres in units, from the best's down
     uint64_t bins[kBins + 64];      // first by place (n modulo 4096, and a place for each lane's values that are in none), then
                                     // masses from the best's down; blocks' masses
-    uint64_t work[kBins];           // sums over ranges
+    alignas(16) uint64_t work[kBins];   // sums over ranges; a few values side by side
     uint64_t list[kList];           // index << 32 | key, in any order
     uint64_t wave[2 * kWavesOf];
     int found, n;
@@ -157,6 +157,19 @@ __device__ __forceinline__ uint64_t wave_incl(uint64_t v) {
     v += dpp64<0x143, 0xc>(v);
     return v;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp32(uint32_t v) { return __builtin_amdgcn_update_dpp(0u, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ uint32_t wave_incl(uint32_t v) {
+    v += dpp32<0x111, 0xf>(v);
+    v += dpp32<0x112, 0xf>(v);
+    v += dpp32<0x114, 0xf>(v);
+    v += dpp32<0x118, 0xf>(v);
+    v += dpp32<0x142, 0xa>(v);
+    v += dpp32<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) { return lane64(v, lane); }
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane64(wave_incl(v), 63); }
 __device__ __forceinline__ uint32_t wave_max(uint32_t b) {
     b = __builtin_elementwise_max(b, dpp_mov_u<kQuadXor1>(b));
@@ -195,39 +208,39 @@ __device__ __forceinline__ uint32_t block_max(uint32_t s, Lds& sh) {
     return wave_max(static_cast<uint32_t>(sh.wave[threadIdx.x & 15]));
 }
 
-// Where the sum of x(0), x(1), ... x(4095) reaches `need` (> 0): the place (4096: nowhere) and what is missing in front of it.
-// Every wave sums 256 of them; the one where it is looks at its own again.
-template <typename F>
-__device__ __forceinline__ int cut(F x, uint64_t need, uint64_t* left, Lds& sh) {
+// Where the sum of x(0), x(1), ... x(4095), of type T, reaches `need` (> 0): the place (4096: nowhere), what is missing in front of
+// it, and (*all, not null) the sum. Every wave sums 256 of them; the one where it is looks at its own again.
+template <typename T, typename F>
+__device__ __forceinline__ int cut(F x, T need, T* left, T* all, Lds& sh) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint64_t v[kEach], sum = 0;
+    T v[kEach], sum = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         v[e] = x(256 * wave + 64 * e + lane);
         sum += v[e];
     }
-    sum = wave_sum(sum);
+    sum = lane_of(wave_incl(sum), 63);
     __syncthreads();
     if (lane == 0) sh.wave[wave] = sum;
     __syncthreads();
-    const uint64_t to = wave_incl(sh.wave[lane & 15]);
-    const uint64_t upto = lane64(to, wave), before = upto - sum;
-    if (wave == 0 && lane64(to, 15) < need && lane == 0) sh.found = kBins;
+    const T to = wave_incl(static_cast<T>(sh.wave[lane & 15])), upto = lane_of(to, wave), before = upto - sum, total = lane_of(to, 15);
+    if (all) *all = total;
+    if (wave == 0 && total < need && lane == 0) sh.found = kBins;
     if (before < need && upto >= need) {
-        uint64_t at = before;
+        T at = before;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const uint64_t y = at + wave_incl(v[e]);
+            const T y = at + wave_incl(v[e]);
             if (y - v[e] < need && y >= need) {
                 sh.found = 256 * wave + 64 * e + lane;
                 sh.left = need - (y - v[e]);
             }
-            at = lane64(y, 63);
+            at = lane_of(y, 63);
         }
     }
     __syncthreads();
     const int found = __builtin_amdgcn_readfirstlane(sh.found);
-    *left = sh.left;
+    *left = static_cast<T>(sh.left);
     __syncthreads();
     return found;
 }
@@ -276,7 +289,7 @@ __device__ __forceinline__ uint32_t narrow(int n, const uint32_t (&at)[kEach], u
         for (int e = 0; e < kEach; ++e)
             if (x[e]) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.work[(at[e] - from) >> shift]), static_cast<unsigned long long>(x[e]));
         __syncthreads();
-        const int range = cut([&](int i) { return sh.work[i]; }, *need, need, sh);
+        const int range = cut<uint64_t>([&](int i) { return sh.work[i]; }, *need, need, nullptr, sh);
         from += static_cast<uint32_t>(range < kBins ? range : kBins - 1) << shift;
         if (shift == 0) return from;
 #pragma unroll
@@ -590,7 +603,7 @@ __device__ __forceinline__ int choose_block(const Row& w, Limit limit, Lds& sh) 
 #pragma unroll
     for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
     all = block_sum(s, sh);
-    const int i0 = cut([&](int i) { return sh.bins[i]; }, w.place(all) + 1, &left, sh) * kBlock, i = i0 + kPer * threadIdx.x;
+    const int i0 = cut<uint64_t>([&](int i) { return sh.bins[i]; }, w.place(all) + 1, &left, nullptr, sh) * kBlock, i = i0 + kPer * threadIdx.x;
     float v[kPer];
     uint64_t x[kPer], sum = 0;
     unpack8<DT>(load_raw8<DT>(w.x, i, w.V), v);
@@ -679,7 +692,7 @@ __device__ __forceinline__ Limit limit_by_digits(const Row& w, int bin, Limit no
             }
         });
         __syncthreads();
-        const int d = cut([&](int i) { return sh.work[i]; }, need, &need, sh);
+        const int d = cut<uint64_t>([&](int i) { return sh.work[i]; }, need, &need, nullptr, sh);
         prefix |= static_cast<uint32_t>(255 - (d < 256 ? d : 255)) << shift;
         if (d >= 256) need = 1;
     }
@@ -720,6 +733,68 @@ __device__ __forceinline__ Limit limit_in_row(const Row& w, int bin, Limit now, 
     return limit_in<MASS>(w, n, bin, now, need, [&](float v) { return w.units(v, sh); }, sh);
 }
 
+// Few values in LDS (n <= kFew), one a thread: how many of them come before thread i's in the order, and their units.
+struct Few {
+    uint64_t code, units, before;   // code: larger comes first
+    int rank;
+};
+struct alignas(16) Pair {
+    uint64_t a, b;
+};
+__device__ __forceinline__ Pair* pairs_of(Lds& sh) { return reinterpret_cast<Pair*>(sh.work); }
+__device__ __forceinline__ Few rank_few(int n, uint64_t units, Lds& sh) {
+    Few f{0, units, 0, 0};
+    const int i = threadIdx.x;
+    if (i < n) {
+        const uint64_t x = sh.list[i];
+        f.code = x << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(x >> 32));
+    }
+    if (i < kFew) pairs_of(sh)[i] = Pair{f.code, units};
+    __syncthreads();
+    if (i < n)
+#pragma unroll 8
+        for (int j = 0; j < (n + 7) / 8 * 8; ++j) {
+            const Pair y = pairs_of(sh)[j];
+            const bool ahead = y.a > f.code;        // (places behind n are 0)
+            f.rank += ahead;
+            f.before += ahead ? y.b : 0;
+        }
+    return f;
+}
+// The sum over the first four waves, of which only these are left.
+__device__ __forceinline__ uint64_t four_sum(uint64_t s, Lds& sh) {
+    s = wave_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return sh.wave[0] + sh.wave[1] + sh.wave[2] + sh.wave[3];
+}
+
+// choose_listed for n <= kFew: the last thing that a workgroup does, by its first four waves.
+__device__ __forceinline__ void choose_few(const Row& w, int n, int64_t* token, Lds& sh) {
+    if (threadIdx.x >= kFew) return;
+    const int i = threadIdx.x;
+    const float v = i < n ? value_of(static_cast<uint32_t>(sh.list[i])) : kNone;
+    Few f = rank_few(n, i < n ? w.units(v) : 0, sh);
+    bool in = i < n && (!w.k_limits() || f.rank < w.k);
+    if (w.p_limits()) {
+        const uint64_t need = w.part(four_sum(in ? f.units : 0, sh));
+        in = in && f.before < need;
+    }
+    const uint64_t x = in && v >= w.floor ? f.units : 0, t = w.place(four_sum(x, sh));
+    const uint32_t mine = static_cast<uint32_t>(sh.list[i] >> 32);
+    pairs_of(sh)[i] = Pair{mine, x};
+    __syncthreads();
+    uint64_t to = 0;
+    if (x)
+#pragma unroll 8
+        for (int j = 0; j < (n + 7) / 8 * 8; ++j) {
+            const Pair y = pairs_of(sh)[j];         // (behind n: nothing)
+            to += static_cast<uint32_t>(y.a) < mine ? y.b : 0;
+        }
+    if (x && to <= t && to + x > t) *token = mine;
+}
+
 // The token of n values in LDS, all that k (the bin that it cuts and what it keeps of that; 4096: none) may keep.
 __device__ __forceinline__ int choose_listed(const Row& w, int n, int k_bin, uint64_t k_left, Lds& sh) {
     Limit limit{0, w.V};
@@ -744,7 +819,7 @@ __device__ __forceinline__ int choose_listed(const Row& w, int n, int k_bin, uin
             atomicAdd(reinterpret_cast<unsigned long long*>(&sh.work[static_cast<int>(w.depth(v))]), static_cast<unsigned long long>(z));
         });
         s = block_sum(s, sh);
-        const int bin = cut([&](int i) { return sh.work[i]; }, w.part(s), &left, sh);
+        const int bin = cut<uint64_t>([&](int i) { return sh.work[i]; }, w.part(s), &left, nullptr, sh);
         limit = limit_in<true>(w, n, bin, limit, left, units, sh);
     }
     uint64_t s = 0;
@@ -763,7 +838,19 @@ __device__ __forceinline__ int choose_cut(const Row& w, int n, int bin, uint64_t
     auto units = [&](float v) { return w.units(v, sh); };
     Limit limit{0, w.V};
     if (n <= kList) {
-        limit = limit_in<true>(w, n, bin, limit, left, units, sh);
+        if (n <= kFew) {
+            // the limit is the last one in front of which less than `left` lies
+            const float v = static_cast<int>(threadIdx.x) < n ? value_of(static_cast<uint32_t>(sh.list[threadIdx.x])) : kNone;
+            const Few f = rank_few(n, static_cast<int>(threadIdx.x) < n ? units(v) : 0, sh);
+            const bool in = static_cast<int>(threadIdx.x) < n && (f.before < left || f.rank == 0);
+            const uint32_t last = block_max(in ? static_cast<uint32_t>(f.rank) + 1 : 0u, sh);
+            if (in && f.rank + 1 == static_cast<int>(last)) sh.left = f.code;
+            __syncthreads();
+            limit = Limit{static_cast<uint32_t>(sh.left >> 32), static_cast<int>(~static_cast<uint32_t>(sh.left))};
+            __syncthreads();
+        } else {
+            limit = limit_in<true>(w, n, bin, limit, left, units, sh);
+        }
         listed(n, sh, [&](int e, float v, int i) {
             if (v >= w.floor && limit.keeps(key_of(v), i))
                 atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[i / kBlock]), static_cast<unsigned long long>(units(v)));
@@ -828,15 +915,12 @@ __device__ __forceinline__ void place_again(Row& w) {
 // Where numbers of the bins (by place) cut k: the bin (4096: nowhere), what it keeps, and how many values that bin and those above
 // it have.
 __device__ __forceinline__ int cut_number(const Row& w, int base, uint64_t* left, uint64_t* held, Lds& sh) {
-    auto number = [&](int d) { return sh.bins[(base + d) & kMask] >> w.number; };
-    const int bin = cut(number, static_cast<uint64_t>(w.k), left, sh);
-    uint64_t s = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int d = kThreads * e + threadIdx.x;
-        s += d <= bin ? number(d) : 0;
-    }
-    *held = block_sum(s, sh);
+    auto number = [&](int d) { return static_cast<uint32_t>(sh.bins[(base + d) & kMask] >> w.number); };
+    uint32_t rest, all;
+    const uint32_t k = static_cast<uint32_t>(w.k);
+    const int bin = cut<uint32_t>(number, k, &rest, &all, sh);
+    *left = rest;
+    *held = bin < kBins ? k - rest + number(bin) : all;
     return bin;
 }
 
@@ -872,7 +956,7 @@ __device__ __attribute__((noinline)) int by_readings(Row w, Lds& sh) {
         for (int e = 0; e < kEach; ++e) s += kThreads * e + threadIdx.x < bin ? sh.bins[kThreads * e + threadIdx.x] : 0;
         const uint64_t above = block_sum(s, sh), need = w.part(above + mass);
         left = need - above;
-        if (need <= above) bin = cut([&](int i) { return sh.bins[i]; }, need, &left, sh);
+        if (need <= above) bin = cut<uint64_t>([&](int i) { return sh.bins[i]; }, need, &left, nullptr, sh);
         if (bin < kBins) limit = limit_in_row<DT, true>(w, bin, limit, left, sh);
     }
     block_masses<DT, true>(w, 0, w.V, kBins, limit, sh);
@@ -900,7 +984,7 @@ __device__ __forceinline__ int cut_mass(const Row& w, uint64_t* left, Lds& sh) {
     uint64_t s = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) s += sh.bins[kThreads * e + threadIdx.x];
-    return cut([&](int i) { return sh.bins[i]; }, w.part(block_sum(s, sh)), left, sh);
+    return cut<uint64_t>([&](int i) { return sh.bins[i]; }, w.part(block_sum(s, sh)), left, nullptr, sh);
 }
 
 template <int DT>
@@ -922,6 +1006,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
             if (held <= kList) {
                 empty_list(sh);
                 collect<DT>(w, 0, w.V, 0, bin < kBins ? bin : kBins - 1, sh);
+                if (sh.n <= kFew) {
+                    choose_few(w, sh.n, a.token + r, sh);
+                    return;
+                }
                 token = choose_listed(w, sh.n, bin, left, sh);
             } else {
                 token = by_readings<DT>(w, sh);
@@ -1075,6 +1163,10 @@ __global__ void __launch_bounds__(kThreads) sample_second_kernel(SampleArgs a) {
     if (!w.k_limits())
         for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = static_cast<int64_t>(i) * kBlock < w.V ? receive(s.blocks + i) : 0;
     __syncthreads();
+    if (w.k_limits() && n <= kFew) {
+        choose_few(w, n, a.token + blockIdx.y, sh);
+        return;
+    }
     if (w.k_limits()) token = choose_listed(w, n, bin, left, sh);
     else token = bin < kBins ? choose_cut<DT>(w, n, bin, left, sh) : choose_block<DT>(w, Limit{0, w.V}, sh);
     if (threadIdx.x == 0) a.token[blockIdx.y] = token;
