@@ -3,12 +3,13 @@
 //
 //   softmax over [shared keys, own keys] = both parts' unnormalised outputs over a common maximum, divided by both sums
 //
-// Three kernels. The plan (once for all layers of a step) finds the groups. The second takes the rows of a group (its
-// sequences' query heads of one cache head) as tiles of 16 RT rows over the shared keys and leaves, for every sequence and
-// head, output, maximum and sum over them in fp32. The third is the single-token kernel over each sequence's own keys,
-// which adds that part before it divides.
+// The plan (once for all layers of a step) finds the groups. The first kernel takes the rows of a group (its sequences' query
+// heads of one cache head) as tiles of 16 RT rows over the shared keys, cut into as many pieces as there are compute units;
+// the second joins the pieces of every row; the third is the single-token kernel over each sequence's own keys, which adds that
+// part before it divides. (Pieces joined by the workgroup that brings the last one, as the single-token kernel does it:
+// 32 sequences over 32000 tokens 160 us instead of XX, most of it one workgroup's waiting for 17 x 64 rows.)
 //
-// The second kernel is the single-token kernel's plan with more rows: HBM-bound where a group has few of them, keys and
+// The first kernel is the single-token kernel's plan with more rows: HBM-bound where a group has few of them, keys and
 // values go straight from the pages into registers, each wave with 32 keys of a tile and all rows. At 64 rows (RT = 4) a
 // wave's 32 keys of 128 values cost 64 products of 16 cycles and some 1500 cycles of softmax against the 16 KB that it
 // waits for, a fifth of what HBM brings a compute unit in that time, so larger groups, whose tiles read the keys again from
@@ -32,25 +33,32 @@ constexpr int kPlanThreads = 1024;
 //
 // Sequences belong together if their first pages are the same; what a group shares is the shortest run of equal pages
 // of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency.
+// ON_CHIP: working space in LDS (up to kPlanRows sequences), else behind the plan.
+constexpr int kPlanRows = 2048;
+
 // (What atomics have changed is read past the first level cache.)
 __device__ __forceinline__ int latest(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+template <bool ON_CHIP>
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* table, int64_t ld, int B, int width,
                                                                     const int* lens, int page_shift, int* plan) {
     __shared__ int wave_sum[2][kPlanThreads / 64];
+    __shared__ int space[ON_CHIP ? 4 * kPlanRows : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int* start = plan + SharedPlan::start();
     int* members = plan + SharedPlan::members(B);
     int* groups = plan + SharedPlan::groups(B);
-    int* key = plan + SharedPlan::work(B);          // first page
-    int* lead = key + B;                            // first sequence with it
-    int* tokens = lead + B;                         // of a lead: what its group shares
-    int* count = tokens + B;                        // of a lead: members
+    int* group_at = plan + SharedPlan::group_at(B);
+    int* rank_at = plan + SharedPlan::rank_at(B);
+    int* work = plan + SharedPlan::work(B);
+    int* key = ON_CHIP ? space : work;                                  // first page
+    int* lead = ON_CHIP ? space + kPlanRows : work + B;                 // first sequence with it
+    int* tokens = ON_CHIP ? space + 2 * kPlanRows : work + 2 * static_cast<int64_t>(B);    // of a lead: what its group shares
+    int* count = ON_CHIP ? space + 3 * kPlanRows : work + 3 * static_cast<int64_t>(B);     // of a lead: members
     for (int b = tid; b < B; b += kPlanThreads) {
         key[b] = lens[b] > 0 && width > 0 ? table[b * ld] : -1;
         tokens[b] = 0x7fffffff;
         count[b] = 0;
-        start[b] = 0;
     }
     __syncthreads();
     for (int b = tid; b < B; b += kPlanThreads) {
@@ -64,24 +72,30 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
         lead[b] = l;
     }
     __syncthreads();
-    // a wave a sequence: entries that it has in common with its lead
+    // a wave a sequence: entries that it has in common with its lead, 256 at a time
     for (int b = wave; b < B; b += kPlanThreads / 64) {
         const int l = lead[b];
-        if (l < 0 || latest(count + l) < 2) continue;
+        if (l < 0 || l == b || latest(count + l) < 2) continue;
         const int most = lens[b] < lens[l] ? lens[b] : lens[l];
         const int entries = static_cast<int>((static_cast<int64_t>(most) + (1 << page_shift) - 1) >> page_shift);
         const int n = entries < width ? entries : width;
         int same = n;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const int i = i0 + lane;
-            bool differ = false;
-            if (i < n) {
-                const int x = table[b * ld + i];
-                differ = x < 0 || x != table[l * ld + i];
+        for (int i0 = 0; i0 < n; i0 += 256) {
+            int x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = i0 + 64 * e + lane < n ? i0 + 64 * e + lane : n - 1;
+                x[e] = table[b * ld + i];
+                y[e] = table[l * ld + i];
             }
-            const uint64_t any = __ballot(differ);
-            if (any) {
-                same = i0 + __builtin_ctzll(any);
+            int first = n;
+#pragma unroll
+            for (int e = 3; e >= 0; --e) {
+                const uint64_t any = __ballot(x[e] < 0 || x[e] != y[e]);
+                if (any) first = i0 + 64 * e + __builtin_ctzll(any);
+            }
+            if (first < n) {
+                same = first;
                 break;
             }
         }
@@ -116,19 +130,24 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
             to[1] = b;
             to[2] = member0 + m - n;
             to[3] = n;
-            count[b] = -(member0 + m - n) - 1;      // a group: where its members begin
+            key[b] = group0 + g - 1;                // a group: its number, where its members begin
+            count[b] = -(member0 + m - n) - 1;
         }
         group0 += all_g;
         member0 += all_m;
         __syncthreads();
     }
     for (int b = tid; b < B; b += kPlanThreads) {
-        const int l = lead[b];
-        if (l < 0 || latest(count + l) >= 0) continue;
+        const int l = lead[b], begin = l < 0 ? 0 : latest(count + l);
+        const bool in = begin < 0;
         int before = 0;
-        for (int x = l; x < b; ++x) before += lead[x] == l;
-        members[-latest(count + l) - 1 + before] = b;
-        start[b] = latest(tokens + l);
+        if (in) {
+            for (int x = l; x < b; ++x) before += lead[x] == l;
+            members[-begin - 1 + before] = b;
+        }
+        start[b] = in ? latest(tokens + l) : 0;
+        group_at[b] = in ? key[l] : -1;
+        rank_at[b] = before;
     }
     if (tid == 0) {
         plan[0] = group0;
@@ -155,10 +174,96 @@ __device__ __forceinline__ Group group_of(const AttnArgs& a, int g) {
     return r;
 }
 
+constexpr int kSharedTile = kSharedWaves * kKeys;
+
+__device__ __forceinline__ int groups_of(const AttnArgs& a) {
+    const int n = a.plan[0], most = static_cast<int>(a.B) / 2;
+    return n < 0 ? 0 : n < most ? n : most;
+}
+
+// The line of tiles: a group takes up its tiles for each (cache head, row tile) pair.
+__device__ __forceinline__ int tiles_of(const Group& r) { return (r.tokens + kSharedTile - 1) / kSharedTile; }
+template <int ROWS>
+__device__ __forceinline__ int row_tiles_of(const AttnArgs& a, const Group& r) { return (r.count * (a.Hq / a.H) + ROWS - 1) / ROWS; }
+// Its places (they fit 32 bits: the host refuses tables that could hold more), and those of the groups in front of group g.
+template <int ROWS>
+__device__ __forceinline__ int line_of(const AttnArgs& a, int n_groups, int g, int* before) {
+    int all = 0, front = 0;
+    for (int x = threadIdx.x & 63; x < n_groups; x += 64) {
+        const Group r = group_of(a, x);
+        const int n = tiles_of(r) * row_tiles_of<ROWS>(a, r) * a.H;
+        all += n;
+        front += x < g ? n : 0;
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        all += __shfl_xor(all, s);
+        front += __shfl_xor(front, s);
+    }
+    *before = __builtin_amdgcn_readfirstlane(front);
+    return __builtin_amdgcn_readfirstlane(all);
+}
+
+// The pieces of every row together, in their order: a wave a row (of a sequence and query head).
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int pieces_most) {
+    const int64_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    if (at >= a.B * a.Hq) return;
+    const int b = static_cast<int>(at / a.Hq), hq = static_cast<int>(at % a.Hq), lane = threadIdx.x & 63;
+    const int g = a.plan[SharedPlan::group_at(a.B) + b], rank = a.plan[SharedPlan::rank_at(a.B) + b], n_groups = groups_of(a);
+    if (g < 0 || g >= n_groups || rank < 0) return;
+    const Group r = group_of(a, g);
+    if (r.tokens == 0 || rank >= r.count) return;
+    int before;
+    const int total = line_of<ROWS>(a, n_groups, g, &before), piece = (total + pieces_most - 1) / pieces_most;
+    const int group = a.Hq / a.H, h = hq / group, of = rank * group + hq % group, nt = tiles_of(r);
+    const int s0 = before + (h * row_tiles_of<ROWS>(a, r) + of / ROWS) * nt, row = of % ROWS;
+    const int p0 = s0 / piece, p1 = (s0 + nt - 1) / piece, slots = 2 * pieces_most;
+    constexpr int V = DP == 256 ? 4 : DP == 128 ? 2 : 1, kAhead = 8;
+    const int d = V * lane;
+    float top = kNegInf, sum = 0.0f, y[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = 0.0f;
+    bool some = false;
+    for (int p = p0; p <= p1; p += kAhead) {
+        float2 st[kAhead];
+        float z[kAhead][V];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int x = p + i < p1 ? p + i : p1, slot = 2 * x + (x * piece < s0);
+            st[i] = *reinterpret_cast<const float2*>(part_stat(a, ROWS, slots, slot) + 2 * row);
+            const float* from = part_out(a, ROWS, slot) + row * a.D + (d < a.D ? d : 0);
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[i][e] = from[e];
+        }
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) most = p + i <= p1 && st[i].y >= 0.0f ? __builtin_fmaxf(most, st[i].x) : most;
+        const float ref = most == kNegInf ? 0.0f : most, f = __builtin_amdgcn_exp2f(top - ref);
+        top = most;
+        sum *= f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] *= f;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (p + i > p1 || st[i].y < 0.0f) continue;                 // nothing seen there
+            some = true;
+            const float fz = __builtin_amdgcn_exp2f(st[i].x - ref);
+            sum += st[i].y * fz;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] += z[i][e] * fz;
+        }
+    }
+    if (d < a.D)
+#pragma unroll
+        for (int e = 0; e < V; ++e) a.shared_out[at * a.D + d + e] = y[e];
+    if (lane == 0) reinterpret_cast<float2*>(a.shared_stat)[at] = make_float2(top, some ? sum : -1.0f);
+}
+
 template <int DP, int DT, bool I8, bool SMALL>
 __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnArgs a, bool quads) {
     constexpr int RT = rows16_of(DP), kTileRows = 16 * RT;
-    constexpr int kWaves = kSharedWaves, kTile = kWaves * kKeys;
+    constexpr int kWaves = kSharedWaves, kTile = kSharedTile;
     constexpr int E = I8 ? 1 : 2;
     constexpr int VE = DP / 16;
     constexpr int kSteps = DP / 32;
@@ -172,25 +277,16 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
     __shared__ float sm_out[kWaves][16][DP + 4];
     __shared__ float sm_m[kWaves][kTileRows], sm_l[kWaves][kTileRows];
     __shared__ int sm_any[kWaves];
-    __shared__ int sm_last;
+    // the query rows, as the products take them: [row tile][step][lane]
+    __shared__ Frag sm_q[RT][kSteps][64], sm_q2[kSplit ? RT : 1][kSplit ? kSteps : 1][64];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int group = a.Hq / a.H;
     const int B = static_cast<int>(a.B);
-    const int found = a.plan[0], n_groups = found < 0 ? 0 : found < B / 2 ? found : B / 2;
-    // the line of tiles: group x takes up its tiles for each (cache head, row tile) pair
-    auto tiles_of = [&](const Group& r) { return (r.tokens + kTile - 1) / kTile; };
-    auto pairs_of = [&](const Group& r) { return (r.count * group + kTileRows - 1) / kTileRows * a.H; };
-    // (its places fit 32 bits: the host refuses tables that could hold more)
-    int total = 0;
-    for (int x = lane; x < n_groups; x += 64) {
-        const Group r = group_of(a, x);
-        total += tiles_of(r) * pairs_of(r);
-    }
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
-    total = __builtin_amdgcn_readfirstlane(total);
+    const int n_groups = groups_of(a);
+    int front;
+    const int total = line_of<kTileRows>(a, n_groups, 0, &front);
     const int piece = (total + gridDim.x - 1) / gridDim.x;
     const int t0 = blockIdx.x * piece, t1 = t0 + piece < total ? t0 + piece : total;
     if (t0 >= t1) return;
@@ -209,15 +305,15 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
     for (int t = t0; t < t1;) {
         // the segment: tiles i0 .. i1 - 1 of group gi's cache head and row tile, whose tile 0 is place s0
         Group r = group_of(a, gi);      // (uniform: the plan is read at the same place by all lanes)
-        while (t - before >= tiles_of(r) * pairs_of(r)) {
-            before += tiles_of(r) * pairs_of(r);
+        while (t - before >= tiles_of(r) * row_tiles_of<kTileRows>(a, r) * a.H) {
+            before += tiles_of(r) * row_tiles_of<kTileRows>(a, r) * a.H;
             ++gi;
             r = group_of(a, gi);
         }
         const int nt = tiles_of(r), pair = (t - before) / nt;
         const int s0 = before + pair * nt;
         const int i0 = t - s0, i1 = t1 - s0 < nt ? t1 - s0 : nt;
-        const int rtiles = (r.count * group + kTileRows - 1) / kTileRows;
+        const int rtiles = row_tiles_of<kTileRows>(a, r);
         const int h = pair / rtiles, row0 = pair % rtiles * kTileRows;
         const int rows = r.count * group - row0 < kTileRows ? r.count * group - row0 : kTileRows;
         const int* table = a.table + static_cast<int64_t>(r.lead) * a.ld_table;
@@ -234,9 +330,7 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
             *hq = h * group + at % group;
         };
 
-        Frag q[RT][kSteps], q2[kSplit ? RT : 1][kSplit ? kSteps : 1];
-#pragma unroll
-        for (int x = 0; x < RT; ++x) {
+        for (int x = wave; x < RT; x += kWaves) {
             int seq = -1, hq = 0;
             if (16 * x + c < rows) row_of(16 * x + c, &seq, &hq);
             const uint16_t* row = static_cast<const uint16_t*>(a.q) + (seq < 0 ? 0 : seq) * a.q_token + hq * a.q_head;
@@ -245,18 +339,17 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
                 const int d = I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
                 uint4 y = make_uint4(0, 0, 0, 0);
                 if (seq >= 0 && d < a.D) y = *reinterpret_cast<const uint4*>(row + d);
-                q[x][s] = Frag{{y.x, y.y, y.z, y.w}};
+                Frag q{{y.x, y.y, y.z, y.w}};
                 if constexpr (kSplit) {
+                    Frag q2;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t hi, lo;
-                        split_f16(q[x][s].w[j], &hi, &lo);
-                        q[x][s].w[j] = hi;
-                        q2[x][s].w[j] = lo;
-                    }
+                    for (int j = 0; j < 4; ++j) split_f16(q.w[j], &q.w[j], &q2.w[j]);
+                    sm_q2[x][s][lane] = q2;
                 }
+                sm_q[x][s][lane] = q;
             }
         }
+        __syncthreads();
 
         Raw<KB> kr[2][2][KL];
         Raw<VE * E> vr[2][8];
@@ -366,13 +459,21 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
 #pragma unroll
             for (int x = 0; x < RT; ++x) {
                 float p[8];
+                // (read here every time: kept from tile to tile, all rows' would push others out of the registers)
+                asm volatile("" ::: "memory");
+                Frag q[kSteps], q2[kSplit ? kSteps : 1];
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) {
+                    q[st] = sm_q[x][st][lane];
+                    if constexpr (kSplit) q2[st] = sm_q2[x][st][lane];
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     f32x4 s = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int st = 0; st < kSteps; ++st) {
-                        s = mfma16<MT>(k[u][st], q[x][st], s);
-                        if constexpr (kSplit) s = mfma16<MT>(k[u][st], q2[x][st], s);
+                        s = mfma16<MT>(k[u][st], q[st], s);
+                        if constexpr (kSplit) s = mfma16<MT>(k[u][st], q2[st], s);
                     }
 #pragma unroll
                     for (int y = 0; y < 4; ++y) p[4 * u + y] = s[y] * scale * (I8 ? ksc[buf][u][y] : 1.0f);
@@ -460,7 +561,6 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
 
         // the waves' parts together, 16 rows at a time: rows c, values VE (4 g + y) + e
         const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < s0);
-        const bool complete = i0 == 0 && i1 == nt;
         if (lane == 0) sm_any[wave] = any;
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
@@ -499,63 +599,10 @@ __global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnA
                     y[2] = __builtin_fmaf(f, z.z, y[2]);
                     y[3] = __builtin_fmaf(f, z.w, y[3]);
                 }
-                if (complete) {
-                    int seq, hq;
-                    row_of(row, &seq, &hq);
-                    if (seq < 0) continue;
-                    const int64_t at = static_cast<int64_t>(seq) * a.Hq + hq;
-                    *reinterpret_cast<float4*>(a.shared_out + at * a.D + d) = make_float4(y[0], y[1], y[2], y[3]);
-                    if (d == 0) reinterpret_cast<float2*>(a.shared_stat)[at] = make_float2(top + kShift, some ? sum : -1.0f);
-                } else {
-                    float* to = part_out(a, kTileRows, slot) + row * a.D + d;
-                    send(to, y[0], y[1]);
-                    send(to + 2, y[2], y[3]);
-                    if (d == 0) send(part_stat(a, kTileRows, slots, slot) + 2 * row, top, some ? sum : -1.0f);
-                }
-            }
-        }
-        if (!complete) {
-            // the pieces of the segment: workgroups p0 .. p1 of the line; the last to arrive joins them in their order
-            const int p0 = s0 / piece, p1 = (s0 + nt - 1) / piece;
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const int64_t at = (static_cast<int64_t>(r.first) * group / kTileRows + gi + row0 / kTileRows) * a.H + h;
-                int* count = a.counters + at;
-                const int old = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (old == p1 - p0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                sm_last = old == p1 - p0;
-            }
-            __syncthreads();
-            if (sm_last) {
-                for (int e = threadIdx.x; e < rows * (DP / 4); e += 64 * kWaves) {
-                    const int row = e / (DP / 4), d = 4 * (e % (DP / 4));
-                    if (d >= a.D) continue;
-                    float top = kNegInf, sum = 0.0f, y[4] = {0, 0, 0, 0};
-                    bool some = false;
-                    for (int p = p0; p <= p1; ++p) {
-                        const int from = 2 * p + (p * piece < s0);
-                        const float2 st = receive(part_stat(a, kTileRows, slots, from) + 2 * row);
-                        const float* z = part_out(a, kTileRows, from) + row * a.D + d;
-                        const float2 z0 = receive(z), z1 = receive(z + 2);
-                        if (st.y < 0.0f) continue;      // nothing seen there
-                        some = true;
-                        const float mx = __builtin_fmaxf(top, st.x), ref = mx == kNegInf ? 0.0f : mx;
-                        const float f = __builtin_amdgcn_exp2f(top - ref), fz = __builtin_amdgcn_exp2f(st.x - ref);
-                        top = mx;
-                        sum = sum * f + st.y * fz;
-                        y[0] = y[0] * f + z0.x * fz;
-                        y[1] = y[1] * f + z0.y * fz;
-                        y[2] = y[2] * f + z1.x * fz;
-                        y[3] = y[3] * f + z1.y * fz;
-                    }
-                    int seq, hq;
-                    row_of(row, &seq, &hq);
-                    if (seq < 0) continue;
-                    const int64_t at = static_cast<int64_t>(seq) * a.Hq + hq;
-                    *reinterpret_cast<float4*>(a.shared_out + at * a.D + d) = make_float4(y[0], y[1], y[2], y[3]);
-                    if (d == 0) reinterpret_cast<float2*>(a.shared_stat)[at] = make_float2(top + kShift, some ? sum : -1.0f);
-                }
+                float* to = part_out(a, kTileRows, slot) + row * a.D + d;
+                *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                if (d == 0)
+                    *reinterpret_cast<float2*>(part_stat(a, kTileRows, slots, slot) + 2 * row) = make_float2(top + kShift, some ? sum : -1.0f);
             }
         }
         __syncthreads();                                // what is in LDS has been read
@@ -572,6 +619,9 @@ int shared_width(const AttnArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL((attn_shared_kernel<DP, DT, I8, false>), grid, dim3(64 * kSharedWaves), 0, stream, a, quads);
     else
         hipLaunchKernelGGL((attn_shared_kernel<DP, DT, I8, true>), grid, dim3(64 * kSharedWaves), 0, stream, a, quads);
+    const int64_t rows = a.B * a.Hq;
+    hipLaunchKernelGGL((attn_shared_join_kernel<DP, 16 * rows16_of(DP)>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream,
+                       a, static_cast<int>(grid.x));
     return launch_status("paged_attention_shared");
 }
 
@@ -594,11 +644,7 @@ int64_t attn_shared_workspace_bytes(int Hq, int H, int D, int64_t B) {
     return (single > parts ? single : parts) + B * Hq * (D + 2) * 4;
 }
 
-int64_t attn_shared_counters(int Hq, int H, int64_t B) {
-    const int64_t single = attn_decode_counters(Hq, H, B);
-    const int64_t parts = (B * (Hq / H) / 32 + B / 2 + 2) * H;      // tiles of at least 32 rows
-    return single > parts ? single : parts;                         // zero between the two kernels
-}
+int64_t attn_shared_counters(int Hq, int H, int64_t B) { return attn_decode_counters(Hq, H, B); }
 
 int launch_attn_shared(const AttnArgs& args, hipStream_t stream) {
     AttnArgs a = args;
@@ -615,8 +661,8 @@ int launch_attn_shared(const AttnArgs& args, hipStream_t stream) {
 
 int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t width, const int* lens, int page_shift,
                      int* plan, hipStream_t stream) {
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, table, ld_table, static_cast<int>(rows),
-                       static_cast<int>(width), lens, page_shift, plan);
+    hipLaunchKernelGGL(rows <= kPlanRows ? shared_plan_kernel<true> : shared_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0,
+                       stream, table, ld_table, static_cast<int>(rows), static_cast<int>(width), lens, page_shift, plan);
     return launch_status("kv_shared");
 }
 
