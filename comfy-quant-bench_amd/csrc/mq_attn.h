@@ -71,5 +71,40 @@ __device__ __forceinline__ void split_f16(uint32_t w, uint32_t* hi, uint32_t* lo
     *lo = bf16_exact2(la, lb);
 }
 
+// 32 x 32 products, and exchanges between lanes l and l ^ 32, which hold a row of them.
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
+    if constexpr (DT == kDtF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float max2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum2(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// LDS by its own addresses.
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v* LdsShort4;
+
+// Sixteen bytes per active lane from `src` to LDS bytes dst + 16 lane (dst the same in all lanes). Written as asm: the
+// compiler would wait for the builtin's stores before any LDS read that it cannot tell apart. m0, which says where to,
+// is left as it was: the compiler may keep a value there and takes no word that it is overwritten (it is reserved).
+__device__ __forceinline__ void load_lds16(const char* src, uint32_t dst) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 }  // namespace
 }  // namespace mq

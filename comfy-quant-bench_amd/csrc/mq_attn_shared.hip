@@ -157,8 +157,10 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
 
 // ---------------------------------------------------------------------------------------- the shared keys
 
-constexpr int kSharedWaves = 4;
-constexpr int rows16_of(int dp) { return dp == 256 ? 2 : 4; }     // 16-row tiles that a wave holds
+constexpr int kSharedRows = 128;            // rows of a tile, 32 a wave
+constexpr int tile_keys(int dp) { return dp == 256 ? 32 : 64; }
+constexpr int tile_waves(int dp) { return dp == 128 ? 8 : 4; }
+constexpr int tiles_ahead(int dp) { return dp == 64 ? 7 : 3; }      // on their way while one is worked on
 
 struct Group {
     int tokens, lead, first, count;
@@ -174,24 +176,35 @@ __device__ __forceinline__ Group group_of(const AttnArgs& a, int g) {
     return r;
 }
 
-constexpr int kSharedTile = kSharedWaves * kKeys;
-
 __device__ __forceinline__ int groups_of(const AttnArgs& a) {
     const int n = a.plan[0], most = static_cast<int>(a.B) / 2;
     return n < 0 ? 0 : n < most ? n : most;
 }
 
-// The line of tiles: a group takes up its tiles for each (cache head, row tile) pair.
-__device__ __forceinline__ int tiles_of(const Group& r) { return (r.tokens + kSharedTile - 1) / kSharedTile; }
-template <int ROWS>
-__device__ __forceinline__ int row_tiles_of(const AttnArgs& a, const Group& r) { return (r.count * (a.Hq / a.H) + ROWS - 1) / ROWS; }
-// Its places (they fit 32 bits: the host refuses tables that could hold more), and those of the groups in front of group g.
-template <int ROWS>
-__device__ __forceinline__ int line_of(const AttnArgs& a, int n_groups, int g, int* before) {
+// The line of tiles (of `tile` keys): a group takes up its tiles for each (cache head, row tile) pair. (Its places fit 32 bits:
+// the host refuses tables that could hold more.)
+__device__ __forceinline__ int tiles_of(const Group& r, int tile) { return static_cast<int>((static_cast<uint32_t>(r.tokens) + tile - 1) / tile); }
+__device__ __forceinline__ int row_tiles_of(const AttnArgs& a, const Group& r) {
+    return (r.count * (a.Hq / a.H) + kSharedRows - 1) / kSharedRows;
+}
+__device__ __forceinline__ int places_of(const AttnArgs& a, const Group& r, int tile) { return tiles_of(r, tile) * row_tiles_of(a, r) * a.H; }
+
+// Lane x: group g0 + x.
+__device__ __forceinline__ Group groups_from(const AttnArgs& a, int g0) {
+    const int at = g0 + (threadIdx.x & 63), most = static_cast<int>(a.B) / 2;
+    Group r = group_of(a, at < most ? at : 0);          // (a group is read with their number: one wait less)
+    if (at >= groups_of(a)) r.tokens = 0;
+    return r;
+}
+__device__ __forceinline__ Group group_from(const Group& mine, int x) {
+    return Group{__builtin_amdgcn_readlane(mine.tokens, x), __builtin_amdgcn_readlane(mine.lead, x),
+                 __builtin_amdgcn_readlane(mine.first, x), __builtin_amdgcn_readlane(mine.count, x)};
+}
+// All places, and those of the groups in front of group g. mine: groups_from(a, 0).
+__device__ __forceinline__ int line_of(const AttnArgs& a, const Group& mine, int n_groups, int g, int tile, int* before) {
     int all = 0, front = 0;
-    for (int x = threadIdx.x & 63; x < n_groups; x += 64) {
-        const Group r = group_of(a, x);
-        const int n = tiles_of(r) * row_tiles_of<ROWS>(a, r) * a.H;
+    for (int g0 = 0; g0 < n_groups; g0 += 64) {
+        const int x = g0 + (threadIdx.x & 63), n = places_of(a, g0 ? groups_from(a, g0) : mine, tile);
         all += n;
         front += x < g ? n : 0;
     }
@@ -203,22 +216,47 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int n_groups, int g, i
     *before = __builtin_amdgcn_readfirstlane(front);
     return __builtin_amdgcn_readfirstlane(all);
 }
+// The group that has place t of the line, and the places in front of it.
+__device__ __forceinline__ Group group_at_place(const AttnArgs& a, const Group& mine, int n_groups, int t, int tile, int* before) {
+    int front = 0;
+    for (int g0 = 0; g0 < n_groups; g0 += 64) {
+        const Group r = g0 ? groups_from(a, g0) : mine;
+        const int n = places_of(a, r, tile);
+        int sum = n;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int y = __shfl_up(sum, s);
+            sum += (threadIdx.x & 63) >= s ? y : 0;
+        }
+        const uint64_t behind = __ballot(front + sum > t);
+        if (behind) {
+            const int x = __builtin_ctzll(behind);
+            *before = front + __builtin_amdgcn_readlane(sum - n, x);
+            return group_from(r, x);
+        }
+        front += __builtin_amdgcn_readlane(sum, 63);
+    }
+    *before = front;
+    return Group{0, 0, 0, 0};
+}
 
-// The pieces of every row together, in their order: a wave a row (of a sequence and query head).
-template <int DP, int ROWS>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int pieces_most) {
+// The pieces of every row whose tiles more than one workgroup has, in their order: a wave a row (of a sequence and query head).
+// rows_most: rows that a workgroup's place in the workspace has room for.
+template <int DP>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int pieces_most, int rows_most) {
     const int64_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
     if (at >= a.B * a.Hq) return;
     const int b = static_cast<int>(at / a.Hq), hq = static_cast<int>(at % a.Hq), lane = threadIdx.x & 63;
     const int g = a.plan[SharedPlan::group_at(a.B) + b], rank = a.plan[SharedPlan::rank_at(a.B) + b], n_groups = groups_of(a);
     if (g < 0 || g >= n_groups || rank < 0) return;
-    const Group r = group_of(a, g);
+    const Group r = group_of(a, g), mine = groups_from(a, 0);
     if (r.tokens == 0 || rank >= r.count) return;
     int before;
-    const int total = line_of<ROWS>(a, n_groups, g, &before), piece = (total + pieces_most - 1) / pieces_most;
-    const int group = a.Hq / a.H, h = hq / group, of = rank * group + hq % group, nt = tiles_of(r);
-    const int s0 = before + (h * row_tiles_of<ROWS>(a, r) + of / ROWS) * nt, row = of % ROWS;
+    const int total = line_of(a, mine, n_groups, g, tile_keys(DP), &before), piece = (total + pieces_most - 1) / pieces_most;
+    const int group = a.Hq / a.H, h = hq / group, of = rank * group + hq % group, nt = tiles_of(r, tile_keys(DP));
+    const int s0 = before + (h * row_tiles_of(a, r) + of / kSharedRows) * nt, row = of % kSharedRows;
     const int p0 = s0 / piece, p1 = (s0 + nt - 1) / piece, slots = 2 * pieces_most;
+    if (p0 == p1) return;                               // written by that workgroup
     constexpr int V = DP == 256 ? 4 : DP == 128 ? 2 : 1, kAhead = 8;
     const int d = V * lane;
     float top = kNegInf, sum = 0.0f, y[V];
@@ -231,8 +269,8 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int p
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int x = p + i < p1 ? p + i : p1, slot = 2 * x + (x * piece < s0);
-            st[i] = *reinterpret_cast<const float2*>(part_stat(a, ROWS, slots, slot) + 2 * row);
-            const float* from = part_out(a, ROWS, slot) + row * a.D + (d < a.D ? d : 0);
+            st[i] = *reinterpret_cast<const float2*>(part_stat(a, rows_most, slots, slot) + 2 * row);
+            const float* from = part_out(a, rows_most, slot) + row * a.D + (d < a.D ? d : 0);
 #pragma unroll
             for (int e = 0; e < V; ++e) z[i][e] = from[e];
         }
@@ -260,368 +298,418 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int p
     if (lane == 0) reinterpret_cast<float2*>(a.shared_stat)[at] = make_float2(top, some ? sum : -1.0f);
 }
 
-template <int DP, int DT, bool I8, bool SMALL>
-__global__ void __launch_bounds__(64 * kSharedWaves, 1) attn_shared_kernel(AttnArgs a, bool quads) {
-    constexpr int RT = rows16_of(DP), kTileRows = 16 * RT;
-    constexpr int kWaves = kSharedWaves, kTile = kSharedTile;
-    constexpr int E = I8 ? 1 : 2;
-    constexpr int VE = DP / 16;
-    constexpr int kSteps = DP / 32;
-    constexpr int KB = 16;
-    constexpr int KL = DP * E / 4 / KB;
-    constexpr bool kSplit = I8 && DT == kDtF16;
-    constexpr int MT = I8 ? kDtBf16 : DT;
-    constexpr float kLift = MT == kDtF16 ? 14.0f - 8.0f : 0.0f;     // of fp16 probabilities; kSlack below what they may reach
-    constexpr float kShift = MT == kDtF16 ? 8.0f : 0.0f;            // what the single-token kernel lifts them by beyond that
-    constexpr float kSlack = 8.0f;
-    __shared__ float sm_out[kWaves][16][DP + 4];
-    __shared__ float sm_m[kWaves][kTileRows], sm_l[kWaves][kTileRows];
-    __shared__ int sm_any[kWaves];
-    // the query rows, as the products take them: [row tile][step][lane]
-    __shared__ Frag sm_q[RT][kSteps][64], sm_q2[kSplit ? RT : 1][kSplit ? kSteps : 1][64];
+template <int DP, bool I8>
+struct __attribute__((aligned(16))) SharedLds {
+    static constexpr int kTile = tile_keys(DP), kRing = tiles_ahead(DP) + 1, kWide = I8 ? 2 : kRing, kPages = DP == 64 ? 16 : 8;
+    uint16_t k[kWide][kTile * DP], v[kWide][kTile * DP];    // tiles of 16 bits, chunks of 8 values in the order kswap and vswap
+    int8_t kr[I8 ? kRing : 1][I8 ? kTile * DP : 16], vr[I8 ? kRing : 1][I8 ? kTile * DP : 16];  // int8 caches: as they come
+    float scale[I8 ? kRing : 1][2][64];
+    int page[tile_waves(DP)][kPages][64];    // a wave's own: where a tile's keys are
+};
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int group = a.Hq / a.H;
-    const int B = static_cast<int>(a.B);
+// 4 bytes per active lane from `src` to LDS bytes dst + 4 lane; loads on their way, up to N of a wave's newest
+__device__ __forceinline__ void load_lds4(const void* src, uint32_t dst) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_but() {
+    static_assert(N >= 0 && N < 64);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// (__syncthreads without a wait for loads that are meant to be on their way)
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache. rows_most: as above.
+template <int DP, int DT, bool I8>
+__global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(AttnArgs a, int rows_most) {
+    using Lds = SharedLds<DP, I8>;
+    constexpr int E = I8 ? 1 : 2, kTile = Lds::kTile, kRing = Lds::kRing, kAhead = kRing - 1, kPages = Lds::kPages, kThreads = 64 * tile_waves(DP);
+    static_assert(kPages >= 2 * kRing - 1);
+    constexpr bool kSplit = I8 && DT == kDtF16;         // fp16 rows against int8 keys: bf16 products of hi + lo
+    constexpr int MT = I8 ? kDtBf16 : DT;               // type of the products
+    constexpr float kSlack = 8.0f;                      // how far a row's maximum may pass its reference (log2)
+    constexpr float kLift = MT == kDtF16 ? 6.0f : 0.0f; // fp16 probabilities are held 2^6 times as large, ...
+    constexpr float kShift = MT == kDtF16 ? 8.0f : 0.0f;    // ... by 2^8 less than in the single-token kernel, which adds these
+    constexpr int kSteps = DP / 16;                     // products over the width
+    constexpr int kBlocks = DP / 32;                    // value blocks of the output
+    constexpr int kV = 16 / E;                          // values of a 16-byte chunk in the cache
+    constexpr int kPerKey = DP / kV;                    // chunks per key
+    constexpr int KC = kTile * kPerKey / kThreads;           // chunks of keys (and of values) that a thread brings
+    static_assert(KC > 0);
+    constexpr int kLoads = 2 * KC + (I8 ? 1 : 0) + 1;   // a wave's loads for a tile: chunks, scales, pages of a later one
+    extern __shared__ char lds_raw[];
+    Lds& sm = *reinterpret_cast<Lds*>(lds_raw);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = lane & 31, hf = lane >> 5;
+    const int group = a.Hq / a.H, B = static_cast<int>(a.B);
+    const Group first = groups_from(a, 0);
     const int n_groups = groups_of(a);
     int front;
-    const int total = line_of<kTileRows>(a, n_groups, 0, &front);
+    const int total = line_of(a, first, n_groups, 0, kTile, &front);
     const int piece = (total + gridDim.x - 1) / gridDim.x;
     const int t0 = blockIdx.x * piece, t1 = t0 + piece < total ? t0 + piece : total;
     if (t0 >= t1) return;
-
     const int mask = (1 << a.page_shift) - 1;
-    const int last_page = static_cast<int>(a.pages) - 1;
-    const uint32_t tok = static_cast<uint32_t>(a.c_token) * E;
-    uint32_t ko[KL], vo[4];
-#pragma unroll
-    for (int x = 0; x < KL; ++x) ko[x] = (SMALL ? 0 : c * tok) + (KB / E * (4 * x + g) < a.D ? KB * (4 * x + g) : 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vo[r] = (SMALL ? 0 : (4 * g + r) * tok) + (VE * c < a.D ? VE * E * c : 0);
-    const float scale = a.scale * kLog2e;
+    auto kswap = [](int key) { return key & 7; };
+    auto vswap = [](int key) { return DP == 64 ? 4 * (key >> 1 & 1) : 4 * (key & 3); };
+    const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_offset(I8 ? (const void*)sm.kr : (const void*)sm.k) + wave * 1024);
+    const uint32_t lds_v = __builtin_amdgcn_readfirstlane(lds_offset(I8 ? (const void*)sm.vr : (const void*)sm.v) + wave * 1024);
+    const uint32_t lds_scale = __builtin_amdgcn_readfirstlane(lds_offset(sm.scale) + (wave & 1) * 256);
+    const uint32_t lds_page = __builtin_amdgcn_readfirstlane(lds_offset(sm.page[wave]));
+    const float size = __builtin_fabsf(a.scale * kLog2e), scale = size < 0x1p-100f ? 0x1p-100f : size;   // (0 times -infinity)
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    auto clear = [&] {                                  // what no load writes: keys and values beyond the heads' width
+        if (!I8 && DP > a.D)
+            for (int e = tid; e < Lds::kWide * kTile * DP / 8; e += kThreads) {
+                reinterpret_cast<uint4*>(sm.k)[e] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sm.v)[e] = make_uint4(0, 0, 0, 0);
+            }
+    };
+    clear();
 
-    int gi = 0, before = 0;
     for (int t = t0; t < t1;) {
-        // the segment: tiles i0 .. i1 - 1 of group gi's cache head and row tile, whose tile 0 is place s0
-        Group r = group_of(a, gi);      // (uniform: the plan is read at the same place by all lanes)
-        while (t - before >= tiles_of(r) * row_tiles_of<kTileRows>(a, r) * a.H) {
-            before += tiles_of(r) * row_tiles_of<kTileRows>(a, r) * a.H;
-            ++gi;
-            r = group_of(a, gi);
-        }
-        const int nt = tiles_of(r), pair = (t - before) / nt;
+        // the segment: tiles i0 .. i1 - 1 of a group's cache head and row tile, whose tile 0 is place s0
+        int before;
+        const Group r = group_at_place(a, first, n_groups, t, kTile, &before);
+        const int nt = tiles_of(r, kTile), pair = (t - before) / nt;
         const int s0 = before + pair * nt;
         const int i0 = t - s0, i1 = t1 - s0 < nt ? t1 - s0 : nt;
-        const int rtiles = row_tiles_of<kTileRows>(a, r);
-        const int h = pair / rtiles, row0 = pair % rtiles * kTileRows;
-        const int rows = r.count * group - row0 < kTileRows ? r.count * group - row0 : kTileRows;
+        const int rtiles = row_tiles_of(a, r);
+        const int h = pair / rtiles, row0 = pair % rtiles * kSharedRows;
+        const int rows = r.count * group - row0 < kSharedRows ? r.count * group - row0 : kSharedRows;
         const int* table = a.table + static_cast<int64_t>(r.lead) * a.ld_table;
         const char* kbase = static_cast<const char*>(a.kc) + static_cast<int64_t>(h) * a.c_head * E;
         const char* vbase = static_cast<const char*>(a.vc) + static_cast<int64_t>(h) * a.c_head * E;
-        const float* ksb = I8 ? a.k_scale + h * a.s_head : nullptr;
-        const float* vsb = I8 ? a.v_scale + h * a.s_head : nullptr;
-        const int last = r.tokens - 1;
-        // row x of the tile: its sequence (-1: none of the batch) and query head
-        auto row_of = [&](int x, int* seq, int* hq) {
-            const int at = row0 + x;
-            const int s = a.plan[SharedPlan::members(a.B) + r.first + at / group];
-            *seq = s >= 0 && s < B ? s : -1;
-            *hq = h * group + at % group;
-        };
+        const float* sbase = (wave & 1 ? a.v_scale : a.k_scale) + static_cast<int64_t>(h) * a.s_head;
+        const uint32_t last = static_cast<uint32_t>(r.tokens) - 1;   // (no further than the table: group_of)
 
-        for (int x = wave; x < RT; x += kWaves) {
-            int seq = -1, hq = 0;
-            if (16 * x + c < rows) row_of(16 * x + c, &seq, &hq);
-            const uint16_t* row = static_cast<const uint16_t*>(a.q) + (seq < 0 ? 0 : seq) * a.q_token + hq * a.q_head;
+        const uint32_t pages = static_cast<uint32_t>(a.pages);
+
+        // Where tile i's keys are, into the wave's own list
+        auto look_up = [&](int i) __attribute__((always_inline)) {
+            const uint32_t at = (static_cast<uint32_t>(i) * kTile + lane) >> a.page_shift, most = static_cast<uint32_t>(a.width) - 1;
+            load_lds4(table + (at < most ? at : most), lds_page + (i & (kPages - 1)) * 256);
+        };
+        // key x of tile i: its page, or -1
+        auto page_of = [&](int i, int x) __attribute__((always_inline)) {
+            const int p = sm.page[wave][i & (kPages - 1)][x];
+            return (i < i1) & (static_cast<uint32_t>(i) * kTile + x <= last) & (static_cast<uint32_t>(p) < pages) ? p : -1;
+        };
+        // Tile i on its way to ring place i % kRing (a key that is not held: the cache's first). 16-bit caches: 16-byte chunk c of
+        // key x at c ^ kswap(x) and c ^ vswap(x)
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const uint32_t place = static_cast<uint32_t>(i & (kRing - 1)) * kTile * DP * E;
+            int64_t at[KC];
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const int d = I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-                uint4 y = make_uint4(0, 0, 0, 0);
-                if (seq >= 0 && d < a.D) y = *reinterpret_cast<const uint4*>(row + d);
-                Frag q{{y.x, y.y, y.z, y.w}};
-                if constexpr (kSplit) {
-                    Frag q2;
+            for (int x = 0; x < KC; ++x) {
+                const int key = tid / kPerKey + kThreads / kPerKey * x, p = page_of(i, key);
+                at[x] = p < 0 ? 0 : static_cast<int64_t>(p) * a.c_page + ((static_cast<uint32_t>(i) * kTile + key) & mask) * a.c_token;
+            }
+            const int slot = tid % kPerKey, key0 = tid / kPerKey;       // (the order is the same for all of a thread's keys)
+            const int kc = I8 ? slot : slot ^ kswap(key0), vc = I8 ? slot : slot ^ vswap(key0);
+            if (kV * kc < a.D)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) split_f16(q.w[j], &q.w[j], &q2.w[j]);
-                    sm_q2[x][s][lane] = q2;
+                for (int x = 0; x < KC; ++x) load_lds16(kbase + at[x] * E + 16 * kc, lds_k + place + 16 * kThreads * x);
+            if (kV * vc < a.D)
+#pragma unroll
+                for (int x = 0; x < KC; ++x) load_lds16(vbase + at[x] * E + 16 * vc, lds_v + place + 16 * kThreads * x);
+            if constexpr (I8) {
+                if (lane < kTile) {
+                    const int p = page_of(i, lane);
+                    load_lds4(sbase + (p < 0 ? 0 : static_cast<int64_t>(p) * a.s_page + ((static_cast<uint32_t>(i) * kTile + lane) & mask) * a.s_token),
+                              lds_scale + (i & (kRing - 1)) * 512);
                 }
-                sm_q[x][s][lane] = q;
+            }
+            look_up(i + kAhead);
+        };
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) look_up(i0 + x);
+
+        // a wave's rows, and the 32 keys of a tile that it takes: eight waves take one half each, and so do four for few rows
+        const bool few = kTile == 64 && rows <= kSharedRows / 2, split = kTile == 64 && (few || kThreads == 512);
+        const int blocks = few ? 2 : 4, block = wave & (blocks - 1), part = wave / blocks;
+        const int u0 = split ? part : 0, u1 = split ? part + 1 : kTile / 32, row = block * 32 + q;
+        const bool active = block * 32 < rows && part < 2;
+        // this lane's row: its sequence (-1: none) and query head
+        int seq = -1, hq = 0;
+        if (row < rows) {
+            const int at = row0 + row;
+            seq = a.plan[SharedPlan::members(a.B) + r.first + at / group];
+            seq = seq >= 0 && seq < B ? seq : -1;
+            hq = h * group + at % group;
+        }
+        Frag qf[kSteps], qf2[kSplit ? kSteps : 1];
+        const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + (seq < 0 ? 0 : seq) * a.q_token + hq * a.q_head;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int d = 16 * s + 8 * hf;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (seq >= 0 && d < a.D) x = *reinterpret_cast<const uint4*>(qrow + d);
+            qf[s] = Frag{{x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign}};
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_f16(qf[s].w[j], &qf[s].w[j], &qf2[s].w[j]);
             }
         }
-        __syncthreads();
+        // (The rows are here before the first tiles are sent for: a wait for them behind that would be one for all of those.)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(qf[s].w[0]), "+v"(qf[s].w[1]), "+v"(qf[s].w[2]), "+v"(qf[s].w[3]));
+        f32x16 o[kBlocks];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[i][x] = 0.0f;
+        float m = kNegInf, l = 0.0f;                    // reference maximum (of the scaled scores), sum of the lane's keys
+        bool any = false;
 
-        Raw<KB> kr[2][2][KL];
-        Raw<VE * E> vr[2][8];
-        float ksc[2][2][4], vsc[2][2][4];
-        uint32_t held[2];
-        auto first_key = [&](int i) { return i * kTile + wave * kKeys; };
-        // the 32 keys from j on: every address is inside the cache (a key that is not held reads page 0)
-        auto load = [&](int buf, int j) __attribute__((always_inline)) {
-            held[buf] = 0;
-            const int ne = static_cast<int>(a.width) - 1;
-            if constexpr (!SMALL) {
+        // 16-bit caches: this thread's own values of tile i whose keys are hidden: 0 (what is there may be an infinity)
+        auto hide_own = [&](int i, uint64_t held) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int at = (j + 16 * u) >> a.page_shift;
-                    const int p = scalar_word(table + __builtin_amdgcn_readfirstlane(at < ne ? at : ne));
-                    const bool ok = p >= 0 && p <= last_page && at <= ne;
-                    held[buf] |= ok ? 0xffffu << (16 * u) : 0u;
-                    const int pg = ok ? p : 0, slot = (j + 16 * u) & mask;
-                    const int64_t off = (pg * a.c_page + slot * a.c_token) * E;
-                    const char* kp = kbase + off;
-                    const char* vp = vbase + off;
+            for (int x = 0; x < KC; ++x)
+                if (!(held >> (tid / kPerKey + kThreads / kPerKey * x) & 1))
+                    reinterpret_cast<uint4*>(sm.v[i & (kRing - 1)])[tid + kThreads * x] = make_uint4(0, 0, 0, 0);
+        };
+        // int8 caches: this thread's own chunks of tile i in 16 bits
+        auto widen = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
+            for (int x = 0; x < KC; ++x) {
+                const int e = tid + kThreads * x, key = e / kPerKey, c = e % kPerKey;
+                uint4 y[2] = {reinterpret_cast<const uint4*>(sm.kr[I8 ? i & (kRing - 1) : 0])[e],
+                              reinterpret_cast<const uint4*>(sm.vr[I8 ? i & (kRing - 1) : 0])[e]};
+                if (kV * c >= a.D) y[0] = y[1] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) vr[buf][4 * u + y] = load_row<VE * E, E>(vp, vo[y], VE * c, a.D);
-                    if constexpr (I8) {
-                        const int64_t so = pg * a.s_page + slot * a.s_token;
-                        if (quads) {
-                            const float4 x = *reinterpret_cast<const float4*>(ksb + so + 4 * g);
-                            const float4 y = *reinterpret_cast<const float4*>(vsb + so + 4 * g);
-                            ksc[buf][u][0] = x.x; ksc[buf][u][1] = x.y; ksc[buf][u][2] = x.z; ksc[buf][u][3] = x.w;
-                            vsc[buf][u][0] = y.x; vsc[buf][u][1] = y.y; vsc[buf][u][2] = y.z; vsc[buf][u][3] = y.w;
-                        } else {
+                for (int z = 0; z < 2; ++z) {
+                    float f[4][4];
+                    i8x4(y[z].x, f[0]);
+                    i8x4(y[z].y, f[1]);
+                    i8x4(y[z].z, f[2]);
+                    i8x4(y[z].w, f[3]);
+                    uint16_t* to = (z ? sm.v[i & 1] : sm.k[i & 1]) + key * DP;
+                    const int swap = z ? vswap(key) : kswap(key);
 #pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                ksc[buf][u][y] = ksb[so + (4 * g + y) * a.s_token];
-                                vsc[buf][u][y] = vsb[so + (4 * g + y) * a.s_token];
-                            }
-                        }
-                    }
-                }
-            } else {
-                const int mine = j + (lane & 31), at = mine >> a.page_shift;
-                const int p = table[at < ne ? at : ne];
-                const bool ok = p >= 0 && p <= last_page && at <= ne;
-                held[buf] = static_cast<uint32_t>(__ballot(ok));
-                const int code = ok ? (p << a.page_shift) | (mine & mask) : 0;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int ck = __shfl(code, 16 * u + c);
-                    const char* kp = kbase + (static_cast<int64_t>(ck >> a.page_shift) * a.c_page + (ck & mask) * a.c_token) * E;
-#pragma unroll
-                    for (int x = 0; x < KL; ++x) kr[buf][u][x] = load_raw<KB>(kp + ko[x]);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const int cv = __shfl(code, 16 * u + 4 * g + y);
-                        const int64_t pg = cv >> a.page_shift, slot = cv & mask;
-                        vr[buf][4 * u + y] = load_row<VE * E, E>(vbase + (pg * a.c_page + slot * a.c_token) * E, vo[y], VE * c, a.D);
-                        if constexpr (I8) {
-                            ksc[buf][u][y] = ksb[pg * a.s_page + slot * a.s_token];
-                            vsc[buf][u][y] = vsb[pg * a.s_page + slot * a.s_token];
-                        }
-                    }
+                    for (int w = 0; w < 2; ++w)
+                        *reinterpret_cast<uint4*>(to + 8 * ((2 * c + w) ^ swap)) =
+                            make_uint4(bf16_exact2(f[2 * w][0], f[2 * w][1]), bf16_exact2(f[2 * w][2], f[2 * w][3]),
+                                       bf16_exact2(f[2 * w + 1][0], f[2 * w + 1][1]), bf16_exact2(f[2 * w + 1][2], f[2 * w + 1][3]));
                 }
             }
         };
-        f32x4 o[RT][VE];
-        float m[RT], l[RT];
+        // a lane's places in the LDS rows (as in mq_attn_prompt.hip)
+        const int kx = hf ^ (q & 7), vn = lane & 15;
+        auto v_frag = [&](int buf, int u, int i, int x) __attribute__((always_inline)) {
+            const int at = 4 * hf + (vn >> 2);
+            const uint32_t base = lds_offset(sm.v[0]) + buf * kTile * DP * 2 + (32 * u + at) * DP * 2 +
+                                  16 * ((4 * (i & 3)) ^ vswap(at)) + 32 * (lane >> 4 & 1) + 8 * (vn & 3);
+            const LdsShort4 p = (LdsShort4)(base) + (256 * (i >> 2) + 16 * x * DP * 2) / 8;
+            const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+            const auto z = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p + DP * 2);
+            const uint2 yw = __builtin_bit_cast(uint2, y), zw = __builtin_bit_cast(uint2, z);
+            return Frag{{yw.x, yw.y, zw.x, zw.y}};
+        };
+        // keys 32 u .. 32 u + 31 of the tile
+        auto work = [&](int buf, int ring, uint64_t held_all, int u) __attribute__((always_inline)) {
+            const uint32_t held = static_cast<uint32_t>(held_all >> (32 * u));
+            if (held == 0) return;
+            any = true;
+            // (All of the keys are sent for before the first product, and the values before the softmax: an LDS read takes as long
+            // as four products, and a wave has only one other beside it.)
+            const char* krow = reinterpret_cast<const char*>(sm.k[buf]) + (32 * u + q) * DP * 2;
+            Frag k[kSteps];
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-            m[x] = kNegInf;
-            l[x] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) o[x][i] = f32x4{0, 0, 0, 0};
-        }
-        bool any = false;           // a key that is held (the same for all rows)
-        auto work = [&](int buf, int j) __attribute__((always_inline)) {
-            const bool whole = held[buf] == 0xffffffffu && j + kKeys - 1 <= last;
-            uint32_t see = 0xffu;
-            if (!whole) {
-                see = 0;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const int at = 16 * (x >> 2) + 4 * g + (x & 3);
-                    see |= ((held[buf] >> at) & 1) && j + at <= last ? 1u << x : 0u;
-                }
+            for (int st = 0; st < kSteps; ++st) {
+                const uint4 x = *reinterpret_cast<const uint4*>(krow + 16 * ((2 * (st & 3)) ^ kx) + (st >> 2) * 128);
+                k[st] = Frag{{x.x, x.y, x.z, x.w}};
             }
-            any = any || whole || __ballot(see != 0) != 0;
-            Frag k[2][kSteps];
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 s;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int x = 0; x < 16; ++x) s[x] = 0.0f;
 #pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    if constexpr (I8) {
-                        float f0[4], f1[4];
-                        i8x4(kr[buf][u][st >> 1].w[2 * (st & 1)], f0);
-                        i8x4(kr[buf][u][st >> 1].w[2 * (st & 1) + 1], f1);
-                        k[u][st] = Frag{{bf16_exact2(f0[0], f0[1]), bf16_exact2(f0[2], f0[3]), bf16_exact2(f1[0], f1[1]),
-                                         bf16_exact2(f1[2], f1[3])}};
-                    } else {
-                        k[u][st] = Frag{{kr[buf][u][st].w[0], kr[buf][u][st].w[1], kr[buf][u][st].w[2], kr[buf][u][st].w[3]}};
-                    }
-                    const int d = I8 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1) : 32 * st + 8 * g;
-                    if (d >= a.D) k[u][st] = Frag{{0, 0, 0, 0}};
-                }
-            Frag pf[RT], pf2[kSplit ? RT : 1];
-#pragma unroll
-            for (int x = 0; x < RT; ++x) {
-                float p[8];
-                // (read here every time: kept from tile to tile, all rows' would push others out of the registers)
-                asm volatile("" ::: "memory");
-                Frag q[kSteps], q2[kSplit ? kSteps : 1];
-#pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    q[st] = sm_q[x][st][lane];
-                    if constexpr (kSplit) q2[st] = sm_q2[x][st][lane];
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f32x4 s = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        s = mfma16<MT>(k[u][st], q[st], s);
-                        if constexpr (kSplit) s = mfma16<MT>(k[u][st], q2[st], s);
-                    }
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) p[4 * u + y] = s[y] * scale * (I8 ? ksc[buf][u][y] : 1.0f);
-                }
-                if (!whole)
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) p[y] = (see >> y) & 1 ? p[y] : kNegInf;
-                float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3])),
-                                            __builtin_fmaxf(__builtin_fmaxf(p[4], p[5]), __builtin_fmaxf(p[6], p[7])));
-                top = max4(top);
-                const bool move = top > m[x] + kSlack;
-                if (__ballot(move)) {
-                    const float f = move ? __builtin_amdgcn_exp2f(m[x] - top) : 1.0f;
-                    m[x] = move ? top : m[x];
-                    l[x] *= f;
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) o[x][i] *= f;
-                }
-                const float base = m[x] == kNegInf ? 0.0f : m[x];
-#pragma unroll
-                for (int y = 0; y < 8; ++y) p[y] = __builtin_amdgcn_exp2f(p[y] - base + kLift);
-                l[x] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                if constexpr (I8) {
-#pragma unroll
-                    for (int y = 0; y < 8; ++y)         // a key that is not seen has weight 0 whatever its scale holds
-                        p[y] = (see >> y) & 1 ? p[y] * vsc[buf][y >> 2][y & 3] : 0.0f;
-                }
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    pf[x].w[y] = pack_16x2(p[2 * y], p[2 * y + 1], MT);
-                    if constexpr (kSplit)
-                        pf2[x].w[y] = pack_16x2(p[2 * y] - bf16lo(pf[x].w[y]), p[2 * y + 1] - bf16hi(pf[x].w[y]), MT);
-                }
+            for (int st = 0; st < kSteps; ++st) {
+                s = mfma32<MT>(k[st], qf[st], s);
+                if constexpr (kSplit) s = mfma32<MT>(k[st], qf2[st], s);
             }
-            if (!I8 && !whole) {        // 0 times an infinity or NaN: values that are not seen become 0
+            Frag v[kBlocks][2];
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
+            for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                    for (int e = 0; e < VE * E / 4; ++e) vr[buf][x].w[e] = (see >> x) & 1 ? vr[buf][x].w[e] : 0u;
-            }
+                for (int x = 0; x < 2; ++x) v[i][x] = v_frag(buf, u, i, x);
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (I8) {
 #pragma unroll
-                for (int w = 0; w < VE / 4; ++w) {
-                    float f8[8][4];
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const float4 x = *reinterpret_cast<const float4*>(&sm.scale[ring][0][32 * u + 8 * r4 + 4 * hf]);
+                    s[4 * r4] *= x.x;
+                    s[4 * r4 + 1] *= x.y;
+                    s[4 * r4 + 2] *= x.z;
+                    s[4 * r4 + 3] *= x.w;
+                }
+            }
+            const uint32_t see = held >> (4 * hf);          // bit 8 (x / 4) + x % 4: that key is seen (by every row)
+            if (held != 0xffffffffu) {
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) i8x4(vr[buf][x].w[w], f8[x]);
+                for (int x = 0; x < 16; ++x) s[x] = (see >> (8 * (x >> 2) + (x & 3))) & 1 ? s[x] : kNegInf;
+            }
+            float top = kNegInf;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        Frag v;
+            for (int x = 0; x < 16; ++x) top = __builtin_fmaxf(top, s[x]);
+            top = max2(top) * scale;
+            const bool move = top > m + kSlack;
+            if (__ballot(move)) {
+                const float f = move ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+                m = move ? top : m;
+                l *= f;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) v.w[x] = bf16_exact2(f8[2 * x][i], f8[2 * x + 1][i]);
+                for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                        for (int x = 0; x < RT; ++x) {
-                            o[x][4 * w + i] = mfma16<MT>(v, pf[x], o[x][4 * w + i]);
-                            if constexpr (kSplit) o[x][4 * w + i] = mfma16<MT>(v, pf2[x], o[x][4 * w + i]);
+                    for (int x = 0; x < 16; ++x) o[i][x] *= f;
+            }
+            const float base = kLift - (m == kNegInf ? 0.0f : m);
+            float sum[4] = {0, 0, 0, 0};
+            Frag p[2], p2[kSplit ? 2 : 1];
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                float e[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    e[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * r4 + x], scale, base));
+                    sum[x] += e[x];
+                }
+                if constexpr (I8) {
+                    const float4 x = *reinterpret_cast<const float4*>(&sm.scale[ring][1][32 * u + 8 * r4 + 4 * hf]);
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) e[y] *= xs[y];
+                    if (held != 0xffffffffu)            // (0 times whatever a hidden key's scale is)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) e[y] = (see >> (8 * r4 + y)) & 1 ? e[y] : 0.0f;
+                }
+                const int x = r4 >> 1, w = 2 * (r4 & 1);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    p[x].w[w + y] = pack_16x2(e[2 * y], e[2 * y + 1], MT);
+                    if constexpr (kSplit)
+                        p2[x].w[w + y] = pack_16x2(e[2 * y] - bf16lo(p[x].w[w + y]), e[2 * y + 1] - bf16hi(p[x].w[w + y]), MT);
+                }
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    o[i] = mfma32<MT>(v[i][x], p[x], o[i]);
+                    if constexpr (kSplit) o[i] = mfma32<MT>(v[i][x], p2[x], o[i]);
+                }
+        };
+
+        // kAhead tiles are on their way while one is worked on. A tile's place in the ring is loaded again behind the barrier that
+        // every wave reaches only when it is through with it, and each wave waits for its own loads in front of the barrier that the
+        // others read them behind.
+        wait_but<0>();
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) fetch(i0 + x);
+        for (int i = i0; i < i1; ++i) {
+            wait_but<(kAhead - 1) * kLoads>();
+            const uint64_t held = __ballot(page_of(i, lane) >= 0) & (~uint64_t(0) >> (64 - kTile));
+            if constexpr (I8) widen(i);
+            else if (held != ~uint64_t(0) >> (64 - kTile)) hide_own(i, held);
+            barrier_lds();
+            fetch(i + kAhead);
+            if (active)
+#pragma unroll 1
+                for (int u = u0; u < u1; ++u) work(I8 ? i & 1 : i & (kRing - 1), i & (kRing - 1), held, u);
+        }
+        wait_but<0>();
+        barrier_lds();
+        l = sum2(l);
+        // a row's two parts together, the second's through LDS where the tiles were
+        if (split) {
+            constexpr int kRow = DP + 4;                // (rows begin 4 banks apart)
+            float* sm_o = reinterpret_cast<float*>(lds_raw) + row * kRow;
+            float2* sm_m = reinterpret_cast<float2*>(reinterpret_cast<float*>(lds_raw) + kSharedRows * kRow) + row;
+            if (part == 1) {
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4)
+                        *reinterpret_cast<float4*>(sm_o + 32 * i + 8 * r4 + 4 * hf) =
+                            make_float4(o[i][4 * r4], o[i][4 * r4 + 1], o[i][4 * r4 + 2], o[i][4 * r4 + 3]);
+                if (hf == 0) *sm_m = make_float2(m, any ? l : -1.0f);
+            }
+            __syncthreads();
+            if (part == 0) {
+                const float2 other = *sm_m;
+                if (!(other.y == -1.0f)) {              // (of a part that saw nothing: sums of 0, a maximum of -infinity)
+                    const float top = __builtin_fmaxf(m, other.x), ref = top == kNegInf ? 0.0f : top;
+                    const float f = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(other.x - ref);
+                    m = top;
+                    l = l * f + other.y * f1;
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i) {
+                        float4 y[4];
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) y[r4] = *reinterpret_cast<const float4*>(sm_o + 32 * i + 8 * r4 + 4 * hf);
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            o[i][4 * r4] = o[i][4 * r4] * f + y[r4].x * f1;
+                            o[i][4 * r4 + 1] = o[i][4 * r4 + 1] * f + y[r4].y * f1;
+                            o[i][4 * r4 + 2] = o[i][4 * r4 + 2] * f + y[r4].z * f1;
+                            o[i][4 * r4 + 3] = o[i][4 * r4 + 3] * f + y[r4].w * f1;
                         }
                     }
+                    any = true;
                 }
-            } else {
+            }
+        }
+        if (part == 0 && row < rows) {
+            const bool complete = i0 == 0 && i1 == nt;
+            const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < s0);
+            const int64_t at = static_cast<int64_t>(seq < 0 ? 0 : seq) * a.Hq + hq;
+            float* to = complete ? a.shared_out + at * a.D : part_out(a, rows_most, slot) + static_cast<int64_t>(row) * a.D;
+            float* stat = complete ? a.shared_stat + 2 * at : part_stat(a, rows_most, slots, slot) + 2 * row;
+            if (seq >= 0 || !complete) {
 #pragma unroll
-                for (int w = 0; w < VE / 2; ++w) {
-                    Frag v0, v1;
+                for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        v0.w[x] = pair16<0>(vr[buf][2 * x].w[w], vr[buf][2 * x + 1].w[w]);
-                        v1.w[x] = pair16<1>(vr[buf][2 * x].w[w], vr[buf][2 * x + 1].w[w]);
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const int d = 32 * i + 8 * r4 + 4 * hf;
+                        if (d < a.D)
+                            *reinterpret_cast<float4*>(to + d) = make_float4(o[i][4 * r4], o[i][4 * r4 + 1], o[i][4 * r4 + 2], o[i][4 * r4 + 3]);
                     }
-#pragma unroll
-                    for (int x = 0; x < RT; ++x) {
-                        o[x][2 * w] = mfma16<MT>(v0, pf[x], o[x][2 * w]);
-                        o[x][2 * w + 1] = mfma16<MT>(v1, pf[x], o[x][2 * w + 1]);
-                    }
-                }
-            }
-        };
-        load(0, first_key(i0));
-        int i = i0;
-        for (; i + 1 < i1; i += 2) {
-            load(1, first_key(i + 1));
-            work(0, first_key(i));
-            if (i + 2 < i1) load(0, first_key(i + 2));
-            work(1, first_key(i + 1));
-        }
-        if (i < i1) work(0, first_key(i));
-
-        // the waves' parts together, 16 rows at a time: rows c, values VE (4 g + y) + e
-        const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < s0);
-        if (lane == 0) sm_any[wave] = any;
-#pragma unroll
-        for (int x = 0; x < RT; ++x) {
-            const float sum = sum4(l[x]);
-            if (g == 0) {
-                sm_m[wave][16 * x + c] = m[x];
-                sm_l[wave][16 * x + c] = sum;
+                if (hf == 0) *reinterpret_cast<float2*>(stat) = make_float2(m + kShift, any ? l : -1.0f);
             }
         }
-#pragma unroll
-        for (int x = 0; x < RT; ++x) {
-            __syncthreads();
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) sm_out[wave][c][VE * (4 * g + y) + e] = o[x][e][y];
-            __syncthreads();
-            int some = 0;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) some |= sm_any[w];
-            for (int e = threadIdx.x; e < 16 * DP / 4; e += 64 * kWaves) {
-                const int row = 16 * x + e / (DP / 4), d = 4 * (e % (DP / 4));
-                if (row >= rows || d >= a.D) continue;
-                float top = kNegInf;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) top = __builtin_fmaxf(top, sm_m[w][row]);
-                const float base = top == kNegInf ? 0.0f : top;
-                float sum = 0.0f, y[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(sm_m[w][row] - base);
-                    sum += f * sm_l[w][row];
-                    const float4 z = *reinterpret_cast<const float4*>(&sm_out[w][row & 15][d]);
-                    y[0] = __builtin_fmaf(f, z.x, y[0]);
-                    y[1] = __builtin_fmaf(f, z.y, y[1]);
-                    y[2] = __builtin_fmaf(f, z.z, y[2]);
-                    y[3] = __builtin_fmaf(f, z.w, y[3]);
-                }
-                float* to = part_out(a, kTileRows, slot) + row * a.D + d;
-                *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
-                if (d == 0)
-                    *reinterpret_cast<float2*>(part_stat(a, kTileRows, slots, slot) + 2 * row) = make_float2(top + kShift, some ? sum : -1.0f);
-            }
-        }
-        __syncthreads();                                // what is in LDS has been read
         t = s0 + i1;
+        if (t < t1) {
+            __syncthreads();                            // what is in LDS has been read
+            if (split) clear();                           // (over the part that was there)
+        }
     }
+}
+
+// Rows of a workgroup's place in the workspace: no tile has more.
+int rows_most_of(int Hq, int H, int64_t B) {
+    const int64_t rows = B * (Hq / H);
+    return static_cast<int>(rows < kSharedRows ? rows : kSharedRows);
 }
 
 template <int DP, int DT, bool I8>
 int shared_width(const AttnArgs& a, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(decode_groups()));
-    const bool quads = I8 && a.s_token == 1 && a.s_page % 4 == 0 && a.s_head % 4 == 0 &&
-                       (reinterpret_cast<uintptr_t>(a.k_scale) | reinterpret_cast<uintptr_t>(a.v_scale)) % 16 == 0;
-    if (a.page_shift >= 4)
-        hipLaunchKernelGGL((attn_shared_kernel<DP, DT, I8, false>), grid, dim3(64 * kSharedWaves), 0, stream, a, quads);
-    else
-        hipLaunchKernelGGL((attn_shared_kernel<DP, DT, I8, true>), grid, dim3(64 * kSharedWaves), 0, stream, a, quads);
+    const int groups = decode_groups(), rows_most = rows_most_of(a.Hq, a.H, a.B);
+    const size_t lds = sizeof(SharedLds<DP, I8>);
+    static_assert(sizeof(SharedLds<DP, I8>) <= 160 * 1024 && sizeof(SharedLds<DP, I8>) >= sizeof(float) * kSharedRows * (DP + 6));
+    auto kern = attn_shared_kernel<DP, DT, I8>;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(lds)) != hipSuccess) {
+        (void)hipGetLastError();
+        set_error("paged_attention_shared: cannot reserve %zu bytes of LDS", lds);
+        return -3;
+    }
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(groups)), dim3(64 * tile_waves(DP)), lds, stream, a, rows_most);
     const int64_t rows = a.B * a.Hq;
-    hipLaunchKernelGGL((attn_shared_join_kernel<DP, 16 * rows16_of(DP)>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream,
-                       a, static_cast<int>(grid.x));
+    hipLaunchKernelGGL((attn_shared_join_kernel<DP>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a, groups, rows_most);
     return launch_status("paged_attention_shared");
 }
 
@@ -632,15 +720,13 @@ int shared_type(const AttnArgs& a, hipStream_t stream) {
     return shared_width<256, DT, I8>(a, stream);
 }
 
-int rows_of(int D) { return 16 * rows16_of(D <= 64 ? 64 : D <= 128 ? 128 : 256); }
-
-int64_t parts_bytes(int D) { return 2 * static_cast<int64_t>(decode_groups()) * rows_of(D) * (D + 2) * 4; }
+int64_t parts_bytes(int Hq, int H, int D, int64_t B) { return 2 * static_cast<int64_t>(decode_groups()) * rows_most_of(Hq, H, B) * (D + 2) * 4; }
 
 }  // namespace
 
 int64_t attn_shared_workspace_bytes(int Hq, int H, int D, int64_t B) {
     // both kernels' pieces (one behind the other in time), then the shared parts
-    const int64_t single = attn_decode_workspace_bytes(Hq, H, D), parts = parts_bytes(D);
+    const int64_t single = attn_decode_workspace_bytes(Hq, H, D), parts = parts_bytes(Hq, H, D, B);
     return (single > parts ? single : parts) + B * Hq * (D + 2) * 4;
 }
 
@@ -648,7 +734,7 @@ int64_t attn_shared_counters(int Hq, int H, int64_t B) { return attn_decode_coun
 
 int launch_attn_shared(const AttnArgs& args, hipStream_t stream) {
     AttnArgs a = args;
-    const int64_t single = attn_decode_workspace_bytes(a.Hq, a.H, a.D), parts = parts_bytes(a.D);
+    const int64_t single = attn_decode_workspace_bytes(a.Hq, a.H, a.D), parts = parts_bytes(a.Hq, a.H, a.D, a.B);
     a.shared_out = reinterpret_cast<float*>(static_cast<char*>(a.work) + (single > parts ? single : parts));
     a.shared_stat = a.shared_out + a.B * a.Hq * a.D;
     a.start = a.plan + SharedPlan::start();
