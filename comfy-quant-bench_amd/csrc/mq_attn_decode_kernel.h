@@ -205,34 +205,107 @@ __device__ __forceinline__ Raw<BYTES> load_row(const char* row, uint32_t off, in
 }
 
 // SHARED: four values of query row hq of sequence b, unnormalised over maximum m and sum l (`some`: of any key), with
-// the part of the keys that its group shares.
-__device__ __forceinline__ void add_shared(const AttnArgs& a, int b, int hq, int d, float& m, float& l, bool& some, float (&x)[4]) {
-    const int64_t row = static_cast<int64_t>(b) * a.Hq + hq;
-    const float2 st = reinterpret_cast<const float2*>(a.shared_stat)[row];
-    if (st.y < 0.0f) return;                            // nothing seen there
-    const float4 y = *reinterpret_cast<const float4*>(a.shared_out + row * a.D + d);
-    if (!some) {
-        m = st.x;
-        l = st.y;
-        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-        some = true;
-        return;
+// the part of the keys that its group shares. That is whole, or in the pieces of several workgroups of the launch before: slot
+// 2 p of piece p, the first one's as it says; every parts-th is added, from `part` on. (Indexes are clamped, as they may come
+// from a plan that is none.)
+__device__ __forceinline__ void add_shared(const AttnArgs& a, int b, int hq, int d, int part, int parts, float& m, float& l,
+                                           bool& some, float (&x)[4]) {
+    constexpr int kAhead = 8;
+    const int64_t at = static_cast<int64_t>(b) * a.Hq + hq;
+    const int4 rec = reinterpret_cast<const int4*>(a.shared_rows)[at];
+    const float2 st0 = reinterpret_cast<const float2*>(a.shared_stat)[at];
+    const float4 y0 = *reinterpret_cast<const float4*>(a.shared_out + at * a.D + d);
+    const int pieces = static_cast<int>(gridDim.x), first = rec.x > 0 ? rec.x < 2 * pieces ? rec.x : 2 * pieces - 1 : 0;
+    const int p0 = first >> 1, p1 = rec.y < pieces ? rec.y : pieces - 1;
+    const int row = rec.z > 0 ? rec.z < a.shared_most ? rec.z : a.shared_most - 1 : 0;
+    const float* stats = a.shared_parts + static_cast<int64_t>(2 * pieces) * a.shared_most * a.D;
+    if (p1 < 0 && part > 0) return;
+    for (int p = p0 + part; p1 < 0 || p <= p1; p += kAhead * parts) {
+        float2 st[kAhead];
+        float4 y[kAhead];
+        if (p1 < 0) {
+            st[0] = st0;
+            y[0] = y0;
+#pragma unroll
+            for (int i = 1; i < kAhead; ++i) {
+                st[i] = make_float2(kNegInf, -1.0f);
+                y[i] = make_float4(0, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int w = p + i * parts < p1 ? p + i * parts : p1;
+                const int64_t slot = w <= p0 ? first : 2 * w;
+                st[i] = reinterpret_cast<const float2*>(stats)[slot * a.shared_most + row];
+                y[i] = *reinterpret_cast<const float4*>(a.shared_parts + (slot * a.shared_most + row) * a.D + d);
+                if (p + i * parts > p1) st[i].y = -1.0f;
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) top = st[i].y < 0.0f ? top : __builtin_fmaxf(top, st[i].x);
+        const float ref = top == kNegInf ? 0.0f : top, f = some ? __builtin_amdgcn_exp2f(m - ref) : 0.0f;
+        m = top;
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= f;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (st[i].y < 0.0f) continue;               // nothing seen there
+            some = true;
+            const float fi = __builtin_amdgcn_exp2f(st[i].x - ref);
+            l += st[i].y * fi;
+            x[0] += y[i].x * fi;
+            x[1] += y[i].y * fi;
+            x[2] += y[i].z * fi;
+            x[3] += y[i].w * fi;
+        }
+        if (p1 < 0) return;
     }
-    const float top = __builtin_fmaxf(m, st.x), ref = top == kNegInf ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(m - ref), fs = __builtin_amdgcn_exp2f(st.x - ref);
-    m = top;
-    l = l * f + st.y * fs;
-    x[0] = x[0] * f + y.x * fs;
-    x[1] = x[1] * f + y.y * fs;
-    x[2] = x[2] * f + y.z * fs;
-    x[3] = x[3] * f + y.w * fs;
+}
+
+// A part's place in LDS: maximum, sum (-1: nothing seen) and values of each of the threads that share a row's pieces.
+constexpr int shared_threads(int dp) { return 64 * waves_of(dp) > 4 * dp ? 64 * waves_of(dp) : 4 * dp; }
+struct SharedPart {
+    float m, l, x[4];
+};
+
+// SHARED: those of rows hq0 .. hq0 + rows - 1 of sequence b, by all threads; returns how many have a row's four values.
+template <int DP>
+__device__ __forceinline__ int gather_shared(const AttnArgs& a, int b, int hq0, int rows, SharedPart* buf) {
+    constexpr int kQuads = DP / 4, kThreads = 64 * waves_of(DP);
+    const int items = rows * kQuads, parts = items >= kThreads ? 1 : kThreads / items;
+    for (int e = threadIdx.x; e < items * parts; e += kThreads) {
+        const int part = e / items, item = e % items, d = 4 * (item % kQuads);
+        SharedPart y{kNegInf, 0.0f, {0, 0, 0, 0}};
+        bool some = false;
+        if (d < a.D) add_shared(a, b, hq0 + item / kQuads, d, part, parts, y.m, y.l, some, y.x);
+        if (!some) y.l = -1.0f;
+        buf[e] = y;
+    }
+    return parts;
+}
+__device__ __forceinline__ void add_gathered(const SharedPart* buf, int items, int parts, int item, float& m, float& l, bool& some,
+                                             float (&x)[4]) {
+    for (int p = 0; p < parts; ++p) {
+        const SharedPart y = buf[p * items + item];
+        if (y.l < 0.0f) continue;
+        const float top = __builtin_fmaxf(m, y.m), ref = top == kNegInf ? 0.0f : top;
+        const float f = some ? __builtin_amdgcn_exp2f(m - ref) : 0.0f, fy = __builtin_amdgcn_exp2f(y.m - ref);
+        m = top;
+        l = l * f + y.l * fy;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = x[e] * f + y.x[e] * fy;
+        some = true;
+    }
 }
 
 // A split sequence's pieces p0 .. p1 together, for the query rows of one tile: groups of threads take every
 // parts-th piece with a running maximum, four pieces' loads at a time, and are then added in LDS (buf).
 template <int DP, int DT, bool SHARED>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, int rows, int rows_most, int slots, int s0, int piece, int p0,
-                                            int p1, int b, int hq0, [[maybe_unused]] int from, float* buf) {
+                                            int p1, int b, int hq0, [[maybe_unused]] const SharedPart* shared,
+                                            [[maybe_unused]] int shared_parts, float* buf) {
     constexpr int kQuads = DP / 4;                      // float4 of a row
     constexpr int kThreads = 64 * waves_of(DP);
     const int items = rows * kQuads, parts = items >= kThreads ? 1 : kThreads / items;
@@ -302,7 +375,7 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, int rows, int row
         }
         if (mine && part == 0) {
             if constexpr (SHARED)
-                if (from > 0) add_shared(a, b, hq0 + row, d, m, l, some, x);
+                add_gathered(shared, items, shared_parts, item, m, l, some, x);
             const float inv = some ? 1.0f / l : 0.0f;
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + b * a.o_token + (hq0 + row) * a.o_head + d) =
                 make_uint2(pack_16x2(x[0] * inv, x[1] * inv, DT), pack_16x2(x[2] * inv, x[3] * inv, DT));
@@ -334,6 +407,7 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
     constexpr float kLift = MT == kDtF16 ? 14.0f : 0.0f;
     __shared__ float sm_out[kWaves][16][DP + 4];
     __shared__ float sm_m[kWaves][16], sm_l[kWaves][16];
+    __shared__ SharedPart sm_shared[SHARED ? shared_threads(DP) : 1];
     __shared__ int sm_any[kWaves];
     __shared__ int sm_last;
 
@@ -352,7 +426,7 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
                     const int row = x / (a.D / 4), d = 4 * (x % (a.D / 4));
                     float m = kNegInf, l = 0.0f, y[4] = {0, 0, 0, 0};
                     bool some = false;
-                    add_shared(a, e, row, d, m, l, some, y);
+                    add_shared(a, e, row, d, 0, 1, m, l, some, y);
                     const float inv = some ? 1.0f / l : 0.0f;
                     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + e * a.o_token + row * a.o_head + d) =
                         make_uint2(pack_16x2(y[0] * inv, y[1] * inv, DT), pack_16x2(y[2] * inv, y[3] * inv, DT));
@@ -660,6 +734,9 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
 
         // the waves' parts together: rows c, values VE (4 g + r) + i
         __syncthreads();
+        int shared_parts = 0;
+        if constexpr (SHARED)
+            if (whole && cur_from > 0) shared_parts = gather_shared<DP>(a, cur_b, hq0, rows, sm_shared);
         if (lane == 0) sm_any[wave] = any;
         if (c < rows) {
             if (g == 0) {
@@ -696,8 +773,7 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             }
             if (whole) {
                 bool seen = some;
-                if constexpr (SHARED)
-                    if (cur_from > 0) add_shared(a, cur_b, hq0 + row, d, top, sum, seen, x);
+                if constexpr (SHARED) add_gathered(sm_shared, rows * (DP / 4), shared_parts, e, top, sum, seen, x);
                 const float inv = seen ? 1.0f / sum : 0.0f;     // nothing seen: zeros
                 uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + cur_b * a.o_token +
                                                             (hq0 + row) * a.o_head + d);
@@ -726,7 +802,13 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
             }
             __syncthreads();
             if (sm_last) {
-                join_pieces<DP, DT, SHARED>(a, rows, rows_most, slots, cur_s0, piece, p0, p1, cur_b, hq0, cur_from, &sm_out[0][0][0]);
+                if constexpr (SHARED)
+                    if (cur_from > 0) {
+                        shared_parts = gather_shared<DP>(a, cur_b, hq0, rows, sm_shared);
+                        __syncthreads();
+                    }
+                join_pieces<DP, DT, SHARED>(a, rows, rows_most, slots, cur_s0, piece, p0, p1, cur_b, hq0, sm_shared, shared_parts,
+                                            &sm_out[0][0][0]);
             }
         }
         if (!kAcross && more) {

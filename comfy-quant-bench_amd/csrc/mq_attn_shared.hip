@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
 
 constexpr int kSharedRows = 128;            // rows of a tile, 32 a wave
 constexpr int tile_keys(int dp) { return dp == 256 ? 32 : 64; }
+constexpr int kLeastTiles = 2;              // of a workgroup
 constexpr int tile_waves(int dp) { return dp == 128 ? 8 : 4; }
 constexpr int tiles_ahead(int dp) { return dp == 64 ? 7 : 3; }      // on their way while one is worked on
 
@@ -200,20 +201,12 @@ __device__ __forceinline__ Group group_from(const Group& mine, int x) {
     return Group{__builtin_amdgcn_readlane(mine.tokens, x), __builtin_amdgcn_readlane(mine.lead, x),
                  __builtin_amdgcn_readlane(mine.first, x), __builtin_amdgcn_readlane(mine.count, x)};
 }
-// All places, and those of the groups in front of group g. mine: groups_from(a, 0).
-__device__ __forceinline__ int line_of(const AttnArgs& a, const Group& mine, int n_groups, int g, int tile, int* before) {
-    int all = 0, front = 0;
-    for (int g0 = 0; g0 < n_groups; g0 += 64) {
-        const int x = g0 + (threadIdx.x & 63), n = places_of(a, g0 ? groups_from(a, g0) : mine, tile);
-        all += n;
-        front += x < g ? n : 0;
-    }
+// All places. mine: groups_from(a, 0).
+__device__ __forceinline__ int line_of(const AttnArgs& a, const Group& mine, int n_groups, int tile) {
+    int all = 0;
+    for (int g0 = 0; g0 < n_groups; g0 += 64) all += places_of(a, g0 ? groups_from(a, g0) : mine, tile);
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        all += __shfl_xor(all, s);
-        front += __shfl_xor(front, s);
-    }
-    *before = __builtin_amdgcn_readfirstlane(front);
+    for (int s = 1; s < 64; s <<= 1) all += __shfl_xor(all, s);
     return __builtin_amdgcn_readfirstlane(all);
 }
 // The group that has place t of the line, and the places in front of it.
@@ -240,64 +233,6 @@ __device__ __forceinline__ Group group_at_place(const AttnArgs& a, const Group& 
     return Group{0, 0, 0, 0};
 }
 
-// The pieces of every row whose tiles more than one workgroup has, in their order: a wave a row (of a sequence and query head).
-// rows_most: rows that a workgroup's place in the workspace has room for.
-template <int DP>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int pieces_most, int rows_most) {
-    const int64_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    if (at >= a.B * a.Hq) return;
-    const int b = static_cast<int>(at / a.Hq), hq = static_cast<int>(at % a.Hq), lane = threadIdx.x & 63;
-    const int g = a.plan[SharedPlan::group_at(a.B) + b], rank = a.plan[SharedPlan::rank_at(a.B) + b], n_groups = groups_of(a);
-    if (g < 0 || g >= n_groups || rank < 0) return;
-    const Group r = group_of(a, g), mine = groups_from(a, 0);
-    if (r.tokens == 0 || rank >= r.count) return;
-    int before;
-    const int total = line_of(a, mine, n_groups, g, tile_keys(DP), &before), piece = (total + pieces_most - 1) / pieces_most;
-    const int group = a.Hq / a.H, h = hq / group, of = rank * group + hq % group, nt = tiles_of(r, tile_keys(DP));
-    const int s0 = before + (h * row_tiles_of(a, r) + of / kSharedRows) * nt, row = of % kSharedRows;
-    const int p0 = s0 / piece, p1 = (s0 + nt - 1) / piece, slots = 2 * pieces_most;
-    if (p0 == p1) return;                               // written by that workgroup
-    constexpr int V = DP == 256 ? 4 : DP == 128 ? 2 : 1, kAhead = 8;
-    const int d = V * lane;
-    float top = kNegInf, sum = 0.0f, y[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) y[e] = 0.0f;
-    bool some = false;
-    for (int p = p0; p <= p1; p += kAhead) {
-        float2 st[kAhead];
-        float z[kAhead][V];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int x = p + i < p1 ? p + i : p1, slot = 2 * x + (x * piece < s0);
-            st[i] = *reinterpret_cast<const float2*>(part_stat(a, rows_most, slots, slot) + 2 * row);
-            const float* from = part_out(a, rows_most, slot) + row * a.D + (d < a.D ? d : 0);
-#pragma unroll
-            for (int e = 0; e < V; ++e) z[i][e] = from[e];
-        }
-        float most = top;
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) most = p + i <= p1 && st[i].y >= 0.0f ? __builtin_fmaxf(most, st[i].x) : most;
-        const float ref = most == kNegInf ? 0.0f : most, f = __builtin_amdgcn_exp2f(top - ref);
-        top = most;
-        sum *= f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[e] *= f;
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (p + i > p1 || st[i].y < 0.0f) continue;                 // nothing seen there
-            some = true;
-            const float fz = __builtin_amdgcn_exp2f(st[i].x - ref);
-            sum += st[i].y * fz;
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] += z[i][e] * fz;
-        }
-    }
-    if (d < a.D)
-#pragma unroll
-        for (int e = 0; e < V; ++e) a.shared_out[at * a.D + d + e] = y[e];
-    if (lane == 0) reinterpret_cast<float2*>(a.shared_stat)[at] = make_float2(top, some ? sum : -1.0f);
-}
-
 template <int DP, bool I8>
 struct __attribute__((aligned(16))) SharedLds {
     static constexpr int kTile = tile_keys(DP), kRing = tiles_ahead(DP) + 1, kWide = I8 ? 2 : kRing, kPages = DP == 64 ? 16 : 8;
@@ -321,9 +256,9 @@ __device__ __forceinline__ void wait_but() {
 // (__syncthreads without a wait for loads that are meant to be on their way)
 __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache. rows_most: as above.
+// DP: head width rounded up to 64, 128 or 256; DT: type of the tokens; I8: int8 cache.
 template <int DP, int DT, bool I8>
-__global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(AttnArgs a, int rows_most) {
+__global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(AttnArgs a) {
     using Lds = SharedLds<DP, I8>;
     constexpr int E = I8 ? 1 : 2, kTile = Lds::kTile, kRing = Lds::kRing, kAhead = kRing - 1, kPages = Lds::kPages, kThreads = 64 * tile_waves(DP);
     static_assert(kPages >= 2 * kRing - 1);
@@ -346,9 +281,8 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
     const int group = a.Hq / a.H, B = static_cast<int>(a.B);
     const Group first = groups_from(a, 0);
     const int n_groups = groups_of(a);
-    int front;
-    const int total = line_of(a, first, n_groups, 0, kTile, &front);
-    const int piece = (total + gridDim.x - 1) / gridDim.x;
+    const int total = line_of(a, first, n_groups, kTile);
+    const int even = (total + gridDim.x - 1) / gridDim.x, piece = even > kLeastTiles ? even : kLeastTiles;
     const int t0 = blockIdx.x * piece, t1 = t0 + piece < total ? t0 + piece : total;
     if (t0 >= t1) return;
     const int mask = (1 << a.page_shift) - 1;
@@ -663,12 +597,13 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
                 }
             }
         }
+        // a tile's rows that one workgroup has seen all keys of are complete, others' pieces are in one of its two slots
         if (part == 0 && row < rows) {
             const bool complete = i0 == 0 && i1 == nt;
-            const int slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < s0);
+            const int64_t slots = 2 * gridDim.x, slot = 2 * blockIdx.x + (t0 < s0), place = slot * a.shared_most + row;
             const int64_t at = static_cast<int64_t>(seq < 0 ? 0 : seq) * a.Hq + hq;
-            float* to = complete ? a.shared_out + at * a.D : part_out(a, rows_most, slot) + static_cast<int64_t>(row) * a.D;
-            float* stat = complete ? a.shared_stat + 2 * at : part_stat(a, rows_most, slots, slot) + 2 * row;
+            float* to = complete ? a.shared_out + at * a.D : a.shared_parts + place * a.D;
+            float* stat = complete ? a.shared_stat + 2 * at : a.shared_parts + slots * a.shared_most * a.D + 2 * place;
             if (seq >= 0 || !complete) {
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i)
@@ -680,6 +615,8 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
                     }
                 if (hf == 0) *reinterpret_cast<float2*>(stat) = make_float2(m + kShift, any ? l : -1.0f);
             }
+            if (hf == 0 && seq >= 0 && i0 == 0)
+                reinterpret_cast<int4*>(a.shared_rows)[at] = make_int4(static_cast<int>(slot), complete ? -1 : (s0 + nt - 1) / piece, row, 0);
         }
         t = s0 + i1;
         if (t < t1) {
@@ -689,16 +626,9 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
     }
 }
 
-// Rows of a workgroup's place in the workspace: no tile has more.
-int rows_most_of(int Hq, int H, int64_t B) {
-    const int64_t rows = B * (Hq / H);
-    return static_cast<int>(rows < kSharedRows ? rows : kSharedRows);
-}
-
 template <int DP, int DT, bool I8>
 int shared_width(const AttnArgs& a, hipStream_t stream) {
-    const int groups = decode_groups(), rows_most = rows_most_of(a.Hq, a.H, a.B);
-    const size_t lds = sizeof(SharedLds<DP, I8>);
+        const size_t lds = sizeof(SharedLds<DP, I8>);
     static_assert(sizeof(SharedLds<DP, I8>) <= 160 * 1024 && sizeof(SharedLds<DP, I8>) >= sizeof(float) * kSharedRows * (DP + 6));
     auto kern = attn_shared_kernel<DP, DT, I8>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -707,9 +637,7 @@ int shared_width(const AttnArgs& a, hipStream_t stream) {
         set_error("paged_attention_shared: cannot reserve %zu bytes of LDS", lds);
         return -3;
     }
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(groups)), dim3(64 * tile_waves(DP)), lds, stream, a, rows_most);
-    const int64_t rows = a.B * a.Hq;
-    hipLaunchKernelGGL((attn_shared_join_kernel<DP>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a, groups, rows_most);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(decode_groups())), dim3(64 * tile_waves(DP)), lds, stream, a);
     return launch_status("paged_attention_shared");
 }
 
@@ -720,23 +648,30 @@ int shared_type(const AttnArgs& a, hipStream_t stream) {
     return shared_width<256, DT, I8>(a, stream);
 }
 
+// Rows of a slot: no tile has more.
+int rows_most_of(int Hq, int H, int64_t B) {
+    const int64_t rows = B * (Hq / H);
+    return static_cast<int>(rows < kSharedRows ? rows : kSharedRows);
+}
 int64_t parts_bytes(int Hq, int H, int D, int64_t B) { return 2 * static_cast<int64_t>(decode_groups()) * rows_most_of(Hq, H, B) * (D + 2) * 4; }
 
 }  // namespace
 
 int64_t attn_shared_workspace_bytes(int Hq, int H, int D, int64_t B) {
-    // both kernels' pieces (one behind the other in time), then the shared parts
-    const int64_t single = attn_decode_workspace_bytes(Hq, H, D), parts = parts_bytes(Hq, H, D, B);
-    return (single > parts ? single : parts) + B * Hq * (D + 2) * 4;
+    // the single-token kernel's pieces, the shared keys' pieces, their whole parts, where a row's are
+    return attn_decode_workspace_bytes(Hq, H, D) + parts_bytes(Hq, H, D, B) + B * Hq * (D + 2 + 4) * 4;
 }
 
 int64_t attn_shared_counters(int Hq, int H, int64_t B) { return attn_decode_counters(Hq, H, B); }
 
 int launch_attn_shared(const AttnArgs& args, hipStream_t stream) {
     AttnArgs a = args;
-    const int64_t single = attn_decode_workspace_bytes(a.Hq, a.H, a.D), parts = parts_bytes(a.Hq, a.H, a.D, a.B);
-    a.shared_out = reinterpret_cast<float*>(static_cast<char*>(a.work) + (single > parts ? single : parts));
-    a.shared_stat = a.shared_out + a.B * a.Hq * a.D;
+    // (each of them a multiple of 16 bytes: heads are of 8 values at least, slots and the slots' rows come in pairs of two floats)
+    a.shared_most = rows_most_of(a.Hq, a.H, a.B);
+    a.shared_parts = reinterpret_cast<float*>(static_cast<char*>(a.work) + attn_decode_workspace_bytes(a.Hq, a.H, a.D));
+    a.shared_out = a.shared_parts + parts_bytes(a.Hq, a.H, a.D, a.B) / 4;
+    a.shared_rows = reinterpret_cast<int*>(a.shared_out + a.B * a.Hq * a.D);
+    a.shared_stat = reinterpret_cast<float*>(a.shared_rows + a.B * a.Hq * 4);
     a.start = a.plan + SharedPlan::start();
     const bool i8 = a.k_scale != nullptr;
     int rc;

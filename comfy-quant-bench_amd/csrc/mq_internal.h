@@ -261,6 +261,9 @@ struct AttnArgs {
     const int* start;         // [B], keys of a sequence that its group's part covers
     float* shared_out;        // [B, Hq, D], the part over those keys, unnormalised
     float* shared_stat;       // [B, Hq, 2], its maximum (base 2) and sum; sum -1: nothing seen
+    float* shared_parts;      // of rows whose part is in pieces: those, [slots, shared_most, D], and their maxima and sums
+    int* shared_rows;         // [B, Hq, 4], first slot, last piece (-1: not in pieces), row in them
+    int shared_most;
 };
 int launch_attn_prompt(const AttnArgs& a, hipStream_t stream);
 int launch_attn_decode(const AttnArgs& a, hipStream_t stream);
