@@ -4,24 +4,32 @@
 //   softmax over [shared keys, own keys] = both parts' unnormalised outputs over a common maximum, divided by both sums
 //
 // The plan (once for all layers of a step) finds the groups. The first kernel takes the rows of a group (its sequences' query
-// heads of one cache head) as tiles of 16 RT rows over the shared keys, cut into as many pieces as there are compute units;
-// the second joins the pieces of every row; the third is the single-token kernel over each sequence's own keys, which adds that
-// part before it divides. (Pieces joined by the workgroup that brings the last one, as the single-token kernel does it:
-// 32 sequences over 32000 tokens 160 us instead of XX, most of it one workgroup's waiting for 17 x 64 rows.)
+// heads of one cache head) as tiles of 128 rows over the shared keys, cut into as many pieces as there are compute units. The
+// second is the single-token kernel over each sequence's own keys; where it divides a row by its sum it adds the row's pieces of
+// the first. (In a launch of their own the pieces cost 7 to 10 us a layer instead of 4 to 8. The workgroup that brings a
+// tile's last piece, as in the single-token kernel, would have 128 rows of up to 17 pieces by itself.)
 //
-// The first kernel is the single-token kernel's plan with more rows: HBM-bound where a group has few of them, keys and
-// values go straight from the pages into registers, each wave with 32 keys of a tile and all rows. At 64 rows (RT = 4) a
-// wave's 32 keys of 128 values cost 64 products of 16 cycles and some 1500 cycles of softmax against the 16 KB that it
-// waits for, a fifth of what HBM brings a compute unit in that time, so larger groups, whose tiles read the keys again from
-// the caches, are still served at that rate.
-//
-//   S^T = K Q^T, O^T = V^T P^T   operands and lanes as in mq_attn_decode_kernel.h, once per 16 rows; keys are unpacked
-//                                and values paired once for all of them
+//   S^T = K Q^T, O^T = V^T P^T   products of 32 x 32 x 16. A wave has 32 rows, one a lane (and its partner), as B and P^T's
+//                                operand straight from S^T's registers, as in mq_attn_prompt.hip
 //   softmax                      base 2, fp32; the reference maximum of a row moves (and its sums are rescaled) only when
 //                                the row's maximum passes it by 2^8
 //
 // All rows of a group see all of its shared keys, so what is hidden (behind the shared length, in pages that are none) is
 // hidden from every row.
+//
+// What bounds the first kernel: HBM, as it reads a tile of keys once for 128 rows, if enough is on its way (a compute unit's
+// share of 5 TB/s over 2 us is 40 KB) and nothing else takes a tile's time (64 keys of 128 values, 32 KB: 1.6 us). So:
+//   loads      go to LDS by themselves into a ring of tiles, three ahead of the one that is worked on, with the table's entries
+//              of the tiles behind those among them: the loop has no other loads, and its one wait leaves those of the later
+//              tiles on their way (in registers, one tile ahead: 54 us instead of 46)
+//   LDS reads  of a tile's keys are all sent for before the first product, and its values before the softmax (each in front of
+//              its product: 57 us)
+//   waves      eight at 128 values a head, so that a matrix unit has one wave's products while another's softmax runs; each
+//              takes 32 of the 64 keys, or with up to 64 rows four do. 64 values: four, as a tile is half as long; 256: four,
+//              whose sums need the registers of two
+//   int8       16 bytes of a row by each thread, in 16 bits for all waves' products once
+// 32 sequences of 32 heads over 32000 shared tokens of 8 cache heads, 131 MB: 46 us, 2.9 TB/s and 366 TFLOP/s (16 rows a
+// wave with keys straight to registers, read again for every 64 rows: 68 us).
 #include "mq_attn_decode_kernel.h"
 
 namespace mq {
@@ -32,7 +40,9 @@ constexpr int kPlanThreads = 1024;
 // ---------------------------------------------------------------------------------------- the plan
 //
 // Sequences belong together if their first pages are the same; what a group shares is the shortest run of equal pages
-// of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency.
+// of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency, of
+// one workgroup (64 sequences of 9000 tokens in pages of 16: 11 us; each row's look for its first with a thread's loop, and a
+// wave's tables one behind the other: 14).
 // ON_CHIP: working space in LDS (up to kPlanRows sequences), else behind the plan.
 constexpr int kPlanRows = 2048;
 
@@ -43,64 +53,93 @@ template <bool ON_CHIP>
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* table, int64_t ld, int B, int width,
                                                                     const int* lens, int page_shift, int* plan) {
     __shared__ int wave_sum[2][kPlanThreads / 64];
-    __shared__ int space[ON_CHIP ? 4 * kPlanRows : 1];
+    __shared__ int space[ON_CHIP ? 6 * kPlanRows : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int* start = plan + SharedPlan::start();
     int* members = plan + SharedPlan::members(B);
     int* groups = plan + SharedPlan::groups(B);
-    int* group_at = plan + SharedPlan::group_at(B);
-    int* rank_at = plan + SharedPlan::rank_at(B);
     int* work = plan + SharedPlan::work(B);
     int* key = ON_CHIP ? space : work;                                  // first page
     int* lead = ON_CHIP ? space + kPlanRows : work + B;                 // first sequence with it
     int* tokens = ON_CHIP ? space + 2 * kPlanRows : work + 2 * static_cast<int64_t>(B);    // of a lead: what its group shares
     int* count = ON_CHIP ? space + 3 * kPlanRows : work + 3 * static_cast<int64_t>(B);     // of a lead: members
+    int* rank = ON_CHIP ? space + 5 * kPlanRows : work + 4 * static_cast<int64_t>(B);      // members in front of it
+    int* held_by = ON_CHIP ? space + 4 * kPlanRows : start;             // tokens of a sequence
     for (int b = tid; b < B; b += kPlanThreads) {
-        key[b] = lens[b] > 0 && width > 0 ? table[b * ld] : -1;
+        const int n = lens[b], k = width > 0 ? table[b * ld] : -1;
+        key[b] = n > 0 ? k : -1;
         tokens[b] = 0x7fffffff;
-        count[b] = 0;
+        held_by[b] = n;
     }
     __syncthreads();
-    for (int b = tid; b < B; b += kPlanThreads) {
-        const int k = key[b];
-        int l = -1;
-        if (k >= 0) {
-            l = 0;
-            while (key[l] != k) ++l;
-            atomicAdd(&count[l], 1);
-        }
-        lead[b] = l;
-    }
-    __syncthreads();
-    // a wave a sequence: entries that it has in common with its lead, 256 at a time
+    // a wave a sequence: the first with its first page, how many in front of it have that, how many all in all
     for (int b = wave; b < B; b += kPlanThreads / 64) {
-        const int l = lead[b];
-        if (l < 0 || l == b || latest(count + l) < 2) continue;
-        const int most = lens[b] < lens[l] ? lens[b] : lens[l];
-        const int entries = static_cast<int>((static_cast<int64_t>(most) + (1 << page_shift) - 1) >> page_shift);
-        const int n = entries < width ? entries : width;
-        int same = n;
-        for (int i0 = 0; i0 < n; i0 += 256) {
-            int x[4], y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = i0 + 64 * e + lane < n ? i0 + 64 * e + lane : n - 1;
-                x[e] = table[b * ld + i];
-                y[e] = table[l * ld + i];
+        const int k = key[b];
+        int l = -1, before = 0, all = 0;
+        if (k >= 0)
+#pragma unroll 4
+            for (int x0 = 0; x0 < B; x0 += 64) {
+                const int x = x0 + lane;
+                const uint64_t same = __ballot(x < B && key[x < B ? x : 0] == k);
+                if (same && l < 0) l = x0 + __builtin_ctzll(same);
+                all += __builtin_popcountll(same);
+                before += __builtin_popcountll(x0 + 64 <= b ? same : x0 <= b ? same & ((uint64_t(1) << (b - x0)) - 1) : 0);
             }
-            int first = n;
-#pragma unroll
-            for (int e = 3; e >= 0; --e) {
-                const uint64_t any = __ballot(x[e] < 0 || x[e] != y[e]);
-                if (any) first = i0 + 64 * e + __builtin_ctzll(any);
-            }
-            if (first < n) {
-                same = first;
-                break;
-            }
+        if (lane == 0) {
+            lead[b] = l;
+            rank[b] = before;
+            if (l == b) count[b] = all;
         }
-        const int64_t held = static_cast<int64_t>(same) << page_shift;
-        if (lane == 0) atomicMin(&tokens[l], held < most ? static_cast<int>(held) : most);
+    }
+    __syncthreads();
+    // a wave four sequences: entries that each has in common with its lead, 256 at a time
+    constexpr int kFour = 4;
+    for (int b0 = wave; b0 < B; b0 += kFour * (kPlanThreads / 64)) {
+        int l[kFour], most[kFour], n[kFour], same[kFour], longest = 0;
+        const int* mine[kFour];
+        const int* first_of[kFour];
+        bool open[kFour];
+#pragma unroll
+        for (int s = 0; s < kFour; ++s) {
+            const int b = b0 + s * (kPlanThreads / 64), at = b < B ? b : b0;
+            l[s] = __builtin_amdgcn_readfirstlane(lead[at]);
+            open[s] = b < B && l[s] >= 0 && l[s] != b;
+            const int of = open[s] ? l[s] : at, x = held_by[at], y = held_by[of];
+            most[s] = __builtin_amdgcn_readfirstlane(x < y ? x : y);
+            const int64_t entries = (static_cast<int64_t>(most[s]) + (1 << page_shift) - 1) >> page_shift;
+            n[s] = !open[s] ? 0 : entries < width ? static_cast<int>(entries) : width;
+            same[s] = n[s];
+            mine[s] = table + at * ld;
+            first_of[s] = table + of * ld;
+            longest = longest > n[s] ? longest : n[s];
+        }
+        for (int i0 = 0; i0 < longest; i0 += 256) {
+            int x[kFour][4], y[kFour][4];
+#pragma unroll
+            for (int s = 0; s < kFour; ++s)
+                if (i0 < same[s])                       // (no difference yet)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = i0 + 64 * e + lane < n[s] ? i0 + 64 * e + lane : n[s] - 1;
+                        x[s][e] = mine[s][i];
+                        y[s][e] = first_of[s][i];
+                    }
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[s][e] = y[s][e] = 0;
+#pragma unroll
+            for (int s = 0; s < kFour; ++s)
+#pragma unroll
+                for (int e = 3; e >= 0; --e) {
+                    const uint64_t any = __ballot(x[s][e] < 0 || x[s][e] != y[s][e]);
+                    if (any) same[s] = i0 + 64 * e + __builtin_ctzll(any);
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < kFour; ++s) {
+            const int64_t held = static_cast<int64_t>(same[s]) << page_shift;
+            if (lane == 0 && open[s]) atomicMin(&tokens[l[s]], held < most[s] ? static_cast<int>(held) : most[s]);
+        }
     }
     __syncthreads();
     // groups in the order of their first sequences, members in their own
@@ -130,8 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
             to[1] = b;
             to[2] = member0 + m - n;
             to[3] = n;
-            key[b] = group0 + g - 1;                // a group: its number, where its members begin
-            count[b] = -(member0 + m - n) - 1;
+            count[b] = -(member0 + m - n) - 1;      // a group: where its members begin
         }
         group0 += all_g;
         member0 += all_m;
@@ -140,14 +178,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
     for (int b = tid; b < B; b += kPlanThreads) {
         const int l = lead[b], begin = l < 0 ? 0 : latest(count + l);
         const bool in = begin < 0;
-        int before = 0;
-        if (in) {
-            for (int x = l; x < b; ++x) before += lead[x] == l;
-            members[-begin - 1 + before] = b;
-        }
+        if (in) members[-begin - 1 + rank[b]] = b;
         start[b] = in ? latest(tokens + l) : 0;
-        group_at[b] = in ? key[l] : -1;
-        rank_at[b] = before;
     }
     if (tid == 0) {
         plan[0] = group0;
@@ -158,8 +190,10 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
 // ---------------------------------------------------------------------------------------- the shared keys
 
 constexpr int kSharedRows = 128;            // rows of a tile, 32 a wave
-constexpr int tile_keys(int dp) { return dp == 256 ? 32 : 64; }
-constexpr int kLeastTiles = 2;              // of a workgroup
+constexpr int tile_keys(int dp) { return dp == 256 ? 32 : 64; }     // keys and values of 16 or 32 KB
+// Tiles of a workgroup at least: a piece more is one more to add for every row. (16 rows over 2000 tokens of 4 heads, both
+// kernels: 1 tile 27.5 us, 2 27.3, 4 28.6)
+constexpr int kLeastTiles = 2;
 constexpr int tile_waves(int dp) { return dp == 128 ? 8 : 4; }
 constexpr int tiles_ahead(int dp) { return dp == 64 ? 7 : 3; }      // on their way while one is worked on
 
@@ -307,7 +341,9 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
         // the segment: tiles i0 .. i1 - 1 of a group's cache head and row tile, whose tile 0 is place s0
         int before;
         const Group r = group_at_place(a, first, n_groups, t, kTile, &before);
-        const int nt = tiles_of(r, kTile), pair = (t - before) / nt;
+        const int nt = tiles_of(r, kTile);
+        if (nt == 0) return;                            // (of a plan that is none)
+        const int pair = (t - before) / nt;
         const int s0 = before + pair * nt;
         const int i0 = t - s0, i1 = t1 - s0 < nt ? t1 - s0 : nt;
         const int rtiles = row_tiles_of(a, r);

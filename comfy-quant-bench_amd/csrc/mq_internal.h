@@ -279,17 +279,14 @@ int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t w
 
 // The groups of sequences that hold the same first pages, as int32: their number; three words unused; start[b], the
 // tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
-// shared, the sequence whose pages are read, its first member's place and their number; each sequence's group (-1: none) and
-// its place among the members; working space.
+// shared, the sequence whose pages are read, its first member's place and their number; working space.
 struct SharedPlan {
     static constexpr int kHead = 4, kGroup = 4;
-    static int64_t ints(int64_t B) { return kHead + 10 * B; }
+    static int64_t ints(int64_t B) { return kHead + 9 * B; }
     __host__ __device__ static int64_t start() { return kHead; }
     __host__ __device__ static int64_t members(int64_t B) { return kHead + B; }
     __host__ __device__ static int64_t groups(int64_t B) { return kHead + 2 * B; }
-    __host__ __device__ static int64_t group_at(int64_t B) { return kHead + 4 * B; }
-    __host__ __device__ static int64_t rank_at(int64_t B) { return kHead + 5 * B; }
-    __host__ __device__ static int64_t work(int64_t B) { return kHead + 6 * B; }
+    __host__ __device__ static int64_t work(int64_t B) { return kHead + 4 * B; }
 };
 
 // --- 4-bit weights, floating activations (mq_w4a16.hip)

@@ -250,7 +250,7 @@ def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int) -
 
 
 def _plan_ints(b: int) -> int:
-    return 4 + 10 * b      # mq_kv_shared_ints
+    return 4 + 9 * b      # mq_kv_shared_ints
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

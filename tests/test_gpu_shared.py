@@ -268,3 +268,66 @@ def test_the_same_every_time(gpu_device):
     want = s.run()
     for _ in range(5):
         assert torch.equal(s.run(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [31, 32, 33, 64, 65, 97, 128, 129, 257])
+@pytest.mark.parametrize("d,int8", [(64, False), (64, True), (128, False), (128, True), (256, False), (256, True), (72, False), (144, True)])
+def test_rows_of_a_tile(gpu_device, rows, d, int8):
+    """Groups whose rows end at every boundary between waves and tiles, over a few tiles and over many workgroups' pieces."""
+    print(f"[shared] {rows} rows x {d} int8 {int8}", flush=True)
+    s = Forks(gpu_device, [(200, [i % 2 for i in range(rows)]), (3000, [3] * 5)], 2, 2, d, page=8, int8=int8, dtype=torch.float16 if rows % 2 else torch.bfloat16)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [32, 33, 64, 65, 128, 192, 193, 256, 257, 320, 449, 512, 513, 577, 1024])
+@pytest.mark.parametrize("d,int8", [(64, False), (64, True), (128, False), (128, True), (256, False), (256, True)])
+def test_tiles(gpu_device, tokens, d, int8):
+    """One tile to more than a ring holds, in one piece and with the next group's behind them in the same workgroup."""
+    s = Forks(gpu_device, [(tokens, [1, 2, 0])] + [(tokens - 1, [2, 1])] * 9, 8, 8, d, page=1, int8=int8)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+def test_long_and_short_groups(gpu_device):
+    """Workgroups that end one group's tiles, have others whole and begin a third's; more groups than lanes."""
+    groups = [(20000, [5] * 3)] + [(1 + 13 * i % 90, [i % 4, 1]) for i in range(150)] + [(7000, [60, 1, 9])]
+    s = Forks(gpu_device, groups, 4, 4, 128, page=4)
+    s.check(s.run())
+
+
+@pytest.mark.gpu
+def test_two_at_once(gpu_device):
+    """Calls of two streams and of two threads at the same time do not share working space."""
+    import threading
+    sets = [Forks(gpu_device, [(4000, [50] * 12), (90, [3, 5])], 8, 2, 128, seed=i) for i in range(2)]
+    want = [s.run() for s in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(sets[i].run())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys) and len(got[0]) == len(got[1]) == 20
+
+
+@pytest.mark.gpu
+def test_plan_of_anything(gpu_device):
+    """A plan that kv_shared did not write: whatever its numbers say, every access stays inside, and the next call is right."""
+    s = Forks(gpu_device, MIXED, 8, 2, 64)
+    want, plan = s.run(), s.plan()
+    g = torch.Generator().manual_seed(1)
+    for i in range(12):
+        odd = torch.randint(-3, 40, plan.shape, generator=g, dtype=torch.int32) if i % 3 else torch.randint(-2 ** 31, 2 ** 31 - 1, plan.shape, generator=g, dtype=torch.int64).int()
+        odd[0] = (i % 4) * 3
+        s.run(odd.to(gpu_device))
+    assert torch.equal(s.run(), want)
