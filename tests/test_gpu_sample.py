@@ -1,5 +1,5 @@
-"""kitchen_amd.sample against plain numpy in 64 bits, row by row: tokens have to be equal. (Weights are exact to 1e-15 and sums
-to 2^-45 of the largest weight on both sides: a token could only differ where u, top_p or min_p lies within that of a border.)"""
+"""kitchen_amd.sample against plain numpy in 64 bits, row by row: tokens have to be equal. (A weight is off by 1e-9 of itself at
+most, and sums are of integers: a token could only differ where u, top_p or min_p lies that close to a border of the sums.)"""
 import numpy as np
 import pytest
 import torch
@@ -146,3 +146,90 @@ def test_strides_streams_and_graphs(gpu_device):
         torch.cuda.synchronize()
         assert torch.equal(a, ck.sample(x, u, top_k=30)) and torch.equal(b, ck.sample(x, u, temperature=0.7, top_p=p))
         assert torch.equal(c, ck.sample(x, u))
+
+
+ODD = [dict(), dict(top_k=9), dict(top_k=4500), dict(top_p=0.6), dict(top_k=6000, top_p=0.95, min_p=0.01), dict(min_p=0.3), dict(top_p=0.02)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", ODD, ids=str)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_rows_of_large_batches(gpu_device, kw, dtype):
+    """More rows than are cut into parts, of several blocks."""
+    check(gpu_device, logits(140, 40003, dtype, 11), uniform(140), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", ODD + [dict(top_k=100000), dict(top_k=131071, top_p=0.5)], ids=str)
+@pytest.mark.parametrize("vocab", [131072, 262144, 300007])
+def test_thousands_alike(gpu_device, kw, vocab):
+    """All alike, two values, a few hundred, and values that crowd in one bin: more to choose from than is held at once."""
+    print(f"[sample] alike {vocab} {kw}", flush=True)
+    g = torch.Generator().manual_seed(14)
+    x = torch.stack([torch.full((vocab,), -3.5), torch.randint(0, 2, (vocab,), generator=g) * 20.0,
+                     torch.randint(0, 300, (vocab,), generator=g) * 1e-6, torch.rand(vocab, generator=g) * 1e-3 - 50])
+    x[3, 77] = 1.0
+    check(gpu_device, x, [0.37, 0.62, 0.11, 0.93], **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1e-28, 1e-10, 1e-4, 30.0, 1e4, 1e10, 1e30, float("inf")])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20), dict(top_p=0.7), dict(top_p=0.7, top_k=5000), dict(min_p=0.1)], ids=str)
+def test_temperatures(gpu_device, t, kw):
+    print(f"[sample] T {t} {kw}", flush=True)
+    check(gpu_device, logits(6, 20011, torch.float32, 15), uniform(6), temperature=t, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1e-42, 1e-30, 1e4, 6e4, 1e30, 3e38])
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.0), dict(top_k=3), dict(top_p=0.7), dict(temperature=1e3, top_k=50, top_p=0.9)], ids=str)
+def test_sizes_of_logits(gpu_device, dtype, size, kw):
+    """Up to the type's largest, down to what is not normal."""
+    big = torch.finfo(dtype).max
+    x = (torch.rand((5, 9001), generator=torch.Generator().manual_seed(16)).double() * 2 - 1) * size
+    x[1] = x[1].abs()
+    x[2] = -x[2].abs()
+    check(gpu_device, x.clamp(-big, big).to(dtype), uniform(5), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [900, 70001])
+def test_every_kind_of_nan(gpu_device, vocab):
+    """Quiet and signalling, of either sign: never chosen, in rows of one part and of several."""
+    bits = {torch.bfloat16: ([0x7f81, 0x7fc0, -1, -0x7f], torch.int16), torch.float16: ([0x7c01, 0x7e00, -1, -0x3ff], torch.int16),
+            torch.float32: ([0x7f800001, 0x7fc00000, -1, -0x7fffff], torch.int32)}
+    for dtype, (patterns, like) in bits.items():
+        x = logits(4, vocab, dtype, 17)
+        for i, b in enumerate(patterns):
+            nan = torch.tensor([b], dtype=like).view(dtype)
+            assert nan.isnan().all()
+            x[i, i::2] = nan
+            if i == 3:
+                x[i] = nan
+        for kw in (dict(), dict(top_k=5), dict(top_p=0.5), dict(temperature=0.0)):
+            check(gpu_device, x, uniform(4), **kw)
+
+
+@pytest.mark.gpu
+def test_two_at_once(gpu_device):
+    """Calls of two streams and of two threads at the same time do not share working space."""
+    import threading
+    x = [logits(20, 100003, torch.bfloat16, 18 + i).to(gpu_device) for i in range(2)]
+    u = uniform(20).to(gpu_device)
+    want = [ck.sample(y, u, top_p=0.9, top_k=800) for y in x]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got[i].append(ck.sample(x[i], u, top_p=0.9, top_k=800))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys) and len(got[0]) == len(got[1]) == 30
