@@ -143,6 +143,6 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
             _SAMPLE_WS[key] = nbytes
         work = _scratch(nbytes, dev, stream) if nbytes else None
         _lib.call("mq_sample", x.data_ptr(), _lib.DTYPE_CODE[x.dtype], x.stride(0), rows, vocab, u.data_ptr(), t[0], float(t[1]),
-                  k[0], int(k[1]), p[0], float(p[1]), least[0], float(least[1]), token.data_ptr(),
+                  k[0], min(max(int(k[1]), -1), 1 << 24), p[0], float(p[1]), least[0], float(least[1]), token.data_ptr(),
                   None if work is None else work.data_ptr(), nbytes, stream)
     return token

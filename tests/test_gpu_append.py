@@ -249,3 +249,27 @@ def test_the_same_as_the_cache_method_in_a_graph(gpu_device):
             at = int(cache.page_table[b, (n[b] - 1) // 16]), slice(None), (n[b] - 1) % 16
             assert torch.equal(cache.k[1][at], other.k[1][at]) and torch.equal(cache.v[1][at], v[b])
     assert not cache.k[0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_pages_far_into_a_cache(gpu_device, int8):
+    """Offsets beyond 32 bits, in values and in bytes: what is written is what a cache of these pages alone gets."""
+    r = ck.Rotary(128)
+    s = Batch(gpu_device, [70, 9, 130], [70, 2, 66], 4, 4, 128, page=64, int8=int8)
+    want, n = s.run(r), s.pages
+    near = [x.clone() for x in (s.kc, s.vc, *((s.ks, s.vs) if int8 else ()))]
+    pages = (1 << 32) // (4 * 64 * 128) + n + 5
+    far = torch.arange(pages - 1, pages - 1 - n, -1, device=gpu_device)
+
+    def spread(fill, x):
+        y = torch.empty((pages, *x.shape[1:]), dtype=x.dtype, device=gpu_device)
+        y[far] = fill
+        return y
+
+    s.kc, s.vc = spread(3, s.kc), spread(3, s.vc)
+    if int8:
+        s.ks, s.vs = spread(9.0, s.ks), spread(9.0, s.vs)
+    s.table = torch.where(s.table < 0, s.table, pages - 1 - s.table)
+    assert torch.equal(s.run(r), want)
+    assert all(torch.equal(x[far], y) for x, y in zip((s.kc, s.vc, *((s.ks, s.vs) if int8 else ())), near))

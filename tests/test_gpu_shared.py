@@ -331,3 +331,24 @@ def test_plan_of_anything(gpu_device):
         odd[0] = (i % 4) * 3
         s.run(odd.to(gpu_device))
     assert torch.equal(s.run(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_pages_far_into_a_cache(gpu_device, int8):
+    """Offsets beyond 32 bits, in values and in bytes: the same as in a cache that holds these pages alone."""
+    s = Forks(gpu_device, [(500, [40, 0, 7]), (100, [300, 2])], 8, 4, 128, page=64, int8=int8)
+    want, n = s.run(), s.k.shape[0]
+    pages = (1 << 32) // (4 * 64 * 128) + n + 5
+    far = torch.arange(pages - 1, pages - 1 - n, -1, device=gpu_device)
+
+    def spread(x):
+        y = torch.empty((pages, *x.shape[1:]), dtype=x.dtype, device=gpu_device)
+        y[far] = x
+        return y
+
+    s.k, s.v = spread(s.k), spread(s.v)
+    if int8:
+        s.ks, s.vs = spread(s.ks), spread(s.vs)
+    s.table = torch.where(s.table < 0, s.table, pages - 1 - s.table)
+    assert torch.equal(s.run(), want)
