@@ -207,12 +207,13 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     value rounded once (codes of an int8 cache are of the unrounded ones). A query without a position (of a sequence that
     holds nothing) is passed as it is; rows behind the last sequence's are not written."""
     dev = _device_of(q, "q")
-    if k.shape != v.shape or k.dtype != v.dtype or k.device != dev or v.device != dev:
+    qs, shape, dtype = q.shape, k.shape, k.dtype
+    if shape != v.shape or dtype != v.dtype or k.device != dev or v.device != dev:
         raise ValueError(f"k and v must be alike and on {dev}, got {list(k.shape)} {k.dtype} and {list(v.shape)} {v.dtype}")
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype:
+    if len(qs) != 3 or len(shape) != 3 or qs[0] != shape[0] or qs[2] != shape[2] or q.dtype != dtype:
         raise ValueError(f"q must be [tokens, heads, head_dim] beside k, got {list(q.shape)} {q.dtype} and {list(k.shape)} {k.dtype}")
     q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    t, h, d = k.shape
+    t, h, d = shape
     if rotary.dim > d:
         raise ValueError(f"{rotary.dim} values to turn in heads of {d}")
     if rotary.turns.device != dev:
@@ -221,12 +222,12 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     page_table = _apart(page_table)
     tables = _table_args(page_table, kv_lens, cu_q, t, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
+        out = q.new_empty(qs)
+    elif out.shape != qs or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
             or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with rows at multiples of 16 bytes")
-    _lib.call("mq_kv_append", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), q.shape[1],
-              k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _CODE[k.dtype], t, h, d, *cache,
+    _lib.call("mq_kv_append", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), qs[1],
+              k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _CODE[dtype], t, h, d, *cache,
               *tables, rotary.turns.data_ptr(), rotary.dim, int(rotary.interleaved), rotary.size, _lib.stream_of_device(dev))
     return out
 

@@ -45,6 +45,11 @@ def _rows(x: torch.Tensor, what: str, like: torch.Tensor | None = None) -> torch
     return x
 
 
+def _new(x: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of x's shape (a call with one argument is half a microsecond shorter)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _norm_args(x, weight, residual, eps):
     x2 = _rows(x, "x")
     m, k = x2.shape
@@ -55,7 +60,7 @@ def _norm_args(x, weight, residual, eps):
             raise ValueError(f"weight must be floating-point [{k}] on {x2.device}, got {weight.dtype} {list(weight.shape)} on {weight.device}")
         weight = weight.contiguous()
     r2 = None if residual is None else _rows(residual, "residual", x)
-    h = None if residual is None else torch.empty((m, k), dtype=x2.dtype, device=x2.device)
+    h = None if residual is None else _new(x)
     args = (x2.data_ptr(), _lib.DTYPE_CODE[x2.dtype], x2.stride(0), None if r2 is None else r2.data_ptr(),
             0 if r2 is None else r2.stride(0), None if weight is None else weight.data_ptr(),
             _lib.DT_BF16 if weight is None else _lib.DTYPE_CODE[weight.dtype], float(eps))
@@ -68,11 +73,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torc
     fp32 and rounded once to x's type. x: bfloat16, float16 or float32 of any strides, rows of up to 32768 values; weight: floating [K],
     None for ones. Returns y, or with a residual (y, h), both contiguous in x's shape."""
     x2, m, k, h, args, hargs, _keep = _norm_args(x, weight, residual, eps)
-    y = torch.empty((m, k), dtype=x2.dtype, device=x2.device)
+    y = _new(x)
     if m:
         _lib.call("mq_rms_norm", *args, *hargs, y.data_ptr(), k, m, k, _lib.stream_of_device(x2.device))
-    y = y if x.dim() == 2 else y.reshape(x.shape)
-    return y if h is None else (y, h if x.dim() == 2 else h.reshape(x.shape))
+    return y if h is None else (y, h)
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -90,7 +94,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, resid
     if m:
         _lib.call("mq_rms_norm_quant", *args, int(convrot_groupsize or 0), *hargs, q.data_ptr(), k, s.data_ptr(), m, k,
                   _lib.stream_of_device(x2.device))
-    return (q, s) if h is None else (q, s, h if x.dim() == 2 else h.reshape(x.shape))
+    return (q, s) if h is None else (q, s, h)
 
 
 def _setting(value, name: str, rows: int, dtype, device):
