@@ -383,12 +383,16 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t r) {
     Row w;
     w.x = static_cast<const char*>(a.x) + r * a.ld * (DT == kDtF32 ? 4 : 2);
     w.V = static_cast<int>(a.V);
-    w.T = uniform(a.temperature ? a.temperature[r] : a.temperature1);
+    // (Read at once, not one behind the other. What is not given is read from u and not used.)
+    const float u = a.u[r], t = (a.temperature ? a.temperature : a.u)[r], p = (a.top_p ? a.top_p : a.u)[r],
+                least = (a.min_p ? a.min_p : a.u)[r];
+    const int k = (a.top_k ? a.top_k : reinterpret_cast<const int*>(a.u))[r];
+    w.T = uniform(a.temperature ? t : a.temperature1);
     w.T = w.T < 0x1p120f ? w.T : w.T >= 0x1p120f ? 0x1p120f : 0.0f;     // (NaN: 0)
-    w.p = uniform(a.top_p ? a.top_p[r] : a.top_p1);
-    w.least = uniform(a.min_p ? a.min_p[r] : a.min_p1);
-    w.k = a.top_k ? __builtin_amdgcn_readfirstlane(a.top_k[r]) : a.top_k1;
-    w.u = uniform(a.u[r]);
+    w.p = uniform(a.top_p ? p : a.top_p1);
+    w.least = uniform(a.min_p ? least : a.min_p1);
+    w.k = a.top_k ? __builtin_amdgcn_readfirstlane(k) : a.top_k1;
+    w.u = uniform(u);
     int log2 = 0;
     while ((1 << log2) < w.V) ++log2;
     w.bits = 62 - log2 < 51 ? 62 - log2 : 51;
@@ -1090,10 +1094,13 @@ __global__ void __launch_bounds__(kThreads) sample_second_kernel(SampleArgs a) {
     const int parts = gridDim.x, part = blockIdx.x;
     const Share s = share_of(a, blockIdx.y, parts);
     Row w = row_of<DT>(a, blockIdx.y);
-    uint32_t best = 0;
+    uint32_t best = 0, bests[kMostParts];               // (all read at once)
     int of = 0, token;
-    for (int y = 0; y < parts; ++y)
-        if (s.best[y] > best) { best = s.best[y]; of = y; }
+#pragma unroll
+    for (int y = 0; y < kMostParts; ++y) bests[y] = s.best[y < parts ? y : 0];
+#pragma unroll
+    for (int y = 0; y < kMostParts; ++y)
+        if (y < parts && bests[y] > best) { best = bests[y]; of = y; }
     w.best = uniform(value_of(__builtin_amdgcn_readfirstlane(best)));
     w.first = static_cast<int>(s.first[of]);
     // what one workgroup does alone
@@ -1115,15 +1122,26 @@ __global__ void __launch_bounds__(kThreads) sample_second_kernel(SampleArgs a) {
     if (w.k_limits() || w.p_limits()) {
         // the parts' bins together, those of a lower best further down
         uint64_t x[kEach] = {0, 0, 0, 0};
-        for (int y = 0; y < parts; ++y) {
-            const float far = w.top - __builtin_rintf(value_of(s.best[y]) * w.per_step);
-            if (!(far < static_cast<float>(kBins))) continue;
-            const int up = static_cast<int>(far);
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int d = kThreads * e + static_cast<int>(threadIdx.x) - up;
-                if (d >= 0) x[e] += s.bins[y * kBins + d];
+        for (int y0 = 0; y0 < kMostParts; y0 += 4) {    // (four parts' at once)
+            if (y0 >= parts) break;
+            uint64_t z[4][kEach];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int y = y0 + j;
+                const float far = w.top - __builtin_rintf(value_of(bests[y]) * w.per_step);
+                const int up = y < parts && far < static_cast<float>(kBins) ? static_cast<int>(far) : kBins;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int d = kThreads * e + static_cast<int>(threadIdx.x) - up;
+                    z[j][e] = s.bins[(y < parts ? y : 0) * kBins + (d < 0 ? 0 : d)];
+                    if (d < 0) z[j][e] = 0;
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) x[e] += z[j][e];
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) sh.bins[kThreads * e + threadIdx.x] = x[e];
