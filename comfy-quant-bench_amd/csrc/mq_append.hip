@@ -14,8 +14,8 @@
 // 29 us, 3.3 TB/s: a workgroup a token has 6 KB, one round of loads between its angles and its scales. 64 single tokens:
 // 3.9 us, chains of dependent loads (length, table, row) and the angles.
 //
-// A row is 8 values a lane on the 2^k lanes that hold it; a
-// lane of a turned row of halves holds four values of each half, so that it has both of a pair.
+// A row is 8 values a lane on the 2^k lanes that hold it; a lane of a turned row of halves holds four values of each half, so
+// that it has both of a pair.
 #include "mq_device.h"
 #include "mq_internal.h"
 
