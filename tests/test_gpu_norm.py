@@ -196,3 +196,21 @@ def test_streams_and_graphs(gpu_device):
         wy, wh = ck.rms_norm(x, None, r)
         wq, ws = ck.rms_norm_quantize(wy)
         assert torch.equal(y, wy) and torch.equal(h, wh) and torch.equal(q, wq) and torch.equal(s, ws)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(1023, 520), (1024, 512), (1024, 513), (1025, 1537), (1100, 2570), (1030, 5000), (1024, 8191), (1500, 3)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows(gpu_device, m, k, dtype):
+    """Where a wave has two pieces of a row instead of one, odd numbers of waves, rows that share a workgroup and its last one."""
+    print(f"[norm] {m} x {k} {dtype}", flush=True)
+    x, r = rows(m, k, dtype, gpu_device, 1), rows(m, k, dtype, gpu_device, 3)
+    y, h = ck.rms_norm(x, None, r)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    check_float(y, h, None, dtype)
+    q, s = ck.rms_norm_quantize(x)
+    check_codes(q, s, x, None, 0)
+    if k > 16:
+        k = k // 16 * 16
+        q, s = ck.rms_norm_quantize(x[:, :k], convrot_groupsize=16)
+        check_codes(q, s, x[:, :k], None, 16)

@@ -233,3 +233,12 @@ def test_two_at_once(gpu_device):
     for t in threads:
         t.join()
     assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys) and len(got[0]) == len(got[1]) == 30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [(1 << 24) - 3, 1 << 24])
+def test_the_longest_rows(gpu_device, vocab):
+    x = logits(1, vocab, torch.bfloat16, 21)
+    check(gpu_device, x, [0.613])
+    check(gpu_device, x, [0.272], top_p=0.9, temperature=0.8)
+    check(gpu_device, x, [0.272], top_k=64)
