@@ -179,7 +179,7 @@ int mq_paged_attention(const void* q, int64_t q_token, int64_t q_head, int dtype
 int64_t mq_kv_shared_ints(int64_t rows) { return rows < 0 || rows >= (kMost >> 4) ? 0 : SharedPlan::ints(rows); }
 
 int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, const int32_t* lens,
-                 int page_size, int32_t* plan, void* stream) {
+                 int page_size, int64_t least_bytes, int32_t* plan, void* stream) {
     clear_error();
     MQ_REQUIRE(rows >= 0 && width >= 0 && rows < (kMost >> 4) && width < kMost, "kv_shared: bad shape rows=%lld width=%lld",
                (long long)rows, (long long)width);
@@ -190,7 +190,9 @@ int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int6
     MQ_REQUIRE(rows == 0 || (lens && aligned(lens, 4)), "kv_shared: lens must be non-null and 4-byte aligned");
     MQ_REQUIRE(rows == 0 || width == 0 || (page_table && aligned(page_table, 4) && ld_table >= width),
                "kv_shared: page_table must be non-null and 4-byte aligned with ld_table >= width");
-    return launch_kv_shared(page_table, ld_table, rows, width, lens, log2_of(page_size), plan, static_cast<hipStream_t>(stream));
+    const int64_t kib = least_bytes < 0 ? 0 : least_bytes >> 10;
+    return launch_kv_shared(page_table, ld_table, rows, width, lens, log2_of(page_size), static_cast<int>(kib < kMost ? kib : kMost), plan,
+                            static_cast<hipStream_t>(stream));
 }
 
 int64_t mq_paged_attention_shared_counters(int64_t Hq, int64_t H, int64_t B) {

@@ -81,12 +81,19 @@ __device__ __forceinline__ int scalar_word(const int* p) {
     return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
 }
 
+// SHARED: whether the groups save enough reading for a kernel of their own. (Otherwise no sequence shares anything: what
+// several read of the same comes from the caches for all but the first.)
+__device__ __forceinline__ bool worth_sharing(const AttnArgs& a) {
+    const int64_t token = static_cast<int64_t>(a.H) * a.D * (a.k_scale ? 2 : 4);
+    return scalar_word(a.plan + 1) * token >= static_cast<int64_t>(scalar_word(a.plan + 2)) << 10;
+}
+
 // SHARED: the keys of sequence b, len of them, that its group's part covers: none if it has lost some of them since
 // (or is empty).
 template <bool SHARED>
 __device__ __forceinline__ int covered(const AttnArgs& a, int b, int len) {
     if constexpr (!SHARED) return 0;
-    const int from = a.start[b];
+    const int from = a.start ? a.start[b] : 0;
     return from > 0 && from <= len ? from : 0;
 }
 
@@ -416,6 +423,8 @@ __global__ void __launch_bounds__(64 * waves_of(DP), waves_of(DP) / 4) attn_deco
     const int group = a.Hq / a.H;
     const int rows_most = group < 16 ? group : 16;
     const int per = a.H * row_tiles, extra = a.B * per > gridDim.x ? kExtra : 0;
+    if constexpr (SHARED)
+        if (!worth_sharing(a)) a.start = nullptr;
     // sequences that see nothing have no tiles: zeros
     for (int e = blockIdx.x; e < a.B; e += gridDim.x) {
         const int len = scalar_word(a.lens + e), from = covered<SHARED>(a, e, len);

@@ -51,7 +51,8 @@ __device__ __forceinline__ int latest(const int* p) { return __hip_atomic_load(p
 
 template <bool ON_CHIP>
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* table, int64_t ld, int B, int width,
-                                                                    const int* lens, int page_shift, int* plan) {
+                                                                    const int* lens, int page_shift, int least_kib, int* plan) {
+    __shared__ unsigned long long saved;
     __shared__ int wave_sum[2][kPlanThreads / 64];
     __shared__ int space[ON_CHIP ? 6 * kPlanRows : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
     int* count = ON_CHIP ? space + 3 * kPlanRows : work + 3 * static_cast<int64_t>(B);     // of a lead: members
     int* rank = ON_CHIP ? space + 5 * kPlanRows : work + 4 * static_cast<int64_t>(B);      // members in front of it
     int* held_by = ON_CHIP ? space + 4 * kPlanRows : start;             // tokens of a sequence
+    if (tid == 0) saved = 0;
     for (int b = tid; b < B; b += kPlanThreads) {
         const int n = lens[b], k = width > 0 ? table[b * ld] : -1;
         key[b] = n > 0 ? k : -1;
@@ -169,6 +171,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
             to[1] = b;
             to[2] = member0 + m - n;
             to[3] = n;
+            atomicAdd(&saved, static_cast<unsigned long long>(n - 1) * keys);
             count[b] = -(member0 + m - n) - 1;      // a group: where its members begin
         }
         group0 += all_g;
@@ -183,7 +186,9 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
     }
     if (tid == 0) {
         plan[0] = group0;
-        plan[1] = plan[2] = plan[3] = 0;
+        plan[1] = saved < 0x7fffffff ? static_cast<int>(saved) : 0x7fffffff;
+        plan[2] = least_kib;
+        plan[3] = 0;
     }
 }
 
@@ -213,7 +218,7 @@ __device__ __forceinline__ Group group_of(const AttnArgs& a, int g) {
 
 __device__ __forceinline__ int groups_of(const AttnArgs& a) {
     const int n = a.plan[0], most = static_cast<int>(a.B) / 2;
-    return n < 0 ? 0 : n < most ? n : most;
+    return n < 0 || !worth_sharing(a) ? 0 : n < most ? n : most;
 }
 
 // The line of tiles (of `tile` keys): a group takes up its tiles for each (cache head, row tile) pair. (Its places fit 32 bits:
@@ -717,9 +722,9 @@ int launch_attn_shared(const AttnArgs& args, hipStream_t stream) {
 }
 
 int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t width, const int* lens, int page_shift,
-                     int* plan, hipStream_t stream) {
+                     int least_kib, int* plan, hipStream_t stream) {
     hipLaunchKernelGGL(rows <= kPlanRows ? shared_plan_kernel<true> : shared_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0,
-                       stream, table, ld_table, static_cast<int>(rows), static_cast<int>(width), lens, page_shift, plan);
+                       stream, table, ld_table, static_cast<int>(rows), static_cast<int>(width), lens, page_shift, least_kib, plan);
     return launch_status("kv_shared");
 }
 

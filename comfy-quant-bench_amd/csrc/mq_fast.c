@@ -117,9 +117,9 @@ ENTRY_F(mq_kv_append, 41,
         fn_mq_kv_append(P(0), L(1), L(2), P(3), L(4), L(5), L(6), P(7), L(8), L(9), P(10), L(11), L(12),
                         I(13), L(14), L(15), L(16), P(17), P(18), I(19), L(20), L(21), L(22), P(23), P(24), L(25), L(26),
                         L(27), L(28), I(29), P(30), L(31), L(32), L(33), P(34), P(35), P(36), L(37), I(38), F(39), P(40)))
-ENTRY(mq_kv_shared, 8,
-      B(0) | B(4) | B(6) | B(7),
-      fn_mq_kv_shared(P(0), L(1), L(2), L(3), P(4), I(5), P(6), P(7)))
+ENTRY(mq_kv_shared, 9,
+      B(0) | B(4) | B(7) | B(8),
+      fn_mq_kv_shared(P(0), L(1), L(2), L(3), P(4), I(5), L(6), P(7), P(8)))
 ENTRY_F(mq_paged_attention_shared, 34,
         B(0) | B(8) | B(9) | B(14) | B(15) | B(21) | B(24) | B(25) | B(27) | B(30) | B(32) | B(33),
         B(26),

@@ -275,9 +275,10 @@ int launch_attn_shared(const AttnArgs& a, hipStream_t stream);
 int64_t attn_shared_workspace_bytes(int Hq, int H, int D, int64_t B);
 int64_t attn_shared_counters(int Hq, int H, int64_t B);
 int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t width, const int* lens, int page_shift,
-                     int* plan, hipStream_t stream);
+                     int least_kib, int* plan, hipStream_t stream);
 
-// The groups of sequences that hold the same first pages, as int32: their number; three words unused; start[b], the
+// The groups of sequences that hold the same first pages, as int32: their number; the tokens that reading each group's
+// once saves; the least of their bytes, in KiB, that is worth it; a word unused; start[b], the
 // tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
 // shared, the sequence whose pages are read, its first member's place and their number; working space.
 struct SharedPlan {

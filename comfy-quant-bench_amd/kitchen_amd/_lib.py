@@ -93,7 +93,7 @@ _SIGNATURES = {
                       c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
                       c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_float, c_vp], c_int),
     "mq_kv_shared_ints": ([c_i64], c_i64),
-    "mq_kv_shared": ([c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp], c_int),
+    "mq_kv_shared": ([c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_i64, c_vp, c_vp], c_int),
     "mq_paged_attention_shared_workspace_bytes": ([c_i64, c_i64, c_i64, c_i64], c_i64),
     "mq_paged_attention_shared_counters": ([c_i64, c_i64, c_i64], c_i64),
     "mq_paged_attention_shared": ([c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_i64,

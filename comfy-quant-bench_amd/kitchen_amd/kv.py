@@ -232,10 +232,18 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     return out
 
 
-def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int) -> torch.Tensor:
+# Keys and values, bytes, that a plan has to save reading for. Sharing costs a launch more and the parts' joining, 8 to 16 us, and
+# saves little time a byte, as the second reading of a page comes from the caches. (us, every sequence alone / shared: 16 / 4
+# heads of 128, 4 over 4096 tokens, 25 MB saved, 20 / 25; 8 groups of 8 over 1024, 117 MB, 25 / 27; 16 over 4096, 126 MB, 33 / 28;
+# 32 / 8 heads, 8 groups of 8 over 256, 59 MB, 21 / 30; over 1024, 235 MB, 42 / 37; int8, 4 over 16384, 101 MB, 41 / 39)
+LEAST_SHARED = 100 << 20
+
+
+def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, least: int | None = None) -> torch.Tensor:
     """Which sequences hold the same first pages (forks of one another), as a plan for paged_attention(shared=): int32 on the
     device, the same for all layers. It holds while sequences grow, and until one is freed or forked to, or a shared entry of
-    the table changes. page_size: the cache's."""
+    the table changes. page_size: the cache's. least: where the plan saves the reading of fewer bytes of keys and values than
+    that (as many as the attention's heads and type make of its tokens), every sequence is attended by itself; None: 100 MiB."""
     dev = _device_of(page_table, "page_table")
     page_table = _apart(page_table)
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
@@ -246,7 +254,7 @@ def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int) -
         raise ValueError(f"kv_lens must be contiguous int32 [{b}] on {dev}")
     plan = torch.empty(_plan_ints(b), dtype=torch.int32, device=dev)
     _lib.call("mq_kv_shared", page_table.data_ptr(), max(page_table.stride(0), width), b, width, kv_lens.data_ptr(),
-              int(page_size), plan.data_ptr(), _lib.stream_of_device(dev))
+              int(page_size), min(max(LEAST_SHARED if least is None else int(least), 0), 1 << 40), plan.data_ptr(), _lib.stream_of_device(dev))
     return plan
 
 
@@ -509,10 +517,10 @@ class PagedKVCache:
         kc, vc, ks, vs = self._layer(layer)
         return kv_append(q, k, v, kc, vc, self.page_table, self.lens if lens is None else lens, rotary, cu_q, ks, vs, out)
 
-    def shared(self, lens: torch.Tensor | None = None) -> torch.Tensor:
+    def shared(self, lens: torch.Tensor | None = None, least: int | None = None) -> torch.Tensor:
         """The plan of the pages that sequences share, for attend: until a sequence is freed or forked to. lens: other lengths than
-        the cache's own (a sequence of length 0 takes no part)."""
-        return kv_shared(self.page_table, self.lens if lens is None else lens, self.page_size)
+        the cache's own (a sequence of length 0 takes no part); least: kv_shared's."""
+        return kv_shared(self.page_table, self.lens if lens is None else lens, self.page_size, least)
 
     def attend(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor | None = None, scale: float | None = None,
                window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,

@@ -556,14 +556,16 @@ int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int6
 /*
  * mq_kv_shared: which sequences hold the same first pages, to plan: int32 [mq_kv_shared_ints(rows)], whose words only
  * mq_paged_attention_shared reads. A group shares the tokens of the longest run of table entries that are equal in all its
- * sequences. mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
+ * sequences; least_bytes: of keys and values that are read once instead of once per sequence, all groups together, below which
+ * nothing is shared (a multiple of 1024 below 2^41; about 100 million is where the additional launch pays).
+ * mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
  * keys and values that a group shares are read once for all of it. The plan holds for any cache and layer with these tables,
  * until a shared entry changes or a sequence that shares them is emptied and filled again; sequences may grow.
  *   workspace, counters: as for mq_paged_attention, with the sizes of the functions below
  */
 int64_t mq_kv_shared_ints(int64_t rows);
 int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int64_t width, const int32_t* lens,
-                 int page_size, int32_t* plan, void* stream);
+                 int page_size, int64_t least_bytes, int32_t* plan, void* stream);
 int64_t mq_paged_attention_shared_workspace_bytes(int64_t Hq, int64_t H, int64_t D, int64_t B);
 int64_t mq_paged_attention_shared_counters(int64_t Hq, int64_t H, int64_t B);
 int mq_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t B, int64_t Hq, int64_t H,

@@ -67,7 +67,7 @@ class Forks:
         return x.permute([perm.index(i) for i in range(4)])
 
     def plan(self):
-        return ck.kv_shared(self.table, self.kv_lens, self.page)
+        return ck.kv_shared(self.table, self.kv_lens, self.page, least=0)
 
     def run(self, plan=None, **kw):
         return ck.paged_attention(self.q, self.k, self.v, self.table, self.kv_lens, k_scale=self.ks, v_scale=self.vs,
@@ -329,6 +329,8 @@ def test_plan_of_anything(gpu_device):
     for i in range(12):
         odd = torch.randint(-3, 40, plan.shape, generator=g, dtype=torch.int32) if i % 3 else torch.randint(-2 ** 31, 2 ** 31 - 1, plan.shape, generator=g, dtype=torch.int64).int()
         odd[0] = (i % 4) * 3
+        if i % 2:
+            odd[1], odd[2] = 2 ** 31 - 1, 0                 # worth sharing
         s.run(odd.to(gpu_device))
     assert torch.equal(s.run(), want)
 
@@ -352,3 +354,18 @@ def test_pages_far_into_a_cache(gpu_device, int8):
         s.ks, s.vs = spread(s.ks), spread(s.vs)
     s.table = torch.where(s.table < 0, s.table, pages - 1 - s.table)
     assert torch.equal(s.run(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+def test_what_sharing_has_to_save(gpu_device, int8):
+    """Below `least` bytes every sequence is attended by itself, bit for bit; at it the groups' are shared."""
+    s = Forks(gpu_device, [(128, [5, 1, 20]), (64, [0, 3]), (0, [70])], 8, 2, 64, page=64, int8=int8)
+    alone = ck.paged_attention(s.q, s.k, s.v, s.table, s.kv_lens, k_scale=s.ks, v_scale=s.vs)
+    shared = s.run()
+    saved = (2 * 128 + 64) * 2 * 64 * 2 * (1 if int8 else 2)
+    assert saved % 1024 == 0 and not torch.equal(alone, shared)
+    for least, want in ((0, shared), (saved, shared), (saved + 1024, alone), (ck.kv.LEAST_SHARED, alone), (1 << 60, alone)):
+        assert torch.equal(s.run(ck.kv_shared(s.table, s.kv_lens, 64, least)), want)
+    assert torch.equal(s.run(ck.kv_shared(s.table, s.kv_lens, 64)), alone)
+    assert read(ck.kv_shared(s.table, s.kv_lens, 64), 6) == read(s.plan(), 6)

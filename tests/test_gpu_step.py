@@ -29,8 +29,9 @@ def forked(config=None, int8=False, seed=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("window", [None, 24])
-def test_forks_share_their_pages(gpu_device, int8, window):
+def test_forks_share_their_pages(gpu_device, monkeypatch, int8, window):
     print(f"[step] int8 {int8} window {window}", flush=True)
+    monkeypatch.setattr(ck.kv, "LEAST_SHARED", 0)
     a, b = (forked(small(window=window, sinks=2 if window else 0), int8) for _ in range(2))
     b.cache.forked = False                          # this one reads every sequence's pages for itself
     plan = a.cache.shared().cpu().tolist()
@@ -62,8 +63,9 @@ def test_sequences_that_sit_a_step_out(gpu_device):
 
 
 @pytest.mark.gpu
-def test_a_step_in_a_graph(gpu_device):
+def test_a_step_in_a_graph(gpu_device, monkeypatch):
     """Growing, attending with a plan, sampling: captured once, replayed with other tokens and random numbers, against eager steps."""
+    monkeypatch.setattr(ck.kv, "LEAST_SHARED", 0)
     a, b = forked(seed=3), forked(seed=3)
     rows = torch.arange(6, dtype=torch.int32, device=gpu_device)
     tokens, u = torch.zeros(6, dtype=torch.int64, device=gpu_device), torch.zeros(6, device=gpu_device)

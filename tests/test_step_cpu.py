@@ -20,7 +20,7 @@ APPEND = dict(q=A, q_token=1024, q_head=128, out=A, o_token=1024, o_head=128, Hq
               v_head=128, dtype=0, T=3, H=4, D=128, kc=A, vc=A, cdt=0, c_page=8192, c_head=2048, c_token=128, ks=None, vs=None,
               s_page=0, s_head=0, s_token=0, pages=9, page=16, table=A, ld=4, B=3, width=4, lens=A, cu=None, freq=A, turn=128,
               interleaved=0, size=1.0, stream=None)
-PLAN = dict(table=A, ld=4, rows=3, width=4, lens=A, page=16, plan=A, stream=None)
+PLAN = dict(table=A, ld=4, rows=3, width=4, lens=A, page=16, least=0, plan=A, stream=None)
 SHARED = dict(q=A, q_token=1024, q_head=128, dtype=0, B=3, Hq=8, H=4, D=128, kc=A, vc=A, cdt=0, c_page=8192, c_head=2048,
               c_token=128, ks=None, vs=None, s_page=0, s_head=0, s_token=0, pages=9, page=16, table=A, ld=4, width=4,
               lens=A, plan=A, scale=0.1, out=A, out_token=1024, out_head=128, work=A, work_bytes=1 << 30, counters=A, stream=None)
