@@ -11,8 +11,9 @@
 // serve all heads from LDS.
 //
 // Memory-bound: each value is read once and written once. 17.5 k tokens of 48 heads of 128 in bf16, 429 MB: 85 us, 5.0 TB/s (a copy 5.1). 8.5 k tokens of 24 heads of 128 into int8, 96 MB:
-// 29 us, 3.3 TB/s: a workgroup a token has 6 KB, one round of loads between its angles and its scales. 64 single tokens:
-// 3.9 us, chains of dependent loads (length, table, row) and the angles.
+// 29 us, 3.3 TB/s beside the angles in fp64 and eight divisions a lane (a row's values loaded in front of the angles, the next
+// row's in front of a row's work: 32 us, 93 instead of 89 into 16 bits). 64 single tokens: 3.9 us, chains of dependent loads
+// (length, table, row) and the angles.
 //
 // A row is 8 values a lane on the 2^k lanes that hold it; a lane of a turned row of halves holds four values of each half, so
 // that it has both of a pair.
