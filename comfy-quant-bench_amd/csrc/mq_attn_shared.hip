@@ -41,8 +41,8 @@ constexpr int kPlanThreads = 1024;
 //
 // Sequences belong together if their first pages are the same; what a group shares is the shortest run of equal pages
 // of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency, of
-// one workgroup (64 sequences of 9000 tokens in pages of 16: 11 us; each row's look for its first with a thread's loop, and a
-// wave's tables one behind the other: 14).
+// one workgroup (64 sequences of 9000 tokens in pages of 16: 11 us, a wave's tables one behind the other 14; 704 sequences that
+// share nothing: 30 us, with a wave for each sequence's look at all the others 104).
 // ON_CHIP: working space in LDS (up to kPlanRows sequences), else behind the plan.
 constexpr int kPlanRows = 2048;
 
@@ -73,24 +73,35 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
         tokens[b] = 0x7fffffff;
         held_by[b] = n;
     }
+    if (ON_CHIP && tid < 8 && B + tid < ((B + 7) & ~7)) key[B + tid] = -2;
     __syncthreads();
-    // a wave a sequence: the first with its first page, how many in front of it have that, how many all in all
-    for (int b = wave; b < B; b += kPlanThreads / 64) {
-        const int k = key[b];
-        int l = -1, before = 0, all = 0;
-        if (k >= 0)
-#pragma unroll 4
-            for (int x0 = 0; x0 < B; x0 += 64) {
-                const int x = x0 + lane;
-                const uint64_t same = __ballot(x < B && key[x < B ? x : 0] == k);
-                if (same && l < 0) l = x0 + __builtin_ctzll(same);
-                all += __builtin_popcountll(same);
-                before += __builtin_popcountll(x0 + 64 <= b ? same : x0 <= b ? same & ((uint64_t(1) << (b - x0)) - 1) : 0);
+    // a lane a sequence: the first with its first page, how many in front of it have that, how many all in all (from the last
+    // sequence down; on chip the list goes on to a multiple of 8 with what no page is)
+    for (int b0 = 64 * wave; b0 < B; b0 += kPlanThreads) {
+        const int b = b0 + lane, k = b < B ? key[b] : -1;
+        int l = -1, in_front = 0, in_wave = 0, behind = 0;
+        auto look = [&](int from, int end, int& n, bool own) __attribute__((always_inline)) {
+            for (int x0 = end - 8; x0 >= from; x0 -= 8) {
+                int other[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) other[x] = key[ON_CHIP || x0 + x < B ? x0 + x : B - 1];
+#pragma unroll
+                for (int x = 7; x >= 0; --x) {
+                    const bool same = other[x] == k && (ON_CHIP || x0 + x < B);
+                    n += same;
+                    if (own) in_wave += same && x0 + x < b;
+                    l = same ? x0 + x : l;
+                }
             }
-        if (lane == 0) {
-            lead[b] = l;
-            rank[b] = before;
-            if (l == b) count[b] = all;
+        };
+        const int end = (B + 7) & ~7, own_end = b0 + 64 < end ? b0 + 64 : end;
+        look(own_end, end, behind, false);
+        look(b0, own_end, behind, true);
+        look(0, b0, in_front, false);
+        if (b < B) {
+            lead[b] = k < 0 ? -1 : l;
+            rank[b] = in_front + in_wave;
+            if (k >= 0 && l == b) count[b] = in_front + behind;
         }
     }
     __syncthreads();

@@ -369,3 +369,14 @@ def test_what_sharing_has_to_save(gpu_device, int8):
         assert torch.equal(s.run(ck.kv_shared(s.table, s.kv_lens, 64, least)), want)
     assert torch.equal(s.run(ck.kv_shared(s.table, s.kv_lens, 64)), alone)
     assert read(ck.kv_shared(s.table, s.kv_lens, 64), 6) == read(s.plan(), 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [7, 8, 9, 63, 64, 65, 127, 129, 705, 1023, 1024, 1025, 2047, 2048, 2049])
+def test_plans_of_many_sequences(gpu_device, rows):
+    g = torch.Generator().manual_seed(rows)
+    table = torch.randint(-1, max(2, rows // 5), (rows, 1), generator=g).repeat(1, 9)
+    table[:, 5] += torch.randint(0, 2, (rows,), generator=g)
+    lens = torch.randint(0, 73, (rows,), generator=g)
+    plan = ck.kv_shared(table.int().to(gpu_device), lens.int().to(gpu_device), 8, least=0)
+    assert read(plan, rows) == step.shared(table.tolist(), lens.tolist(), 8)
