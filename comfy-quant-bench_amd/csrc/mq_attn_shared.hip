@@ -41,7 +41,7 @@ constexpr int kPlanThreads = 1024;
 //
 // Sequences belong together if their first pages are the same; what a group shares is the shortest run of equal pages
 // of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency, of
-// one workgroup (64 sequences of 9000 tokens in pages of 16: 11 us, a wave's tables one behind the other 14; 704 sequences that
+// one workgroup (64 sequences of 9000 tokens in pages of 16: 12 us, a wave's tables one behind the other 14; 704 sequences that
 // share nothing: 30 us, with a wave for each sequence's look at all the others 104).
 // ON_CHIP: working space in LDS (up to kPlanRows sequences), else behind the plan.
 constexpr int kPlanRows = 2048;
