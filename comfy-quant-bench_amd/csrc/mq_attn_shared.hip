@@ -344,12 +344,16 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
     const uint32_t lds_page = __builtin_amdgcn_readfirstlane(lds_offset(sm.page[wave]));
     const float size = __builtin_fabsf(a.scale * kLog2e), scale = size < 0x1p-100f ? 0x1p-100f : size;   // (0 times -infinity)
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-    auto clear = [&] {                                  // what no load writes: keys and values beyond the heads' width
-        if (!I8 && DP > a.D)
+    // What no load writes, keys and values beyond the heads' width. (The zeros go over all of the ring: every wave's are there
+    // before any wave's loads into it are sent for.)
+    auto clear = [&] {
+        if (!I8 && DP > a.D) {
             for (int e = tid; e < Lds::kWide * kTile * DP / 8; e += kThreads) {
                 reinterpret_cast<uint4*>(sm.k)[e] = make_uint4(0, 0, 0, 0);
                 reinterpret_cast<uint4*>(sm.v)[e] = make_uint4(0, 0, 0, 0);
             }
+            __syncthreads();
+        }
     };
     clear();
 
