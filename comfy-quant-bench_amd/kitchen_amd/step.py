@@ -106,7 +106,8 @@ def _setting(value, name: str, rows: int, dtype, device):
     if (value.dtype == dtype) if dtype is torch.int32 else value.is_floating_point():
         value = value.to(dtype).contiguous()
     elif dtype is torch.int32 and value.dtype in (torch.int64, torch.int16, torch.uint8, torch.int8):
-        value = value.clamp(-1, (1 << 31) - 1).to(dtype)
+        # (the bounds are no numbers of the smaller types)
+        value = (value.clamp(-1, (1 << 31) - 1) if value.dtype is torch.int64 else value).to(dtype).contiguous()
     else:
         raise ValueError(f"{name} must be {'whole numbers' if dtype is torch.int32 else 'floating-point'}, got {value.dtype}")
     return value.data_ptr(), 0, value

@@ -1,0 +1,27 @@
+"""The host side of the calls around a step's linears, on the CPU: what settings, classes and shapes they take, and what is handed
+to the library. Host tensors stand for device tensors and nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+import kitchen_amd as ck
+from kitchen_amd import _lib, kv
+from test_step_cpu import host  # noqa: F401  (the library's calls, recorded)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_top_k_of_any_whole_number_type(host, dtype):
+    """The kernel reads int32: every type of whole numbers comes as that, int64 beyond its range at its end."""
+    from kitchen_amd import step
+
+    values = [0, 5, 100] if dtype is torch.uint8 else [-1, 5, 100]
+    _, _, got = step._setting(torch.tensor(values, dtype=dtype), "top_k", 3, torch.int32, torch.device("cpu"))
+    assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == values
+    strided = torch.tensor([v for x in values for v in (x, 1)], dtype=dtype)[::2]
+    assert step._setting(strided, "top_k", 3, torch.int32, torch.device("cpu"))[2].tolist() == values
+    ck.sample(torch.zeros((3, 50)), torch.zeros(3), top_k=torch.tensor(values, dtype=dtype))
+    assert host[-1][0] == "mq_sample"
+    if dtype is torch.int64:
+        far = step._setting(torch.tensor([1 << 40, -(1 << 40), 3]), "top_k", 3, torch.int32, torch.device("cpu"))[2]
+        assert far.tolist() == [(1 << 31) - 1, -1, 3]
