@@ -222,7 +222,8 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     page_table = _apart(page_table)
     tables = _table_args(page_table, kv_lens, cu_q, t, dev)
     if out is None:
-        out = q.new_empty(qs)
+        # a plain tensor whatever q's class (new_empty keeps the class; it is the cheaper call)
+        out = q.new_empty(qs) if type(q) is torch.Tensor else torch.empty(qs, dtype=dtype, device=dev)
     elif out.shape != qs or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
             or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with rows at multiples of 16 bytes")

@@ -25,3 +25,26 @@ def test_top_k_of_any_whole_number_type(host, dtype):
     if dtype is torch.int64:
         far = step._setting(torch.tensor([1 << 40, -(1 << 40), 3]), "top_k", 3, torch.int32, torch.device("cpu"))[2]
         assert far.tolist() == [(1 << 31) - 1, -1, 3]
+
+
+def test_outputs_are_plain_tensors(host, monkeypatch):
+    """The outputs are the library's own buffers, not the class of what goes in."""
+    class Tagged(torch.Tensor):
+        pass
+
+    def tagged(t):
+        return t.as_subclass(Tagged)
+
+    x, w = tagged(torch.zeros((3, 64), dtype=torch.bfloat16)), tagged(torch.ones(64))
+    norms = [ck.rms_norm(x, w), *ck.rms_norm(x, w, x), *ck.rms_norm_quantize(x, w, x), ck.rms_norm(x[:, ::2]),
+             ck.rms_norm(torch.nn.Parameter(torch.zeros(3, 64)))]
+    q = tagged(torch.zeros((3, 8, 64), dtype=torch.bfloat16))
+    cache, table, lens = torch.zeros((5, 8, 16, 64), dtype=torch.bfloat16), torch.zeros((3, 2), dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    turned = ck.kv_append(q, q, q, cache, cache, table, lens, ck.Rotary(64, device="cpu"))
+    monkeypatch.setattr(kv, "_ATTN_WS", {(None, 3, 8, 8, 64, 3, True, False): (0, 0)})
+    attended = ck.paged_attention(q, cache, cache, table, lens, shared=ck.kv_shared(tagged(table), tagged(lens), 16))
+    token = ck.sample(tagged(torch.zeros((3, 50))), tagged(torch.zeros(3)))
+    for y in (*norms, turned, attended, token):
+        assert type(y) is torch.Tensor and not y.requires_grad
+    assert [(type(y), y.dtype, y.shape) for y in (ck.rms_norm(x[:2, :32]), turned)] == \
+        [(torch.Tensor, torch.bfloat16, (2, 32)), (torch.Tensor, torch.bfloat16, (3, 8, 64))]
