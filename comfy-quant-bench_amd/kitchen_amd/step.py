@@ -12,6 +12,8 @@ reads from it.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -38,7 +40,8 @@ def _rows(x: torch.Tensor, what: str, like: torch.Tensor | None = None) -> torch
         raise ValueError(f"{what} needs at least one dimension")
     k = x.shape[-1]
     if x.dim() != 2:
-        x = x.reshape(-1, k)
+        # (rows of no values: how many is not -1's to say)
+        x = x.reshape(-1 if k else math.prod(x.shape[:-1]), k)
     s0, s1 = x.stride()
     if (s1 != 1 and k > 1) or (x.shape[0] > 1 and s0 < k):
         x = x.contiguous()

@@ -48,3 +48,12 @@ def test_outputs_are_plain_tensors(host, monkeypatch):
         assert type(y) is torch.Tensor and not y.requires_grad
     assert [(type(y), y.dtype, y.shape) for y in (ck.rms_norm(x[:2, :32]), turned)] == \
         [(torch.Tensor, torch.bfloat16, (2, 32)), (torch.Tensor, torch.bfloat16, (3, 8, 64))]
+
+
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (2, 3, 0), (2, 0, 5, 0)])
+def test_rows_without_values_are_refused(host, shape):
+    for call in (ck.rms_norm, ck.rms_norm_quantize):
+        for residual in (None, torch.zeros(shape)):
+            with pytest.raises(ValueError, match="rows of 1 to"):
+                call(torch.zeros(shape), residual=residual)
+    assert not host and ck.rms_norm(torch.zeros((2, 0, 5))).shape == (2, 0, 5) and not host
