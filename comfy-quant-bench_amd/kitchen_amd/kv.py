@@ -165,7 +165,7 @@ class Rotary:
     * "linear": every frequency divided by factor
     * "yarn": pairs that turn fewer than beta_slow times over the original context are divided by factor, those of more than
       beta_fast turns stay, linearly between them by their number; queries and keys are multiplied by
-      0.1 ln(factor) + 1 (or by `size`)
+      0.1 ln(factor) + 1, and by 1 for factors below 1 (or by `size`)
 
     The frequencies are held as 64-bit fractions of a turn on the device, so that positions of any size lose nothing."""
 
@@ -189,7 +189,7 @@ class Rotary:
             for i in range(n):
                 part = min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001)))
                 f[i] = f[i] / factor * part + f[i] * (1 - part)
-            own_size = 0.1 * math.log(factor) + 1.0
+            own_size = 0.1 * math.log(max(factor, 1.0)) + 1.0
         elif scaling is not None:
             raise ValueError(f"scaling must be None, 'linear' or 'yarn', got {scaling!r}")
         self.dim, self.interleaved = dim, bool(interleaved)

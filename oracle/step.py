@@ -36,7 +36,7 @@ def frequencies(dim, base=10000.0, scaling=None, factor=1.0, original=4096, fast
     at = dim / 2 * np.log(original / (2 * np.pi * turns)) / np.log(base)
     lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
     part = np.clip((i - lo) / max(hi - lo, 0.001), 0, 1)
-    return f * (part / factor + 1 - part), 0.1 * math.log(factor) + 1
+    return f * (part / factor + 1 - part), 0.1 * math.log(max(factor, 1)) + 1
 
 
 def turn(x, pos, f, size=1.0, interleaved=False):

@@ -1,6 +1,7 @@
 """The host side of the calls around a step's linears, on the CPU: what settings, classes and shapes they take, and what is handed
 to the library. Host tensors stand for device tensors and nothing is launched."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -57,3 +58,14 @@ def test_rows_without_values_are_refused(host, shape):
             with pytest.raises(ValueError, match="rows of 1 to"):
                 call(torch.zeros(shape), residual=residual)
     assert not host and ck.rms_norm(torch.zeros((2, 0, 5))).shape == (2, 0, 5) and not host
+
+
+def test_yarn_of_shorter_contexts_keeps_the_size():
+    """The size makes up for scores over longer contexts: 0.1 ln(factor) + 1 above 1, else 1."""
+    from oracle import step
+
+    for factor, size in ((0.25, 1.0), (0.999, 1.0), (1.0, 1.0), (math.e, 1.1), (math.exp(10), 2.0)):
+        r = ck.Rotary(64, scaling="yarn", factor=factor, device="cpu")
+        assert math.isclose(r.size, size) and math.isclose(step.frequencies(64, scaling="yarn", factor=factor)[1], size)
+    assert ck.Rotary(64, scaling="yarn", factor=0.25, size=0.7, device="cpu").size == 0.7
+    assert ck.Rotary(64, scaling="linear", factor=8.0, device="cpu").size == 1.0
