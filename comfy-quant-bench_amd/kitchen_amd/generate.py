@@ -142,6 +142,12 @@ class Decoder:
         return self._logits(self._forward(tokens, None, lens, cache.shared(lens) if cache.forked else None))
 
 
+def next_tokens(logits: torch.Tensor, u: torch.Tensor, *settings) -> torch.Tensor:
+    """sample's tokens as the next step takes them: a row of logits that holds no number has none (-1), and its sequence goes on
+    with token 0."""
+    return step.sample(logits, u, *settings).clamp_(min=0)
+
+
 def main(argv: list[str] | None = None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--prompts", type=int, default=4)
@@ -184,7 +190,7 @@ def main(argv: list[str] | None = None) -> int:
             live = cache.compact()
             rows = rows[:-a.prompts]
             print(f"{int(live)} pages are held after {a.prompts} sequences ended")
-        tokens = step.sample(model.step(tokens, rows), u[i], a.temperature, a.top_k, a.top_p, a.min_p)
+        tokens = next_tokens(model.step(tokens, rows), u[i], a.temperature, a.top_k, a.top_p, a.min_p)
         answers.append(tokens)
     cache.check()
     t3 = clock()
