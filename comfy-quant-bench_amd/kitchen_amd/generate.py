@@ -139,7 +139,7 @@ class Decoder:
         cache, before = self.cache, self.cache.lens.clone()
         cache.grow(rows, torch.ones_like(rows))
         lens = cache.lens * (cache.lens > before)        # nothing is written where nothing has grown
-        return self._logits(self._forward(tokens, None, lens, cache.shared(lens) if cache.forked else None))
+        return self._logits(self._forward(tokens, None, lens, cache.shared(lens) if cache.may_share() else None))
 
 
 def next_tokens(logits: torch.Tensor, u: torch.Tensor, *settings) -> torch.Tensor:
