@@ -191,7 +191,8 @@ int mq_kv_shared(const int32_t* page_table, int64_t ld_table, int64_t rows, int6
     MQ_REQUIRE(rows == 0 || width == 0 || (page_table && aligned(page_table, 4) && ld_table >= width),
                "kv_shared: page_table must be non-null and 4-byte aligned with ld_table >= width");
     const int64_t kib = least_bytes < 0 ? 0 : least_bytes >> 10;
-    return launch_kv_shared(page_table, ld_table, rows, width, lens, log2_of(page_size), static_cast<int>(kib < kMost ? kib : kMost), plan,
+    const int least_kib = kib < SharedPlan::kNever ? static_cast<int>(kib) : SharedPlan::kNever;
+    return launch_kv_shared(page_table, ld_table, rows, width, lens, log2_of(page_size), least_kib, plan,
                             static_cast<hipStream_t>(stream));
 }
 

@@ -85,7 +85,8 @@ __device__ __forceinline__ int scalar_word(const int* p) {
 // several read of the same comes from the caches for all but the first.)
 __device__ __forceinline__ bool worth_sharing(const AttnArgs& a) {
     const int64_t token = static_cast<int64_t>(a.H) * a.D * (a.k_scale ? 2 : 4);
-    return scalar_word(a.plan + 1) * token >= static_cast<int64_t>(scalar_word(a.plan + 2)) << 10;
+    const int least = scalar_word(a.plan + 2);
+    return least != SharedPlan::kNever && scalar_word(a.plan + 1) * token >= static_cast<int64_t>(least) << 10;
 }
 
 // SHARED: the keys of sequence b, len of them, that its group's part covers: none if it has lost some of them since

@@ -278,11 +278,11 @@ int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t w
                      int least_kib, int* plan, hipStream_t stream);
 
 // The groups of sequences that hold the same first pages, as int32: their number; the tokens that reading each group's
-// once saves; the least of their bytes, in KiB, that is worth it; a word unused; start[b], the
+// once saves; the least of their bytes, in KiB, that is worth it (kNever: no number of them); a word unused; start[b], the
 // tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
 // shared, the sequence whose pages are read, its first member's place and their number; working space.
 struct SharedPlan {
-    static constexpr int kHead = 4, kGroup = 4;
+    static constexpr int kHead = 4, kGroup = 4, kNever = 0x7fffffff;
     static int64_t ints(int64_t B) { return kHead + 9 * B; }
     __host__ __device__ static int64_t start() { return kHead; }
     __host__ __device__ static int64_t members(int64_t B) { return kHead + B; }

@@ -255,7 +255,7 @@ def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, l
         raise ValueError(f"kv_lens must be contiguous int32 [{b}] on {dev}")
     plan = torch.empty(_plan_ints(b), dtype=torch.int32, device=dev)
     _lib.call("mq_kv_shared", page_table.data_ptr(), max(page_table.stride(0), width), b, width, kv_lens.data_ptr(),
-              int(page_size), min(max(LEAST_SHARED if least is None else int(least), 0), 1 << 40), plan.data_ptr(), _lib.stream_of_device(dev))
+              int(page_size), min(max(LEAST_SHARED if least is None else int(least), 0), (1 << 63) - 1), plan.data_ptr(), _lib.stream_of_device(dev))
     return plan
 
 

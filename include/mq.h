@@ -557,7 +557,8 @@ int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int6
  * mq_kv_shared: which sequences hold the same first pages, to plan: int32 [mq_kv_shared_ints(rows)], whose words only
  * mq_paged_attention_shared reads. A group shares the tokens of the longest run of table entries that are equal in all its
  * sequences; least_bytes: of keys and values that are read once instead of once per sequence, all groups together, below which
- * nothing is shared (a multiple of 1024 below 2^41; about 100 million is where the additional launch pays).
+ * nothing is shared (in units of 1024, rounded down; from 2^41 - 1024 on: nothing ever is; about 100 million is where the
+ * additional launch pays).
  * mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
  * keys and values that a group shares are read once for all of it. The plan holds for any cache and layer with these tables,
  * until a shared entry changes or a sequence that shares them is emptied and filled again; sequences may grow.
