@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int* ta
         plan[0] = group0;
         plan[1] = saved < 0x7fffffff ? static_cast<int>(saved) : 0x7fffffff;
         plan[2] = least_kib;
-        plan[3] = 0;
+        plan[3] = page_shift;
     }
 }
 

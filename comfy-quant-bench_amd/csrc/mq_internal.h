@@ -278,8 +278,8 @@ int launch_kv_shared(const int* table, int64_t ld_table, int64_t rows, int64_t w
                      int least_kib, int* plan, hipStream_t stream);
 
 // The groups of sequences that hold the same first pages, as int32: their number; the tokens that reading each group's
-// once saves; the least of their bytes, in KiB, that is worth it (kNever: no number of them); a word unused; start[b], the
-// tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
+// once saves; the least of their bytes, in KiB, that is worth it (kNever: no number of them); log2 of the page size; start[b],
+// the tokens of sequence b that its group shares (0: none); the groups' members behind each other; for each group the tokens
 // shared, the sequence whose pages are read, its first member's place and their number; working space.
 struct SharedPlan {
     static constexpr int kHead = 4, kGroup = 4, kNever = 0x7fffffff;

@@ -243,8 +243,9 @@ LEAST_SHARED = 100 << 20
 def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, least: int | None = None) -> torch.Tensor:
     """Which sequences hold the same first pages (forks of one another), as a plan for paged_attention(shared=): int32 on the
     device, the same for all layers. It holds while sequences grow, and until one is freed or forked to, or a shared entry of
-    the table changes. page_size: the cache's. least: where the plan saves the reading of fewer bytes of keys and values than
-    that (as many as the attention's heads and type make of its tokens), every sequence is attended by itself; None: 100 MiB."""
+    the table changes. page_size: the cache's (with another one nothing is shared). least: where the plan saves the reading of fewer
+    bytes of keys and values than that (as many as the attention's heads and type make of its tokens), every sequence is attended by
+    itself; None: 100 MiB."""
     dev = _device_of(page_table, "page_table")
     page_table = _apart(page_table)
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):

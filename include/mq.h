@@ -561,7 +561,8 @@ int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int6
  * additional launch pays).
  * mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
  * keys and values that a group shares are read once for all of it. The plan holds for any cache and layer with these tables,
- * until a shared entry changes or a sequence that shares them is emptied and filled again; sequences may grow.
+ * until a shared entry changes or a sequence that shares them is emptied and filled again; sequences may grow. A plan of another
+ * page size than the cache's shares nothing.
  *   workspace, counters: as for mq_paged_attention, with the sizes of the functions below
  */
 int64_t mq_kv_shared_ints(int64_t rows);
