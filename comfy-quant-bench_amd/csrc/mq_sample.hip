@@ -696,6 +696,14 @@ __device__ __forceinline__ Limit limit_by_digits(const Row& w, int bin, Limit no
             }
         });
         __syncthreads();
+        if (shift == 24) {
+            // no more than there is: `need` may come from the bin's mass, which these units' sum misses by a few
+            uint64_t all = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) all += sh.work[kThreads * e + threadIdx.x];
+            all = block_sum(all, sh);
+            need = need < all ? need : all;
+        }
         const int d = cut<uint64_t>([&](int i) { return sh.work[i]; }, need, &need, nullptr, sh);
         prefix |= static_cast<uint32_t>(255 - (d < 256 ? d : 255)) << shift;
         if (d >= 256) need = 1;
