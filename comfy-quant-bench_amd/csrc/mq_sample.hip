@@ -8,13 +8,16 @@
 // in every order, so the result does not depend on how a row is split or on which atomic comes first. (With fp32 weights the
 // sum of a hundred thousand of them would be off by more than the share of a single token; a fp64 exponential for every
 // value takes four times as long as all of the rest.) A weight is a table's entry (fp64, 1e-15) for the nearest multiple of a
-// power of two, `step`, of which 4096 reach as far down as anything weighs (32 T), times 1 + e for the rest of l: that is
-// exact in fp32, below T / 128, and its series takes four fp32 products: 1e-9 at most, of random signs.
+// power of two, `step`, of which 4096 reach as far down as anything weighs ((B + 1) ln 2 T: 32 T for V = 2^17, 36 T for short
+// rows), times 1 + e for the rest of l: that is exact in fp32, below T / 110, and its series takes four fp32 products. A weight is off
+// by 2e-9 of itself and a unit at most.
 //
 // First reading: the largest value, and numbers and masses of the 4096 bins around those multiples below it, in LDS. The
 // bins are places n modulo 4096, so that they stay where they are as the largest value seen rises; those that fall out of
 // reach are cleared. A bin is one 64-bit sum: a value adds 1 in the upper bits and 2^fine (e + 1/32) in the lower ones; the bin's
-// mass is its centre's weight times (number + sum of e). Sums over the bins from the top say which bin the limit cuts.
+// mass is its centre's weight times (number + sum of e). Sums over the bins from the top say which bin the limit cuts. (2^fine
+// leaves room for V values: 2^33 up to V = 2^17. What a value adds is rounded to fp32 and to a whole number, so masses are off by 4e-9
+// of themselves up to V = 2^19, beyond that by 2^(2 log2(V) - 68), 1e-6 at 2^24.)
 //
 // Second reading: where k limits a row (few values), those of the cut bin and above, into LDS, where everything else is decided;
 // where p does, those of the cut bin alone and the masses of what is above it by blocks of 8192; without either, the masses of
@@ -123,8 +126,12 @@ __device__ __forceinline__ void scan(const void* row, int b, int e, F f) {
     }
 }
 
+// What makes a number of units an fp64 whose last place is 1 (below 2^51.02 they are), and the number back.
+constexpr double kUnits = 0x1p52;
+__device__ __forceinline__ uint64_t units_of(double x) { return __builtin_bit_cast(uint64_t, x) & 0xfffffffffffffull; }
+
 struct Lds {
-    uint64_t weight[kBins];         // of the bins' centres in units, from the best's down
+    double weight[kBins];           // of the bins' centres in units, from the best's down, each kUnits more
     uint64_t bins[kBins + 64];      // first by place (n modulo 4096, and a place for each lane's values that are in none), then
                                     // masses from the best's down; blocks' masses
     alignas(16) uint64_t work[kBins];   // sums over ranges; a few values side by side
@@ -330,13 +337,14 @@ struct Row {
         const float e = __builtin_fmaf(x, 1.0f / 6.0f, 0.5f);
         return __builtin_fmaf(e, x, 1.0f) * x;
     }
-    // A value's weight in units, from the table: the bin's and e times that, both to 31 fractional bits (0 out of reach).
+    // A value's weight in units, from the table (0 out of reach): the bin's c and e c, added where an fp64's last place is a unit, so
+    // that the sum's rounding is the only one. (c's upper 30 bits times e in integers, the rest of c left out, put weights of 2^-22
+    // of the largest off by 1e-5 and those of 2^-32 by 4e-3; with the rest 256 rows of 131072 took 81 us instead of 76.)
     __device__ __forceinline__ uint64_t units(float v, const Lds& sh) const {
         const float d = depth(v), e = excess(v);
         const bool in = d < static_cast<float>(kBins);
-        const uint64_t c = sh.weight[in ? static_cast<int>(d) : kMask];
-        const int64_t more = static_cast<int64_t>(static_cast<int32_t>(c >> (bits - 30))) * static_cast<int32_t>(e * 0x1p31f);
-        return in ? c + static_cast<uint64_t>(more >> (61 - bits)) : 0;
+        const double c = sh.weight[in ? static_cast<int>(d) : kMask];
+        return in ? units_of(__builtin_fma(static_cast<double>(e), c - kUnits, c)) : 0;
     }
     // The same from its own exponential.
     __device__ __forceinline__ uint64_t units(float v) const {
@@ -425,7 +433,7 @@ __device__ __forceinline__ void bins_of(Row& w, int b, int e, bool known, int* b
     const int mine = kPer * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < kBins + 64; i += kThreads) sh.bins[i] = 0;
     const uint64_t one = uint64_t{1} << w.number;
-    const float scale = uniform(__builtin_ldexpf(1.0f, w.fine)), bias = uniform(kBias * scale);
+    const float scale = uniform(__builtin_ldexpf(1.0f, w.fine)), bias = uniform(kBias * scale + 0.5f);    // (rounded, where fp32 has halves)
     int at = 0, parity = 0;
     float top = known ? w.top : kNone;
     uint32_t best = key_of(kNone);
@@ -512,7 +520,7 @@ __device__ __forceinline__ void weigh_bins(const Row& w, Lds& sh) {
     if (threadIdx.x == 128)
         small[128] = exp2((static_cast<double>(w.top) * static_cast<double>(w.step) - static_cast<double>(w.best)) * (1.4426950408889634074 / static_cast<double>(w.T)) + w.bits);
     __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.weight[b] = static_cast<uint64_t>(__builtin_rint(small[128] * small[64 + (b >> 6)] * small[b & 63]));
+    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.weight[b] = __builtin_rint(small[128] * small[64 + (b >> 6)] * small[b & 63]) + kUnits;
     __syncthreads();
 }
 
@@ -525,7 +533,7 @@ __device__ __forceinline__ void masses_of(const Row& w, int base, Lds& sh) {
         const uint64_t s = sh.bins[(base + d) & kMask], part = s & ((uint64_t{1} << w.number) - 1);
         const double n = static_cast<double>(s >> w.number);
         const double sum = static_cast<double>(part) * __builtin_ldexp(1.0, -w.fine) - n * static_cast<double>(kBias);
-        x[e] = static_cast<uint64_t>(__builtin_rint(static_cast<double>(sh.weight[d]) * (n + sum)));
+        x[e] = static_cast<uint64_t>(__builtin_rint((sh.weight[d] - kUnits) * (n + sum)));
     }
     __syncthreads();
 #pragma unroll

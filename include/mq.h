@@ -584,8 +584,9 @@ int mq_paged_attention_shared(const void* q, int64_t q_token, int64_t q_head, in
  * part whose weight reaches top_p of theirs (>= 1: all; at least one), of those w_i >= min_p; the token is the first i, in
  * the order of i, whose kept weight up to i exceeds u times all kept weight. T < 2^-100 (or NaN): the first largest. Logits that
  * are NaN count as -infinity; a row without any other gets -1; where +infinities are, only they have weight. u below
- * 0 (or NaN) counts as 0, u >= 1 takes the last one kept. Weights are off by 1e-9 of themselves at most, their sums exact in
- * units of 2^-45 of the largest for V = 2^17 (2^(log2(V) - 62), at least 2^-51): the same inputs always give the same token.
+ * 0 (or NaN) counts as 0, u >= 1 takes the last one kept. Weights are off by 2e-9 of themselves and a unit at most, a unit being
+ * 2^-45 of the largest for V = 2^17 (2^(log2(V) - 62), at least 2^-51), and their sums exact; those that say where top_p cuts are off
+ * by 4e-9 of themselves more up to V = 2^19, beyond that by 2^(2 log2(V) - 68). The same inputs always give the same token.
  *   logits [rows, V] of type dtype (bf16, fp16, fp32), row stride ld, V <= 2^24; temperature, top_p, min_p fp32 [rows]
  *   and top_k int32 [rows], or NULL for the value *_all of every row
  *   workspace: mq_sample_workspace_bytes(rows, V) bytes, 16-byte aligned (nothing in it has to start at zero)

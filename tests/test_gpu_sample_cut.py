@@ -43,3 +43,31 @@ def test_a_cut_next_to_the_end_of_thousands_alike(gpu_device, case, rows):
     for y, t in zip(u, want):
         got = ck.sample(logits, torch.full((rows,), float(y), device=gpu_device), top_p=0.5)
         assert got.tolist() == [t] * rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [-15.03, -15.71, -16.22, -16.64, -17.05, -17.4])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_tokens_among_small_weights(gpu_device, v, rows):
+    """A best value (weight 1) and n = 131071 equal ones of weight w = 2^-25.1 to 2^-21.7 behind it: where token i is chosen, u lies
+    (1 - u) / w = n - i weights in front of the end of all of them. A weight off by 2e-9 of itself and a unit (2^-45) moves that
+    place by (n - i) (2e-9 + 2^-45 / w) <= 0.14 tokens at w = 2^-25.1, so a place in the middle third of a token stays in it."""
+    vocab = 1 << 17
+    x = np.full(vocab, np.float32(v), dtype=np.float32)
+    x[0] = 0.0
+    w, n = float(np.exp(np.float64(x[1]))), vocab - 1
+    us = []
+    for i in (3, 70, 1000, 20000, 65536, 100000, 131000):
+        u = np.float32((1 + (i + 0.5) * w) / (1 + n * w))
+        for _ in range(64):                             # the next one whose place is in the middle third
+            at = (float(u) * (1 + n * w) - 1) / w
+            if 1 / 3 < at % 1 < 2 / 3 and 0 < at < n:
+                us.append((u, 1 + int(at)))
+                break
+            u = np.nextafter(u, np.float32(0 if i == 131000 else 2))
+    assert len(us) == 7
+    logits = torch.from_numpy(x).to(gpu_device).expand(rows, -1)
+    logits = logits if rows == 1 else logits.contiguous()
+    for u, t in us:
+        assert step.sample(x, u) == t                    # the oracle's sums of fp64 say the same
+        assert ck.sample(logits, torch.full((rows,), float(u), device=gpu_device)).tolist() == [t] * rows, (float(u), t)
