@@ -11,8 +11,12 @@
 //
 //   S^T = K Q^T, O^T = V^T P^T   products of 32 x 32 x 16. A wave has 32 rows, one a lane (and its partner), as B and P^T's
 //                                operand straight from S^T's registers, as in mq_attn_prompt.hip
-//   softmax                      base 2, fp32; the reference maximum of a row moves (and its sums are rescaled) only when
-//                                the row's maximum passes it by 2^8
+//   softmax                      base 2, fp32, against a row's running maximum; its sums are rescaled where it moves. The
+//                                probabilities are rounded to the products' 16 bits as in the single-token kernel, the largest
+//                                exact. (Moving only when the maximum passes its reference by 2^8, with fp16 probabilities held
+//                                2^8 smaller for it: 2 % faster, but the output is off by 2.09e-3 instead of 1.85e-3 in bf16, where
+//                                rounding it alone is 1.65e-3, and by 2.58e-4 instead of 2.32e-4 in fp16, and fp16
+//                                probabilities below 2^-20 of the largest lose bits.)
 //
 // All rows of a group see all of its shared keys, so what is hidden (behind the shared length, in pages that are none) is
 // hidden from every row.
@@ -314,9 +318,8 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
     static_assert(kPages >= 2 * kRing - 1);
     constexpr bool kSplit = I8 && DT == kDtF16;         // fp16 rows against int8 keys: bf16 products of hi + lo
     constexpr int MT = I8 ? kDtBf16 : DT;               // type of the products
-    constexpr float kSlack = 8.0f;                      // how far a row's maximum may pass its reference (log2)
-    constexpr float kLift = MT == kDtF16 ? 6.0f : 0.0f; // fp16 probabilities are held 2^6 times as large, ...
-    constexpr float kShift = MT == kDtF16 ? 8.0f : 0.0f;    // ... by 2^8 less than in the single-token kernel, which adds these
+    // fp16 probabilities are held 2^14 times as large, as in the single-token kernel, which adds these
+    constexpr float kLift = MT == kDtF16 ? 14.0f : 0.0f;
     constexpr int kSteps = DP / 16;                     // products over the width
     constexpr int kBlocks = DP / 32;                    // value blocks of the output
     constexpr int kV = 16 / E;                          // values of a 16-byte chunk in the cache
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
 #pragma unroll
             for (int x = 0; x < 16; ++x) top = __builtin_fmaxf(top, s[x]);
             top = max2(top) * scale;
-            const bool move = top > m + kSlack;
+            const bool move = top > m;
             if (__ballot(move)) {
                 const float f = move ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
                 m = move ? top : m;
@@ -669,7 +672,7 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), 1) attn_shared_kernel(Att
                         if (d < a.D)
                             *reinterpret_cast<float4*>(to + d) = make_float4(o[i][4 * r4], o[i][4 * r4 + 1], o[i][4 * r4 + 2], o[i][4 * r4 + 3]);
                     }
-                if (hf == 0) *reinterpret_cast<float2*>(stat) = make_float2(m + kShift, any ? l : -1.0f);
+                if (hf == 0) *reinterpret_cast<float2*>(stat) = make_float2(m, any ? l : -1.0f);
             }
             if (hf == 0 && seq >= 0 && i0 == 0)
                 reinterpret_cast<int4*>(a.shared_rows)[at] = make_int4(static_cast<int>(slot), complete ? -1 : (s0 + nt - 1) / piece, row, 0);
