@@ -317,6 +317,10 @@ struct W4A16Args {
 int launch_w4a16(const W4A16Args& a, hipStream_t stream);
 
 
+// Threads of a launch along x at most: the runtime counts them in 32 bits, and with more leaves workgroups out without an error.
+// Calls of more rows than that go in several launches.
+constexpr int64_t kMostThreads = int64_t(1) << 31;
+
 // --- norms (mq_norm.hip)
 struct NormArgs {
     const void* x;            // [M, K] of type dtype

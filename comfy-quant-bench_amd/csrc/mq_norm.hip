@@ -267,7 +267,8 @@ int launch_units(const NormArgs& a, int waves, hipStream_t stream) {
     // rows of a few waves share a workgroup of four
     const int rows = waves < 4 ? 4 / waves : 1;
     const size_t lds = BLK > 0 ? sizeof(float) * kTrWave * waves * rows : 0;
-    const int64_t groups = (a.M + rows - 1) / rows;
+    const int64_t most = kMostThreads / (64 * waves * rows) * rows;         // rows of a launch
+    const int64_t es = DT == kDtF32 ? 4 : 2;
     auto kern = norm_kernel<DT, BLK, UNITS>;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(lds)) != hipSuccess) {
@@ -275,7 +276,16 @@ int launch_units(const NormArgs& a, int waves, hipStream_t stream) {
         set_error("rms_norm: cannot reserve %zu bytes of LDS", lds);
         return -3;
     }
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(groups)), dim3(64 * waves * rows), lds, stream, a, waves);
+    for (int64_t m = 0; m < a.M; m += most) {
+        NormArgs b = a;
+        b.x = static_cast<const char*>(a.x) + m * a.ldx * es;
+        b.r = a.r ? static_cast<const char*>(a.r) + m * a.ldr * es : nullptr;
+        b.h = a.h ? static_cast<char*>(a.h) + m * a.ldh * es : nullptr;
+        b.y = static_cast<char*>(a.y) + m * a.ldy * (BLK >= 0 ? 1 : es);
+        b.s = a.s ? a.s + m : nullptr;
+        b.M = a.M - m < most ? a.M - m : most;
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((b.M + rows - 1) / rows)), dim3(64 * waves * rows), lds, stream, b, waves);
+    }
     return launch_status("rms_norm");
 }
 
