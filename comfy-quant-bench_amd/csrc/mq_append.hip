@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppendArgs a) {
     __shared__ float2 turn[kMostPairs];
     const KvWriteArgs& w = a.w;
     const int lanes = 1 << w.row_shift;                     // lanes per row
-    const int64_t t = blockIdx.x;
+    const int64_t t = a.first + blockIdx.x;
     int64_t b = t, pos;
     if (w.cu_q) {
         // the sequence of token t: cu_q[b] <= t < cu_q[b + 1]
@@ -146,10 +146,14 @@ template <int DT>
 int launch_type(const KvAppendArgs& a, bool i8, hipStream_t stream) {
     // workgroups: one a token, and for few tokens as many as have rows for all their lanes
     const int64_t rows = a.Hq + 2 * a.w.H, per = 256 >> a.w.row_shift;
-    const int64_t steps = (rows + per - 1) / per, want = (1024 + a.w.T - 1) / a.w.T;
-    const dim3 grid(static_cast<unsigned>(a.w.T), static_cast<unsigned>(steps < want ? steps : want));
-    if (i8) hipLaunchKernelGGL((kv_append_kernel<DT, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((kv_append_kernel<DT, false>), grid, dim3(256), 0, stream, a);
+    const int64_t steps = (rows + per - 1) / per, want = (1024 + a.w.T - 1) / a.w.T, most = kMostThreads / 256;
+    for (int64_t t = 0; t < a.w.T; t += most) {
+        KvAppendArgs b = a;
+        b.first = t;
+        const dim3 grid(static_cast<unsigned>(a.w.T - t < most ? a.w.T - t : most), static_cast<unsigned>(steps < want ? steps : want));
+        if (i8) hipLaunchKernelGGL((kv_append_kernel<DT, true>), grid, dim3(256), 0, stream, b);
+        else hipLaunchKernelGGL((kv_append_kernel<DT, false>), grid, dim3(256), 0, stream, b);
+    }
     return launch_status("kv_append");
 }
 

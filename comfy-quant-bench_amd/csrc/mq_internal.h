@@ -185,6 +185,10 @@ struct KvWriteArgs {
 };
 int launch_kv_write(const KvWriteArgs& a, int dtype, bool i8, hipStream_t stream);
 
+// Threads of a launch along x at most: the runtime counts them in 32 bits, and with more leaves workgroups out without an error.
+// Calls of more rows than that go in several launches.
+constexpr int64_t kMostThreads = int64_t(1) << 31;
+
 // --- new tokens turned by their positions and written (mq_append.hip)
 struct KvAppendArgs {
     KvWriteArgs w;
@@ -197,6 +201,7 @@ struct KvAppendArgs {
     int turn;                 // values of a head that are turned
     int interleaved;          // pairs are neighbours, else halves
     float size;               // what cosines and sines are multiplied by
+    int64_t first;            // the first token of a launch
 };
 int launch_kv_append(const KvAppendArgs& a, int dtype, bool i8, hipStream_t stream);
 
@@ -316,10 +321,6 @@ struct W4A16Args {
 };
 int launch_w4a16(const W4A16Args& a, hipStream_t stream);
 
-
-// Threads of a launch along x at most: the runtime counts them in 32 bits, and with more leaves workgroups out without an error.
-// Calls of more rows than that go in several launches.
-constexpr int64_t kMostThreads = int64_t(1) << 31;
 
 // --- norms (mq_norm.hip)
 struct NormArgs {
