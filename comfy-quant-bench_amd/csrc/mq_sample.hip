@@ -1218,7 +1218,19 @@ template <int DT>
 int launch_type(const SampleArgs& a, hipStream_t stream) {
     const int parts = parts_of(a.rows, a.V);
     if (parts == 1) {
-        hipLaunchKernelGGL((sample_kernel<DT>), dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, stream, a);
+        constexpr int64_t most = kMostThreads / kThreads;
+        for (int64_t r = 0; r < a.rows; r += most) {
+            SampleArgs b = a;
+            b.x = static_cast<const char*>(a.x) + r * a.ld * (DT == kDtF32 ? 4 : 2);
+            b.u = a.u + r;
+            b.temperature = a.temperature ? a.temperature + r : nullptr;
+            b.top_p = a.top_p ? a.top_p + r : nullptr;
+            b.min_p = a.min_p ? a.min_p + r : nullptr;
+            b.top_k = a.top_k ? a.top_k + r : nullptr;
+            b.token = a.token + r;
+            b.rows = a.rows - r < most ? a.rows - r : most;
+            hipLaunchKernelGGL((sample_kernel<DT>), dim3(static_cast<unsigned>(b.rows)), dim3(kThreads), 0, stream, b);
+        }
     } else {
         const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(a.rows));
         hipLaunchKernelGGL((sample_first_kernel<DT>), grid, dim3(kThreads), 0, stream, a);

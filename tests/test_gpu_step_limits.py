@@ -49,3 +49,18 @@ def test_appends_of_many_tokens(gpu_device, ragged):
         kd, vd = torch.zeros_like(kc), torch.zeros_like(vc)
         assert torch.equal(y[n], ck.kv_append(q[n], k[n], v[n], kd, vd, table, end, rotary, few))
         assert torch.equal(kc.view(-1, d)[n], kd.view(-1, d)[n])
+
+
+@pytest.mark.gpu
+def test_tokens_of_many_rows(gpu_device):
+    """2^22 rows and some, 1024 threads each, with settings of their own."""
+    rows, vocab, n = (1 << 22) + 3, 5, 1 << 14
+    g = torch.Generator(device=gpu_device).manual_seed(0)
+    x = torch.randn((n, vocab), generator=g, device=gpu_device).repeat(rows // n + 1, 1)[:rows].contiguous()
+    u = torch.rand(n, generator=g, device=gpu_device).repeat(rows // n + 1)[:rows].contiguous()
+    t = torch.rand(n, generator=g, device=gpu_device).repeat(rows // n + 1)[:rows].contiguous()
+    k = torch.randint(0, 5, (n,), generator=g, device=gpu_device, dtype=torch.int32).repeat(rows // n + 1)[:rows].contiguous()
+    y = ck.sample(x, u, t, k, t, t / 4)
+    first = ck.sample(x[:n], u[:n], t[:n], k[:n], t[:n], t[:n] / 4)
+    assert torch.equal(y, first.repeat(rows // n + 1)[:rows])
+    assert torch.equal(ck.sample(x, u, 0.0), x.argmax(-1))
