@@ -244,6 +244,8 @@ int mq_quantize_weight_checked(const void* w, int dtype, int64_t N, int64_t K, i
     MQ_REQUIRE(N < (int64_t(1) << 31), "quantize_weight: N too large");
     MQ_REQUIRE(K <= 32768, "quantize_weight: K=%lld exceeds 32768", (long long)K);
     const bool group = format == MQ_WFMT_U4_ASYM_G64 || format == MQ_WFMT_I4_SYM_G64;
+    // (256 threads a row, and a launch's are counted in 32 bits)
+    MQ_REQUIRE(group || N < (int64_t(1) << 24), "quantize_weight: N too large");
     MQ_REQUIRE(group ? K % 64 == 0 : K % 16 == 0, "quantize_weight: K=%lld must be a multiple of %d", (long long)K,
                group ? 64 : 16);
     MQ_REQUIRE(hblock == 0 || hblock == 16 || hblock == 64 || hblock == 256,

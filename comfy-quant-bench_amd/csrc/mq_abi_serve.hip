@@ -76,7 +76,8 @@ int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, i
     MQ_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16) && k_token % 8 == 0 && k_head % 8 == 0 && v_token % 8 == 0 &&
                    v_head % 8 == 0,
                "kv_write: k and v need 16-byte aligned bases and rows that start at multiples of 16 bytes");
-    MQ_REQUIRE(T * H < (int64_t(1) << 33), "kv_write: too many rows");
+    // (a launch's threads are counted in 32 bits; a row has one for every 8 values, up to a power of two)
+    MQ_REQUIRE(T < 2 * kMost / H && (T * H) << log2_of((D + 7) / 8) <= 2 * kMost - 256, "kv_write: too many rows");
     KvWriteArgs a{};
     a.k = k; a.v = v; a.k_token = k_token; a.k_head = k_head; a.v_token = v_token; a.v_head = v_head;
     a.T = T; a.H = H; a.D = D; a.kc = k_cache; a.vc = v_cache; a.c_page = c_page; a.c_head = c_head; a.c_token = c_token;
