@@ -299,8 +299,10 @@ int launch_block(const NormArgs& a, hipStream_t stream) {
     // rotated 64 x 4096 4.7 / 6.4, 2048 x 4096 14.4 / 15.7; fp32, twice the registers, 8192 x 2560 68 / 74.)
     const bool two = BLK <= 0 && DT != kDtF32 && (pieces >= 16 || (a.M >= kManyRows && pieces > 1));
     if (waves_for(1) <= kMostWaves && !two) return launch_units<DT, BLK, 1>(a, waves_for(1), stream);
-    if (waves_for(2) <= kMostWaves) return launch_units<DT, BLK, 2>(a, waves_for(2), stream);
-    return launch_units<DT, BLK, 4>(a, waves_for(4), stream);
+    // (rotated pieces are twice as long: two a wave are enough for every row)
+    if constexpr (BLK <= 0)
+        if (waves_for(2) > kMostWaves) return launch_units<DT, BLK, 4>(a, waves_for(4), stream);
+    return launch_units<DT, BLK, 2>(a, waves_for(2), stream);
 }
 
 template <int DT>
