@@ -7,13 +7,13 @@
 //
 // Angles: f_i is given as a 64-bit fraction of a turn, so p f_i modulo a turn is the integer product p f_i modulo 2^64,
 // exact for every position (in fp32 a position of 60000 would already be off by 4e-3); its cosine and sine are
-// taken in fp64 and rounded to fp32 once. One workgroup takes one token: its angles are computed once, by one wave, and
-// serve all heads from LDS.
+// taken in fp64 and rounded to fp32 once. A workgroup takes a token, of few tokens a part of one's heads: it computes the angles, a
+// thread a pair, and they serve all its heads from LDS.
 //
-// Memory-bound: each value is read once and written once. 17.5 k tokens of 48 heads of 128 in bf16, 429 MB: 85 us, 5.0 TB/s (a copy 5.1). 8.5 k tokens of 24 heads of 128 into int8, 96 MB:
-// 29 us, 3.3 TB/s beside the angles in fp64 and eight divisions a lane (a row's values loaded in front of the angles, the next
-// row's in front of a row's work: 32 us, 93 instead of 89 into 16 bits). 64 single tokens: 3.9 us, chains of dependent loads
-// (length, table, row) and the angles.
+// Memory-bound: each value is read once and written once. 17.5 k tokens of 48 heads of 128 in bf16, 429 MB: 85 us, 5.0 TB/s (a copy
+// 5.1; under the profiler 89). 8.5 k tokens of 24 heads of 128 into int8, 96 MB: 28 us, 3.4 TB/s beside the angles in fp64 and eight
+// divisions a lane (a row's values loaded in front of the angles, the next row's in front of a row's work: 32 us; into 16 bits, both
+// under the profiler, 93 instead of 89). 64 single tokens: 3.7 us, chains of dependent loads (length, table, row) and the angles.
 //
 // A row is 8 values a lane on the 2^k lanes that hold it; a lane of a turned row of halves holds four values of each half, so
 // that it has both of a pair.

@@ -25,15 +25,15 @@
 // share of 5 TB/s over 2 us is 40 KB) and nothing else takes a tile's time (64 keys of 128 values, 32 KB: 1.6 us). So:
 //   loads      go to LDS by themselves into a ring of tiles, three ahead of the one that is worked on, with the table's entries
 //              of the tiles behind those among them: the loop has no other loads, and its one wait leaves those of the later
-//              tiles on their way (in registers, one tile ahead: 54 us instead of 46)
+//              tiles on their way (in registers, one tile ahead: 8 us more)
 //   LDS reads  of a tile's keys are all sent for before the first product, and its values before the softmax (each in front of
-//              its product: 57 us)
+//              its product: 11 us more)
 //   waves      eight at 128 values a head, so that a matrix unit has one wave's products while another's softmax runs; each
 //              takes 32 of the 64 keys, or with up to 64 rows four do. 64 values: four, as a tile is half as long; 256: four,
 //              whose sums need the registers of two
 //   int8       16 bytes of a row by each thread, in 16 bits for all waves' products once
-// 32 sequences of 32 heads over 32000 shared tokens of 8 cache heads, 131 MB: 46 us, 2.9 TB/s and 366 TFLOP/s (16 rows a
-// wave with keys straight to registers, read again for every 64 rows: 68 us).
+// 32 sequences of 32 heads over 32000 shared tokens of 8 cache heads, 131 MB: 49 us, 2.7 TB/s and 346 TFLOP/s (16 rows a
+// wave with keys straight to registers, read again for every 64 rows: 22 us more).
 #include "mq_attn_decode_kernel.h"
 
 namespace mq {
@@ -44,7 +44,8 @@ constexpr int kPlanThreads = 1024;
 // ---------------------------------------------------------------------------------------- the plan
 //
 // Sequences belong together if their first pages are the same; what a group shares is the shortest run of equal pages
-// of a member and the group's first sequence, no longer than any member. Integers of a few hundred sequences: latency, of
+// of a member and the group's first sequence, no longer than any member. (So one member that has only a common beginning with
+// the others leaves them only that to share, and of beginnings inside beginnings the outermost is shared.) Integers of a few hundred sequences: latency, of
 // one workgroup (64 sequences of 9000 tokens in pages of 16: 12 us, a wave's tables one behind the other 14; 704 sequences that
 // share nothing: 30 us, with a wave for each sequence's look at all the others 104).
 // ON_CHIP: working space in LDS (up to kPlanRows sequences), else behind the plan.

@@ -236,16 +236,17 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
 # Keys and values, bytes, that a plan has to save reading for. Sharing costs a launch more and the parts' joining, 8 to 16 us, and
 # saves little time a byte, as the second reading of a page comes from the caches. (us, every sequence alone / shared: 16 / 4
 # heads of 128, 4 over 4096 tokens, 25 MB saved, 20 / 25; 8 groups of 8 over 1024, 117 MB, 25 / 27; 16 over 4096, 126 MB, 33 / 28;
-# 32 / 8 heads, 8 groups of 8 over 256, 59 MB, 21 / 30; over 1024, 235 MB, 42 / 37; int8, 4 over 16384, 101 MB, 41 / 39)
+# 32 / 8 heads, 8 groups of 8 over 256, 59 MB, 21 / 31; over 1024, 235 MB, 42 / 38; int8, 4 over 16384, 101 MB, 41 / 40)
 LEAST_SHARED = 100 << 20
 
 
 def kv_shared(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, least: int | None = None) -> torch.Tensor:
     """Which sequences hold the same first pages (forks of one another), as a plan for paged_attention(shared=): int32 on the
-    device, the same for all layers. It holds while sequences grow, and until one is freed or forked to, or a shared entry of
-    the table changes. page_size: the cache's (with another one nothing is shared). least: where the plan saves the reading of fewer
-    bytes of keys and values than that (as many as the attention's heads and type make of its tokens), every sequence is attended by
-    itself; None: 100 MiB."""
+    device, the same for all layers. All sequences with the same first page are one group, which shares what all of them have in
+    common: one that soon goes its own way shortens that for the others. It holds while sequences grow, and until one is freed or
+    forked to, or a shared entry of the table changes. page_size: the cache's (with another one nothing is shared). least: where the
+    plan saves the reading of fewer bytes of keys and values than that (as many as the attention's heads and type make of its
+    tokens), every sequence is attended by itself; None: 100 MiB."""
     dev = _device_of(page_table, "page_table")
     page_table = _apart(page_table)
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):

@@ -555,8 +555,8 @@ int mq_kv_append(const void* q, int64_t q_token, int64_t q_head, void* out, int6
 
 /*
  * mq_kv_shared: which sequences hold the same first pages, to plan: int32 [mq_kv_shared_ints(rows)], whose words only
- * mq_paged_attention_shared reads. A group shares the tokens of the longest run of table entries that are equal in all its
- * sequences; least_bytes: of keys and values that are read once instead of once per sequence, all groups together, below which
+ * mq_paged_attention_shared reads. A group is of all sequences with the same first page and shares the tokens of the longest run of
+ * table entries that are equal in all of them; least_bytes: of keys and values that are read once instead of once per sequence, all groups together, below which
  * nothing is shared (in units of 1024, rounded down; from 2^41 - 1024 on: nothing ever is; about 100 million is where the
  * additional launch pays).
  * mq_paged_attention_shared: mq_paged_attention of one new token per sequence (no window), where the
