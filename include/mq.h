@@ -153,7 +153,7 @@ int mq_swiglu_rotquant(const void* h, int h_dtype, int64_t M, int64_t K, int64_t
  *          otherwise) or int8 [N, K] for I8_ROW; row stride ldq bytes
  *   scale  fp16 [N, K/64] (stride ld_scale elements) for the group formats, fp32 [N] otherwise
  *   zero   U4_ASYM_G64 only: packed uint4 [N, ceil(K/128)] (group 2j low nibble), stride ld_zero
- * Requires K % 64 == 0 (group formats) or K % 16 == 0, K % hblock == 0, K <= 32768. Output rows
+ * Requires K % 64 == 0 (group formats) or K % 16 == 0, K % hblock == 0, K <= 32768, N < 2^24 for the row formats. Output rows
  * are written by plain stores; no alignment beyond the element size is needed.
  */
 int mq_quantize_weight(const void* w, int dtype, int64_t N, int64_t K, int64_t ldw, int hblock, int format,
@@ -432,7 +432,8 @@ int mq_linear_w4_group_noalloc(const void* x, int x_dtype, int64_t ldx, int hblo
  *
  * mq_kv_write: k, v [T, H, D] of type dtype (bf16 or fp16) into their pages. int8 cache: per row of D
  * values s = max(max |x| / 127, 1e-10), code = rne(x / s); a row with an infinity or NaN gets codes 0
- * and scale NaN (it reads back as NaN). A token with a position below 0 or behind the table is dropped.
+ * and scale NaN (it reads back as NaN). A token with a position below 0 or behind the table is dropped. T H times D / 8,
+ * rounded up to a power of two, is below 2^32.
  */
 int mq_kv_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                 int dtype, int64_t T, int64_t H, int64_t D, void* k_cache, void* v_cache, int cache_dtype,
