@@ -236,8 +236,8 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
 # Keys and values, bytes, that a plan has to save reading for. Sharing costs a launch more and the parts' joining, 8 to 16 us, and
 # saves little time a byte, as the second reading of a page comes from the caches. (us, every sequence alone / shared: 16 / 4
 # heads of 128, 4 over 4096 tokens, 25 MB saved, 20 / 25; 8 groups of 8 over 1024, 117 MB, 25 / 27; 16 over 4096, 126 MB, 33 / 28;
-# 32 / 8 heads, 8 groups of 8 over 256, 59 MB, 21 / 31; over 1024, 235 MB, 42 / 38; int8, 4 over 16384, 101 MB, 41 / 40. Bytes alone are no sharp rule: 8 / 1 heads, 16 over
-# 16384, 126 MB, 33 / 50; 32 / 8 heads, 64 over 1024, 264 MB, 35 / 40.)
+# 32 / 8 heads, 8 groups of 8 over 256, 59 MB, 21 / 31; over 1024, 235 MB, 42 / 38; int8, 4 over 16384, 101 MB, 41 / 40. Bytes
+# alone are no sharp rule: 8 / 1 heads, 16 over 16384, 126 MB, 33 / 50; 32 / 8 heads, 64 over 1024, 264 MB, 35 / 40.)
 LEAST_SHARED = 100 << 20
 
 
